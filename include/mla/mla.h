@@ -364,6 +364,90 @@ int mla_kv_append_paged(mla_dtype_t dtype, const mla_dims_t* dims, const void* x
                         int32_t page_size, void* c_kv_pages, void* pe_pages, void* workspace,
                         size_t workspace_bytes, hipStream_t stream);
 
+/* ---- Paged cache in 8 bits with a scale for each block of tokens (none in the reference).
+ * The pools hold OCP e4m3 codes, and a scale byte for each block of scale_block tokens and each
+ * part of a row (the rows of one block share a page):
+ *   c_kv_pages [num_pages, page_size, 512], pe_pages [num_pages, page_size, 64]   uint8 codes
+ *   scales     [num_pages, page_size / scale_block, 2]   uint8 E8M0 (OCP MX): [..., 0] is the
+ *              latent's, [..., 1] the rope key's
+ * with value = code * 2^(byte - 127).  The bytes of blocks that hold keys are 1 .. 254; the pool
+ * may hold anything where no sequence has a key.  scale_block is 16, 32 or 64, page_size a
+ * positive multiple of 64, kv_rank 512 and rope 64 (MLA_ERR_UNSUPPORTED otherwise).
+ * block_table [B, max_pages] as above; a table entry outside [0, num_pages) is never followed. */
+
+/* Block tables, positions and slots from request lengths, for a batch of `batch` requests of up
+ * to `sq` new tokens each over a pool of num_pages pages (any cache format).  Request b holds
+ * L = seq_lens[b] tokens (clamped to [0, max_pages * page_size]) in the first
+ * ceil(L / page_size) entries of its table row, and
+ *   new_lens[b] > 0   asks for that many more.  It is granted if it is at most sq, the table's
+ *                     span holds the sum, and the free pages cover the new pages of this request
+ *                     and of every earlier one that met the first two conditions (a request that
+ *                     needs no new page waits for none); else it gets nothing;
+ *   new_lens[b] < 0   drops its last -new_lens[b] tokens (at most L): rejected drafts, or with
+ *                     INT32_MIN a request that ended.  Pages that it no longer touches go back.
+ * Free pages are a ring: free_pages [num_pages] with free_state {head, count}, the free ones at
+ * (head + i) % num_pages, i < count.  Pages are taken from its head, in request and page order;
+ * pages given back go behind its tail in the same order, for later calls (past num_pages of them in
+ * all they are dropped; every page is in the ring or in one table row, so that none is).
+ *   seq_lens_out [B], free_state_out [2]   the state after the call; may be seq_lens, free_state
+ *   block_table  [B, max_pages]            updated in place: new entries only
+ *   granted      [B]       tokens added or (negative) dropped
+ *   positions, slots [B, sq] int64: a request's n new tokens are the last n of its sq rows, as
+ *                attention's causal rule has them; the token's position in its sequence, and its
+ *                row of the pool (page * page_size + row in the page); -1 in the other rows
+ * All of it is device memory; nothing is read back.  positions is what mla_q_absorbed_ragged and
+ * mla_kv_append_paged take (which skips rows at -1), slots what mla_kv_read_fp8blk takes.
+ * batch * sq and num_pages are at most 2^30, batch * max_pages and the span below 2^31. */
+size_t mla_cache_extend_workspace_bytes(int32_t batch);
+int mla_cache_extend(int32_t batch, int32_t sq, int32_t page_size, int32_t max_pages,
+                     int32_t num_pages, const int32_t* new_lens, const int32_t* seq_lens,
+                     const int32_t* free_state, int32_t* block_table, int32_t* free_pages,
+                     int32_t* seq_lens_out, int32_t* free_state_out, int32_t* granted,
+                     int64_t* positions, int64_t* slots, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream);
+
+/* KV-cache append into that cache: mla_kv_append's rows for the last new_lens[b] of the sq rows
+ * of x (clamped to [0, min(sq, seq_lens[b])]; the other rows are padding) go to positions
+ * [seq_lens[b] - new_lens[b], seq_lens[b]) of sequence b, which are also their RoPE positions --
+ * seq_lens and new_lens as mla_cache_extend leaves them (seq_lens_out, granted).  A block's scale
+ * is the smallest power of two, at least 2^-100, under which each finite new value's magnitude is
+ * at most 448; a block that keeps rows before the new ones has at least the scale that it had,
+ * and where that grows those rows are coded again (without error, but for values that become
+ * subnormal).  Codes are the float32 rows rounded once, to nearest even; a value that is not
+ * finite becomes NaN.  Rows at and past seq_lens[b], and blocks without new rows, keep their bytes.
+ * A page with new rows belongs to one sequence (pages that are only read may be shared).
+ * dtype (float32, bf16 or fp16) is that of x, W_kv_a and kv_norm_w; uses dims->batch, sq, hidden,
+ * kv_rank, rope, sk (= max_pages * page_size).  Workspace as mla_kv_append. */
+int mla_kv_append_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const void* x,
+                               const void* W_kv_a, const void* kv_norm_w, const float* inv_freq,
+                               double eps, const int32_t* seq_lens, const int32_t* new_lens,
+                               const int32_t* block_table, int32_t page_size, int32_t num_pages,
+                               int32_t scale_block, void* c_kv_pages, void* pe_pages,
+                               void* scales, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+
+/* Rows of that cache, decoded: for each of n slots (pool rows) latent [n, 512] and rope [n, 64]
+ * in dtype (float32, bf16, fp16; float32 and, in its normal range, bf16 hold the values exactly).
+ * A slot outside the pool (mla_cache_extend's -1) gives rows of zeros. */
+int mla_kv_read_fp8blk(mla_dtype_t dtype, const int64_t* slots, int64_t n,
+                       const void* c_kv_pages, const void* pe_pages, const void* scales,
+                       int32_t page_size, int32_t num_pages, int32_t scale_block, void* latent,
+                       void* rope, hipStream_t stream);
+
+/* Attention over that cache: mla_attention_paged on its values, with bf16 or fp16 queries, W_uv
+ * and output (values enter the products in that type: exact in bf16's normal range, and in
+ * fp16's).  Same block_table, seq_lens and causal rule; a sequence or query that sees no key gives
+ * zero rows, and rows of a page outside the pool count as zeros. */
+size_t mla_attention_paged_fp8blk_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims,
+                                                  int causal, int32_t page_size);
+int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_absorbed,
+                               const void* q_rope, const void* c_kv_pages, const void* pe_pages,
+                               const void* scales, const int32_t* block_table,
+                               const int32_t* seq_lens, int32_t page_size, int32_t num_pages,
+                               int32_t scale_block, const void* W_uv, double scale, int causal,
+                               void* out, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+
 /* Output projection wo: out [B*Sq, hidden] = attn [B*Sq, H*v] @ W_o [H*v, hidden], all in
  * dtype (fp32 accumulation).  attn is mla_attention's output [B, Sq, H, v]. */
 size_t mla_o_proj_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims);

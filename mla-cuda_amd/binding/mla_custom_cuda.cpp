@@ -10,7 +10,9 @@
 // the very kernels the fused calls run, and the path's neighbours: split_wkv_b (weight
 // prep), kv_append (the cache write) and o_proj (wo); mla_attention_paged and
 // kv_append_paged for a ragged, paged cache (q_absorbed takes [B, Sq] positions for it);
-// mla_attention_fp8kv and mla_attention_paged_fp8kv for an e4m3 cache.  This file only
+// mla_attention_fp8kv and mla_attention_paged_fp8kv for an e4m3 cache; cache_extend,
+// kv_append_paged_fp8blk, kv_read_fp8blk and mla_attention_paged_fp8blk for a paged e4m3 cache
+// with a scale for each block of tokens.  This file only
 // validates tensors, allocates outputs and workspace from torch's caching allocator and
 // passes raw pointers and the current HIP stream to the C ABI; all device work lives in
 // libmla_amd.so.
@@ -716,6 +718,214 @@ void op_kv_append_paged(torch::Tensor x, torch::Tensor W_kv_a, torch::Tensor kv_
                  "kv_append_paged");
 }
 
+// ------------------------------------------------------------------ paged cache, block scales
+
+// A paged cache of e4m3 codes with E8M0 scales: pools [pages, page_size, ·] and scales
+// [pages, page_size / block, 2].  Returns the tokens a scale block.
+int32_t check_blocked(const torch::Tensor& ckv, const torch::Tensor& pe, const torch::Tensor& scales) {
+    check_dim(ckv, 3, "c_kv_pages", "[num_pages, page_size, kv_rank]");
+    check_dim(pe, 3, "pe_pages", "[num_pages, page_size, rope]");
+    check_dim(scales, 3, "scales", "[num_pages, page_size / block, 2]");
+    const int64_t P = ckv.size(0), page = ckv.size(1);
+    TORCH_CHECK(pe.size(0) == P && pe.size(1) == page,
+                "pe_pages must be [num_pages, page_size, rope] matching c_kv_pages (got ",
+                pe.sizes(), ")");
+    for (const torch::Tensor* t : {&ckv, &pe})
+        TORCH_CHECK(t->scalar_type() == torch::kFloat8_e4m3fn || t->scalar_type() == torch::kByte,
+                    "MLA: the fp8 cache must be float8_e4m3fn or uint8 codes (got ",
+                    t->scalar_type(), ")");
+    TORCH_CHECK(scales.scalar_type() == torch::kFloat8_e8m0fnu || scales.scalar_type() == torch::kByte,
+                "MLA: scales must be float8_e8m0fnu or uint8 (got ", scales.scalar_type(), ")");
+    TORCH_CHECK(P > 0 && P < INT32_MAX && page > 0 && page < INT32_MAX,
+                "MLA: the pool must have pages and rows (got ", ckv.sizes(), ")");
+    TORCH_CHECK(scales.size(0) == P && scales.size(2) == 2 && scales.size(1) > 0 &&
+                    page % scales.size(1) == 0,
+                "scales must be [num_pages, page_size / block, 2] matching c_kv_pages (got ",
+                scales.sizes(), ")");
+    return (int32_t)(page / scales.size(1));
+}
+
+void check_int32(const torch::Tensor& t, int64_t n, const char* name) {
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == n, name, " must be a 1-D tensor of length ", n,
+                " (got ", t.sizes(), ")");
+    TORCH_CHECK(t.scalar_type() == torch::kInt32, name, " must be int32");
+}
+
+// Block tables, positions and slots from request lengths; block_table and free_pages are updated
+// in place, the rest comes back: [seq_lens, free_state, granted, positions, slots].
+std::vector<torch::Tensor> op_cache_extend(torch::Tensor new_lens, torch::Tensor seq_lens,
+                                           torch::Tensor block_table, torch::Tensor free_pages,
+                                           torch::Tensor free_state, int64_t Sq, int64_t page_size) {
+    check_dim(block_table, 2, "block_table", "[B, max_pages]");
+    TORCH_CHECK(block_table.scalar_type() == torch::kInt32, "block_table must be int32");
+    const int64_t B = block_table.size(0), max_pages = block_table.size(1);
+    TORCH_CHECK(B > 0 && max_pages > 0, "block_table must be [B, max_pages] (got ",
+                block_table.sizes(), ")");
+    check_int32(new_lens, B, "new_lens");
+    check_int32(seq_lens, B, "seq_lens");
+    check_int32(free_state, 2, "free_state");
+    TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) > 0 &&
+                    free_pages.scalar_type() == torch::kInt32,
+                "free_pages must be a 1-D int32 tensor with a place for each page of the pool (got ",
+                free_pages.sizes(), ")");
+    TORCH_CHECK(block_table.is_contiguous() && free_pages.is_contiguous(),
+                "MLA: block_table and free_pages are updated in place and must be contiguous");
+    TORCH_CHECK(Sq > 0 && page_size > 0 && Sq < INT32_MAX && page_size < INT32_MAX &&
+                    B < INT32_MAX && max_pages < INT32_MAX && free_pages.size(0) < INT32_MAX,
+                "MLA: Sq and page_size must be positive, and the sizes below 2^31");
+    check_device({&new_lens, &seq_lens, &block_table, &free_pages, &free_state});
+
+    c10::DeviceGuard guard(block_table.device());
+    auto want = new_lens.contiguous();
+    auto lens = seq_lens.contiguous();
+    auto state = free_state.contiguous();
+    auto lens_out = torch::empty_like(lens);
+    auto state_out = torch::empty_like(state);
+    auto granted = torch::empty_like(lens);
+    auto positions = torch::empty({B, Sq}, lens.options().dtype(torch::kLong));
+    auto slots = torch::empty_like(positions);
+    const size_t wsb = mla_cache_extend_workspace_bytes((int32_t)B);
+    auto ws = workspace(wsb, lens);
+    check_status(mla_cache_extend((int32_t)B, (int32_t)Sq, (int32_t)page_size, (int32_t)max_pages,
+                                  (int32_t)free_pages.size(0), want.data_ptr<int32_t>(),
+                                  lens.data_ptr<int32_t>(), state.data_ptr<int32_t>(),
+                                  block_table.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(),
+                                  lens_out.data_ptr<int32_t>(), state_out.data_ptr<int32_t>(),
+                                  granted.data_ptr<int32_t>(), positions.data_ptr<int64_t>(),
+                                  slots.data_ptr<int64_t>(), ws.data_ptr(), wsb, current_stream()),
+                 "cache_extend");
+    return {lens_out, state_out, granted, positions, slots};
+}
+
+// KV-cache append into the blocked 8-bit cache, in place: the last new_lens[b] rows of x[b] become
+// the last tokens of sequence b, which has seq_lens[b] with them.
+void op_kv_append_paged_fp8blk(torch::Tensor x, torch::Tensor W_kv_a, torch::Tensor kv_norm_w,
+                               torch::Tensor seq_lens, torch::Tensor new_lens,
+                               torch::Tensor block_table, torch::Tensor c_kv_pages,
+                               torch::Tensor pe_pages, torch::Tensor scales, double eps) {
+    check_dim(x, 3, "x", "[B, Sq, hidden]");
+    check_dim(W_kv_a, 2, "W_kv_a", "[hidden, kv_rank + rope]");
+    check_dim(block_table, 2, "block_table", "[B, max_pages]");
+    const int32_t block = check_blocked(c_kv_pages, pe_pages, scales);
+    const int64_t B = x.size(0), Sq = x.size(1), hidden = x.size(2);
+    const int64_t page = c_kv_pages.size(1), R = c_kv_pages.size(2), D = pe_pages.size(2);
+    TORCH_CHECK(W_kv_a.size(0) == hidden && W_kv_a.size(1) == R + D,
+                "W_kv_a must be [hidden, kv_rank + rope] (got ", W_kv_a.sizes(), ")");
+    TORCH_CHECK(block_table.size(0) == B && block_table.scalar_type() == torch::kInt32,
+                "block_table must be an int32 [B, max_pages] tensor");
+    TORCH_CHECK(kv_norm_w.dim() == 1 && kv_norm_w.size(0) == R,
+                "kv_norm_w must be a 1-D tensor of length kv_rank (got ", kv_norm_w.sizes(), ")");
+    TORCH_CHECK(D > 0 && D % 2 == 0, "MLA: the rope width must be positive and even");
+    check_int32(seq_lens, B, "seq_lens");
+    check_int32(new_lens, B, "new_lens");
+    TORCH_CHECK(c_kv_pages.is_contiguous() && pe_pages.is_contiguous() && scales.is_contiguous(),
+                "MLA: c_kv_pages, pe_pages and scales are updated in place and must be contiguous");
+    const mla_dtype_t dt = to_mla_dtype(x, "x");
+    check_same_dtype(x, W_kv_a, "W_kv_a");
+    check_same_dtype(x, kv_norm_w, "kv_norm_w");
+    check_device({&x, &W_kv_a, &kv_norm_w, &seq_lens, &new_lens, &block_table, &c_kv_pages, &pe_pages,
+                  &scales});
+
+    c10::DeviceGuard guard(x.device());
+    auto xc = x.contiguous();
+    auto wa = W_kv_a.contiguous();
+    auto g = kv_norm_w.contiguous();
+    auto lens = seq_lens.contiguous();
+    auto fresh = new_lens.contiguous();
+    auto tab = block_table.contiguous();
+    auto inv_freq = device_inv_freq(D, x.device());
+    mla_dims_t d{};
+    d.batch = (int32_t)B; d.sq = (int32_t)Sq; d.hidden = (int32_t)hidden;
+    d.kv_rank = (int32_t)R; d.rope = (int32_t)D;
+    TORCH_CHECK(block_table.size(1) * page < INT32_MAX, "MLA: block_table spans too many keys");
+    d.sk = (int32_t)(block_table.size(1) * page);
+    const size_t wsb = mla_kv_append_workspace_bytes(dt, &d);
+    auto ws = workspace(wsb, x);
+    check_status(mla_kv_append_paged_fp8blk(dt, &d, xc.data_ptr(), wa.data_ptr(), g.data_ptr(),
+                                            inv_freq.data_ptr<float>(), eps,
+                                            lens.data_ptr<int32_t>(), fresh.data_ptr<int32_t>(),
+                                            tab.data_ptr<int32_t>(), (int32_t)page,
+                                            (int32_t)c_kv_pages.size(0), block,
+                                            c_kv_pages.data_ptr(), pe_pages.data_ptr(),
+                                            scales.data_ptr(), ws.data_ptr(), wsb,
+                                            current_stream()),
+                 "kv_append_paged_fp8blk");
+}
+
+// Rows of the blocked 8-bit cache by slot, decoded: [latent [.., 512], rope [.., 64]] in dtype.
+std::vector<torch::Tensor> op_kv_read_fp8blk(torch::Tensor slots, torch::Tensor c_kv_pages,
+                                             torch::Tensor pe_pages, torch::Tensor scales,
+                                             torch::ScalarType dtype) {
+    const int32_t block = check_blocked(c_kv_pages, pe_pages, scales);
+    TORCH_CHECK(slots.scalar_type() == torch::kLong, "slots must be int64 (got ", slots.scalar_type(),
+                ")");
+    const int64_t R = c_kv_pages.size(2), D = pe_pages.size(2);
+    TORCH_CHECK(R == 512 && D == 64, "MLA: a cache with block scales needs kv_rank 512 and rope 64 "
+                "(got ", R, ", ", D, ")");
+    const mla_dtype_t dt = to_mla_dtype(torch::empty({0}, torch::TensorOptions().dtype(dtype)),
+                                        "dtype");
+    check_device({&slots, &c_kv_pages, &pe_pages, &scales});
+    c10::DeviceGuard guard(slots.device());
+    auto sl = slots.contiguous();
+    auto ck = c_kv_pages.contiguous();
+    auto pe = pe_pages.contiguous();
+    auto sc = scales.contiguous();
+    auto shape = sl.sizes().vec();
+    shape.push_back(R);
+    auto lat = torch::empty(shape, sl.options().dtype(dtype));
+    shape.back() = D;
+    auto rot = torch::empty(shape, sl.options().dtype(dtype));
+    check_status(mla_kv_read_fp8blk(dt, sl.data_ptr<int64_t>(), sl.numel(), ck.data_ptr(),
+                                    pe.data_ptr(), sc.data_ptr(), (int32_t)ck.size(1),
+                                    (int32_t)ck.size(0), block, lat.data_ptr(), rot.data_ptr(),
+                                    current_stream()),
+                 "kv_read_fp8blk");
+    return {lat, rot};
+}
+
+// Attention over the blocked 8-bit cache: as mla_attention_paged on its values, with bf16 or fp16
+// queries, W_uv and output.
+torch::Tensor op_mla_attention_paged_fp8blk(torch::Tensor q_absorbed, torch::Tensor q_rope,
+                                            torch::Tensor c_kv_pages, torch::Tensor pe_pages,
+                                            torch::Tensor scales, torch::Tensor block_table,
+                                            torch::Tensor seq_lens, torch::Tensor W_uv,
+                                            double scale, bool causal) {
+    int64_t page = 0;
+    mla_dims_t d = paged_dims(q_absorbed, q_rope, c_kv_pages, pe_pages, block_table, &seq_lens,
+                              &W_uv, &page);
+    const int32_t block = check_blocked(c_kv_pages, pe_pages, scales);
+    const mla_dtype_t dt = to_mla_dtype(q_absorbed, "q_absorbed");
+    check_same_dtype(q_absorbed, q_rope, "q_rope");
+    check_same_dtype(q_absorbed, W_uv, "W_uv");
+    TORCH_CHECK(dt == MLA_DTYPE_BF16 || dt == MLA_DTYPE_F16,
+                "MLA: a cache with block scales is read with bfloat16 or float16 queries "
+                "(q_absorbed has dtype ", q_absorbed.scalar_type(), ")");
+    check_device({&q_absorbed, &q_rope, &c_kv_pages, &pe_pages, &scales, &block_table, &seq_lens,
+                  &W_uv});
+
+    c10::DeviceGuard guard(q_absorbed.device());
+    auto qa = q_absorbed.contiguous();
+    auto qr = q_rope.contiguous();
+    auto ck = c_kv_pages.contiguous();
+    auto pe = pe_pages.contiguous();
+    auto sc = scales.contiguous();
+    auto tab = block_table.contiguous();
+    auto lens = seq_lens.contiguous();
+    auto wuv = W_uv.contiguous();
+    auto out = torch::empty({d.batch, d.sq, d.heads, d.v}, qa.options());
+    const size_t wsb = mla_attention_paged_fp8blk_workspace_bytes(dt, &d, causal ? 1 : 0,
+                                                                  (int32_t)page);
+    auto ws = workspace(wsb, qa);
+    check_status(mla_attention_paged_fp8blk(dt, &d, qa.data_ptr(), qr.data_ptr(), ck.data_ptr(),
+                                            pe.data_ptr(), sc.data_ptr(), tab.data_ptr<int32_t>(),
+                                            lens.data_ptr<int32_t>(), (int32_t)page,
+                                            (int32_t)ck.size(0), block, wuv.data_ptr(), scale,
+                                            causal ? 1 : 0, out.data_ptr(), ws.data_ptr(), wsb,
+                                            current_stream()),
+                 "mla_attention_paged_fp8blk");
+    return out;
+}
+
 // ------------------------------------------------------------------ neighbours of the path
 
 // Weight prep once at load: the W_uk / W_uv halves of wkv_b as contiguous tensors.
@@ -892,4 +1102,27 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "KV-cache append into a paged cache: token (b, s) to slot positions[b, s]",
           py::arg("x"), py::arg("W_kv_a"), py::arg("kv_norm_w"), py::arg("positions"),
           py::arg("block_table"), py::arg("c_kv_pages"), py::arg("pe_pages"), py::arg("eps"));
+    m.def("cache_extend", &op_cache_extend,
+          "Block tables, positions and slots from request lengths: requests grow by new_lens[b] "
+          "(at most Sq) tokens or drop some, pages come from and go to the ring of free ones; "
+          "block_table and free_pages in place, returns [seq_lens, free_state, granted, positions, "
+          "slots]",
+          py::arg("new_lens"), py::arg("seq_lens"), py::arg("block_table"), py::arg("free_pages"),
+          py::arg("free_state"), py::arg("Sq"), py::arg("page_size"));
+    m.def("kv_append_paged_fp8blk", &op_kv_append_paged_fp8blk,
+          "KV-cache append in place into a paged cache of e4m3 codes with a power-of-two scale for "
+          "each block of tokens: the last new_lens[b] rows of x[b] are the last tokens of sequence b",
+          py::arg("x"), py::arg("W_kv_a"), py::arg("kv_norm_w"), py::arg("seq_lens"),
+          py::arg("new_lens"), py::arg("block_table"), py::arg("c_kv_pages"), py::arg("pe_pages"),
+          py::arg("scales"), py::arg("eps"));
+    m.def("kv_read_fp8blk", &op_kv_read_fp8blk,
+          "Rows of that cache by slot, decoded: returns [latent [.., 512], rope [.., 64]]; zeros "
+          "for slots outside the pool",
+          py::arg("slots"), py::arg("c_kv_pages"), py::arg("pe_pages"), py::arg("scales"),
+          py::arg("dtype"));
+    m.def("mla_attention_paged_fp8blk", &op_mla_attention_paged_fp8blk,
+          "Attention over that cache (bf16 or fp16 queries and output): returns out [B, Sq, H, v]",
+          py::arg("q_absorbed"), py::arg("q_rope"), py::arg("c_kv_pages"), py::arg("pe_pages"),
+          py::arg("scales"), py::arg("block_table"), py::arg("seq_lens"), py::arg("W_uv"),
+          py::arg("scale"), py::arg("causal") = false);
 }

@@ -769,6 +769,53 @@ int check_pages(const mla_dims_t* d, int32_t page_size) {
     return MLA_OK;
 }
 
+// x @ W_kv_a (or its *nsplit split-K partials) into the workspace.
+int run_kv_product(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, const void* W_kv_a,
+                   GemmPlan plan, void* workspace, int* nsplit, hipStream_t stream) {
+    float* acc = at<float>(workspace, 0);
+    GemmProblem gp = kv_problem(dtype, dims, x, W_kv_a, acc);
+    *nsplit = 1;
+    if (plan.split > 1) {
+        *nsplit = plan.split;
+        plan.workspace_bytes = 0;
+        MLA_TRY_HIP(launch_gemm_partials(gp, plan, acc, stream), "kv GEMM launch");
+    } else {
+        MLA_TRY_HIP(launch_gemm(gp, plan, nullptr, stream), "kv GEMM launch");
+    }
+    return ok();
+}
+
+// The blocked 8-bit pools: their pages and scale blocks, and with dims the widths and the table.
+int check_blocked_pool(int32_t page_size, int32_t num_pages, int32_t scale_block) {
+    if (page_size <= 0 || page_size % 64 != 0)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "page_size must be a positive multiple of 64 (got %d)",
+                    page_size);
+    MLA_CHECK(check_pos(num_pages, "num_pages"));
+    if (scale_block != 16 && scale_block != 32 && scale_block != 64)
+        return fail(MLA_ERR_UNSUPPORTED, "scale_block must be 16, 32 or 64 tokens (got %d)", scale_block);
+    return MLA_OK;
+}
+int check_fp8blk(const mla_dims_t* d, int32_t page_size, int32_t num_pages, int32_t scale_block) {
+    if (d->kv_rank != 512 || d->rope != 64)
+        return fail(MLA_ERR_UNSUPPORTED, "a cache with block scales needs kv_rank 512 and rope 64 "
+                    "(got %d, %d)", d->kv_rank, d->rope);
+    MLA_CHECK(check_pages(d, page_size));
+    return check_blocked_pool(page_size, num_pages, scale_block);
+}
+int check_fp8blk_attn(mla_dtype_t dtype, const mla_dims_t* d, int causal, int32_t page_size,
+                      int32_t num_pages, int32_t scale_block) {
+    if (!is_half(dtype))
+        return fail(MLA_ERR_UNSUPPORTED, "a cache with block scales is read with bf16 or fp16 queries "
+                    "(dtype %d)", (int)dtype);
+    MLA_CHECK(check_attn_dims(dtype, d, causal));
+    MLA_CHECK(check_fp8blk(d, page_size, num_pages, scale_block));
+    // the pass forms 32-bit per-lane offsets within one sequence's query rows
+    if ((int64_t)d->sq * d->heads * d->kv_rank * 2 >= 0x7fffffff)
+        return fail(MLA_ERR_UNSUPPORTED, "Sq * heads * kv_rank * 2 must be below 2^31 bytes (Sq %d, "
+                    "heads %d)", d->sq, d->heads);
+    return MLA_OK;
+}
+
 // KV append: x @ W_kv_a into the workspace, then the fused norm / RoPE / scatter kernel.
 // Dense: rows start_row + s of a [B, cache_rows] cache.  Paged (block_table): the rows of
 // slots positions[b*Sq + s] through the table.
@@ -807,15 +854,8 @@ int kv_append_impl(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, con
     const int bq = dims->batch * dims->sq;
     const int n = dims->kv_rank + dims->rope;
     float* acc = at<float>(workspace, 0);
-    GemmProblem gp = kv_problem(dtype, dims, x, W_kv_a, acc);
     int nsplit = 1;
-    if (plan.split > 1) {
-        nsplit = plan.split;
-        plan.workspace_bytes = 0;
-        MLA_TRY_HIP(launch_gemm_partials(gp, plan, acc, stream), "kv GEMM launch");
-    } else {
-        MLA_TRY_HIP(launch_gemm(gp, plan, nullptr, stream), "kv GEMM launch");
-    }
+    MLA_CHECK(run_kv_product(dtype, dims, x, W_kv_a, plan, workspace, &nsplit, stream));
     MLA_TRY_HIP(launch_kv_append(acc, nsplit, (int64_t)bq * n, kv_norm_w, positions, inv_freq,
                                  c_kv, pe_cache, storage_out(dtype), dims->batch, dims->sq,
                                  dims->kv_rank, dims->rope, start_row, cache_rows, (float)eps,
@@ -1075,16 +1115,25 @@ FlashProblem fp8_problem(const mla_dims_t* d, const void* qa, const void* qr, co
     return p;
 }
 
-// ragged: the paged pool's plan (the balanced work list and its partial slots)
-Fp8Layout fp8_layout(const mla_dims_t* d, bool ragged = false) {
+// block scales: 16-bit queries of either format
+FlashProblem fp8blk_problem(mla_dtype_t dt, const mla_dims_t* d, const void* qa, const void* qr,
+                            const void* ckv, const void* pe, const void* scales, int scale_block,
+                            double scale, int causal) {
+    FlashProblem p = flash_problem(dt, d, qa, qr, ckv, pe, scale, causal);
+    p.fp8_kv = true;
+    p.scales = static_cast<const uint8_t*>(scales);
+    p.scale_block = scale_block;
+    return p;
+}
+
+// the workspace of a pass over an fp8 cache (`fp`, whose pointers do not matter) and 3d
+Fp8Layout fp8_layout_of(mla_dtype_t dt, const mla_dims_t* d, const FlashProblem& fp) {
     Fp8Layout L;
     const size_t rows = (size_t)d->batch * d->sq * d->heads;
-    FlashProblem fp = fp8_problem(d, nullptr, nullptr, nullptr, nullptr, 1.f, 1.0, 0);
-    fp.ragged = ragged;
     L.flash = plan_flash(fp);
     L.ctx16 = flash_ctx16_ok(fp, L.flash);
-    L.out = L.ctx16 ? plan_gemm(out_problem16(MLA_DTYPE_BF16, d, nullptr, nullptr, nullptr))
-                    : plan_gemm(out_problem(MLA_DTYPE_BF16, d, nullptr, nullptr, nullptr, nullptr));
+    L.out = L.ctx16 ? plan_gemm(out_problem16(dt, d, nullptr, nullptr, nullptr))
+                    : plan_gemm(out_problem(dt, d, nullptr, nullptr, nullptr, nullptr));
     size_t o = 0;
     L.off_rowsum = o; o = align_up(o + rows * sizeof(float));
     L.off_ctx = o;    o = align_up(o + rows * d->kv_rank * sizeof(float));
@@ -1092,6 +1141,17 @@ Fp8Layout fp8_layout(const mla_dims_t* d, bool ragged = false) {
     L.off_part = o;   o = align_up(o + L.flash.partial_bytes);
     L.total = o;
     return L;
+}
+// ragged: the paged pool's plan (the balanced work list and its partial slots)
+Fp8Layout fp8_layout(const mla_dims_t* d, bool ragged = false) {
+    FlashProblem fp = fp8_problem(d, nullptr, nullptr, nullptr, nullptr, 1.f, 1.0, 0);
+    fp.ragged = ragged;
+    return fp8_layout_of(MLA_DTYPE_BF16, d, fp);
+}
+Fp8Layout fp8blk_layout(mla_dtype_t dt, const mla_dims_t* d) {
+    FlashProblem fp = fp8blk_problem(dt, d, nullptr, nullptr, nullptr, nullptr, nullptr, 64, 1.0, 0);
+    fp.ragged = true;
+    return fp8_layout_of(dt, d, fp);
 }
 
 int check_fp8_attn(mla_dtype_t dtype, const mla_dims_t* dims, int causal, float kv_scale) {
@@ -1445,6 +1505,157 @@ int mla_attention(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_absor
     MLA_TRY_HIP(launch_gemm(cp, L.ctx, at<void>(workspace, L.off_ctx_ws), stream), "3c launch");
     // 3d
     GemmProblem op = out_problem(dtype, dims, ctx, row_sum, W_uv, out);
+    MLA_TRY_HIP(launch_gemm(op, L.out, at<void>(workspace, L.off_out_ws), stream), "3d launch");
+    return ok();
+}
+
+// ------------------------------------------------------------------ 8-bit blocked cache
+
+size_t mla_cache_extend_workspace_bytes(int32_t batch) {
+    return batch > 0 ? align_up(cache_extend_workspace(batch)) : 0;
+}
+
+int mla_cache_extend(int32_t batch, int32_t sq, int32_t page_size, int32_t max_pages,
+                     int32_t num_pages, const int32_t* new_lens, const int32_t* seq_lens,
+                     const int32_t* free_state, int32_t* block_table, int32_t* free_pages,
+                     int32_t* seq_lens_out, int32_t* free_state_out, int32_t* granted,
+                     int64_t* positions, int64_t* slots, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream) {
+    MLA_CHECK(check_pos(batch, "batch"));
+    MLA_CHECK(check_pos(sq, "sq"));
+    MLA_CHECK(check_pos(max_pages, "max_pages"));
+    MLA_CHECK(check_pos(num_pages, "num_pages"));
+    if (page_size <= 0 || page_size % 64 != 0)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "page_size must be a positive multiple of 64 (got %d)",
+                    page_size);
+    constexpr int64_t kMost = (int64_t)1 << 30;   // the kernels' sums of these stay in 32 bits
+    if ((int64_t)batch * sq > kMost || num_pages > kMost)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "batch * sq and num_pages must be at most 2^30");
+    if ((int64_t)max_pages * page_size > kMaxI32 || (int64_t)batch * max_pages > kMaxI32)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "max_pages * page_size and batch * max_pages must be "
+                    "below 2^31");
+    MLA_CHECK(check_ptr(new_lens, "new_lens"));
+    MLA_CHECK(check_ptr(seq_lens, "seq_lens"));
+    MLA_CHECK(check_ptr(free_state, "free_state"));
+    MLA_CHECK(check_ptr(block_table, "block_table"));
+    MLA_CHECK(check_ptr(free_pages, "free_pages"));
+    MLA_CHECK(check_ptr(seq_lens_out, "seq_lens_out"));
+    MLA_CHECK(check_ptr(free_state_out, "free_state_out"));
+    MLA_CHECK(check_ptr(granted, "granted"));
+    MLA_CHECK(check_ptr(positions, "positions"));
+    MLA_CHECK(check_ptr(slots, "slots"));
+    MLA_CHECK(check_ws(workspace, workspace_bytes, mla_cache_extend_workspace_bytes(batch)));
+    CacheExtend p;
+    p.B = batch; p.Sq = sq; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
+    p.new_lens = new_lens; p.seq_lens = seq_lens; p.free_state = free_state;
+    p.block_table = block_table; p.free_pages = free_pages;
+    p.seq_lens_out = seq_lens_out; p.free_state_out = free_state_out; p.granted = granted;
+    p.positions = positions; p.slots = slots;
+    MLA_TRY_HIP(launch_cache_extend(p, workspace, stream), "cache extend launch");
+    return ok();
+}
+
+int mla_kv_append_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const void* x,
+                               const void* W_kv_a, const void* kv_norm_w, const float* inv_freq,
+                               double eps, const int32_t* seq_lens, const int32_t* new_lens,
+                               const int32_t* block_table, int32_t page_size, int32_t num_pages,
+                               int32_t scale_block, void* c_kv_pages, void* pe_pages,
+                               void* scales, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream) {
+    MLA_CHECK(check_dtype(dtype));
+    MLA_CHECK(check_kv_dims(dtype, dims));
+    MLA_CHECK(check_fp8blk(dims, page_size, num_pages, scale_block));
+    MLA_CHECK(check_ptr(x, "x"));
+    MLA_CHECK(check_ptr(W_kv_a, "W_kv_a"));
+    MLA_CHECK(check_ptr(kv_norm_w, "kv_norm_w"));
+    MLA_CHECK(check_ptr(inv_freq, "inv_freq"));
+    MLA_CHECK(check_ptr(seq_lens, "seq_lens"));
+    MLA_CHECK(check_ptr(new_lens, "new_lens"));
+    MLA_CHECK(check_ptr(block_table, "block_table"));
+    MLA_CHECK(check_ptr(c_kv_pages, "c_kv_pages"));
+    MLA_CHECK(check_ptr(pe_pages, "pe_pages"));
+    MLA_CHECK(check_ptr(scales, "scales"));
+    if (!(eps >= 0.0) || !std::isfinite(eps))
+        return fail(MLA_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
+    GemmPlan plan;
+    const size_t need = kv_ws_bytes(dtype, dims, &plan);
+    MLA_CHECK(check_ws(workspace, workspace_bytes, need));
+    KvAppendBlk p;
+    MLA_CHECK(run_kv_product(dtype, dims, x, W_kv_a, plan, workspace, &p.nsplit, stream));
+    p.in = at<float>(workspace, 0);
+    p.split_stride = (int64_t)dims->batch * dims->sq * (dims->kv_rank + dims->rope);
+    p.gain = kv_norm_w; p.gain_type = storage_out(dtype); p.inv_freq = inv_freq;
+    p.seq_lens = seq_lens; p.new_lens = new_lens; p.block_table = block_table;
+    p.c_kv = c_kv_pages; p.pe = pe_pages; p.scales = scales;
+    p.B = dims->batch; p.Sq = dims->sq; p.page_size = page_size;
+    p.max_pages = dims->sk / page_size; p.num_pages = num_pages; p.block = scale_block;
+    p.eps = (float)eps;
+    MLA_TRY_HIP(launch_kv_append_blk(p, stream), "kv append launch");
+    return ok();
+}
+
+int mla_kv_read_fp8blk(mla_dtype_t dtype, const int64_t* slots, int64_t n,
+                       const void* c_kv_pages, const void* pe_pages, const void* scales,
+                       int32_t page_size, int32_t num_pages, int32_t scale_block, void* latent,
+                       void* rope, hipStream_t stream) {
+    MLA_CHECK(check_dtype(dtype));
+    if (n < 0 || n > ((int64_t)1 << 40))
+        return fail(MLA_ERR_INVALID_ARGUMENT, "n must be in [0, 2^40] (got %lld)", (long long)n);
+    MLA_CHECK(check_blocked_pool(page_size, num_pages, scale_block));
+    if (n == 0) return ok();
+    MLA_CHECK(check_ptr(slots, "slots"));
+    MLA_CHECK(check_ptr(c_kv_pages, "c_kv_pages"));
+    MLA_CHECK(check_ptr(pe_pages, "pe_pages"));
+    MLA_CHECK(check_ptr(scales, "scales"));
+    MLA_CHECK(check_ptr(latent, "latent"));
+    MLA_CHECK(check_ptr(rope, "rope"));
+    KvReadBlk p;
+    p.slots = slots; p.n = n; p.rows = (int64_t)num_pages * page_size;
+    p.c_kv = c_kv_pages; p.pe = pe_pages; p.scales = scales;
+    p.lat = latent; p.rot = rope; p.out_type = storage_out(dtype); p.block = scale_block;
+    MLA_TRY_HIP(launch_kv_read_blk(p, stream), "kv read launch");
+    return ok();
+}
+
+size_t mla_attention_paged_fp8blk_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims,
+                                                  int causal, int32_t page_size) {
+    if (!dims || check_fp8blk_attn(dtype, dims, causal, page_size, 1, 64) != MLA_OK) return 0;
+    return fp8blk_layout(dtype, dims).total;
+}
+
+int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_absorbed,
+                               const void* q_rope, const void* c_kv_pages, const void* pe_pages,
+                               const void* scales, const int32_t* block_table,
+                               const int32_t* seq_lens, int32_t page_size, int32_t num_pages,
+                               int32_t scale_block, const void* W_uv, double scale, int causal,
+                               void* out, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream) {
+    MLA_CHECK(check_fp8blk_attn(dtype, dims, causal, page_size, num_pages, scale_block));
+    MLA_CHECK(check_scale(scale));
+    MLA_CHECK(check_ptr(q_absorbed, "q_absorbed"));
+    MLA_CHECK(check_ptr(q_rope, "q_rope"));
+    MLA_CHECK(check_ptr(c_kv_pages, "c_kv_pages"));
+    MLA_CHECK(check_ptr(pe_pages, "pe_pages"));
+    MLA_CHECK(check_ptr(scales, "scales"));
+    MLA_CHECK(check_ptr(block_table, "block_table"));
+    MLA_CHECK(check_ptr(seq_lens, "seq_lens"));
+    MLA_CHECK(check_ptr(W_uv, "W_uv"));
+    MLA_CHECK(check_ptr(out, "out"));
+    const Fp8Layout L = fp8blk_layout(dtype, dims);
+    MLA_CHECK(check_ws(workspace, workspace_bytes, L.total));
+    float* row_sum = at<float>(workspace, L.off_rowsum);
+    float* ctx = at<float>(workspace, L.off_ctx);
+    FlashProblem fp = fp8blk_problem(dtype, dims, q_absorbed, q_rope, c_kv_pages, pe_pages, scales,
+                                     scale_block, scale, causal);
+    fp.seq_lens = seq_lens;
+    fp.block_table = block_table;
+    fp.page_size = page_size;
+    fp.num_pages = num_pages;
+    MLA_TRY_HIP(launch_flash(fp, L.flash, ctx, row_sum, at<float>(workspace, L.off_part), stream,
+                             true, L.ctx16 ? ctx : nullptr),
+                "blocked fp8-cache attention launch");
+    GemmProblem op = L.ctx16 ? out_problem16(dtype, dims, ctx, W_uv, out)
+                             : out_problem(dtype, dims, ctx, row_sum, W_uv, out);
     MLA_TRY_HIP(launch_gemm(op, L.out, at<void>(workspace, L.off_out_ws), stream), "3d launch");
     return ok();
 }

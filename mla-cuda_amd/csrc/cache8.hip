@@ -1,0 +1,464 @@
+// The paged cache in 8 bits with a power-of-two scale for each block of tokens: block tables,
+// positions and slots from request lengths (extend), the append that writes it and the reader
+// of its rows.  Attention over it is flash16x8_kernel (flash.hip).
+//
+// Format: pools of pages of page_size rows, e4m3 codes [num_pages, page_size, 512] (latent) and
+// [num_pages, page_size, 64] (rope key), and E8M0 scale bytes [num_pages, page_size / G, 2], one
+// for each block of G tokens and each part: value = code * 2^(byte - 127).  The two parts have a
+// scale each because a latent row is RMS-normalised and a rope key is not.  Powers of two cost an
+// e4m3 code no precision (it has an exponent of its own), and they let a block whose scale grows
+// be coded again without error but for values that become subnormal.
+
+#include "common.h"
+#include "kernels.h"
+
+#include <algorithm>
+
+namespace mla {
+
+namespace {
+
+typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
+typedef float v2f_t __attribute__((ext_vector_type(2)));
+
+// ---- extend ---------------------------------------------------------------------------------
+// Request b holds L = seq_lens[b] tokens and asks for new_lens[b] more (or fewer).  What it needs,
+// pages(L + n) - pages(L), is summed over the requests in order, and a request is granted while
+// the running sum stays within the free pages; the same sums place its pages in the ring of free
+// ones.  So the whole plan is two prefix sums over the requests (pages asked for, pages given
+// back), made by one workgroup; then every table entry, ring entry, position and slot follows from
+// its request's four numbers {L, granted, first page taken, first page given back} alone, in any
+// order: taken pages come from the ring's free ones and given ones go to places that hold none, and
+// a new token's page is an old table entry or a free one, so nothing written here is read here.
+// It is bound by latency (a decode step's tables are a few KB).
+constexpr int kExtendThreads = 1024;
+constexpr int kExtendWaves = kExtendThreads / 64;
+
+struct ExtendArgs {
+    int B, Sq, page_size, max_pages, num_pages;
+    const int* new_lens;
+    const int* seq_lens;
+    const int* free_state;   // {head, count}
+    int* table;
+    int* ring;
+    int* lens_out;
+    int* state_out;
+    int* granted;
+    int64_t* positions;
+    int64_t* slots;
+    int4* info;              // [B + 1]: the requests' four numbers, then {head, count, 0, 0}
+};
+
+__device__ __forceinline__ int extend_pages(int tokens, int page_size) {
+    return tokens / page_size + (tokens % page_size != 0);
+}
+
+// The part that follows from `info` (in LDS or memory), by `threads` threads of which this is
+// number `t`: a wave per request for its pages, a thread per position.
+__device__ __forceinline__ void extend_fill(const ExtendArgs& a, const int4* info, int head, int count,
+                                            int t, int threads) {
+    const uint32_t N = (uint32_t)a.num_pages;   // head, count <= N <= 2^30: the sums below fit
+    const int lane = t & 63;
+    for (int b = t >> 6; b < a.B; b += threads >> 6) {
+        const int4 r = info[b];
+        const int have = extend_pages(r.x, a.page_size), end = extend_pages(r.x + r.y, a.page_size);
+        int* row = a.table + (int64_t)b * a.max_pages;
+        for (int j = have + lane; j < end; j += 64) row[j] = a.ring[(uint32_t)(head + r.z + j - have) % N];
+        // past `room` there is no place left behind the tail: a page that is in the ring already
+        const int room = (int)N - count - r.w;
+        for (int j = end + lane; j < have && j - end < room; j += 64)
+            a.ring[((uint32_t)head + (uint32_t)count + (uint32_t)(r.w + j - end)) % N] = row[j];
+    }
+    const int total = a.B * a.Sq;
+    for (int i = t; i < total; i += threads) {
+        const int b = i / a.Sq, s = i - b * a.Sq;
+        const int4 r = info[b];
+        int64_t pos = -1, slot = -1;
+        if (s >= a.Sq - r.y) {
+            const int p = r.x + r.y - a.Sq + s, j = p / a.page_size, have = extend_pages(r.x, a.page_size);
+            const int page = j < have ? a.table[(int64_t)b * a.max_pages + j]
+                                      : a.ring[(uint32_t)(head + r.z + j - have) % N];
+            pos = p;
+            slot = (int64_t)page * a.page_size + p % a.page_size;
+        }
+        a.positions[i] = pos;
+        a.slots[i] = slot;
+    }
+}
+
+// ONE: `info` stays in LDS (B <= kExtendThreads) and this workgroup does the rest too.
+template <bool ONE>
+__global__ void __launch_bounds__(kExtendThreads) cache_extend_kernel(ExtendArgs a) {
+    __shared__ int w_ask[kExtendWaves], w_back[kExtendWaves], w_take[kExtendWaves];
+    __shared__ int4 info_lds[ONE ? kExtendThreads : 1];
+    int4* info = ONE ? info_lds : a.info;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int N = a.num_pages, span = a.max_pages * a.page_size;
+    int head = a.free_state[0] % N;
+    if (head < 0) head += N;
+    const int count = min(max(a.free_state[1], 0), N);
+    const int per = (a.B + kExtendThreads - 1) / kExtendThreads;
+    const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+    // pages asked for by a request that its own limits allow, and given back by one that shrinks
+    auto plan = [&](int b, int* L, int* n, int* ask, int* back) __attribute__((always_inline)) {
+        *L = min(max(a.seq_lens[b], 0), span);
+        *n = a.new_lens[b];
+        *ask = *back = 0;
+        const int have = extend_pages(*L, a.page_size);
+        if (*n > 0) {
+            if (*n > a.Sq || *n > span - *L) *n = 0;
+            else *ask = extend_pages(*L + *n, a.page_size) - have;
+        } else {
+            *n = max(*n, -*L);
+            *back = have - extend_pages(*L + *n, a.page_size);
+        }
+    };
+    int ask = 0, back = 0;
+    for (int b = b0; b < b1; ++b) {
+        int L, n, k, r;
+        plan(b, &L, &n, &k, &r);
+        ask += k;
+        back += r;
+    }
+    int ia = ask, ib = back;   // inclusive scans within the wave, then the waves before
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(ia, d), y = __shfl_up(ib, d);
+        if (lane >= d) { ia += x; ib += y; }
+    }
+    if (lane == 63) { w_ask[wave] = ia; w_back[wave] = ib; }
+    __syncthreads();
+    int asked = ia - ask, pushed = ib - back, all_back = 0;
+    for (int w = 0; w < kExtendWaves; ++w) {
+        if (w < wave) { asked += w_ask[w]; pushed += w_back[w]; }
+        all_back += w_back[w];
+    }
+    int taken = 0;   // pages taken by the requests up to this thread's last granted one
+    for (int b = b0; b < b1; ++b) {
+        int L, n, k, r;
+        plan(b, &L, &n, &k, &r);
+        const int first = asked;
+        asked += k;
+        if (k > 0) {
+            if (asked <= count) taken = asked;
+            else n = 0;
+        }
+        info[b] = make_int4(L, n, first, pushed);
+        pushed += r;
+        a.lens_out[b] = L + n;
+        a.granted[b] = n;
+    }
+    for (int d = 32; d > 0; d >>= 1) taken = max(taken, __shfl_xor(taken, d));
+    if (lane == 0) w_take[wave] = taken;
+    __syncthreads();
+    for (int w = 0; w < kExtendWaves; ++w) taken = max(taken, w_take[w]);
+    if (tid == 0) {
+        a.state_out[0] = (int)(((uint32_t)head + (uint32_t)taken) % (uint32_t)N);
+        a.state_out[1] = count - taken + min(all_back, N - count);
+        if (!ONE) info[a.B] = make_int4(head, count, 0, 0);
+    }
+    if (ONE) extend_fill(a, info, head, count, tid, kExtendThreads);
+}
+
+__global__ void __launch_bounds__(256) cache_extend_fill_kernel(ExtendArgs a) {
+    const int4 s = a.info[a.B];
+    extend_fill(a, a.info, s.x, s.y, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+}
+
+// ---- append ---------------------------------------------------------------------------------
+// A workgroup owns one block of G tokens of one sequence: it forms the block's new rows from the
+// product x @ W_kv_a (or its split-K partials), takes the largest magnitude of each part over
+// them, and codes them.  Nothing of a block is shared between workgroups, so the scale needs no
+// atomics and the result no order.  A wave makes a row at a time (8 latent columns and, in the
+// lower half, one rope pair a lane: the norm is a wave reduction), four rows a wave in registers
+// across the one barrier that the block's maxima need.
+//   scale: 2^e with the smallest e >= -100 such that every finite magnitude is <= 448 * 2^e (448,
+//     e4m3's largest value, is 1.75 * 2^8: e from the exponent and one comparison); where the block
+//     keeps rows written before, at least the scale that they have.  If that grew, they are
+//     coded again: code * 2^(e_old - e), exact but for values that become subnormal.
+//   codes: v * 2^-e rounded once, to nearest even, from the fp32 row; a value that is not finite
+//     becomes the NaN code and has no part in the scale.
+struct AppendBlkArgs {
+    const float* in;         // [nsplit][B*Sq][576], split_stride floats apart
+    int nsplit;
+    int64_t split_stride;
+    const void* gain;
+    const float* inv_freq;
+    const int* seq_lens;     // after the append
+    const int* new_lens;
+    const int* table;
+    uint8_t* c_kv;
+    uint8_t* pe;
+    uint8_t* scales;
+    int B, Sq, page_size, max_pages, num_pages, blocks;
+    float eps;
+};
+
+constexpr int kA8R = 512, kA8D = 64, kA8Row = kA8R + kA8D;
+constexpr int kA8RowsPerWave = 4;
+constexpr int kScaleMin = 127 - 100;
+
+__device__ __forceinline__ float finite_abs(float v) {
+    const float m = fabsf(v);
+    return m < INFINITY ? m : 0.f;
+}
+// the E8M0 byte of the smallest scale that holds magnitudes up to amax (finite, >= 0)
+__device__ __forceinline__ int scale_byte(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    return max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u), kScaleMin);
+}
+__device__ __forceinline__ float scale_value(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+__device__ __forceinline__ float code_input(float v, float inv) {
+    return fabsf(v) < INFINITY ? v * inv : __uint_as_float(0x7fc00000u);
+}
+__device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+// four codes to the values that they have under `scale`, a power of two
+__device__ __forceinline__ v4f decode4(uint32_t w, float scale) {
+    const v2f_t lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false);
+    const v2f_t hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
+    return v4f{lo[0], lo[1], hi[0], hi[1]};
+}
+
+template <int OUT, int G>
+__global__ void __launch_bounds__(64 * G / kA8RowsPerWave) kv_append_blk_kernel(AppendBlkArgs a) {
+    constexpr int kWaves = G / kA8RowsPerWave;
+    __shared__ float red[2][kWaves];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x / a.blocks, t = blockIdx.x % a.blocks;
+    const int L = min(max(a.seq_lens[b], 0), a.max_pages * a.page_size);
+    const int n = min(max(a.new_lens[b], 0), min(a.Sq, L));
+    const int first = L - n, p0 = (first / G + t) * G;
+    if (n == 0 || p0 >= L) return;
+    const int page = a.table[(int64_t)b * a.max_pages + p0 / a.page_size];
+    if (page < 0 || page >= a.num_pages) return;   // not a page of the pool: skipped
+    const int64_t row0 = (int64_t)page * a.page_size + p0 % a.page_size;
+    uint8_t* sc = a.scales + 2 * (row0 / G);
+    int old[2] = {0, 0};
+    if (first > p0) { old[0] = sc[0]; old[1] = sc[1]; }
+
+    float lat[kA8RowsPerWave][8], rot[kA8RowsPerWave][2];
+    float top = 0.f, top_r = 0.f;
+    float gain[8];
+    #pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if constexpr (OUT == kOutF32) gain[k] = static_cast<const float*>(a.gain)[8 * lane + k];
+        else gain[k] = Store16<OUT>::to_f32(static_cast<const uint16_t*>(a.gain)[8 * lane + k]);
+    }
+    #pragma unroll
+    for (int q = 0; q < kA8RowsPerWave; ++q) {
+        const int pos = p0 + wave + kWaves * q;
+        if (pos < first || pos >= L) continue;   // wave-uniform
+        const float* base = a.in + ((int64_t)b * a.Sq + (pos - L + a.Sq)) * kA8Row;
+        const float* lp = base + 8 * lane;
+        const float* rp = base + kA8R + 2 * (lane & 31);
+        v4f s0 = v4f{0.f, 0.f, 0.f, 0.f}, s1 = s0;
+        v2f_t sr = v2f_t{0.f, 0.f};
+        constexpr int kWin = 4;   // splits' loads in flight
+        for (int i = 0; i < a.nsplit; i += kWin) {
+            v4f x0[kWin], x1[kWin];
+            v2f_t xr[kWin];
+            #pragma unroll
+            for (int k = 0; k < kWin; ++k) {
+                const int64_t o = (int64_t)min(i + k, a.nsplit - 1) * a.split_stride;
+                x0[k] = *reinterpret_cast<const v4f*>(lp + o);
+                x1[k] = *reinterpret_cast<const v4f*>(lp + o + 4);
+                xr[k] = *reinterpret_cast<const v2f_t*>(rp + o);
+            }
+            #pragma unroll
+            for (int k = 0; k < kWin; ++k)
+                if (i + k < a.nsplit) { s0 += x0[k]; s1 += x1[k]; sr += xr[k]; }
+        }
+        float ss = 0.f;
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) ss += s0[k] * s0[k] + s1[k] * s1[k];
+        const float inv = rsqrtf(wave_reduce(ss, OpSum()) / (float)kA8R + a.eps);
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            lat[q][k] = (k < 4 ? s0[k] : s1[k - 4]) * inv * gain[k];
+            top = fmaxf(top, finite_abs(lat[q][k]));
+        }
+        float c, s;
+        rope_cos_sin(rope_angle(pos, a.inv_freq[lane & 31]), &c, &s);
+        rot[q][0] = rope_even(sr[0], sr[1], c, s);
+        rot[q][1] = rope_odd(sr[0], sr[1], c, s);
+        top_r = fmaxf(top_r, fmaxf(finite_abs(rot[q][0]), finite_abs(rot[q][1])));
+    }
+    top = wave_reduce(top, OpMax());
+    top_r = wave_reduce(top_r, OpMax());
+    if (lane == 0) { red[0][wave] = top; red[1][wave] = top_r; }
+    __syncthreads();
+    #pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        top = fmaxf(top, red[0][w]);
+        top_r = fmaxf(top_r, red[1][w]);
+    }
+    const int e_lat = max(scale_byte(top), old[0]), e_rot = max(scale_byte(top_r), old[1]);
+    if (threadIdx.x == 0) { sc[0] = (uint8_t)e_lat; sc[1] = (uint8_t)e_rot; }
+    const float inv_l = scale_value(254 - min(e_lat, 254)), inv_r = scale_value(254 - min(e_rot, 254));
+    const bool again_l = first > p0 && e_lat != old[0], again_r = first > p0 && e_rot != old[1];
+    #pragma unroll
+    for (int q = 0; q < kA8RowsPerWave; ++q) {
+        const int pos = p0 + wave + kWaves * q;
+        uint8_t* cl = a.c_kv + (row0 + wave + kWaves * q) * kA8R + 8 * lane;
+        uint8_t* cr = a.pe + (row0 + wave + kWaves * q) * kA8D + 2 * (lane & 31);
+        if (pos >= L) continue;
+        if (pos >= first) {
+            const float* v = lat[q];
+            auto in = [&](int k) __attribute__((always_inline)) { return code_input(v[k], inv_l); };
+            *reinterpret_cast<v2u_t*>(cl) =
+                v2u_t{code4(in(0), in(1), in(2), in(3)), code4(in(4), in(5), in(6), in(7))};
+            if (lane < 32)
+                *reinterpret_cast<uint16_t*>(cr) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(
+                    code_input(rot[q][0], inv_r), code_input(rot[q][1], inv_r), 0, false);
+            continue;
+        }
+        // rows of before, under a larger scale: 2^(e_old - e), at least 2^-100 (which leaves nothing)
+        if (again_l) {
+            const float f = scale_value(127 - min(e_lat - old[0], 100));
+            const v2u_t w = *reinterpret_cast<const v2u_t*>(cl);
+            const v4f x = decode4(w[0], f), y = decode4(w[1], f);
+            *reinterpret_cast<v2u_t*>(cl) = v2u_t{code4(x[0], x[1], x[2], x[3]), code4(y[0], y[1], y[2], y[3])};
+        }
+        if (again_r && lane < 32) {
+            const float f = scale_value(127 - min(e_rot - old[1], 100));
+            const v2f_t x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(
+                (uint32_t)*reinterpret_cast<const uint16_t*>(cr), f, false);
+            *reinterpret_cast<uint16_t*>(cr) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        }
+    }
+}
+
+// ---- read -----------------------------------------------------------------------------------
+// Rows by slot, decoded: a wave takes four rows at a time (their 8 codes a lane, then the rope
+// codes of all four by 16 lanes each), all loads before the first store.  Bound by the bytes.
+struct ReadBlkArgs {
+    const int64_t* slots;
+    int64_t n, rows;         // slots asked for; rows of the pool
+    const uint8_t* c_kv;
+    const uint8_t* pe;
+    const uint8_t* scales;
+    void* lat;               // [n, 512]
+    void* rot;               // [n, 64]
+    int block_shift;         // log2 of the tokens a block
+};
+
+template <int OUT>
+__device__ __forceinline__ void store4(void* dst, int64_t at, v4f v) {
+    if constexpr (OUT == kOutF32)
+        *reinterpret_cast<v4f*>(static_cast<float*>(dst) + at) = v;
+    else
+        *reinterpret_cast<v2u_t*>(static_cast<uint16_t*>(dst) + at) =
+            v2u_t{Store16<OUT>::pack2(v[0], v[1]), Store16<OUT>::pack2(v[2], v[3])};
+}
+
+template <int OUT>
+__global__ void __launch_bounds__(256) kv_read_blk_kernel(ReadBlkArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t waves = (int64_t)gridDim.x * 4;
+    for (int64_t r0 = 4 * ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)); r0 < a.n; r0 += 4 * waves) {
+        v2u_t c[4];
+        float f[4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t s = r0 + i < a.n ? a.slots[r0 + i] : -1;
+            const bool in = s >= 0 && s < a.rows;
+            c[i] = in ? reinterpret_cast<const v2u_t*>(a.c_kv + s * kA8R)[lane] : v2u_t{0, 0};
+            f[i] = in ? scale_value(a.scales[2 * (s >> a.block_shift)]) : 1.f;
+        }
+        const int64_t rr = r0 + (lane >> 4);
+        const int64_t s = rr < a.n ? a.slots[rr] : -1;
+        const bool in = s >= 0 && s < a.rows;
+        const uint32_t p = in ? reinterpret_cast<const uint32_t*>(a.pe + s * kA8D)[lane & 15] : 0;
+        const float fp = in ? scale_value(a.scales[2 * (s >> a.block_shift) + 1]) : 1.f;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (r0 + i >= a.n) break;
+            store4<OUT>(a.lat, (r0 + i) * kA8R + 8 * lane, decode4(c[i][0], f[i]));
+            store4<OUT>(a.lat, (r0 + i) * kA8R + 8 * lane + 4, decode4(c[i][1], f[i]));
+        }
+        if (rr < a.n) store4<OUT>(a.rot, rr * kA8D + 4 * (lane & 15), decode4(p, fp));
+    }
+}
+
+}  // namespace
+
+// Up to this many positions one workgroup does everything; past it a second, wide launch fills.
+constexpr int kExtendOneFill = 8192;
+
+size_t cache_extend_workspace(int B) { return ((size_t)B + 1) * sizeof(int4); }
+
+hipError_t launch_cache_extend(const CacheExtend& p, void* workspace, hipStream_t stream) {
+    ExtendArgs a;
+    a.B = p.B; a.Sq = p.Sq; a.page_size = p.page_size; a.max_pages = p.max_pages; a.num_pages = p.num_pages;
+    a.new_lens = p.new_lens; a.seq_lens = p.seq_lens; a.free_state = p.free_state;
+    a.table = p.block_table; a.ring = p.free_pages;
+    a.lens_out = p.seq_lens_out; a.state_out = p.free_state_out; a.granted = p.granted;
+    a.positions = p.positions; a.slots = p.slots;
+    a.info = static_cast<int4*>(workspace);
+    if (p.B <= kExtendThreads && (int64_t)p.B * p.Sq <= kExtendOneFill) {
+        hipLaunchKernelGGL(cache_extend_kernel<true>, dim3(1), dim3(kExtendThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(cache_extend_kernel<false>, dim3(1), dim3(kExtendThreads), 0, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t wgs = std::max<int64_t>(((int64_t)p.B * p.Sq + 1023) / 1024, (p.B + 3) / 4);
+    hipLaunchKernelGGL(cache_extend_fill_kernel, dim3((unsigned)std::min<int64_t>(wgs, 8 * kNumCUs)),
+                       dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+namespace {
+template <int OUT>
+hipError_t launch_append_blk(const AppendBlkArgs& a, int block, hipStream_t stream) {
+    const dim3 grid((unsigned)(a.B * a.blocks));
+    if (block == 16)
+        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 16>), grid, dim3(256), 0, stream, a);
+    else if (block == 32)
+        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 32>), grid, dim3(512), 0, stream, a);
+    else
+        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 64>), grid, dim3(1024), 0, stream, a);
+    return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_kv_append_blk(const KvAppendBlk& p, hipStream_t stream) {
+    if ((p.block != 16 && p.block != 32 && p.block != 64) || p.page_size % p.block != 0)
+        return hipErrorInvalidValue;
+    AppendBlkArgs a;
+    a.in = p.in; a.nsplit = p.nsplit; a.split_stride = p.split_stride;
+    a.gain = p.gain; a.inv_freq = p.inv_freq; a.seq_lens = p.seq_lens; a.new_lens = p.new_lens;
+    a.table = p.block_table;
+    a.c_kv = static_cast<uint8_t*>(p.c_kv); a.pe = static_cast<uint8_t*>(p.pe);
+    a.scales = static_cast<uint8_t*>(p.scales);
+    a.B = p.B; a.Sq = p.Sq; a.page_size = p.page_size; a.max_pages = p.max_pages;
+    a.num_pages = p.num_pages; a.eps = p.eps;
+    a.blocks = (p.Sq + p.block - 2) / p.block + 1;   // blocks that Sq tokens in a row can touch
+    if ((int64_t)a.B * a.blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (p.gain_type == kOutF32) return launch_append_blk<kOutF32>(a, p.block, stream);
+    if (p.gain_type == kOutBF16) return launch_append_blk<kOutBF16>(a, p.block, stream);
+    return launch_append_blk<kOutF16>(a, p.block, stream);
+}
+
+hipError_t launch_kv_read_blk(const KvReadBlk& p, hipStream_t stream) {
+    if (p.n <= 0) return hipSuccess;
+    ReadBlkArgs a;
+    a.slots = p.slots; a.n = p.n; a.rows = p.rows;
+    a.c_kv = static_cast<const uint8_t*>(p.c_kv); a.pe = static_cast<const uint8_t*>(p.pe);
+    a.scales = static_cast<const uint8_t*>(p.scales);
+    a.lat = p.lat; a.rot = p.rot;
+    a.block_shift = p.block == 16 ? 4 : p.block == 32 ? 5 : 6;
+    const unsigned grid = (unsigned)std::min<int64_t>((p.n + 15) / 16, 16 * kNumCUs);
+    if (p.out_type == kOutF32)
+        hipLaunchKernelGGL(kv_read_blk_kernel<kOutF32>, dim3(grid), dim3(256), 0, stream, a);
+    else if (p.out_type == kOutBF16)
+        hipLaunchKernelGGL(kv_read_blk_kernel<kOutBF16>, dim3(grid), dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL(kv_read_blk_kernel<kOutF16>, dim3(grid), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace mla

@@ -85,6 +85,10 @@ struct FlashArgs {
     // already normalised and rounded to the storage format, (o_scale O) (1 / l) -- what
     // 3d's A staging forms from ctx and row_sum -- at ctx16[row][R]
     void* ctx16;
+    // block scales of an fp8 cache (flash16x8_kernel<.., true>): E8M0 bytes
+    // [num_pages, page_size >> scale_shift, 2], 1 << scale_shift tokens a block
+    const uint8_t* scales;
+    int scale_shift, num_pages;
 };
 
 // What one workgroup of the attention pass computes: batch b, row tile rt, keys
@@ -1278,27 +1282,42 @@ constexpr int k8Ahead = k8NS - 2;                      // blocks in flight past 
 
 typedef int32_t v2i __attribute__((ext_vector_type(2)));
 
-// eight e4m3 codes (bytes 0..7) -> eight bf16 in operand order
-__device__ __forceinline__ v4u fp8x8_bf16(v2u r) {
-    auto lo2 = [](uint32_t w) __attribute__((always_inline)) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+// eight e4m3 codes (bytes 0..7) -> eight values of format TL, times 2^(exponent of scale), in
+// operand order
+template <typename TL>
+__device__ __forceinline__ v4u fp8x8(v2u r, float scale) {
+    auto two = [&](uint32_t w, auto hi) __attribute__((always_inline)) {
+        constexpr bool kHi = decltype(hi)::value;
+        if constexpr (Half<TL>::kF16)
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, kHi));
+        else
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHi));
     };
-    auto hi2 = [](uint32_t w) __attribute__((always_inline)) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true));
-    };
-    return v4u{lo2(r[0]), hi2(r[0]), lo2(r[1]), hi2(r[1])};
+    constexpr std::integral_constant<bool, false> lo{};
+    constexpr std::integral_constant<bool, true> hi{};
+    return v4u{two(r[0], lo), two(r[0], hi), two(r[1], lo), two(r[1], hi)};
 }
 
+// BS: a scale for each block of tokens and part (paged, bf16 or fp16 queries).  The conversions
+// take a power-of-two scale for nothing, and the 16 keys of a K fragment, or of a V^T fragment's
+// key half, share theirs (blocks are 16, 32 or 64 tokens), so the operands hold the values
+// themselves: no multiplication anywhere, and the softmax and the output scale as in the
+// 16-bit passes.  The scales come through the ring like the codes: P.V wave 2, which has no rope
+// rows to load, brings the block's four bytes (two 16-key halves, two parts) with one load more,
+// zero-extended to a dword each, 256 bytes a stage past the flags; a wave reads its halves'
+// with its fragments.  Keys past the end take scale byte 0, whatever the page holds there (a
+// byte 255 would make their zero codes NaN).
+template <typename TL, bool BS>
 __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
-    typedef bf16_t TL;
-    constexpr float kHeadroom = k2Headroom;
+    constexpr float kHeadroom = Half<TL>::kF16 ? 15.f : k2Headroom;
     constexpr int kPBase = k8NS * k8Stage;                      // 144 KB: two P^T stages
     // the queries at the start: 64 rows of 1 KB (chunk c of row r at c ^ (r & 15)), then 64 rope
     // rows of 128 bytes (chunk c at c ^ ((r >> 1) & 7)), in the last four stages
     constexpr int kQBase = 4 * k8Stage;
     static_assert(kFRows * (kLatBytes + kPeBytes) == 4 * k8Stage, "the queries fill four stages");
     constexpr int kXBase = kPBase + 2 * kXPStage;               // references, sums, flags
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kXBase + 2 * 128 * 4 + 64];
+    constexpr int kSBase = kXBase + 2 * 128 * 4 + 64;           // BS: the stages' scales
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kSBase + (BS ? k8NS * 256 : 0)];
     float* xref = reinterpret_cast<float*>(smem + kXBase);      // [rt][kh][32 rows]
     float* xl = xref + 128;                                     // [rt][kh][32 rows]
     int* flags = reinterpret_cast<int*>(xl + 128);              // [score wave]
@@ -1376,6 +1395,12 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                     asm volatile("" : "+v"(kb0), "+v"(pb0));
                     const uint32_t sbase = (uint32_t)(j % k8NS) * k8Stage;
                     v2u kf[kWin];
+                    float s_lat = 1.f, s_pe = 1.f;
+                    if constexpr (BS) {
+                        const v2u w = *reinterpret_cast<const v2u*>(smem + kSBase + 256 * (j % k8NS) + 8 * kh);
+                        s_lat = __uint_as_float(w[0] << 23);
+                        s_pe = __uint_as_float(w[1] << 23);
+                    }
                     #pragma unroll
                     for (int i = 0; i < kWin; ++i) kf[i] = k_read(sbase, i);
                     // the compiler's own MFMA (not the asm form of the bf16 kernel): the K
@@ -1384,13 +1409,19 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                     sc[0] = sc[1] = v4f{};
                     #pragma unroll
                     for (int s = 0; s < kQSteps; ++s) {
-                        const v4u cur = fp8x8_bf16(kf[s % kWin]);
+                        const v4u cur = fp8x8<TL>(kf[s % kWin], s < kRSteps ? s_lat : s_pe);
                         if (s + kWin < kQSteps) kf[s % kWin] = k_read(sbase, s + kWin);
                         #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(v8bf, cur), __builtin_bit_cast(v8bf, qf[h][s]), sc[h],
-                                0, 0, 0);
+                        for (int h = 0; h < 2; ++h) {
+                            if constexpr (Half<TL>::kF16)
+                                sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    __builtin_bit_cast(v8h, cur), __builtin_bit_cast(v8h, qf[h][s]), sc[h],
+                                    0, 0, 0);
+                            else
+                                sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    __builtin_bit_cast(v8bf, cur), __builtin_bit_cast(v8bf, qf[h][s]), sc[h],
+                                    0, 0, 0);
+                        }
                     }
                     __builtin_amdgcn_sched_barrier(0);
                     const int kq0 = k_lo + k2Keys * j + 16 * kh;
@@ -1503,6 +1534,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     // 16cq .. 16cq+15
     const int wv = cq;
     const bool pe_loader = wv < 2;
+    const bool five = wv < (BS ? 3 : 2);   // waves with a fifth load: rope rows, or (wave 2) scales
     const uint32_t lds0 = lds_addr(smem);
     uint32_t lat_voff[4];
     #pragma unroll
@@ -1519,8 +1551,30 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     auto loads_of = [&](int j) __attribute__((always_inline)) {
         const uint32_t sb = lds0 + (uint32_t)(j % k8NS) * k8Stage;
         const int kb = __builtin_amdgcn_readfirstlane(k_lo + k2Keys * j + 8 * wv);
-        const uint32_t left = (uint32_t)max(0, min(8, k_hi_s - kb));
         Loads d;
+        if constexpr (BS) {
+            // a 32-key block lies in one page (k_lo is a multiple of 32, a page of 64)
+            const int k0 = __builtin_amdgcn_readfirstlane(k_lo + k2Keys * j);
+            const int page = k0 < k_hi_s ? load_uniform(a.block_table + (int64_t)b * a.max_pages + k0 / a.page_size)
+                                         : -1;
+            const bool there = page >= 0 && page < a.num_pages;
+            const int64_t row = there ? (int64_t)page * a.page_size + k0 % a.page_size : 0;
+            const uint32_t left = there ? (uint32_t)max(0, min(8, k_hi_s - kb)) : 0u;
+            d.st = __builtin_amdgcn_readfirstlane(sb + 8 * wv * k8LatBytes);
+            d.rk = rsrc_span(ck_base + (uint64_t)(row + 8 * wv) * kFR, 0, left * kFR);
+            if (wv == 2) {   // the block's two scale bytes, or (blocks of 16) the two halves' four
+                const bool four = a.scale_shift == 4 && k_hi_s - k0 > 16;
+                d.rp = rsrc_span(reinterpret_cast<uint64_t>(a.scales) + 2 * (uint64_t)(row >> a.scale_shift), 0,
+                                 there ? (four ? 4u : 2u) : 0u);
+                d.st_pe = __builtin_amdgcn_readfirstlane(lds0 + kSBase + 256 * (uint32_t)(j % k8NS));
+            } else {
+                const uint32_t left_p = there ? (uint32_t)max(0, min(16, k_hi_s - k0 - 16 * (wv & 1))) : 0u;
+                d.st_pe = __builtin_amdgcn_readfirstlane(sb + k8LatStage + 16 * (wv & 1) * k8PeBytes);
+                d.rp = rsrc_span(pe_base + (uint64_t)(row + 16 * (wv & 1)) * kFD, 0, left_p * kFD);
+            }
+            return d;
+        }
+        const uint32_t left = (uint32_t)max(0, min(8, k_hi_s - kb));
         d.st = __builtin_amdgcn_readfirstlane(sb + 8 * wv * k8LatBytes);
         d.rk = rsrc_span(ck_base + (uint64_t)flash_key_row(a, b, kb, k_hi_s) * kFR, 0, left * kFR);
         // (waves 2 and 3 keep a descriptor they never use)
@@ -1530,20 +1584,23 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         d.rp = rsrc_span(pe_base + (uint64_t)flash_key_row(a, b, kp, k_hi_s) * kFD, 0, left_p * kFD);
         return d;
     };
+    // the scale bytes' offsets: lane 2 half + part; the halves share a block unless it is 16 tokens
+    const uint32_t sc_voff = lane < 4 ? (uint32_t)((lane & 1) + (a.scale_shift == 4 ? (lane & 2) : 0)) : kOob;
     auto issue_one = [&](const Loads& d, int q) __attribute__((always_inline)) {
         if (q < 4) dma16(d.rk, d.st + q * 1024, lat_voff[q]);
-        else dma16(d.rp, d.st_pe, pe_voff);
+        else if (!BS || pe_loader) dma16(d.rp, d.st_pe, pe_voff);
+        else dma_byte(d.rp, d.st_pe, sc_voff);
     };
-    // loads per block: 5 for the rope loaders, 4 for the others; wait until at most n
+    // loads per block: 5 for the rope (and scale) loaders, 4 for the others; wait until at most n
     // blocks' loads are outstanding
     auto issue_block = [&](const Loads& d) __attribute__((always_inline)) {
         #pragma unroll
         for (int q = 0; q < 4; ++q) issue_one(d, q);
-        if (pe_loader) issue_one(d, 4);
+        if (five) issue_one(d, 4);
     };
     auto wait_blocks = [&](auto n_blocks) __attribute__((always_inline)) {
         constexpr int n = decltype(n_blocks)::value;
-        if (pe_loader) wait_vm<5 * n>();
+        if (five) wait_vm<5 * n>();
         else wait_vm<4 * n>();
     };
     // The tile's queries into the last four stages, free until block 4 is issued after barrier
@@ -1599,6 +1656,12 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                 // fragment f (one per two MFMAs, t = 2f and 2f + 1 for the two row tiles):
                 // key half f/4, column block 4cq + f%4
                 constexpr int kVWin = 3;
+                float s_v[2] = {1.f, 1.f};   // the key halves' scales
+                if constexpr (BS) {
+                    const v4u w = *reinterpret_cast<const v4u*>(smem + kSBase + 256 * ((j - 1) % k8NS));
+                    s_v[0] = __uint_as_float(w[0] << 23);
+                    s_v[1] = __uint_as_float(w[2] << 23);
+                }
                 v2u vf[kVWin];
                 #pragma unroll
                 for (int f = 0; f < kVWin; ++f) vf[f] = v_read(sbase, f >> 2, 4 * cq + (f & 3));
@@ -1607,13 +1670,13 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                 for (int t = 0; t < 16; ++t) {
                     const int f = t >> 1;
                     if ((t & 1) == 0) {
-                        cur = fp8x8_bf16(vf[f % kVWin]);
+                        cur = fp8x8<TL>(vf[f % kVWin], s_v[f >> 2]);
                         if (f + kVWin < 8) vf[f % kVWin] = v_read(sbase, (f + kVWin) >> 2, 4 * cq + ((f + kVWin) & 3));
                     }
                     O[t & 7] = mfma32h<TL>(cur, pf[t & 1][f >> 2], O[t & 7]);
                     // block j+6 into stage (j+6) % 8, which block j-2 left at barrier A_j
                     if (t % 3 == 0 && t / 3 < 4) issue_one(next, t / 3);
-                    if (t == 13 && pe_loader) issue_one(next, 4);
+                    if (t == 13 && five) issue_one(next, 4);
                 }
             }
         }
@@ -2943,6 +3006,10 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
 }  // namespace
 
 bool flash_supported(const FlashProblem& p) {
+    if (p.scale_block)   // block scales: an fp8 cache and 16-bit queries
+        return p.fp8_kv && p.half && p.kv_scale == 1.f &&
+               (p.scale_block == 16 || p.scale_block == 32 || p.scale_block == 64) && p.R == kFR &&
+               p.D == kFD && p.B > 0 && p.Sq > 0 && p.H > 0 && p.Sk > 0;
     if (p.fp8_kv && !(p.half && !p.f16 && p.kv_scale > 0.f && std::isfinite(p.kv_scale)))
         return false;   // an fp8 cache is read with bf16 queries and a positive scale
     return p.R == kFR && p.D == kFD && p.B > 0 && p.Sq > 0 && p.H > 0 && p.Sk > 0;
@@ -3043,6 +3110,7 @@ namespace {
 // The 16-bit and fp8-cache kernel the launcher takes for p (the switches below).
 enum class Flash16 { kCodeRing, kSpecPv64, kSpecPv32, kKeySplit };
 Flash16 flash16_choice(const FlashProblem& p) {
+    if (p.scale_block) return Flash16::kCodeRing;   // the one pass that reads block scales
     const char* spec_env = std::getenv("MLA_FLASH16_SPEC");
     const bool spec = !(spec_env && spec_env[0] == '0');
     const char* pv_env = std::getenv("MLA_FLASH16_PV");
@@ -3138,6 +3206,10 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
     a.block_table = p.block_table;
     a.page_size = p.page_size;
     a.max_pages = p.page_size > 0 ? p.Sk / p.page_size : 0;
+    a.scales = p.scales;
+    a.scale_shift = p.scale_block == 16 ? 4 : p.scale_block == 32 ? 5 : 6;
+    a.num_pages = p.num_pages;
+    if (p.scale_block && !(p.scales && p.block_table && p.num_pages > 0)) return hipErrorInvalidValue;
     if (p.block_table && (p.page_size <= 0 || p.page_size % 64 != 0 || p.Sk % p.page_size != 0))
         return hipErrorInvalidValue;
     if (f.balanced) {
@@ -3158,8 +3230,12 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
     // an fp8 cache: the code-ring pass (flash16x8_kernel; cfg4 shape, attention with 3d:
     // 171 us against 220-240 us) unless MLA_FLASH16_FP8=convert asks for the pass that
     // converts each block into a bf16 ring
-    if (p.fp8_kv && k16 == Flash16::kCodeRing)
-        hipLaunchKernelGGL(flash16x8_kernel, dim3(grid), dim3(kXThreads), 0, stream, a);
+    if (p.scale_block && p.f16)
+        hipLaunchKernelGGL((flash16x8_kernel<f16_t, true>), dim3(grid), dim3(kXThreads), 0, stream, a);
+    else if (p.scale_block)
+        hipLaunchKernelGGL((flash16x8_kernel<bf16_t, true>), dim3(grid), dim3(kXThreads), 0, stream, a);
+    else if (p.fp8_kv && k16 == Flash16::kCodeRing)
+        hipLaunchKernelGGL((flash16x8_kernel<bf16_t, false>), dim3(grid), dim3(kXThreads), 0, stream, a);
     else if (p.fp8_kv && spec && pv64)
         hipLaunchKernelGGL((flash16x_kernel<bf16_t, true, true>), dim3(grid), dim3(kXThreads), 0, stream, a);
     else if (p.half && spec && pv64 && p.f16)

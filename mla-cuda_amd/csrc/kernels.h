@@ -171,6 +171,54 @@ hipError_t launch_fp8_dequant(const void* codes, int64_t n, float scale, float* 
 hipError_t launch_split_rows(const void* src, void* dst_a, void* dst_b, int64_t groups,
                              int rows_a, int rows_b, int64_t row_bytes, hipStream_t stream);
 
+// ---------------------------------------------------------------- 8-bit blocked cache (cache8.hip)
+// Pools of e4m3 codes with an E8M0 scale byte for each block of `block` tokens (16, 32 or 64, a
+// divisor of page_size) and part (latent, rope): value = code * 2^(byte - 127).
+// Requests grow or shrink: block-table rows, positions and slots, pages from and to a ring.
+struct CacheExtend {
+    int B = 0, Sq = 0, page_size = 0, max_pages = 0, num_pages = 0;
+    const int* new_lens = nullptr;     // [B]
+    const int* seq_lens = nullptr;     // [B]
+    const int* free_state = nullptr;   // {head, count}
+    int* block_table = nullptr;        // [B, max_pages]
+    int* free_pages = nullptr;         // [num_pages] ring
+    int* seq_lens_out = nullptr;
+    int* free_state_out = nullptr;
+    int* granted = nullptr;            // [B]
+    int64_t* positions = nullptr;      // [B, Sq]
+    int64_t* slots = nullptr;          // [B, Sq]
+};
+size_t cache_extend_workspace(int B);
+hipError_t launch_cache_extend(const CacheExtend& p, void* workspace, hipStream_t stream);
+// KV append, as launch_kv_append's paged form, coded by blocks: the new_lens[b] last tokens of
+// sequence b (seq_lens[b] long with them) are the last of its Sq rows of `in`.
+struct KvAppendBlk {
+    const float* in = nullptr; int nsplit = 1; int64_t split_stride = 0;
+    const void* gain = nullptr; OutType gain_type = kOutF32;
+    const float* inv_freq = nullptr;
+    const int* seq_lens = nullptr;
+    const int* new_lens = nullptr;
+    const int* block_table = nullptr;
+    void* c_kv = nullptr;
+    void* pe = nullptr;
+    void* scales = nullptr;
+    int B = 0, Sq = 0, page_size = 0, max_pages = 0, num_pages = 0, block = 0;
+    float eps = 0.f;
+};
+hipError_t launch_kv_append_blk(const KvAppendBlk& p, hipStream_t stream);
+// Rows `slots` of the pools, decoded to lat [n, 512] and rot [n, 64]; zeros for other slots.
+struct KvReadBlk {
+    const int64_t* slots = nullptr; int64_t n = 0, rows = 0;
+    const void* c_kv = nullptr;
+    const void* pe = nullptr;
+    const void* scales = nullptr;
+    void* lat = nullptr;
+    void* rot = nullptr;
+    OutType out_type = kOutF32;
+    int block = 0;
+};
+hipError_t launch_kv_read_blk(const KvReadBlk& p, hipStream_t stream);
+
 // ---------------------------------------------------------------- 3a scores
 struct ScoresProblem {
     const void* qa = nullptr;    // [B*Sq*H, R]   storage dtype
@@ -228,6 +276,12 @@ struct FlashProblem {
     // one byte per element (rows of R and D bytes)
     bool fp8_kv = false;
     float kv_scale = 1.f;
+    // fp8 cache with a scale for each block of tokens (paged; bf16 or fp16 queries; kv_scale 1):
+    // E8M0 bytes [num_pages, page_size / scale_block, 2] (latent, rope); a table entry outside
+    // [0, num_pages) reads as rows of zeros
+    const uint8_t* scales = nullptr;
+    int scale_block = 0;         // tokens a block: 16, 32 or 64 (0: no block scales)
+    int num_pages = 0;
 };
 struct FlashPlan {
     bool wave = false;           // fp32 pass on 16-row workgroups of key-split waves
