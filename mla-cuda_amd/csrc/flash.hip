@@ -89,6 +89,8 @@ struct FlashArgs {
     // [num_pages, page_size >> scale_shift, 2], 1 << scale_shift tokens a block
     const uint8_t* scales;
     int scale_shift, num_pages;
+    // a list that the workgroups work out themselves (flash_work_small), its item bound
+    int small_list, max_items;
 };
 
 // What one workgroup of the attention pass computes: batch b, row tile rt, keys
@@ -98,6 +100,7 @@ struct FlashWork {
     int b, rt, k_lo, k_len;
     int64_t slot;
     bool direct, skip;
+    int keys;   // of batch b, where known (flash_work_small); else -1
 };
 // Uniform splits: the logical workgroup order is XCD-major (the two row tiles of a batch
 // are neighbours on one XCD, so the second read of a key block hits its L2).  Work list:
@@ -109,6 +112,7 @@ __device__ __forceinline__ FlashWork flash_work(const FlashArgs& a) {
     FlashWork w;
     w.direct = false;
     w.skip = false;
+    w.keys = -1;
     if (!a.wl) {
         if (a.spread) {   // n_split == 1
             spread_tile(blockIdx.x, a.B, a.row_tiles, &w.b, &w.rt);
@@ -158,6 +162,119 @@ __device__ __forceinline__ int64_t flash_key_row(const FlashArgs& a, int b, int 
     if (k >= k_end) return 0;
     const int page = load_uniform(a.block_table + (int64_t)b * a.max_pages + k / a.page_size);
     return (int64_t)page * a.page_size + k % a.page_size;
+}
+
+// The work list of a few sequences (kSmallList, plan_flash) without a launch in front (3.4 to 7 us, and
+// the gap behind it): every workgroup works out the chunk and its own item from the lengths, a sequence a lane, with
+// worklist.h's rules -- the same chunks and partial slots as
+// flash_worklist_kernel, the last chunks of one length bucket in batch order.  Workgroup 0 leaves the
+// sequences' first slots and chunk counts in the list for the merge.
+constexpr int kSmallList = 64;
+// L / c and L % c (0 <= L < 2^24, 0 < c < 2^24)
+__device__ __forceinline__ int divmod24(int L, int c, int* rem) {
+    int q = (int)((float)L * __builtin_amdgcn_rcpf((float)c));   // off by one at most
+    int r = L - q * c;
+    if (r < 0) { --q; r += c; }
+    if (r >= c) { ++q; r -= c; }
+    *rem = r;
+    return q;
+}
+// inclusive sum over the lanes up to this one
+__device__ __forceinline__ int lanes_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+// (packs: an LDS word per wave of the workgroup's kWlTries waves, which try a candidate each)
+__device__ __forceinline__ FlashWork flash_work_small(const FlashArgs& a, int* packs) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool has = lane < a.B;
+    const int L = has ? wl_len(a.seq_lens[lane], a.Sk) : 0;
+    const int tot = wave_sum(L);   // below 64 * 2^21
+    const int mx = (int)wave_reduce((float)L, OpMax{});                       // exact: below 2^24
+    const int mn = -(int)wave_reduce(has ? -(float)L : -16777216.f, OpMax{});
+    int chunk, r, full = 0, cnt = 0, total = 0;
+    if (mn == mx) {
+        chunk = dense_keys_per_split(wl_max(1, mx), a.B * a.row_tiles, kFKeys);
+    } else {
+        const int base = wl_base_blocks(tot, a.row_tiles, kFKeys);
+        chunk = wl_try(base, wave, a.Sk, kFKeys);
+        full = divmod24(L, chunk, &r);
+        const int n = has ? wl_max(1, full + (r > 0)) : 0;
+        // wl_small with the remainder at hand
+        const int small = has && (r > 0 || L == 0) && 2 * r <= chunk - wl_fixed_blocks(kFKeys) * kFKeys;
+        const bool fits = wl_packs(wave_sum(n), wave_sum(small), tot, chunk, a.row_tiles, kFKeys);
+        if (lane == 0) packs[wave] = fits || wave == kWlTries - 1;
+        __syncthreads();
+        const uint64_t tries = __builtin_amdgcn_ballot_w64(lane < kWlTries && packs[lane & (kWlTries - 1)]);
+        chunk = wl_try(base, __builtin_ctzll(tries), a.Sk, kFKeys);
+    }
+    for (;;) {
+        full = divmod24(L, chunk, &r);
+        cnt = has ? wl_max(1, full + (r > 0)) : 0;
+        total = wave_sum(cnt);
+        if (wl_fits(total, a.max_items, chunk, a.Sk)) break;
+        chunk *= 2;
+    }
+    const int n_items = wl_min(total, a.max_items);
+    const int first = lanes_scan(cnt) - cnt, ff = lanes_scan(full) - full, n_full = wave_sum(full);
+    if (blockIdx.x == 0 && threadIdx.x < 64) {
+        int* wl = const_cast<int*>(a.wl);
+        if (has) {
+            wl[kWlHead + lane] = first;
+            wl[kWlHead + a.B + lane] = cnt;
+        }
+        if (lane == 0) { wl[0] = n_items; wl[1] = chunk; }
+    }
+    FlashWork w;
+    w.skip = false;
+    int it = 0;
+    w.rt = 0;
+    if (a.spread) {
+        w.skip = !spread_tile(blockIdx.x, n_items, a.row_tiles, &it, &w.rt);
+    } else {
+        const int x = blockIdx.x % kNumXCDs, q = blockIdx.x / kNumXCDs;
+        it = (q / a.row_tiles) * kNumXCDs + x;
+        w.rt = q % a.row_tiles;
+        w.skip = it >= n_items;
+    }
+    w.b = 0; w.k_lo = 0; w.k_len = 0; w.slot = 0; w.direct = false; w.keys = 0;
+    if (w.skip) return w;
+    int c;
+    if (it < n_full) {
+        w.b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(ff <= it && it < ff + full));
+        c = it - __builtin_amdgcn_readlane(ff, w.b);
+    } else {
+        // the short last chunks: longest first by bucket, then in batch order
+        const bool sh = has && (r > 0 || L == 0);
+        // (the item's place among them picks the lane: one bit of the bucket at a time, then the
+        // place among the lanes that are left)
+        const uint32_t q = (uint32_t)(chunk - 1 - r) * (uint32_t)kWlBuckets / (uint32_t)chunk;
+        uint64_t left = __builtin_amdgcn_ballot_w64(sh);
+        int place = it - n_full;
+        static_assert(kWlBuckets == 256, "eight bits");
+        #pragma unroll
+        for (int bit = 7; bit >= 0; --bit) {
+            const uint64_t low = left & __builtin_amdgcn_ballot_w64(!((q >> bit) & 1));
+            const int n = __builtin_popcountll(low);
+            left = place < n ? low : left & ~low;
+            place -= place < n ? 0 : n;
+        }
+        for (; place > 0; --place) left &= left - 1;
+        w.b = __builtin_ctzll(left);
+        c = __builtin_amdgcn_readlane(full, w.b);
+    }
+    w.k_len = chunk;
+    w.k_lo = c * chunk;
+    w.direct = __builtin_amdgcn_readlane(cnt, w.b) == 1;
+    w.slot = (int64_t)__builtin_amdgcn_readlane(first, w.b) + c;
+    w.keys = __builtin_amdgcn_readlane(L, w.b);
+    return w;
 }
 
 // Chunk permutation of the fp32 pass's LDS rows: 16-byte chunk c of key k sits at
@@ -1324,13 +1441,13 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4, l32 = lane & 31, hw = lane >> 5;
-    const FlashWork work = flash_work(a);
+    const FlashWork work = BS && a.small_list ? flash_work_small(a, flags) : flash_work(a);
     if (work.skip) return;   // past the end of a work list: the whole workgroup leaves
 
     const int b = work.b;
     const int rows_b = a.Sq * a.H;
     const int r0 = work.rt * kFRows;
-    const int skb = flash_batch_keys(a, b);
+    const int skb = BS && work.keys >= 0 ? work.keys : flash_batch_keys(a, b);
     const int k_lo = work.k_lo;
     const int k_end = min(skb, k_lo + work.k_len);
     int k_hi = k_end;
@@ -3060,7 +3177,15 @@ FlashPlan plan_flash(const FlashProblem& p) {
         // grid (flash_worklist_kernel); the partial slots, the list and its grid are sized
         // for its largest case
         f.balanced = true;
-        f.max_items = wl_max_items(p.B, f.row_tiles);
+        f.max_items = p.scale_block ? wl_max_items16(p.B, f.row_tiles) : wl_max_items(p.B, f.row_tiles);
+        // The workgroups work a small list out themselves where they run about once per CU: it costs
+        // each of them more than reading one (launch against none, with 3d, us: one sequence, 512 keys
+        // 24.8 / 21.7; 16 up to 8,192 50.2 / 43.3; 61 up to 4,989 78.4 / 73.4; 32 of 4 queries up to 1,000
+        // 60.6 / 57.0; but four chunks of 333 queries, 2,664 tiles, 736 / 757, one of 700 375 / 435).
+        // MLA_SMALL_LIST=0 keeps the launch (a comparison aid: the same bits)
+        const char* small_env = std::getenv("MLA_SMALL_LIST");
+        f.small_list = p.scale_block && p.B <= kSmallList && base <= kNumCUs &&
+                       !(small_env && small_env[0] == '0');
         f.n_split = 0;
         f.keys_per_split = 0;
         const size_t wl_bytes = ((size_t)wl_ints(p.B, f.max_items) * sizeof(int) + 255) / 256 * 256;
@@ -3209,10 +3334,12 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
     a.scales = p.scales;
     a.scale_shift = p.scale_block == 16 ? 4 : p.scale_block == 32 ? 5 : 6;
     a.num_pages = p.num_pages;
+    a.small_list = f.small_list ? 1 : 0;
+    a.max_items = f.max_items;
     if (p.scale_block && !(p.scales && p.block_table && p.num_pages > 0)) return hipErrorInvalidValue;
     if (p.block_table && (p.page_size <= 0 || p.page_size % 64 != 0 || p.Sk % p.page_size != 0))
         return hipErrorInvalidValue;
-    if (f.balanced) {
+    if (f.balanced && !f.small_list) {
         hipError_t e = launch_flash_worklist(p, f, wl, stream);
         if (e != hipSuccess) return e;
     }

@@ -290,6 +290,7 @@ struct FlashPlan {
     int keys_per_split = 0;      // multiple of the key block
     bool balanced = false;       // ragged keys: a device-built work list of key chunks
     int max_items = 0;           // its largest item count (grid = max_items * row_tiles)
+    bool small_list = false;     // ... that every workgroup works out for itself (no launch)
     size_t partial_bytes = 0;    // scratch: split partials (and the work list)
 };
 bool flash_supported(const FlashProblem& p);

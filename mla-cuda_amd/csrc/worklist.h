@@ -44,6 +44,17 @@ MLA_HD int wl_max_items(int B, int row_tiles) {
     return (kWlPerCu * kNumCUs / row_tiles + B + 1 + kNumXCDs - 1) / kNumXCDs * kNumXCDs;
 }
 
+// The most items that a 16-bit list can have, by the rules below: pieces of at least an equal share
+// of the keys per CU (CUs / row_tiles of them, and a short one more per sequence); with equal lengths
+// the dense splits, one round of CUs below a CU's worth of tiles, past that up to four a sequence
+// (one where the tiles fill whole rounds).  A list's grid and partial slots are sized for it: the
+// workgroups past the list's end cost little, but there were up to five of them for each that works.
+MLA_HD int wl_max_items16(int B, int row_tiles) {
+    const long long base = (long long)B * row_tiles;
+    const int equal = base < kNumCUs || base % kNumCUs == 0 ? B : 4 * B;
+    return (wl_max(kNumCUs / row_tiles + B, equal) + kNumXCDs - 1) / kNumXCDs * kNumXCDs;
+}
+
 // Keys per split of a dense batch of Sk keys, base = B * row_tiles workgroups per split.
 // Below one workgroup per CU: as many splits as fit in one round of CUs (floor(CUs / base)),
 // at least one key block per split.  (Measured at B=1: Sk=512 takes 25.0 us in 32 one-block

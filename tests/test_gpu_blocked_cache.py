@@ -722,3 +722,27 @@ def test_serving_step_in_a_graph(ext):
         for k in ("table", "ring", "c_kv", "pe", "scales", "lens", "state"):
             assert torch.equal(a[k], b[k]), (i, k)
         step(warm)
+
+
+@pytest.mark.parametrize("B,Sq,Sk", [(1, 1, 5000), (2, 1, 63), (7, 1, 4989), (16, 4, 1500), (33, 1, 3000),
+                                     (64, 1, 900), (64, 2, 130), (3, 20, 700), (1, 70, 70)])
+def test_attention_list_without_a_launch(ext, monkeypatch, B, Sq, Sk):
+    """Up to 64 sequences the workgroups work the list out themselves: the same bits as from the
+    list that is built in a launch of its own, for ragged, equal, empty and unlike lengths."""
+    g = torch.Generator().manual_seed(B + Sk)
+    page, block = 64, 32
+    cache = to_gpu(K.new_pool(300, page, block, g))
+    mp = -(-Sk // page)
+    table = torch.randint(0, 300, (B, mp), generator=g).int().to(DEV)   # (read only: pages may be shared)
+    qa, qr, w = (t.to(DEV) for t in K.queries(B, Sq, 128, 128, g, BF))
+    some = torch.randint(0, Sk + 1, (B,), generator=g)
+    long = torch.where(torch.arange(B) == B // 2, Sk, torch.ones(B, dtype=torch.long))
+    for lens in (some, torch.full((B,), Sk), torch.full((B,), Sk // 3), torch.zeros(B, dtype=torch.long), long,
+                 torch.where(torch.arange(B) % 2 == 0, torch.full((B,), Sk), torch.zeros(B, dtype=torch.long)),
+                 some - Sk // 2, some + Sk):
+        outs = []
+        for env in ("0", "1"):
+            monkeypatch.setenv("MLA_SMALL_LIST", env)
+            outs.append(ext.mla_attention_paged_fp8blk(qa, qr, cache["c_kv"], cache["pe"], cache["scales"], table,
+                                                       lens.int().to(DEV), w, SCALE, Sq > 1))
+        assert torch.equal(outs[0], outs[1])
