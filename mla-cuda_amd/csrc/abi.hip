@@ -1651,6 +1651,14 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
     fp.block_table = block_table;
     fp.page_size = page_size;
     fp.num_pages = num_pages;
+    if (out_list_ok(fp, L.flash)) {   // a few tokens: the chunks' merge inside 3d
+        float* part = at<float>(workspace, L.off_part);
+        MLA_TRY_HIP(launch_flash(fp, L.flash, ctx, row_sum, part, stream, false),
+                    "blocked fp8-cache attention launch");
+        MLA_TRY_HIP(launch_out_list(fp, L.flash, ctx, row_sum, part, W_uv, out, dims->v, stream),
+                    "3d launch");
+        return ok();
+    }
     MLA_TRY_HIP(launch_flash(fp, L.flash, ctx, row_sum, at<float>(workspace, L.off_part), stream,
                              true, L.ctx16 ? ctx : nullptr),
                 "blocked fp8-cache attention launch");

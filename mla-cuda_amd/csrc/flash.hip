@@ -2940,6 +2940,153 @@ __global__ void __launch_bounds__(512) flash_merge_many_kernel(const float* __re
     }
 }
 
+// 3d of a few tokens with the merge of their chunks in it: a workgroup takes a head and 64 output
+// columns.  Alone the merge writes a row per token and head that the product then waits a launch for,
+// and a GEMM tile is nearly empty at these token counts; here W_uv's rows are in flight while the
+// chunks' rows are summed.
+//   weights: wave t takes token t: m = max_s m_s, w_s = 2^(m_s - m) / sum_s 2^(m_s - m) l_s.
+//   rows: 128 threads a row (4 columns each), four groups of them; a token's chunks are dealt to four
+//     groups (one token), two (two) or one, 16 rows' loads in flight each, and the groups' sums added
+//     in order.  The two workgroups of a head both read its rows (at most kOutListRows, 2 KB each), so
+//     they run on one XCD and the second read hits its L2: on two XCDs 65,536 keys' 33.5 MB of rows
+//     came twice from memory, 60.4 us with the pass against 58.6 for separate launches.
+//   product: 16x16x32 MFMAs, W_uv's rows by the tokens.  The merged row keeps fp32's precision in two
+//     16-bit terms, v = hi + lo: tokens' hi are columns 0-7, their lo 8-15, added at the end.  Wave w has
+//     rows 16 (w % 4) and K half w / 4; the halves are added through LDS.
+constexpr int kOutListRows = 320;   // chunks' rows a head: Sq * wl_max_items16 at 8 tokens or fewer
+constexpr int kOutListPitch = kFR * 2 + 16;   // bytes of a column in LDS
+template <typename TL>
+__global__ void __launch_bounds__(512) out_list_kernel(const float* __restrict__ o,
+                                                       const float* __restrict__ mp,
+                                                       const float* __restrict__ lp,
+                                                       const float* __restrict__ ctx,
+                                                       const float* __restrict__ row_sum,
+                                                       const int* __restrict__ wl,
+                                                       const uint16_t* __restrict__ W,
+                                                       uint16_t* __restrict__ out, int B, int Sq,
+                                                       int H, int V) {
+    static_assert(kOutListTokens == 8, "hi and lo of the tokens fill 16 columns");
+    __shared__ float wts[kOutListRows];
+    __shared__ v4f sums[kOutListTokens][128];
+    __shared__ __attribute__((aligned(16))) uint8_t cols[2 * kOutListTokens * kOutListPitch];
+    const int vb = (V + 63) / 64;
+    const int wg = xcd_logical_block(blockIdx.x, gridDim.x);
+    const int h = wg / vb, c0 = (wg % vb) * 64;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int M = B * Sq, rows_b = Sq * H;
+    // lane: row l16 of the wave's 16, depths 256 (w / 4) + 32 s + 8 g .. +7 at step s
+    const int vr = 16 * (wave & 3), kh = wave >> 2;
+    v4u wr[8];
+    {
+        const v4u* src = reinterpret_cast<const v4u*>(
+            W + ((int64_t)h * V + min(c0 + vr + l16, V - 1)) * kFR + 256 * kh) + g;
+        #pragma unroll
+        for (int s = 0; s < 8; ++s) wr[s] = src[4 * s];
+    }
+    // a token's chunks (1: its row is in ctx), first partial slot, and place in wts
+    const int first = lane < B ? wl[kWlHead + lane] : 0, count = lane < B ? wl[kWlHead + B + lane] : 0;
+    const int before = lanes_scan(count) - count;
+    auto token = [&](int t, int* n, int64_t* row0, int* at) __attribute__((always_inline)) {
+        const int b = t / Sq, i = (t % Sq) * H + h;
+        *n = __builtin_amdgcn_readlane(count, b);
+        *at = Sq * __builtin_amdgcn_readlane(before, b) + (t % Sq) * *n;
+        *row0 = (int64_t)(*n == 1 ? b : __builtin_amdgcn_readlane(first, b)) * rows_b + i;
+    };
+    // the rows of a group's unit u (token u / parts, chunks u % parts, + parts, ..), kWin at a time; the
+    // first ones' loads go out before the weights'
+    const int parts = M == 1 ? 4 : M == 2 ? 2 : 1;
+    const int group = __builtin_amdgcn_readfirstlane(tid >> 7), c4 = tid & 127;
+    constexpr int kWin = 16;
+    v4f x[kWin];
+    auto load_rows = [&](int u, int s0) __attribute__((always_inline)) {
+        int n, at;
+        int64_t row0;
+        token(u / parts, &n, &row0, &at);
+        const v4f* src = reinterpret_cast<const v4f*>((n == 1 ? ctx : o) + row0 * kFR) + c4;
+        #pragma unroll
+        for (int k = 0; k < kWin; ++k)
+            x[k] = src[(int64_t)min(s0 + k * parts, n - 1) * rows_b * (kFR / 4)];
+    };
+    if (group < M * parts) load_rows(group, group % parts);
+    if (wave < M) {
+        int n, at;
+        int64_t row0;
+        token(wave, &n, &row0, &at);
+        constexpr int kPer = (kOutListRows + 63) / 64;
+        float ms[kPer], ls[kPer], mx = -INFINITY, L = 0.f;
+        #pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int s = lane + 64 * k;
+            const bool in = s < n;
+            const int64_t row = row0 + (in ? (int64_t)s * rows_b : 0);
+            // one chunk: its row is the sum itself
+            ms[k] = !in ? -INFINITY : n == 1 ? 0.f : mp[row];
+            ls[k] = !in ? 0.f : (n == 1 ? row_sum : lp)[row];
+            mx = fmaxf(mx, ms[k]);
+        }
+        mx = wave_reduce(mx, OpMax{});
+        #pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            ms[k] = ms[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[k] - mx);
+            L += ms[k] * ls[k];
+        }
+        L = wave_reduce(L, OpSum{});
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        #pragma unroll
+        for (int k = 0; k < kPer; ++k)
+            if (lane + 64 * k < n) wts[at + lane + 64 * k] = ms[k] * inv;
+    }
+    __syncthreads();
+    for (int u = group; u < M * parts; u += 4) {
+        int n, at;
+        int64_t row0;
+        token(u / parts, &n, &row0, &at);
+        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = u % parts; s0 < n; s0 += kWin * parts) {
+            if (u != group || s0 >= kWin * parts) load_rows(u, s0);
+            #pragma unroll
+            for (int k = 0; k < kWin; ++k)
+                if (s0 + k * parts < n) acc += wts[at + s0 + k * parts] * x[k];
+        }
+        sums[u][c4] = acc;
+    }
+    __syncthreads();
+    for (int t = group; t < M; t += 4) {
+        v4f v = sums[t * parts][c4];
+        for (int q = 1; q < parts; ++q) v += sums[t * parts + q][c4];
+        using S = Half<TL>;
+        const v2u hi = {S::pack2(v[0], v[1]), S::pack2(v[2], v[3])};
+        const v2u lo = {S::pack2(v[0] - S::to_f32(hi[0] & 0xffffu), v[1] - S::to_f32(hi[0] >> 16)),
+                        S::pack2(v[2] - S::to_f32(hi[1] & 0xffffu), v[3] - S::to_f32(hi[1] >> 16))};
+        *reinterpret_cast<v2u*>(cols + t * kOutListPitch + 8 * c4) = hi;
+        *reinterpret_cast<v2u*>(cols + (t + kOutListTokens) * kOutListPitch + 8 * c4) = lo;
+    }
+    __syncthreads();
+    // (a column without a token multiplies whatever is there into its own sums, which nobody reads)
+    v4f d = {0.f, 0.f, 0.f, 0.f};
+    #pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        const v4u c = *reinterpret_cast<const v4u*>(cols + l16 * kOutListPitch + 512 * kh + 64 * s + 16 * g);
+        if constexpr (Half<TL>::kF16)
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, wr[s]),
+                                                       __builtin_bit_cast(v8h, c), d, 0, 0, 0);
+        else
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, wr[s]),
+                                                        __builtin_bit_cast(v8bf, c), d, 0, 0, 0);
+    }
+    if (kh) sums[2 * (wave & 3) + (lane >> 5)][lane & 31] = d;   // (the rows' sums are done with)
+    __syncthreads();
+    if (kh) return;
+    d += sums[2 * wave + (lane >> 5)][lane & 31];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] += dpp_move<0x128>(d[i]);   // row_ror:8: lo beside hi
+    const int v = c0 + vr + 4 * g;
+    if (l16 < M && v < V)
+        *reinterpret_cast<v2u*>(out + ((int64_t)l16 * H + h) * V + v) =
+            v2u{Half<TL>::pack2(d[0], d[1]), Half<TL>::pack2(d[2], d[3])};
+}
+
 // Work list of a ragged batch (one workgroup; key counts are device data).  The chunk rule,
 // the fit check, each batch's chunk counts and the order of the items are the functions of
 // worklist.h; this kernel spreads them over its threads (thread tid owns batches
@@ -3208,6 +3355,34 @@ FlashPlan plan_flash(const FlashProblem& p) {
     return f;
 }
 
+bool out_list_ok(const FlashProblem& p, const FlashPlan& f) {
+    // MLA_OUT_SMALL=0: the merge and 3d launches of their own
+    const char* env = std::getenv("MLA_OUT_SMALL");
+    return p.scale_block && f.balanced && p.B * p.Sq <= kOutListTokens && p.R == kFR &&
+           p.Sq * f.max_items <= kOutListRows && !(env && env[0] == '0');
+}
+
+hipError_t launch_out_list(const FlashProblem& p, const FlashPlan& f, const float* ctx,
+                           const float* row_sum, const float* partials, const void* W_uv, void* out,
+                           int V, hipStream_t stream) {
+    if (!out_list_ok(p, f) || V <= 0) return hipErrorInvalidValue;
+    const size_t rows_b = (size_t)p.Sq * p.H;
+    const size_t wl_bytes = ((size_t)wl_ints(p.B, f.max_items) * sizeof(int) + 255) / 256 * 256;
+    const float* o = reinterpret_cast<const float*>(reinterpret_cast<const char*>(partials) + wl_bytes);
+    const float* m = o + (size_t)f.max_items * rows_b * kFR;
+    const float* l = m + (size_t)f.max_items * rows_b;
+    const int* wl = reinterpret_cast<const int*>(partials);
+    const dim3 grid((unsigned)(p.H * ((V + 63) / 64))), block(512);
+    const uint16_t* W = static_cast<const uint16_t*>(W_uv);
+    if (p.f16)
+        hipLaunchKernelGGL(out_list_kernel<f16_t>, grid, block, 0, stream, o, m, l, ctx, row_sum, wl, W,
+                           static_cast<uint16_t*>(out), p.B, p.Sq, p.H, V);
+    else
+        hipLaunchKernelGGL(out_list_kernel<bf16_t>, grid, block, 0, stream, o, m, l, ctx, row_sum, wl, W,
+                           static_cast<uint16_t*>(out), p.B, p.Sq, p.H, V);
+    return hipGetLastError();
+}
+
 int flash_worklist_ints(const FlashProblem& p, const FlashPlan& f) {
     return f.balanced ? wl_ints(p.B, f.max_items) : 0;
 }
@@ -3389,7 +3564,7 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
         hipLaunchKernelGGL(flash32_kernel<kFStages>, dim3(grid), dim3(kFThreads), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || (!f.balanced && f.n_split == 1)) return e;
-    if (!merge && !f.balanced) return e;   // the caller folds the merge in
+    if (!merge) return e;   // the caller folds the merge in
     const int n = f.n_split;
     if (rows <= kMergeManyRows) {
         const dim3 grid2((unsigned)(2 * rows)), block2(512);

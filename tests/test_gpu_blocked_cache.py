@@ -528,9 +528,11 @@ def test_attention_scales_far_apart(ext, dt):
     check_attention(out, ref, DT[dt], True)
 
 
-def test_attention_equals_one_scale(ext):
+def test_attention_equals_one_scale(ext, monkeypatch):
     """Every scale the same power of two: bit for bit what mla_attention_paged_fp8kv gives, whose
-    one scale it is (a power of two moves no rounding)."""
+    one scale it is (a power of two moves no rounding), with the merge and 3d as launches of their own
+    as that call has them."""
+    monkeypatch.setenv("MLA_OUT_SMALL", "0")
     lens = [700, 64, 1, 333]
     qa, qr, w, cache, table = attention_case(lens, 1, 32, 64, BF, 21, spread=0.0)
     table = table.clamp(min=0)
@@ -746,3 +748,23 @@ def test_attention_list_without_a_launch(ext, monkeypatch, B, Sq, Sk):
             outs.append(ext.mla_attention_paged_fp8blk(qa, qr, cache["c_kv"], cache["pe"], cache["scales"], table,
                                                        lens.int().to(DEV), w, SCALE, Sq > 1))
         assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Sq,H,V", [(1, 1, 128, 128), (2, 1, 128, 128), (4, 2, 128, 128), (1, 8, 128, 128),
+                                      (8, 1, 128, 128), (3, 1, 1, 4), (5, 1, 16, 100), (7, 1, 33, 256)])
+def test_attention_few_tokens(ext, monkeypatch, dt, B, Sq, H, V):
+    """Up to eight tokens the merge of the chunks runs inside 3d: chunked, whole and empty sequences
+    against the plain form, and close to the two launches of their own (MLA_OUT_SMALL=0)."""
+    g = torch.Generator().manual_seed(B * 10 + Sq)
+    lens = [3000] + torch.randint(0, 700, (B - 1,), generator=g).tolist()
+    if B > 3:
+        lens[2], lens[3] = 0, 20
+    qa, qr, w, cache, table = attention_case(lens, Sq, 32, 64, DT[dt], B, H=H, V=V)
+    rows = [torch.nan_to_num(r) for r in K.decode(cache)]
+    ref = K.attention(qa, qr, rows, table, lens, w, SCALE, Sq > 1, 64, cache["c_kv"].size(0))
+    out = attend(ext, qa, qr, w, cache, table, lens, Sq > 1)
+    check_attention(out, ref, DT[dt], True)
+    monkeypatch.setenv("MLA_OUT_SMALL", "0")
+    two = attend(ext, qa, qr, w, cache, table, lens, Sq > 1)
+    check_attention(two, ref, DT[dt], True)
