@@ -169,8 +169,9 @@ __global__ void __launch_bounds__(256) cache_extend_fill_kernel(ExtendArgs a) {
 // product x @ W_kv_a (or its split-K partials), takes the largest magnitude of each part over
 // them, and codes them.  Nothing of a block is shared between workgroups, so the scale needs no
 // atomics and the result no order.  A wave makes a row at a time (8 latent columns and, in the
-// lower half, one rope pair a lane: the norm is a wave reduction), four rows a wave in registers
-// across the one barrier that the block's maxima need.
+// lower half, one rope pair a lane: the norm is a wave reduction) and keeps up to four across the
+// barrier that the block's maxima need.  Few new rows leave waves over: those share the rows' splits
+// (up to 16 of them, whose loads a wave alone would wait for four times), the sums in wave order.
 //   scale: 2^e with the smallest e >= -100 such that every finite magnitude is <= 448 * 2^e (448,
 //     e4m3's largest value, is 1.75 * 2^8: e from the exponent and one comparison); where the block
 //     keeps rows written before, at least the scale that they have.  If that grew, they are
@@ -194,7 +195,7 @@ struct AppendBlkArgs {
 };
 
 constexpr int kA8R = 512, kA8D = 64, kA8Row = kA8R + kA8D;
-constexpr int kA8RowsPerWave = 4;
+constexpr int kA8Waves = 16, kA8Threads = 64 * kA8Waves;
 constexpr int kScaleMin = 127 - 100;
 
 __device__ __forceinline__ float finite_abs(float v) {
@@ -222,9 +223,10 @@ __device__ __forceinline__ v4f decode4(uint32_t w, float scale) {
 }
 
 template <int OUT, int G>
-__global__ void __launch_bounds__(64 * G / kA8RowsPerWave) kv_append_blk_kernel(AppendBlkArgs a) {
-    constexpr int kWaves = G / kA8RowsPerWave;
-    __shared__ float red[2][kWaves];
+__global__ void __launch_bounds__(kA8Threads) kv_append_blk_kernel(AppendBlkArgs a) {
+    constexpr int kRows = G / kA8Waves;   // rows a wave
+    __shared__ float red[2][kA8Waves];
+    __shared__ float part[kA8Waves][kA8Row];   // a team's sums
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.blocks, t = blockIdx.x % a.blocks;
@@ -233,100 +235,134 @@ __global__ void __launch_bounds__(64 * G / kA8RowsPerWave) kv_append_blk_kernel(
     const int first = L - n, p0 = (first / G + t) * G;
     if (n == 0 || p0 >= L) return;
     const int page = a.table[(int64_t)b * a.max_pages + p0 / a.page_size];
-    if (page < 0 || page >= a.num_pages) return;   // not a page of the pool: skipped
-    const int64_t row0 = (int64_t)page * a.page_size + p0 % a.page_size;
-    uint8_t* sc = a.scales + 2 * (row0 / G);
-    int old[2] = {0, 0};
-    if (first > p0) { old[0] = sc[0]; old[1] = sc[1]; }
-
-    float lat[kA8RowsPerWave][8], rot[kA8RowsPerWave][2];
-    float top = 0.f, top_r = 0.f;
     float gain[8];
     #pragma unroll
     for (int k = 0; k < 8; ++k) {
         if constexpr (OUT == kOutF32) gain[k] = static_cast<const float*>(a.gain)[8 * lane + k];
         else gain[k] = Store16<OUT>::to_f32(static_cast<const uint16_t*>(a.gain)[8 * lane + k]);
     }
-    #pragma unroll
-    for (int q = 0; q < kA8RowsPerWave; ++q) {
-        const int pos = p0 + wave + kWaves * q;
-        if (pos < first || pos >= L) continue;   // wave-uniform
-        const float* base = a.in + ((int64_t)b * a.Sq + (pos - L + a.Sq)) * kA8Row;
+    const float freq = a.inv_freq[lane & 31];
+
+    // new rows lo .. hi-1 of the block: with as many waves as rows or fewer, wave w makes rows
+    // w, w + 16, ..; with more, a team of waves shares a row's splits and its first wave goes on
+    const int lo = max(first - p0, 0), hi = min(L - p0, G);
+    int team = 1;
+    while (2 * team * (hi - lo) <= kA8Waves) team *= 2;
+    team = min(team, a.nsplit > 4 ? kA8Waves : 1);   // up to four splits are one wave's loads at once
+    auto row_of = [&](int q) __attribute__((always_inline)) {   // -1: none
+        const int r = team > 1 ? (q ? G : lo + wave / team) : wave + kA8Waves * q;
+        return r >= lo && r < hi ? r : -1;
+    };
+    struct Sums { v4f a, b; v2f_t r; };
+    // splits i0, i0 + step, .. of row r
+    auto sum_splits = [&](int r, int i0, int step) __attribute__((always_inline)) {
+        const float* base = a.in + ((int64_t)b * a.Sq + (p0 + r - L + a.Sq)) * kA8Row;
         const float* lp = base + 8 * lane;
         const float* rp = base + kA8R + 2 * (lane & 31);
-        v4f s0 = v4f{0.f, 0.f, 0.f, 0.f}, s1 = s0;
-        v2f_t sr = v2f_t{0.f, 0.f};
+        Sums s = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v2f_t{0.f, 0.f}};
         constexpr int kWin = 4;   // splits' loads in flight
-        for (int i = 0; i < a.nsplit; i += kWin) {
+        for (int i = i0; i < a.nsplit; i += kWin * step) {
             v4f x0[kWin], x1[kWin];
             v2f_t xr[kWin];
             #pragma unroll
             for (int k = 0; k < kWin; ++k) {
-                const int64_t o = (int64_t)min(i + k, a.nsplit - 1) * a.split_stride;
+                const int64_t o = (int64_t)min(i + k * step, a.nsplit - 1) * a.split_stride;
                 x0[k] = *reinterpret_cast<const v4f*>(lp + o);
                 x1[k] = *reinterpret_cast<const v4f*>(lp + o + 4);
                 xr[k] = *reinterpret_cast<const v2f_t*>(rp + o);
             }
             #pragma unroll
             for (int k = 0; k < kWin; ++k)
-                if (i + k < a.nsplit) { s0 += x0[k]; s1 += x1[k]; sr += xr[k]; }
+                if (i + k * step < a.nsplit) { s.a += x0[k]; s.b += x1[k]; s.r += xr[k]; }
         }
+        return s;
+    };
+    Sums shared_row;
+    if (team > 1) {
+        const int r = row_of(0);
+        if (r >= 0) {
+            shared_row = sum_splits(r, wave % team, team);
+            *reinterpret_cast<v4f*>(&part[wave][8 * lane]) = shared_row.a;
+            *reinterpret_cast<v4f*>(&part[wave][8 * lane + 4]) = shared_row.b;
+            if (lane < 32) *reinterpret_cast<v2f_t*>(&part[wave][kA8R + 2 * lane]) = shared_row.r;
+        }
+        __syncthreads();
+        if (r >= 0 && wave % team == 0)
+            for (int w = wave + 1; w < wave + team; ++w) {
+                shared_row.a += *reinterpret_cast<const v4f*>(&part[w][8 * lane]);
+                shared_row.b += *reinterpret_cast<const v4f*>(&part[w][8 * lane + 4]);
+                shared_row.r += *reinterpret_cast<const v2f_t*>(&part[w][kA8R + 2 * (lane & 31)]);
+            }
+    }
+    const bool mine = team == 1 || wave % team == 0;
+    float lat[kRows][8], rot[kRows][2];
+    float top = 0.f, top_r = 0.f;
+    #pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+        const int r = row_of(q);
+        if (r < 0 || !mine) continue;   // wave-uniform
+        const Sums s = team > 1 ? shared_row : sum_splits(r, 0, 1);
         float ss = 0.f;
         #pragma unroll
-        for (int k = 0; k < 4; ++k) ss += s0[k] * s0[k] + s1[k] * s1[k];
+        for (int k = 0; k < 4; ++k) ss += s.a[k] * s.a[k] + s.b[k] * s.b[k];
         const float inv = rsqrtf(wave_reduce(ss, OpSum()) / (float)kA8R + a.eps);
         #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            lat[q][k] = (k < 4 ? s0[k] : s1[k - 4]) * inv * gain[k];
+            lat[q][k] = (k < 4 ? s.a[k] : s.b[k - 4]) * inv * gain[k];
             top = fmaxf(top, finite_abs(lat[q][k]));
         }
-        float c, s;
-        rope_cos_sin(rope_angle(pos, a.inv_freq[lane & 31]), &c, &s);
-        rot[q][0] = rope_even(sr[0], sr[1], c, s);
-        rot[q][1] = rope_odd(sr[0], sr[1], c, s);
+        float c, sn;
+        rope_cos_sin(rope_angle(p0 + r, freq), &c, &sn);
+        rot[q][0] = rope_even(s.r[0], s.r[1], c, sn);
+        rot[q][1] = rope_odd(s.r[0], s.r[1], c, sn);
         top_r = fmaxf(top_r, fmaxf(finite_abs(rot[q][0]), finite_abs(rot[q][1])));
     }
+    if (page < 0 || page >= a.num_pages) return;   // not a page of the pool: skipped
+    const int64_t row0 = (int64_t)page * a.page_size + p0 % a.page_size;
+    uint8_t* sc = a.scales + 2 * (row0 / G);
+    int old[2] = {0, 0};
+    if (lo > 0) { old[0] = sc[0]; old[1] = sc[1]; }
     top = wave_reduce(top, OpMax());
     top_r = wave_reduce(top_r, OpMax());
     if (lane == 0) { red[0][wave] = top; red[1][wave] = top_r; }
     __syncthreads();
     #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kA8Waves; ++w) {
         top = fmaxf(top, red[0][w]);
         top_r = fmaxf(top_r, red[1][w]);
     }
     const int e_lat = max(scale_byte(top), old[0]), e_rot = max(scale_byte(top_r), old[1]);
     if (threadIdx.x == 0) { sc[0] = (uint8_t)e_lat; sc[1] = (uint8_t)e_rot; }
     const float inv_l = scale_value(254 - min(e_lat, 254)), inv_r = scale_value(254 - min(e_rot, 254));
-    const bool again_l = first > p0 && e_lat != old[0], again_r = first > p0 && e_rot != old[1];
+    auto at_lat = [&](int r) __attribute__((always_inline)) { return a.c_kv + (row0 + r) * kA8R + 8 * lane; };
+    auto at_rot = [&](int r) __attribute__((always_inline)) { return a.pe + (row0 + r) * kA8D + 2 * (lane & 31); };
     #pragma unroll
-    for (int q = 0; q < kA8RowsPerWave; ++q) {
-        const int pos = p0 + wave + kWaves * q;
-        uint8_t* cl = a.c_kv + (row0 + wave + kWaves * q) * kA8R + 8 * lane;
-        uint8_t* cr = a.pe + (row0 + wave + kWaves * q) * kA8D + 2 * (lane & 31);
-        if (pos >= L) continue;
-        if (pos >= first) {
-            const float* v = lat[q];
-            auto in = [&](int k) __attribute__((always_inline)) { return code_input(v[k], inv_l); };
-            *reinterpret_cast<v2u_t*>(cl) =
-                v2u_t{code4(in(0), in(1), in(2), in(3)), code4(in(4), in(5), in(6), in(7))};
-            if (lane < 32)
-                *reinterpret_cast<uint16_t*>(cr) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(
-                    code_input(rot[q][0], inv_r), code_input(rot[q][1], inv_r), 0, false);
-            continue;
-        }
-        // rows of before, under a larger scale: 2^(e_old - e), at least 2^-100 (which leaves nothing)
-        if (again_l) {
-            const float f = scale_value(127 - min(e_lat - old[0], 100));
-            const v2u_t w = *reinterpret_cast<const v2u_t*>(cl);
+    for (int q = 0; q < kRows; ++q) {
+        const int r = row_of(q);
+        if (r < 0 || !mine) continue;
+        auto in = [&](int k) __attribute__((always_inline)) { return code_input(lat[q][k], inv_l); };
+        *reinterpret_cast<v2u_t*>(at_lat(r)) =
+            v2u_t{code4(in(0), in(1), in(2), in(3)), code4(in(4), in(5), in(6), in(7))};
+        if (lane < 32)
+            *reinterpret_cast<uint16_t*>(at_rot(r)) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(
+                code_input(rot[q][0], inv_r), code_input(rot[q][1], inv_r), 0, false);
+    }
+    // rows of before, where the scale grew: times 2^(e_old - e), at least 2^-100 (which leaves nothing)
+    if (lo > 0 && e_lat != old[0]) {
+        const float f = scale_value(127 - min(e_lat - old[0], 100));
+        for (int r = wave; r < lo; r += kA8Waves) {
+            const v2u_t w = *reinterpret_cast<const v2u_t*>(at_lat(r));
             const v4f x = decode4(w[0], f), y = decode4(w[1], f);
-            *reinterpret_cast<v2u_t*>(cl) = v2u_t{code4(x[0], x[1], x[2], x[3]), code4(y[0], y[1], y[2], y[3])};
+            *reinterpret_cast<v2u_t*>(at_lat(r)) =
+                v2u_t{code4(x[0], x[1], x[2], x[3]), code4(y[0], y[1], y[2], y[3])};
         }
-        if (again_r && lane < 32) {
-            const float f = scale_value(127 - min(e_rot - old[1], 100));
+    }
+    if (lo > 0 && e_rot != old[1] && lane < 32) {
+        const float f = scale_value(127 - min(e_rot - old[1], 100));
+        for (int r = wave; r < lo; r += kA8Waves) {
             const v2f_t x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(
-                (uint32_t)*reinterpret_cast<const uint16_t*>(cr), f, false);
-            *reinterpret_cast<uint16_t*>(cr) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+                (uint32_t)*reinterpret_cast<const uint16_t*>(at_rot(r)), f, false);
+            *reinterpret_cast<uint16_t*>(at_rot(r)) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
         }
     }
 }
@@ -415,12 +451,13 @@ namespace {
 template <int OUT>
 hipError_t launch_append_blk(const AppendBlkArgs& a, int block, hipStream_t stream) {
     const dim3 grid((unsigned)(a.B * a.blocks));
+    const dim3 threads(kA8Threads);
     if (block == 16)
-        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 16>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 16>), grid, threads, 0, stream, a);
     else if (block == 32)
-        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 32>), grid, dim3(512), 0, stream, a);
+        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 32>), grid, threads, 0, stream, a);
     else
-        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 64>), grid, dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 64>), grid, threads, 0, stream, a);
     return hipGetLastError();
 }
 }  // namespace
