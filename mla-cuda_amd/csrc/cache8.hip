@@ -222,7 +222,100 @@ __device__ __forceinline__ v4f decode4(uint32_t w, float scale) {
     return v4f{lo[0], lo[1], hi[0], hi[1]};
 }
 
-template <int OUT, int G>
+// A row's product as a wave holds it: latent columns 8 lane .. +7, and rope pair lane % 32.
+struct RowSums { v4f a, b; v2f_t r; };
+
+// The sum of splits i0, i0 + step, .. of the row at `row`.
+__device__ __forceinline__ RowSums sum_splits(const float* row, int nsplit, int64_t split_stride, int i0,
+                                              int step) {
+    const int lane = threadIdx.x & 63;
+    const float* lp = row + 8 * lane;
+    const float* rp = row + kA8R + 2 * (lane & 31);
+    RowSums s = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v2f_t{0.f, 0.f}};
+    constexpr int kWin = 4;   // splits' loads in flight
+    for (int i = i0; i < nsplit; i += kWin * step) {
+        v4f x0[kWin], x1[kWin];
+        v2f_t xr[kWin];
+        #pragma unroll
+        for (int k = 0; k < kWin; ++k) {
+            const int64_t o = (int64_t)min(i + k * step, nsplit - 1) * split_stride;
+            x0[k] = *reinterpret_cast<const v4f*>(lp + o);
+            x1[k] = *reinterpret_cast<const v4f*>(lp + o + 4);
+            xr[k] = *reinterpret_cast<const v2f_t*>(rp + o);
+        }
+        #pragma unroll
+        for (int k = 0; k < kWin; ++k)
+            if (i + k * step < nsplit) { s.a += x0[k]; s.b += x1[k]; s.r += xr[k]; }
+    }
+    return s;
+}
+// The same through LDS, for the waves after this one to add to theirs.
+__device__ __forceinline__ void store_sums(float* part, const RowSums& s) {
+    const int lane = threadIdx.x & 63;
+    *reinterpret_cast<v4f*>(part + 8 * lane) = s.a;
+    *reinterpret_cast<v4f*>(part + 8 * lane + 4) = s.b;
+    if (lane < 32) *reinterpret_cast<v2f_t*>(part + kA8R + 2 * lane) = s.r;
+}
+__device__ __forceinline__ void add_sums(RowSums* s, const float* part) {
+    const int lane = threadIdx.x & 63;
+    s->a += *reinterpret_cast<const v4f*>(part + 8 * lane);
+    s->b += *reinterpret_cast<const v4f*>(part + 8 * lane + 4);
+    s->r += *reinterpret_cast<const v2f_t*>(part + kA8R + 2 * (lane & 31));
+}
+
+template <int OUT>
+__device__ __forceinline__ void load_gain(const void* gain, float (&g)[8]) {
+    const int lane = threadIdx.x & 63;
+    #pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if constexpr (OUT == kOutF32) g[k] = static_cast<const float*>(gain)[8 * lane + k];
+        else g[k] = Store16<OUT>::to_f32(static_cast<const uint16_t*>(gain)[8 * lane + k]);
+    }
+}
+// The cache row of the product `s` at position pos: normalised latent, rotated rope pair.
+__device__ __forceinline__ void make_row(const RowSums& s, const float (&gain)[8], float eps, int pos,
+                                         float freq, float* lat, float* rot) {
+    float ss = 0.f;
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) ss += s.a[k] * s.a[k] + s.b[k] * s.b[k];
+    const float inv = rsqrtf(wave_reduce(ss, OpSum()) / (float)kA8R + eps);
+    #pragma unroll
+    for (int k = 0; k < 8; ++k) lat[k] = (k < 4 ? s.a[k] : s.b[k - 4]) * inv * gain[k];
+    float c, sn;
+    rope_cos_sin(rope_angle(pos, freq), &c, &sn);
+    rot[0] = rope_even(s.r[0], s.r[1], c, sn);
+    rot[1] = rope_odd(s.r[0], s.r[1], c, sn);
+}
+
+// The rows alone, into the place of the first split: where many rows of a block come in many splits,
+// one CU per block would read them all (64 rows in 16 splits: 2.4 MB, 30 us); a workgroup per row
+// spreads that over the chip, and the blocks then read a row once.  Its four waves share the splits.
+template <int OUT>
+__global__ void __launch_bounds__(256) kv_rows_kernel(AppendBlkArgs a) {
+    __shared__ float part[4][kA8Row];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x / a.Sq, i = blockIdx.x % a.Sq;
+    const int L = min(max(a.seq_lens[b], 0), a.max_pages * a.page_size);
+    const int n = min(max(a.new_lens[b], 0), min(a.Sq, L));
+    if (i < a.Sq - n) return;   // padding
+    float* row = const_cast<float*>(a.in) + (int64_t)blockIdx.x * kA8Row;
+    float gain[8];
+    load_gain<OUT>(a.gain, gain);
+    const float freq = a.inv_freq[lane & 31];
+    RowSums s = sum_splits(row, a.nsplit, a.split_stride, wave, 4);
+    store_sums(part[wave], s);
+    __syncthreads();
+    if (wave) return;
+    for (int w = 1; w < 4; ++w) add_sums(&s, part[w]);
+    float lat[8], rot[2];
+    make_row(s, gain, a.eps, L - a.Sq + i, freq, lat, rot);
+    store_sums(row, RowSums{v4f{lat[0], lat[1], lat[2], lat[3]}, v4f{lat[4], lat[5], lat[6], lat[7]},
+                            v2f_t{rot[0], rot[1]}});
+}
+
+// READY: `in` holds the rows themselves (kv_rows_kernel's).
+template <int OUT, int G, bool READY>
 __global__ void __launch_bounds__(kA8Threads) kv_append_blk_kernel(AppendBlkArgs a) {
     constexpr int kRows = G / kA8Waves;   // rows a wave
     __shared__ float red[2][kA8Waves];
@@ -235,64 +328,35 @@ __global__ void __launch_bounds__(kA8Threads) kv_append_blk_kernel(AppendBlkArgs
     const int first = L - n, p0 = (first / G + t) * G;
     if (n == 0 || p0 >= L) return;
     const int page = a.table[(int64_t)b * a.max_pages + p0 / a.page_size];
-    float gain[8];
-    #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        if constexpr (OUT == kOutF32) gain[k] = static_cast<const float*>(a.gain)[8 * lane + k];
-        else gain[k] = Store16<OUT>::to_f32(static_cast<const uint16_t*>(a.gain)[8 * lane + k]);
+    float gain[8], freq = 0.f;
+    if constexpr (!READY) {
+        load_gain<OUT>(a.gain, gain);
+        freq = a.inv_freq[lane & 31];
     }
-    const float freq = a.inv_freq[lane & 31];
 
     // new rows lo .. hi-1 of the block: with as many waves as rows or fewer, wave w makes rows
     // w, w + 16, ..; with more, a team of waves shares a row's splits and its first wave goes on
     const int lo = max(first - p0, 0), hi = min(L - p0, G);
     int team = 1;
     while (2 * team * (hi - lo) <= kA8Waves) team *= 2;
-    team = min(team, a.nsplit > 4 ? kA8Waves : 1);   // up to four splits are one wave's loads at once
+    if (READY || a.nsplit <= 4) team = 1;   // one wave's loads at once
     auto row_of = [&](int q) __attribute__((always_inline)) {   // -1: none
         const int r = team > 1 ? (q ? G : lo + wave / team) : wave + kA8Waves * q;
         return r >= lo && r < hi ? r : -1;
     };
-    struct Sums { v4f a, b; v2f_t r; };
-    // splits i0, i0 + step, .. of row r
-    auto sum_splits = [&](int r, int i0, int step) __attribute__((always_inline)) {
-        const float* base = a.in + ((int64_t)b * a.Sq + (p0 + r - L + a.Sq)) * kA8Row;
-        const float* lp = base + 8 * lane;
-        const float* rp = base + kA8R + 2 * (lane & 31);
-        Sums s = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v2f_t{0.f, 0.f}};
-        constexpr int kWin = 4;   // splits' loads in flight
-        for (int i = i0; i < a.nsplit; i += kWin * step) {
-            v4f x0[kWin], x1[kWin];
-            v2f_t xr[kWin];
-            #pragma unroll
-            for (int k = 0; k < kWin; ++k) {
-                const int64_t o = (int64_t)min(i + k * step, a.nsplit - 1) * a.split_stride;
-                x0[k] = *reinterpret_cast<const v4f*>(lp + o);
-                x1[k] = *reinterpret_cast<const v4f*>(lp + o + 4);
-                xr[k] = *reinterpret_cast<const v2f_t*>(rp + o);
-            }
-            #pragma unroll
-            for (int k = 0; k < kWin; ++k)
-                if (i + k * step < a.nsplit) { s.a += x0[k]; s.b += x1[k]; s.r += xr[k]; }
-        }
-        return s;
+    auto in_row = [&](int r) __attribute__((always_inline)) {
+        return a.in + ((int64_t)b * a.Sq + (p0 + r - L + a.Sq)) * kA8Row;
     };
-    Sums shared_row;
+    RowSums shared_row;
     if (team > 1) {
         const int r = row_of(0);
         if (r >= 0) {
-            shared_row = sum_splits(r, wave % team, team);
-            *reinterpret_cast<v4f*>(&part[wave][8 * lane]) = shared_row.a;
-            *reinterpret_cast<v4f*>(&part[wave][8 * lane + 4]) = shared_row.b;
-            if (lane < 32) *reinterpret_cast<v2f_t*>(&part[wave][kA8R + 2 * lane]) = shared_row.r;
+            shared_row = sum_splits(in_row(r), a.nsplit, a.split_stride, wave % team, team);
+            store_sums(part[wave], shared_row);
         }
         __syncthreads();
         if (r >= 0 && wave % team == 0)
-            for (int w = wave + 1; w < wave + team; ++w) {
-                shared_row.a += *reinterpret_cast<const v4f*>(&part[w][8 * lane]);
-                shared_row.b += *reinterpret_cast<const v4f*>(&part[w][8 * lane + 4]);
-                shared_row.r += *reinterpret_cast<const v2f_t*>(&part[w][kA8R + 2 * (lane & 31)]);
-            }
+            for (int w = wave + 1; w < wave + team; ++w) add_sums(&shared_row, part[w]);
     }
     const bool mine = team == 1 || wave % team == 0;
     float lat[kRows][8], rot[kRows][2];
@@ -301,20 +365,17 @@ __global__ void __launch_bounds__(kA8Threads) kv_append_blk_kernel(AppendBlkArgs
     for (int q = 0; q < kRows; ++q) {
         const int r = row_of(q);
         if (r < 0 || !mine) continue;   // wave-uniform
-        const Sums s = team > 1 ? shared_row : sum_splits(r, 0, 1);
-        float ss = 0.f;
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) ss += s.a[k] * s.a[k] + s.b[k] * s.b[k];
-        const float inv = rsqrtf(wave_reduce(ss, OpSum()) / (float)kA8R + a.eps);
-        #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            lat[q][k] = (k < 4 ? s.a[k] : s.b[k - 4]) * inv * gain[k];
-            top = fmaxf(top, finite_abs(lat[q][k]));
+        const RowSums s = team > 1 ? shared_row : sum_splits(in_row(r), READY ? 1 : a.nsplit, a.split_stride, 0, 1);
+        if constexpr (READY) {
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) lat[q][k] = k < 4 ? s.a[k] : s.b[k - 4];
+            rot[q][0] = s.r[0];
+            rot[q][1] = s.r[1];
+        } else {
+            make_row(s, gain, a.eps, p0 + r, freq, lat[q], rot[q]);
         }
-        float c, sn;
-        rope_cos_sin(rope_angle(p0 + r, freq), &c, &sn);
-        rot[q][0] = rope_even(s.r[0], s.r[1], c, sn);
-        rot[q][1] = rope_odd(s.r[0], s.r[1], c, sn);
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, finite_abs(lat[q][k]));
         top_r = fmaxf(top_r, fmaxf(finite_abs(rot[q][0]), finite_abs(rot[q][1])));
     }
     if (page < 0 || page >= a.num_pages) return;   // not a page of the pool: skipped
@@ -448,16 +509,27 @@ hipError_t launch_cache_extend(const CacheExtend& p, void* workspace, hipStream_
 }
 
 namespace {
+template <int OUT, int G>
+void launch_append_g(const AppendBlkArgs& a, bool rows_first, hipStream_t stream) {
+    const dim3 grid((unsigned)(a.B * a.blocks)), threads(kA8Threads);
+    if (!rows_first) {
+        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, G, false>), grid, threads, 0, stream, a);
+        return;
+    }
+    hipLaunchKernelGGL(kv_rows_kernel<OUT>, dim3((unsigned)(a.B * a.Sq)), dim3(256), 0, stream, a);
+    // the rows are float32 whatever the gain's type
+    hipLaunchKernelGGL((kv_append_blk_kernel<kOutF32, G, true>), grid, threads, 0, stream, a);
+}
 template <int OUT>
 hipError_t launch_append_blk(const AppendBlkArgs& a, int block, hipStream_t stream) {
-    const dim3 grid((unsigned)(a.B * a.blocks));
-    const dim3 threads(kA8Threads);
-    if (block == 16)
-        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 16>), grid, threads, 0, stream, a);
-    else if (block == 32)
-        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 32>), grid, threads, 0, stream, a);
-    else
-        hipLaunchKernelGGL((kv_append_blk_kernel<OUT, 64>), grid, threads, 0, stream, a);
+    // Rows in a launch of their own where a block's are many partial rows and each is more than one
+    // round of loads (one launch / two, with the product, us: 160 tokens in 16 splits, blocks of 64
+    // 49.0 / 24.9; 1,024 in 6, blocks of 64 40.1 / 32.8, of 16 29.6 / 30.7; 16 tokens of 8 sequences
+    // in 14 24.3 / 22.0; 4 of 33 21.0 / 21.7; 4,096 in 3, blocks of 64 67.1 / 69.3).
+    const bool rows_first = a.nsplit > 4 && std::min(a.Sq, block) * a.nsplit >= 160;
+    if (block == 16) launch_append_g<OUT, 16>(a, rows_first, stream);
+    else if (block == 32) launch_append_g<OUT, 32>(a, rows_first, stream);
+    else launch_append_g<OUT, 64>(a, rows_first, stream);
     return hipGetLastError();
 }
 }  // namespace

@@ -269,6 +269,17 @@ def test_append_at_the_layers_width(ext, dt, B, Sq):
     check_append(cache, after, K.append(cache, x, W, gain, lens, new, table, 64, 32), 32)
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("block", [16, 32, 64])
+def test_append_long_rows_in_many_splits(ext, dt, block):
+    """Many new tokens whose product comes in many splits (the rows are made in a launch of their
+    own), with padding, a sequence without new tokens, and blocks that keep rows of before."""
+    lens, new, Sq = [90, 170, 20, 33], [40, 37, 0, 33], 40
+    cache, x, W, gain, table = append_inputs(lens, new, Sq, block, 64, DT[dt], block, hidden=7168)
+    after = run_append(ext, cache, x, W, gain, lens, new, table)
+    check_append(cache, after, K.append(cache, x, W, gain, lens, new, table, 64, block), block)
+
+
 def test_append_scale_grows_and_stays(ext):
     """Token after token into one block, each larger than the last (the rows before are coded again
     every time, down to codes that vanish), then smaller ones, which keep the scale."""
