@@ -170,7 +170,8 @@ __device__ __forceinline__ int64_t flash_key_row(const FlashArgs& a, int b, int 
 // flash_worklist_kernel, the last chunks of one length bucket in batch order.  Workgroup 0 leaves the
 // sequences' first slots and chunk counts in the list for the merge.
 constexpr int kSmallList = 64;
-// L / c and L % c (0 <= L < 2^24, 0 < c < 2^24)
+// L / c and L % c for a quotient below 2^21 (0 <= L < 2^31, 0 < c < 2^24): a dozen instructions where a
+// division takes forty
 __device__ __forceinline__ int divmod24(int L, int c, int* rem) {
     int q = (int)((float)L * __builtin_amdgcn_rcpf((float)c));   // off by one at most
     int r = L - q * c;
@@ -254,7 +255,8 @@ __device__ __forceinline__ FlashWork flash_work_small(const FlashArgs& a, int* p
         const bool sh = has && (r > 0 || L == 0);
         // (the item's place among them picks the lane: one bit of the bucket at a time, then the
         // place among the lanes that are left)
-        const uint32_t q = (uint32_t)(chunk - 1 - r) * (uint32_t)kWlBuckets / (uint32_t)chunk;
+        int rest;
+        const uint32_t q = (uint32_t)divmod24((chunk - 1 - r) * kWlBuckets, chunk, &rest);
         uint64_t left = __builtin_amdgcn_ballot_w64(sh);
         int place = it - n_full;
         static_assert(kWlBuckets == 256, "eight bits");
@@ -3096,7 +3098,7 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
                                                                     int B, int Sk, int row_tiles,
                                                                     int block_keys, int max_items,
                                                                     int* __restrict__ wl) {
-    // reductions and scans run within each wave (__shfl_*), then over the four waves'
+    // reductions and scans run within each wave (DPP), then over the four waves'
     // totals in LDS: a handful of barriers, since this one-workgroup kernel sits on the
     // decode step's critical path
     static_assert(kWlThreads == 256 && kWlBuckets == 256, "one bucket per thread, four waves");
@@ -3131,11 +3133,10 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
         mn = min(mn, L);
         mx = max(mx, L);
     }
-    for (int d = 32; d > 0; d >>= 1) {
-        tot += __shfl_xor(tot, d);
-        mn = min(mn, __shfl_xor(mn, d));
-        mx = max(mx, __shfl_xor(mx, d));
-    }
+    // (a thread's total in two halves: their sums over the wave stay below 2^31)
+    tot = ((long long)wave_sum((int)(tot >> 16)) << 16) + wave_sum((int)(tot & 0xffff));
+    mx = (int)wave_reduce((float)mx, OpMax{});                            // exact: lengths are below 2^24
+    mn = -(int)wave_reduce(b0 < b1 ? -(float)mn : -16777216.f, OpMax{});   // (a wave without a sequence: 2^24)
     if (lane == 0) { w_tot[wave] = tot; w_min[wave] = mn; w_max[wave] = mx; }
     __syncthreads();
     tot = ((w_tot[0] + w_tot[1]) + w_tot[2]) + w_tot[3];
@@ -3154,8 +3155,10 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
             int n = 0, small = 0;
             for (int b = lane; b < B; b += 64) {
                 const int L = b < kLdsLens ? s_len[b] : wl_len(seq_lens[b], Sk);
-                n += wl_chunk_count(L, c);
-                small += wl_small(L, c, block_keys);
+                int r;   // wl_chunk_count and wl_small, from one division
+                const int q = divmod24(L, c, &r);
+                n += wl_max(1, q + (r > 0));
+                small += (r > 0 || L == 0) && 2 * r <= c - wl_fixed_blocks(block_keys) * block_keys;
             }
             n = wave_sum(n);
             small = wave_sum(small);
@@ -3170,12 +3173,12 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
     for (;;) {
         cnt = 0; full = 0;
         for (int b = b0; b < b1; ++b) {
-            const int L = len_of(b);
-            cnt += wl_chunk_count(L, chunk);
-            full += wl_full_count(L, chunk);
+            int r;   // wl_chunk_count and wl_full_count
+            const int q = divmod24(len_of(b), chunk, &r);
+            cnt += wl_max(1, q + (r > 0));
+            full += q;
         }
-        int c = cnt;
-        for (int d = 32; d > 0; d >>= 1) c += __shfl_xor(c, d);
+        const int c = wave_sum(cnt);
         __syncthreads();   // every thread has read the previous round's w_cnt
         if (lane == 0) w_cnt[wave] = c;
         __syncthreads();
@@ -3185,11 +3188,7 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
     }
     // exclusive prefix sums over the threads: inclusive scans within each wave, then the
     // totals of the waves before
-    int ic = cnt, ifl = full;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int c = __shfl_up(ic, d), f = __shfl_up(ifl, d);
-        if (lane >= d) { ic += c; ifl += f; }
-    }
+    const int ic = lanes_scan(cnt), ifl = lanes_scan(full);
     __syncthreads();   // w_cnt of the loop above has been read by every thread
     if (lane == 63) { w_cnt[wave] = ic; w_full[wave] = ifl; }
     __syncthreads();
@@ -3227,19 +3226,23 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
     // (Simulated in-order dispatch at B=128, lengths uniform in [1, 4989]: the makespan
     // drops from 2916 to 2621 key-times against a 2571 lower bound.)
     __shared__ int hist[kWlBuckets], cursor[kWlBuckets];
+    // wl_bucket, from the remainder (chunk <= 2 Sk < 2^23: the product stays below 2^31)
+    auto bucket_of = [&](int r) __attribute__((always_inline)) {
+        int rest;
+        return divmod24((chunk - 1 - r) * kWlBuckets, chunk, &rest);
+    };
     hist[tid] = 0;
     cursor[tid] = 0;
     __syncthreads();
     for (int b = b0; b < b1; ++b) {
         const int L = len_of(b);
-        if (wl_has_short(L, chunk)) atomicAdd(&hist[wl_bucket(L, chunk)], 1);
+        int r;
+        divmod24(L, chunk, &r);
+        if (r > 0 || L == 0) atomicAdd(&hist[bucket_of(r)], 1);
     }
     __syncthreads();
-    int hb = hist[tid], hs = hb;   // exclusive scan of the buckets in order
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(hs, d);
-        if (lane >= d) hs += v;
-    }
+    const int hb = hist[tid];      // exclusive scan of the buckets in order
+    int hs = lanes_scan(hb);
     if (lane == 63) w_rem[wave] = hs;
     __syncthreads();
     for (int w = 0; w < wave; ++w) hs += w_rem[w];
@@ -3247,14 +3250,14 @@ __global__ void __launch_bounds__(kWlThreads) flash_worklist_kernel(const int* _
     __syncthreads();
     for (int b = b0; b < b1; ++b) {
         const int L = len_of(b);
-        const int n = wl_chunk_count(L, chunk);
+        int r;
+        const int nf = divmod24(L, chunk, &r), n = wl_max(1, nf + (r > 0));
         first[b] = slot;
         count[b] = n;
         slot += n;
         for (int c = 0; c < n; ++c) {
-            const bool is_full = (long long)(c + 1) * chunk <= L;
-            const int q = wl_bucket(L, chunk);
-            const int it = is_full ? fi++ : n_full + hist[q] + atomicAdd(&cursor[q], 1);
+            const int q = bucket_of(r);
+            const int it = c < nf ? fi++ : n_full + hist[q] + atomicAdd(&cursor[q], 1);
             if (it < max_items) {   // always (the fit check above); a guard
                 items[2 * it] = b;
                 items[2 * it + 1] = c;
