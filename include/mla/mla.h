@@ -398,7 +398,7 @@ int mla_kv_append_paged(mla_dtype_t dtype, const mla_dims_t* dims, const void* x
  * All of it is device memory; nothing is read back.  positions is what mla_q_absorbed_ragged and
  * mla_kv_append_paged take (which skips rows at -1), slots what mla_kv_read_fp8blk takes.
  * batch * sq and num_pages are at most 2^30, batch * max_pages and the span below 2^31. */
-size_t mla_cache_extend_workspace_bytes(int32_t batch);
+size_t mla_cache_extend_workspace_bytes(int32_t batch, int32_t sq);   /* 0 for a small batch */
 int mla_cache_extend(int32_t batch, int32_t sq, int32_t page_size, int32_t max_pages,
                      int32_t num_pages, const int32_t* new_lens, const int32_t* seq_lens,
                      const int32_t* free_state, int32_t* block_table, int32_t* free_pages,

@@ -784,15 +784,17 @@ std::vector<torch::Tensor> op_cache_extend(torch::Tensor new_lens, torch::Tensor
     auto granted = torch::empty_like(lens);
     auto positions = torch::empty({B, Sq}, lens.options().dtype(torch::kLong));
     auto slots = torch::empty_like(positions);
-    const size_t wsb = mla_cache_extend_workspace_bytes((int32_t)B);
-    auto ws = workspace(wsb, lens);
+    const size_t wsb = mla_cache_extend_workspace_bytes((int32_t)B, (int32_t)Sq);
+    torch::Tensor ws;
+    if (wsb > 0) ws = workspace(wsb, lens);
     check_status(mla_cache_extend((int32_t)B, (int32_t)Sq, (int32_t)page_size, (int32_t)max_pages,
                                   (int32_t)free_pages.size(0), want.data_ptr<int32_t>(),
                                   lens.data_ptr<int32_t>(), state.data_ptr<int32_t>(),
                                   block_table.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(),
                                   lens_out.data_ptr<int32_t>(), state_out.data_ptr<int32_t>(),
                                   granted.data_ptr<int32_t>(), positions.data_ptr<int64_t>(),
-                                  slots.data_ptr<int64_t>(), ws.data_ptr(), wsb, current_stream()),
+                                  slots.data_ptr<int64_t>(), wsb > 0 ? ws.data_ptr() : nullptr, wsb,
+                                  current_stream()),
                  "cache_extend");
     return {lens_out, state_out, granted, positions, slots};
 }

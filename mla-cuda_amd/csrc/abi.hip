@@ -1511,8 +1511,8 @@ int mla_attention(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_absor
 
 // ------------------------------------------------------------------ 8-bit blocked cache
 
-size_t mla_cache_extend_workspace_bytes(int32_t batch) {
-    return batch > 0 ? align_up(cache_extend_workspace(batch)) : 0;
+size_t mla_cache_extend_workspace_bytes(int32_t batch, int32_t sq) {
+    return batch > 0 && sq > 0 ? align_up(cache_extend_workspace(batch, sq)) : 0;
 }
 
 int mla_cache_extend(int32_t batch, int32_t sq, int32_t page_size, int32_t max_pages,
@@ -1544,7 +1544,7 @@ int mla_cache_extend(int32_t batch, int32_t sq, int32_t page_size, int32_t max_p
     MLA_CHECK(check_ptr(granted, "granted"));
     MLA_CHECK(check_ptr(positions, "positions"));
     MLA_CHECK(check_ptr(slots, "slots"));
-    MLA_CHECK(check_ws(workspace, workspace_bytes, mla_cache_extend_workspace_bytes(batch)));
+    MLA_CHECK(check_ws(workspace, workspace_bytes, mla_cache_extend_workspace_bytes(batch, sq)));
     CacheExtend p;
     p.B = batch; p.Sq = sq; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
     p.new_lens = new_lens; p.seq_lens = seq_lens; p.free_state = free_state;

@@ -13,6 +13,7 @@
 #include "kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mla {
 
@@ -20,6 +21,26 @@ namespace {
 
 typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
 typedef float v2f_t __attribute__((ext_vector_type(2)));
+
+// Inclusive sum over the lanes up to this one, and the wave's maximum (of values >= 0).
+__device__ __forceinline__ int lanes_sum_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+__device__ __forceinline__ int lanes_max(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
 
 // ---- extend ---------------------------------------------------------------------------------
 // Request b holds L = seq_lens[b] tokens and asks for new_lens[b] more (or fewer).  What it needs,
@@ -31,11 +52,27 @@ typedef float v2f_t __attribute__((ext_vector_type(2)));
 // order: taken pages come from the ring's free ones and given ones go to places that hold none, and
 // a new token's page is an old table entry or a free one, so nothing written here is read here.
 // It is bound by latency (a decode step's tables are a few KB).
-constexpr int kExtendThreads = 1024;
+constexpr int kExtendThreads = 1024;   // at most
 constexpr int kExtendWaves = kExtendThreads / 64;
+
+// x / d for 0 <= x < 2^31 and a d that the host knows (a division takes forty instructions, and each
+// request's plan has five): with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// x / d = (floor(m x / 2^32) + x) / 2^s, where the sum stays below 2^32.
+struct FastDiv {
+    uint32_t d, m;
+    int s;
+    static FastDiv of(uint32_t d) {
+        int s = 0;
+        while ((1ull << s) < d) ++s;
+        return {d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s};
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t x) const { return (__umulhi(m, x) + x) >> s; }
+    __device__ __forceinline__ uint32_t mod(uint32_t x) const { return x - div(x) * d; }
+};
 
 struct ExtendArgs {
     int B, Sq, page_size, max_pages, num_pages;
+    FastDiv by_page, by_sq;
     const int* new_lens;
     const int* seq_lens;
     const int* free_state;   // {head, count}
@@ -46,40 +83,66 @@ struct ExtendArgs {
     int* granted;
     int64_t* positions;
     int64_t* slots;
-    int4* info;              // [B + 1]: the requests' four numbers, then {head, count, 0, 0}
+    int4* info;              // [B + 1]: the requests' four numbers, then {head, count, long runs, 0}
 };
 
-__device__ __forceinline__ int extend_pages(int tokens, int page_size) {
-    return tokens / page_size + (tokens % page_size != 0);
+__device__ __forceinline__ int extend_pages(const ExtendArgs& a, int tokens) {
+    const uint32_t q = a.by_page.div((uint32_t)tokens);
+    return (int)(q + (q * a.by_page.d != (uint32_t)tokens));
+}
+// Place `at` places past the ring's head (at < 2 num_pages <= 2^31).
+__device__ __forceinline__ int ring_place(const ExtendArgs& a, int head, int at) {
+    uint32_t p = (uint32_t)head + (uint32_t)at;
+    if (p >= (uint32_t)a.num_pages) p -= (uint32_t)a.num_pages;
+    return (int)(p >= (uint32_t)a.num_pages ? p - (uint32_t)a.num_pages : p);
 }
 
-// The part that follows from `info` (in LDS or memory), by `threads` threads of which this is
-// number `t`: a wave per request for its pages, a thread per position.
+// The part that follows from `info` (in LDS or memory), by `threads` threads of which this is number
+// `t`: a thread for each request's first page in or out, a wave for the pages behind it where a
+// request has any (`runs`), a thread for each position.
 __device__ __forceinline__ void extend_fill(const ExtendArgs& a, const int4* info, int head, int count,
-                                            int t, int threads) {
-    const uint32_t N = (uint32_t)a.num_pages;   // head, count <= N <= 2^30: the sums below fit
-    const int lane = t & 63;
-    for (int b = t >> 6; b < a.B; b += threads >> 6) {
+                                            int runs, int t, int threads) {
+    // pages k0, k0 + step, .. of request b's move, kRun of them together: free pages into the table, or
+    // table entries to the ring, as far as there are places behind the tail (else they are in the ring)
+    auto move = [&](int b, int k0, int step, auto run) __attribute__((always_inline)) {
+        constexpr int kRun = decltype(run)::value;
         const int4 r = info[b];
-        const int have = extend_pages(r.x, a.page_size), end = extend_pages(r.x + r.y, a.page_size);
+        const int have = extend_pages(a, r.x), end = extend_pages(a, r.x + r.y);
         int* row = a.table + (int64_t)b * a.max_pages;
-        for (int j = have + lane; j < end; j += 64) row[j] = a.ring[(uint32_t)(head + r.z + j - have) % N];
-        // past `room` there is no place left behind the tail: a page that is in the ring already
-        const int room = (int)N - count - r.w;
-        for (int j = end + lane; j < have && j - end < room; j += 64)
-            a.ring[((uint32_t)head + (uint32_t)count + (uint32_t)(r.w + j - end)) % N] = row[j];
-    }
+        const bool in = have < end;
+        const int n = in ? end - have : min(have - end, a.num_pages - count - r.w);
+        const int from = in ? r.z : count + r.w;   // past the ring's head
+        row += in ? have : end;
+        for (int k = k0; k < n; k += kRun * step) {
+            int page[kRun];
+            #pragma unroll
+            for (int i = 0; i < kRun; ++i) {
+                const int m = min(k + i * step, n - 1);
+                page[i] = in ? a.ring[ring_place(a, head, from + m)] : row[m];
+            }
+            #pragma unroll
+            for (int i = 0; i < kRun; ++i) {
+                const int m = k + i * step;
+                if (m < n) (in ? row[m] : a.ring[ring_place(a, head, from + m)]) = page[i];
+            }
+            if (step == 0) break;
+        }
+    };
+    for (int b = t; b < a.B; b += threads) move(b, 0, 0, std::integral_constant<int, 1>{});
+    if (runs)
+        for (int b = t >> 6; b < a.B; b += threads >> 6)
+            move(b, 1 + (t & 63), 64, std::integral_constant<int, 4>{});
     const int total = a.B * a.Sq;
     for (int i = t; i < total; i += threads) {
-        const int b = i / a.Sq, s = i - b * a.Sq;
+        const int b = (int)a.by_sq.div((uint32_t)i), s = i - b * a.Sq;
         const int4 r = info[b];
         int64_t pos = -1, slot = -1;
         if (s >= a.Sq - r.y) {
-            const int p = r.x + r.y - a.Sq + s, j = p / a.page_size, have = extend_pages(r.x, a.page_size);
+            const int p = r.x + r.y - a.Sq + s, j = (int)a.by_page.div((uint32_t)p), have = extend_pages(a, r.x);
             const int page = j < have ? a.table[(int64_t)b * a.max_pages + j]
-                                      : a.ring[(uint32_t)(head + r.z + j - have) % N];
+                                      : a.ring[ring_place(a, head, r.z + j - have)];
             pos = p;
-            slot = (int64_t)page * a.page_size + p % a.page_size;
+            slot = (int64_t)page * a.page_size + (p - j * a.page_size);
         }
         a.positions[i] = pos;
         a.slots[i] = slot;
@@ -89,79 +152,83 @@ __device__ __forceinline__ void extend_fill(const ExtendArgs& a, const int4* inf
 // ONE: `info` stays in LDS (B <= kExtendThreads) and this workgroup does the rest too.
 template <bool ONE>
 __global__ void __launch_bounds__(kExtendThreads) cache_extend_kernel(ExtendArgs a) {
-    __shared__ int w_ask[kExtendWaves], w_back[kExtendWaves], w_take[kExtendWaves];
+    __shared__ int w_ask[kExtendWaves], w_back[kExtendWaves], w_take[kExtendWaves], w_runs[kExtendWaves];
     __shared__ int4 info_lds[ONE ? kExtendThreads : 1];
     int4* info = ONE ? info_lds : a.info;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int threads = blockDim.x, waves = threads >> 6;
     const int N = a.num_pages, span = a.max_pages * a.page_size;
-    int head = a.free_state[0] % N;
-    if (head < 0) head += N;
-    const int count = min(max(a.free_state[1], 0), N);
-    const int per = (a.B + kExtendThreads - 1) / kExtendThreads;
+    const int per = (a.B + threads - 1) / threads;   // ONE: 1
     const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
     // pages asked for by a request that its own limits allow, and given back by one that shrinks
-    auto plan = [&](int b, int* L, int* n, int* ask, int* back) __attribute__((always_inline)) {
-        *L = min(max(a.seq_lens[b], 0), span);
-        *n = a.new_lens[b];
-        *ask = *back = 0;
-        const int have = extend_pages(*L, a.page_size);
-        if (*n > 0) {
-            if (*n > a.Sq || *n > span - *L) *n = 0;
-            else *ask = extend_pages(*L + *n, a.page_size) - have;
+    struct Plan { int L, n, ask, back; };
+    auto plan = [&](int b) __attribute__((always_inline)) {
+        Plan p = {min(max(a.seq_lens[b], 0), span), a.new_lens[b], 0, 0};
+        const int have = extend_pages(a, p.L);
+        if (p.n > 0) {
+            if (p.n > a.Sq || p.n > span - p.L) p.n = 0;
+            else p.ask = extend_pages(a, p.L + p.n) - have;
         } else {
-            *n = max(*n, -*L);
-            *back = have - extend_pages(*L + *n, a.page_size);
+            p.n = max(p.n, -p.L);
+            p.back = have - extend_pages(a, p.L + p.n);
         }
+        return p;
     };
+    const int head_in = a.free_state[0], count_in = a.free_state[1];
+    Plan own = {0, 0, 0, 0};   // of request b0, where the thread has one alone
     int ask = 0, back = 0;
     for (int b = b0; b < b1; ++b) {
-        int L, n, k, r;
-        plan(b, &L, &n, &k, &r);
-        ask += k;
-        back += r;
+        own = plan(b);
+        ask += own.ask;
+        back += own.back;
     }
-    int ia = ask, ib = back;   // inclusive scans within the wave, then the waves before
-    for (int d = 1; d < 64; d <<= 1) {
-        const int x = __shfl_up(ia, d), y = __shfl_up(ib, d);
-        if (lane >= d) { ia += x; ib += y; }
-    }
+    const int ia = lanes_sum_scan(ask), ib = lanes_sum_scan(back);
     if (lane == 63) { w_ask[wave] = ia; w_back[wave] = ib; }
     __syncthreads();
+    int head = head_in % N;
+    if (head < 0) head += N;
+    const int count = min(max(count_in, 0), N);
     int asked = ia - ask, pushed = ib - back, all_back = 0;
-    for (int w = 0; w < kExtendWaves; ++w) {
+    for (int w = 0; w < waves; ++w) {
         if (w < wave) { asked += w_ask[w]; pushed += w_back[w]; }
         all_back += w_back[w];
     }
     int taken = 0;   // pages taken by the requests up to this thread's last granted one
+    bool runs = false;
     for (int b = b0; b < b1; ++b) {
-        int L, n, k, r;
-        plan(b, &L, &n, &k, &r);
+        Plan p = per == 1 ? own : plan(b);
         const int first = asked;
-        asked += k;
-        if (k > 0) {
+        asked += p.ask;
+        if (p.ask > 0) {
             if (asked <= count) taken = asked;
-            else n = 0;
+            else p.n = 0;
         }
-        info[b] = make_int4(L, n, first, pushed);
-        pushed += r;
-        a.lens_out[b] = L + n;
-        a.granted[b] = n;
+        runs |= max(p.ask, p.back) > 1;
+        info[b] = make_int4(p.L, p.n, first, pushed);
+        pushed += p.back;
+        a.lens_out[b] = p.L + p.n;
+        a.granted[b] = p.n;
     }
-    for (int d = 32; d > 0; d >>= 1) taken = max(taken, __shfl_xor(taken, d));
-    if (lane == 0) w_take[wave] = taken;
+    const int most = lanes_max(taken);
+    const int any = __builtin_amdgcn_ballot_w64(runs) != 0;
+    if (lane == 0) { w_take[wave] = most; w_runs[wave] = any; }
     __syncthreads();
-    for (int w = 0; w < kExtendWaves; ++w) taken = max(taken, w_take[w]);
-    if (tid == 0) {
-        a.state_out[0] = (int)(((uint32_t)head + (uint32_t)taken) % (uint32_t)N);
-        a.state_out[1] = count - taken + min(all_back, N - count);
-        if (!ONE) info[a.B] = make_int4(head, count, 0, 0);
+    int all_runs = 0;
+    for (int w = 0; w < waves; ++w) {
+        taken = max(taken, w_take[w]);
+        all_runs |= w_runs[w];
     }
-    if (ONE) extend_fill(a, info, head, count, tid, kExtendThreads);
+    if (tid == 0) {
+        a.state_out[0] = ring_place(a, head, taken);
+        a.state_out[1] = count - taken + min(all_back, N - count);
+        if (!ONE) info[a.B] = make_int4(head, count, all_runs, 0);
+    }
+    if (ONE) extend_fill(a, info, head, count, all_runs, tid, threads);
 }
 
 __global__ void __launch_bounds__(256) cache_extend_fill_kernel(ExtendArgs a) {
     const int4 s = a.info[a.B];
-    extend_fill(a, a.info, s.x, s.y, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    extend_fill(a, a.info, s.x, s.y, s.z, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ---- append ---------------------------------------------------------------------------------
@@ -485,7 +552,12 @@ __global__ void __launch_bounds__(256) kv_read_blk_kernel(ReadBlkArgs a) {
 // Up to this many positions one workgroup does everything; past it a second, wide launch fills.
 constexpr int kExtendOneFill = 8192;
 
-size_t cache_extend_workspace(int B) { return ((size_t)B + 1) * sizeof(int4); }
+static bool extend_in_one(int B, int Sq) {
+    return B <= kExtendThreads && (int64_t)B * Sq <= kExtendOneFill;
+}
+size_t cache_extend_workspace(int B, int Sq) {
+    return extend_in_one(B, Sq) ? 0 : ((size_t)B + 1) * sizeof(int4);
+}
 
 hipError_t launch_cache_extend(const CacheExtend& p, void* workspace, hipStream_t stream) {
     ExtendArgs a;
@@ -495,8 +567,12 @@ hipError_t launch_cache_extend(const CacheExtend& p, void* workspace, hipStream_
     a.lens_out = p.seq_lens_out; a.state_out = p.free_state_out; a.granted = p.granted;
     a.positions = p.positions; a.slots = p.slots;
     a.info = static_cast<int4*>(workspace);
-    if (p.B <= kExtendThreads && (int64_t)p.B * p.Sq <= kExtendOneFill) {
-        hipLaunchKernelGGL(cache_extend_kernel<true>, dim3(1), dim3(kExtendThreads), 0, stream, a);
+    a.by_page = FastDiv::of((uint32_t)p.page_size);
+    a.by_sq = FastDiv::of((uint32_t)p.Sq);
+    if (extend_in_one(p.B, p.Sq)) {
+        // fewer waves, and with them a shorter way through the barriers, where they have work enough
+        const int threads = p.B <= 32 && p.B * p.Sq <= 256 ? 256 : kExtendThreads;
+        hipLaunchKernelGGL(cache_extend_kernel<true>, dim3(1), dim3(threads), 0, stream, a);
         return hipGetLastError();
     }
     hipLaunchKernelGGL(cache_extend_kernel<false>, dim3(1), dim3(kExtendThreads), 0, stream, a);

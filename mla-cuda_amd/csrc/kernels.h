@@ -188,7 +188,7 @@ struct CacheExtend {
     int64_t* positions = nullptr;      // [B, Sq]
     int64_t* slots = nullptr;          // [B, Sq]
 };
-size_t cache_extend_workspace(int B);
+size_t cache_extend_workspace(int B, int Sq);   // 0 where one launch does it all
 hipError_t launch_cache_extend(const CacheExtend& p, void* workspace, hipStream_t stream);
 // KV append, as launch_kv_append's paged form, coded by blocks: the new_lens[b] last tokens of
 // sequence b (seq_lens[b] long with them) are the last of its Sq rows of `in`.

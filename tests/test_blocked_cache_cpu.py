@@ -59,7 +59,8 @@ EXTEND = dict(batch=2, sq=1, page_size=64, max_pages=4, num_pages=8, new_lens=P1
     (dict(batch=1 << 20, max_pages=1 << 12), INVALID, "2^31"),
     *[({k: None}, INVALID, k) for k, v in EXTEND.items() if v is P16 and k != "workspace"],
     *[({k: ODD}, INVALID, k) for k, v in EXTEND.items() if v is P16 and k != "workspace"],
-    (dict(workspace=None), WORKSPACE, "workspace"), (dict(workspace_bytes=ctypes.c_size_t(47)), WORKSPACE, "small"),
+    (dict(batch=2000, workspace=None), WORKSPACE, "workspace"),
+    (dict(sq=5000, workspace_bytes=ctypes.c_size_t(47)), WORKSPACE, "small"),
 ])
 def test_extend_refuses(lib, change, status, word):
     assert lib.mla_cache_extend(*{**EXTEND, **change}.values()) == status
@@ -135,8 +136,10 @@ def test_attention_refuses(lib, change, status, word):
 
 
 def test_workspace_queries(lib):
-    assert lib.mla_cache_extend_workspace_bytes(0) == 0
-    assert lib.mla_cache_extend_workspace_bytes(1) >= 32
+    assert lib.mla_cache_extend_workspace_bytes(0, 1) == lib.mla_cache_extend_workspace_bytes(1, 0) == 0
+    assert lib.mla_cache_extend_workspace_bytes(64, 8) == 0      # one launch, no workspace
+    assert lib.mla_cache_extend_workspace_bytes(2000, 1) >= 2001 * 16
+    assert lib.mla_cache_extend_workspace_bytes(1, 100000) >= 2 * 16
     d = dims(batch=8, sk=8192)
     q = lib.mla_attention_paged_fp8blk_workspace_bytes
     assert q(BF16, ctypes.byref(d), 0, 64) == q(F16, ctypes.byref(d), 0, 64) > 0

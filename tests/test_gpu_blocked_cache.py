@@ -171,8 +171,8 @@ def test_extend_in_place_state(ext, B, Sq):
     n, ln, t, r, st = (x.to(DEV) for x in (i32(new), i32(lens), table, ring, i32(state)))
     pos = torch.empty(B, Sq, dtype=torch.int64, device=DEV)
     slots = torch.empty_like(pos)
-    wsb = L.mla_cache_extend_workspace_bytes(B)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=DEV)
+    wsb = L.mla_cache_extend_workspace_bytes(B, Sq)
+    ws = torch.empty(max(wsb, 1), dtype=torch.uint8, device=DEV)
     st_code = L.mla_cache_extend(B, Sq, 64, 4, ring.numel(), ptr(n), ptr(ln), ptr(st), ptr(t), ptr(r), ptr(ln),
                                  ptr(st), ptr(n), ptr(pos), ptr(slots), ptr(ws), ctypes.c_size_t(wsb), stream())
     assert st_code == 0, L.mla_last_error()
