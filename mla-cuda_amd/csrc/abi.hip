@@ -1651,7 +1651,7 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
     fp.block_table = block_table;
     fp.page_size = page_size;
     fp.num_pages = num_pages;
-    if (out_list_ok(fp, L.flash)) {   // a few tokens: the chunks' merge inside 3d
+    if (out_list_ok(fp, L.flash)) {   // decode: the chunks' merge inside 3d
         float* part = at<float>(workspace, L.off_part);
         MLA_TRY_HIP(launch_flash(fp, L.flash, ctx, row_sum, part, stream, false),
                     "blocked fp8-cache attention launch");

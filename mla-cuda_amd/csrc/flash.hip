@@ -3089,6 +3089,160 @@ __global__ void __launch_bounds__(512) out_list_kernel(const float* __restrict__
             v2u{Half<TL>::pack2(d[0], d[1]), Half<TL>::pack2(d[2], d[3])};
 }
 
+// The same for more tokens: a workgroup takes a head and 128 output columns, and walks over its share
+// of the tokens, kOutTile at a time.
+//   Wave w multiplies output columns 16 w .. +15: its W_uv rows, all 512 depths, stay in registers, so
+//     W_uv is read once a workgroup (a workgroup a tile read it from L2 again and again: 200 tokens
+//     82 us with the pass against 57 for separate launches).
+//   Of a tile's tokens a wave merges two (a lane 8 columns of a row): their weights and first two
+//     chunks' rows were loaded while it multiplied the tile before (two tiles before gained nothing),
+//     further chunks come four at a time.
+//     The rows go to LDS in two 16-bit terms, hi in columns 0 .. 15, lo in 16 .. 31, and each of
+//     these two blocks is one MFMA a step.  Two tiles' columns alternate, so one barrier a tile is enough.
+// What bounds it is the phases' order (rows, barrier, product: about 3 us a tile) and W_uv's first read.
+// Launches of their own against it, with the pass (us): 9 sequences up to 9,000 keys 38.3 / 37.2, 16 up
+// to 8,192 43.6 / 41.4, 61 up to 4,989 73.9 / 72.5, 64 of up to 300 30.5 / 29.8, 128 up to 8,192 184.5 /
+// 186.0, 32 of 4 queries 57.3 / 59.8; past 128 tokens it loses (200: 57.4 / 66.5) and is not taken.  A row
+// in 16 bits between the launches is the third of the outputs' roundings (P, the row, the output):
+// without it they are 2.4e-3 instead of 2.9e-3 off in bf16, relative, in the 2-norm.
+constexpr int kOutTile = 16;
+template <typename TL>
+__global__ void __launch_bounds__(512, 1) out_merge_kernel(const float* __restrict__ o,
+                                                           const float* __restrict__ mp,
+                                                           const float* __restrict__ lp,
+                                                           const float* __restrict__ ctx,
+                                                           const float* __restrict__ row_sum,
+                                                           const int* __restrict__ wl,
+                                                           const uint16_t* __restrict__ W,
+                                                           uint16_t* __restrict__ out, int B, int Sq,
+                                                           int H, int V, int share) {
+    constexpr int kTok = kOutTile / 8;
+    __shared__ __attribute__((aligned(16))) uint8_t cols[2][2 * kOutTile * kOutListPitch];
+    const int vb = (V + 127) / 128, M = B * Sq, tiles = (M + kOutTile - 1) / kOutTile;
+    const int wg = xcd_logical_block(blockIdx.x, gridDim.x);
+    const int q0 = wg % share, c0 = wg / share % vb * 128, h = wg / share / vb;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rows_b = Sq * H;
+    // the wave's tokens of a tile: chunks, first row among the chunks' or (one chunk) among ctx's, the
+    // chunks' maxima and sums a lane each, the first two chunks' rows
+    int n[kTok];
+    int64_t row0[kTok];
+    float ms[kTok], ls[kTok];
+    v4f x[kTok][2][2];
+    auto row_at = [&](int i, int s) __attribute__((always_inline)) {   // the lane's 8 columns of chunk s
+        return reinterpret_cast<const v4f*>((n[i] == 1 ? ctx : o) +
+                                            (row0[i] + (int64_t)min(s, n[i] - 1) * rows_b) * kFR) + 2 * lane;
+    };
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        #pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+            const int t = min(kOutTile * tile + wave + 8 * i, M - 1), b = t / Sq;
+            n[i] = load_uniform(wl + kWlHead + B + b);
+            row0[i] = (int64_t)(n[i] == 1 ? b : load_uniform(wl + kWlHead + b)) * rows_b + (t - b * Sq) * H + h;
+        }
+        #pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+            const int64_t row = row0[i] + (int64_t)min(lane, n[i] - 1) * rows_b;
+            ms[i] = n[i] == 1 ? 0.f : mp[row];
+            ls[i] = (n[i] == 1 ? row_sum : lp)[row];
+            #pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const v4f* src = row_at(i, s);
+                x[i][s][0] = src[0];
+                x[i][s][1] = src[1];
+            }
+        }
+    };
+    fetch(q0);
+    v4u wr[kFR / 32];
+    {
+        const v4u* src = reinterpret_cast<const v4u*>(
+            W + ((int64_t)h * V + min(c0 + 16 * wave + l16, V - 1)) * kFR) + g;
+        #pragma unroll
+        for (int s = 0; s < kFR / 32; ++s) wr[s] = src[4 * s];
+    }
+    int buf = 0;
+    for (int tile = q0; tile < tiles; tile += share, buf ^= 1) {
+        #pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+            // (chunks past the 64 lanes': a lane takes every 64th)
+            float mx = lane < n[i] ? ms[i] : -INFINITY;
+            for (int s = lane + 64; s < n[i]; s += 64) mx = fmaxf(mx, mp[row0[i] + (int64_t)s * rows_b]);
+            mx = wave_reduce(mx, OpMax{});
+            auto weight = [&](float m) __attribute__((always_inline)) {
+                return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+            };
+            const float w_lane = lane < n[i] ? weight(ms[i]) : 0.f;
+            float L = w_lane * ls[i];
+            for (int s = lane + 64; s < n[i]; s += 64) {
+                const int64_t row = row0[i] + (int64_t)s * rows_b;
+                L += weight(mp[row]) * lp[row];
+            }
+            L = wave_reduce(L, OpSum{});
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            auto w_of = [&](int s) __attribute__((always_inline)) {
+                return s < 64 ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w_lane), s))
+                              : weight(mp[row0[i] + (int64_t)s * rows_b]);
+            };
+            v4f a = w_of(0) * x[i][0][0], b = w_of(0) * x[i][0][1];
+            if (n[i] > 1) {
+                const float w = w_of(1);
+                a += w * x[i][1][0];
+                b += w * x[i][1][1];
+            }
+            for (int s0 = 2; s0 < n[i]; s0 += 4) {
+                v4f y[4][2];
+                #pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const v4f* src = row_at(i, s0 + s);
+                    y[s][0] = src[0];
+                    y[s][1] = src[1];
+                }
+                #pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    if (s0 + s < n[i]) {
+                        const float w = w_of(s0 + s);
+                        a += w * y[s][0];
+                        b += w * y[s][1];
+                    }
+            }
+            a *= inv;
+            b *= inv;
+            using S = Half<TL>;
+            v4u hi, lo;
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float p = k < 2 ? a[2 * k] : b[2 * k - 4], q = k < 2 ? a[2 * k + 1] : b[2 * k - 3];
+                hi[k] = S::pack2(p, q);
+                lo[k] = S::pack2(p - S::to_f32(hi[k] & 0xffffu), q - S::to_f32(hi[k] >> 16));
+            }
+            *reinterpret_cast<v4u*>(cols[buf] + (wave + 8 * i) * kOutListPitch + 16 * lane) = hi;
+            *reinterpret_cast<v4u*>(cols[buf] + (kOutTile + wave + 8 * i) * kOutListPitch + 16 * lane) = lo;
+        }
+        if (tile + share < tiles) fetch(tile + share);
+        lds_barrier();
+        v4f d[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+        #pragma unroll
+        for (int s = 0; s < kFR / 32; ++s)
+            #pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const v4u c = *reinterpret_cast<const v4u*>(cols[buf] + (16 * k + l16) * kOutListPitch + 64 * s + 16 * g);
+                if constexpr (Half<TL>::kF16)
+                    d[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, wr[s]),
+                                                                  __builtin_bit_cast(v8h, c), d[k], 0, 0, 0);
+                else
+                    d[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, wr[s]),
+                                                                   __builtin_bit_cast(v8bf, c), d[k], 0, 0, 0);
+            }
+        const v4f r = d[0] + d[1];
+        const int v = c0 + 16 * wave + 4 * g, t = kOutTile * tile + l16;
+        if (v < V && t < M)
+            *reinterpret_cast<v2u*>(out + ((int64_t)t * H + h) * V + v) =
+                v2u{Half<TL>::pack2(r[0], r[1]), Half<TL>::pack2(r[2], r[3])};
+    }
+}
+
 // Work list of a ragged batch (one workgroup; key counts are device data).  The chunk rule,
 // the fit check, each batch's chunk counts and the order of the items are the functions of
 // worklist.h; this kernel spreads them over its threads (thread tid owns batches
@@ -3358,31 +3512,50 @@ FlashPlan plan_flash(const FlashProblem& p) {
     return f;
 }
 
-bool out_list_ok(const FlashProblem& p, const FlashPlan& f) {
+// which of the kernels above: 0 neither, 1 out_list_kernel, 2 out_merge_kernel
+static int out_list_kind(const FlashProblem& p, const FlashPlan& f) {
     // MLA_OUT_SMALL=0: the merge and 3d launches of their own
     const char* env = std::getenv("MLA_OUT_SMALL");
-    return p.scale_block && f.balanced && p.B * p.Sq <= kOutListTokens && p.R == kFR &&
-           p.Sq * f.max_items <= kOutListRows && !(env && env[0] == '0');
+    if (!p.scale_block || !f.balanced || p.R != kFR || (env && env[0] == '0')) return 0;
+    const int64_t M = (int64_t)p.B * p.Sq;
+    if (M <= kOutListTokens && p.Sq * f.max_items <= kOutListRows) return 1;
+    return M <= kOutMergeTokens ? 2 : 0;
 }
+bool out_list_ok(const FlashProblem& p, const FlashPlan& f) { return out_list_kind(p, f) > 0; }
 
 hipError_t launch_out_list(const FlashProblem& p, const FlashPlan& f, const float* ctx,
                            const float* row_sum, const float* partials, const void* W_uv, void* out,
                            int V, hipStream_t stream) {
-    if (!out_list_ok(p, f) || V <= 0) return hipErrorInvalidValue;
+    const int kind = out_list_kind(p, f);
+    if (kind == 0 || V <= 0) return hipErrorInvalidValue;
     const size_t rows_b = (size_t)p.Sq * p.H;
     const size_t wl_bytes = ((size_t)wl_ints(p.B, f.max_items) * sizeof(int) + 255) / 256 * 256;
     const float* o = reinterpret_cast<const float*>(reinterpret_cast<const char*>(partials) + wl_bytes);
     const float* m = o + (size_t)f.max_items * rows_b * kFR;
     const float* l = m + (size_t)f.max_items * rows_b;
     const int* wl = reinterpret_cast<const int*>(partials);
-    const dim3 grid((unsigned)(p.H * ((V + 63) / 64))), block(512);
     const uint16_t* W = static_cast<const uint16_t*>(W_uv);
+    uint16_t* dst = static_cast<uint16_t*>(out);
+    if (kind == 1) {
+        const dim3 grid((unsigned)(p.H * ((V + 63) / 64)));
+        if (p.f16)
+            hipLaunchKernelGGL(out_list_kernel<f16_t>, grid, dim3(512), 0, stream, o, m, l, ctx, row_sum, wl, W,
+                               dst, p.B, p.Sq, p.H, V);
+        else
+            hipLaunchKernelGGL(out_list_kernel<bf16_t>, grid, dim3(512), 0, stream, o, m, l, ctx, row_sum, wl, W,
+                               dst, p.B, p.Sq, p.H, V);
+        return hipGetLastError();
+    }
+    // one workgroup a CU (a second would read W_uv again: 4 us more at 128 tokens), or a tile each
+    const int heads = p.H * ((V + 127) / 128), tiles = (p.B * p.Sq + kOutTile - 1) / kOutTile;
+    const int share = std::max(1, std::min(tiles, kNumCUs / heads));
+    const dim3 grid((unsigned)(heads * share));
     if (p.f16)
-        hipLaunchKernelGGL(out_list_kernel<f16_t>, grid, block, 0, stream, o, m, l, ctx, row_sum, wl, W,
-                           static_cast<uint16_t*>(out), p.B, p.Sq, p.H, V);
+        hipLaunchKernelGGL(out_merge_kernel<f16_t>, grid, dim3(512), 0, stream, o, m, l, ctx, row_sum, wl, W, dst,
+                           p.B, p.Sq, p.H, V, share);
     else
-        hipLaunchKernelGGL(out_list_kernel<bf16_t>, grid, block, 0, stream, o, m, l, ctx, row_sum, wl, W,
-                           static_cast<uint16_t*>(out), p.B, p.Sq, p.H, V);
+        hipLaunchKernelGGL(out_merge_kernel<bf16_t>, grid, dim3(512), 0, stream, o, m, l, ctx, row_sum, wl, W, dst,
+                           p.B, p.Sq, p.H, V, share);
     return hipGetLastError();
 }
 

@@ -326,10 +326,11 @@ constexpr int kOutSmallMergeM = 4;
 hipError_t launch_out_small(const FlashPartials& fp, const float* ctx, const float* row_sum,
                             const float* W_uv, float* out, int B, int Sq, int H, int R, int V,
                             hipStream_t stream);
-// 3d of a few 16-bit tokens (B * Sq <= kOutListTokens, R = 512) straight from a list's state
-// (launch_flash with merge = false and no ctx16): the merge of each token's chunks and the product with
-// W_uv in one kernel, the merged row in fp32 throughout.  out_list_ok: by the shape and the plan.
-constexpr int kOutListTokens = 8;
+// 3d of up to kOutMergeTokens 16-bit tokens (B * Sq; R = 512) straight from a list's state (launch_flash
+// with merge = false and no ctx16): the merge of each token's chunks and the product with W_uv in one
+// kernel (up to kOutListTokens: one for few tokens), the merged row in two 16-bit terms.
+// out_list_ok: by the shape and the plan.
+constexpr int kOutListTokens = 8, kOutMergeTokens = 128;
 bool out_list_ok(const FlashProblem& p, const FlashPlan& plan);
 hipError_t launch_out_list(const FlashProblem& p, const FlashPlan& plan, const float* ctx,
                            const float* row_sum, const float* partials, const void* W_uv, void* out,

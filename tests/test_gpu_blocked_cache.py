@@ -779,3 +779,21 @@ def test_attention_few_tokens(ext, monkeypatch, dt, B, Sq, H, V):
     monkeypatch.setenv("MLA_OUT_SMALL", "0")
     two = attend(ext, qa, qr, w, cache, table, lens, Sq > 1)
     check_attention(two, ref, DT[dt], True)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Sq,H,V,Sk", [(9, 1, 4, 128, 20000), (13, 1, 128, 128, 2000), (17, 2, 128, 132, 700),
+                                         (64, 2, 16, 64, 300), (11, 9, 3, 260, 900), (128, 1, 128, 128, 400),
+                                         (129, 1, 128, 128, 200)])
+def test_attention_decode_batches(ext, monkeypatch, dt, B, Sq, H, V, Sk):
+    """9 to 128 tokens: the chunks' merge runs inside 3d, a tile of tokens at a time (past 64 chunks a
+    sequence, odd tiles, columns past a block of 128), and one token past it."""
+    g = torch.Generator().manual_seed(B * 10 + Sq)
+    lens = [Sk] + torch.randint(0, min(Sk, 700), (B - 1,), generator=g).tolist()
+    lens[B // 2] = 0
+    qa, qr, w, cache, table = attention_case(lens, Sq, 64, 64, DT[dt], B, H=H, V=V)
+    rows = [torch.nan_to_num(r) for r in K.decode(cache)]
+    ref = K.attention(qa, qr, rows, table, lens, w, SCALE, Sq > 1, 64, cache["c_kv"].size(0))
+    check_attention(attend(ext, qa, qr, w, cache, table, lens, Sq > 1), ref, DT[dt], True)
+    monkeypatch.setenv("MLA_OUT_SMALL", "0")
+    check_attention(attend(ext, qa, qr, w, cache, table, lens, Sq > 1), ref, DT[dt], True)
