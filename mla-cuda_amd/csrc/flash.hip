@@ -1417,6 +1417,27 @@ __device__ __forceinline__ v4u fp8x8(v2u r, float scale) {
     return v4u{two(r[0], lo), two(r[0], hi), two(r[1], lo), two(r[1], hi)};
 }
 
+// A NaN in a key that some of a tile's queries do not see would reach them through P.V, where their P
+// is 0: 0 * NaN.  Queries that do see it have it from their scores, since the latent row is key and
+// value, so V may do without: a P.V wave writes zeros over the NaN codes (0x7F, 0xFF) of its 128
+// columns of a block, whose K has been read by then.  (A causal block that ends past the first row's
+// last key, and in it a NaN score at a hidden place: the score waves note such blocks.)
+__device__ __forceinline__ void f8_zero_nan(uint8_t* stage, int cq, int lane) {
+    const int key = lane >> 1;
+    uint8_t* row = stage + key * k8LatBytes + 256 * (cq >> 1);
+    #pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        v4u* p = reinterpret_cast<v4u*>(row + 16 * ((8 * (cq & 1) + 4 * (lane & 1) + m) ^ swz(key & 15)));
+        v4u w = *p;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t top = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // bit 7 of each NaN
+            w[i] &= ~(top | (top - (top >> 7)));
+        }
+        *p = w;
+    }
+}
+
 // BS: a scale for each block of tokens and part (paged, bf16 or fp16 queries).  The conversions
 // take a power-of-two scale for nothing, and the 16 keys of a K fragment, or of a V^T fragment's
 // key half, share theirs (blocks are 16, 32 or 64 tokens), so the operands hold the values
@@ -1440,6 +1461,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     float* xref = reinterpret_cast<float*>(smem + kXBase);      // [rt][kh][32 rows]
     float* xl = xref + 128;                                     // [rt][kh][32 rows]
     int* flags = reinterpret_cast<int*>(xl + 128);              // [score wave]
+    int* hidden_nan = flags + 8;                                // BS: [block & 1], the block + 1
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4, l32 = lane & 31, hw = lane >> 5;
@@ -1546,6 +1568,15 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                     const int kq0 = k_lo + k2Keys * j + 16 * kh;
                     if (kq0 + 15 > lim_wave) {
                         const int kq = kq0 + 4 * g;
+                        if constexpr (BS) {
+                            // a hidden key with a NaN: the P.V waves take it out of the block's V
+                            bool nan = false;
+                            #pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                nan |= (kq + i > lim0 && sc[0][i] != sc[0][i]) ||
+                                       (kq + i > lim1 && sc[1][i] != sc[1][i]);
+                            if (__builtin_amdgcn_ballot_w64(nan) && lane == 0) hidden_nan[j & 1] = j + 1;
+                        }
                         #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             sc[0][i] = kq + i <= lim0 ? sc[0][i] : -INFINITY;
@@ -1740,6 +1771,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
             dma16(rr, qp + q * 1024,
                   (row0 + 8 * q + (lane >> 3)) * kPeBytes + 16u * ((lane & 7) ^ ((4 * q + (lane >> 4)) & 7)));
     }
+    const int lim_first = skb - a.Sq + r0 / a.H;   // the last key that the tile's first row sees
     v16f O[8];
     for (int pass = 1;; ++pass) {
         #pragma unroll
@@ -1765,6 +1797,8 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
             {
                 asm volatile("" : "+v"(vb0[0]), "+v"(vb0[1]));
                 const uint32_t sbase = (uint32_t)((j - 1) % k8NS) * k8Stage;
+                if (BS && a.causal && k_lo + k2Keys * j - 1 > lim_first && hidden_nan[(j - 1) & 1] == j)
+                    f8_zero_nan(smem + sbase, cq, lane);
                 const uint32_t prs = pr0 + (uint32_t)((j - 1) & 1) * kXPStage;
                 v4u pf[2][2];
                 #pragma unroll

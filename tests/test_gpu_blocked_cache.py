@@ -501,6 +501,26 @@ def test_attention_fewer_keys_than_queries(ext, dt):
             check_attention(out[b:b + 1, Sq - n:], ref[b:b + 1, Sq - n:], DT[dt], True)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("Sq,H,lens,at", [(4, 128, [300, 33, 4], 2), (4, 16, [64, 700, 4], 1), (40, 3, [40, 100, 2000], 17),
+                                          (33, 128, [500, 33, 64], 32), (7, 200, [90, 7, 4000], 0)])
+def test_attention_hidden_nan(ext, monkeypatch, dt, Sq, H, lens, at):
+    """A NaN in a token's row (latent, or rope alone): the queries in front of it keep their bits, it
+    and the ones behind it are NaN."""
+    qa, qr, w, cache, table = attention_case(lens, Sq, 32, 64, DT[dt], Sq, H=H)
+    for fused in ("0", "1"):
+        monkeypatch.setenv("MLA_OUT_SMALL", fused)
+        clean = attend(ext, qa, qr, w, cache, table, lens, True)
+        for name, column in (("c_kv", 77), ("c_kv", 500), ("pe", 9)):
+            bad = {k: v.clone() for k, v in cache.items()}
+            for b, n in enumerate(lens):
+                slot = int(K.slots_of(table, b, n - Sq + at, n - Sq + at + 1, 64)[0])
+                bad[name].view(-1, bad[name].size(2))[slot, column] = 0xFF if b else 0x7F
+            out = attend(ext, qa, qr, w, bad, table, lens, True)
+            assert torch.equal(out[:, :at], clean[:, :at])
+            assert torch.isnan(out[:, at:]).all()
+
+
 @pytest.mark.parametrize("H,V", [(1, 4), (3, 128), (16, 64), (65, 132), (200, 128)])
 def test_attention_heads(ext, H, V):
     lens = [100, 300, 9]
