@@ -373,7 +373,8 @@ int mla_kv_append_paged(mla_dtype_t dtype, const mla_dims_t* dims, const void* x
  * with value = code * 2^(byte - 127).  The bytes of blocks that hold keys are 1 .. 254; the pool
  * may hold anything where no sequence has a key.  scale_block is 16, 32 or 64, page_size a
  * positive multiple of 64, kv_rank 512 and rope 64 (MLA_ERR_UNSUPPORTED otherwise).
- * block_table [B, max_pages] as above; a table entry outside [0, num_pages) is never followed. */
+ * block_table [B, max_pages] as above; a table entry outside [0, num_pages) is never followed.
+ * scales may start at any even address (one layer's pairs of a larger tensor). */
 
 /* Block tables, positions and slots from request lengths, for a batch of `batch` requests of up
  * to `sq` new tokens each over a pool of num_pages pages (any cache format).  Request b holds

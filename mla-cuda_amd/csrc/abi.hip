@@ -785,6 +785,14 @@ int run_kv_product(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, con
     return ok();
 }
 
+// Scale bytes are read by the byte, their pairs kept together: one layer's of a larger tensor may
+// start at any even address.
+int check_scale_ptr(const void* p) {
+    if (!p) return fail(MLA_ERR_INVALID_ARGUMENT, "scales must not be NULL");
+    if (reinterpret_cast<uintptr_t>(p) & 1u)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "scales must be 2-byte aligned");
+    return MLA_OK;
+}
 // The blocked 8-bit pools: their pages and scale blocks, and with dims the widths and the table.
 int check_blocked_pool(int32_t page_size, int32_t num_pages, int32_t scale_block) {
     if (page_size <= 0 || page_size % 64 != 0)
@@ -1574,7 +1582,7 @@ int mla_kv_append_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
     MLA_CHECK(check_ptr(block_table, "block_table"));
     MLA_CHECK(check_ptr(c_kv_pages, "c_kv_pages"));
     MLA_CHECK(check_ptr(pe_pages, "pe_pages"));
-    MLA_CHECK(check_ptr(scales, "scales"));
+    MLA_CHECK(check_scale_ptr(scales));
     if (!(eps >= 0.0) || !std::isfinite(eps))
         return fail(MLA_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
     GemmPlan plan;
@@ -1606,7 +1614,7 @@ int mla_kv_read_fp8blk(mla_dtype_t dtype, const int64_t* slots, int64_t n,
     MLA_CHECK(check_ptr(slots, "slots"));
     MLA_CHECK(check_ptr(c_kv_pages, "c_kv_pages"));
     MLA_CHECK(check_ptr(pe_pages, "pe_pages"));
-    MLA_CHECK(check_ptr(scales, "scales"));
+    MLA_CHECK(check_scale_ptr(scales));
     MLA_CHECK(check_ptr(latent, "latent"));
     MLA_CHECK(check_ptr(rope, "rope"));
     KvReadBlk p;
@@ -1636,7 +1644,7 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
     MLA_CHECK(check_ptr(q_rope, "q_rope"));
     MLA_CHECK(check_ptr(c_kv_pages, "c_kv_pages"));
     MLA_CHECK(check_ptr(pe_pages, "pe_pages"));
-    MLA_CHECK(check_ptr(scales, "scales"));
+    MLA_CHECK(check_scale_ptr(scales));
     MLA_CHECK(check_ptr(block_table, "block_table"));
     MLA_CHECK(check_ptr(seq_lens, "seq_lens"));
     MLA_CHECK(check_ptr(W_uv, "W_uv"));

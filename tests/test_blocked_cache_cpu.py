@@ -20,6 +20,7 @@ OK, INVALID, UNSUPPORTED, WORKSPACE, HIP = range(5)
 F32, BF16, F16, F64 = range(4)
 P16 = ctypes.c_void_p(1 << 20)          # aligned, never dereferenced
 ODD = ctypes.c_void_p((1 << 20) + 4)
+BYTE = ctypes.c_void_p((1 << 20) + 1)
 BIG = ctypes.c_size_t(1 << 40)
 
 
@@ -81,7 +82,7 @@ APPEND = dict(dtype=BF16, dims=None, x=P16, W_kv_a=P16, kv_norm_w=P16, inv_freq=
     (dict(scale_block=48), UNSUPPORTED, "scale_block"), (dict(scale_block=128), UNSUPPORTED, "scale_block"),
     (dict(eps=ctypes.c_double(-1.0)), INVALID, "eps"), (dict(eps=ctypes.c_double(math.nan)), INVALID, "eps"),
     *[({k: None}, INVALID, k) for k, v in APPEND.items() if v is P16 and k != "workspace"],
-    (dict(c_kv_pages=ODD), INVALID, "aligned"), (dict(scales=ODD), INVALID, "aligned"),
+    (dict(c_kv_pages=ODD), INVALID, "aligned"), (dict(scales=BYTE), INVALID, "scales must be 2-byte aligned"),
     (dict(workspace_bytes=ctypes.c_size_t(16)), WORKSPACE, "small"),
 ])
 def test_append_refuses(lib, change, status, word):
@@ -100,7 +101,8 @@ READ = dict(dtype=BF16, slots=P16, n=ctypes.c_int64(5), c_kv_pages=P16, pe_pages
     (dict(page_size=65), INVALID, "page_size"), (dict(num_pages=-2), INVALID, "num_pages"),
     (dict(scale_block=0), UNSUPPORTED, "scale_block"),
     *[({k: None}, INVALID, k) for k, v in READ.items() if v is P16],
-    *[({k: ODD}, INVALID, k) for k, v in READ.items() if v is P16],
+    *[({k: ODD}, INVALID, k) for k, v in READ.items() if v is P16 and k != "scales"],
+    (dict(scales=BYTE), INVALID, "scales must be 2-byte aligned"),
 ])
 def test_read_refuses(lib, change, status, word):
     assert lib.mla_kv_read_fp8blk(*{**READ, **change}.values()) == status
@@ -125,6 +127,7 @@ ATTEND = dict(dtype=BF16, dims=None, q_absorbed=P16, q_rope=P16, c_kv_pages=P16,
     (dict(page_size=0), INVALID, "page_size"), (dict(num_pages=0), INVALID, "num_pages"),
     (dict(scale_block=1), UNSUPPORTED, "scale_block"), (dict(scale=ctypes.c_double(0.0)), INVALID, "scale"),
     *[({k: None}, INVALID, k) for k, v in ATTEND.items() if v is P16 and k != "workspace"],
+    (dict(pe_pages=ODD), INVALID, "aligned"), (dict(scales=BYTE), INVALID, "scales must be 2-byte aligned"),
     (dict(workspace=None), WORKSPACE, "workspace"),
     (dict(workspace_bytes=ctypes.c_size_t(256)), WORKSPACE, "small"),
 ])

@@ -817,3 +817,84 @@ def test_attention_decode_batches(ext, monkeypatch, dt, B, Sq, H, V, Sk):
     check_attention(attend(ext, qa, qr, w, cache, table, lens, Sq > 1), ref, DT[dt], True)
     monkeypatch.setenv("MLA_OUT_SMALL", "0")
     check_attention(attend(ext, qa, qr, w, cache, table, lens, Sq > 1), ref, DT[dt], True)
+
+
+@pytest.mark.parametrize("layer", [1, 2])
+def test_one_layer_of_layered_pools(ext, layer):
+    """Pools of several layers in one tensor: a layer's scale bytes start at any even address (here 6
+    and 12 bytes in).  The same bits as pools of its own, and the other layers' bytes stay."""
+    lens, new, block, page = [100, 30], [70, 30], 64, 64
+    cache, x, W, gain, table = append_inputs(lens, new, 70, block, page, BF, 5, spare=0)
+    assert cache["scales"].numel() == 6
+    alone = to_gpu(cache)
+    stacked = {k: v.unsqueeze(0).repeat(3, *[1] * v.dim()).to(DEV) for k, v in cache.items()}
+    before = {k: v.cpu() for k, v in stacked.items()}
+    one = {k: v[layer] for k, v in stacked.items()}
+    qa, qr, w = (t.to(DEV) for t in K.queries(2, 1, 128, 128, torch.Generator().manual_seed(5), BF))
+    args = [t.to(DEV) for t in (x, W, gain, i32(lens), i32(new), table)]
+    outs = []
+    for c in (alone, one):
+        ext.kv_append_paged_fp8blk(*args, c["c_kv"], c["pe"], c["scales"], 1e-6)
+        outs.append([ext.mla_attention_paged_fp8blk(qa, qr, c["c_kv"], c["pe"], c["scales"], args[5], args[3], w,
+                                                    SCALE, False),
+                     *ext.kv_read_fp8blk(torch.arange(3 * page, device=DEV), c["c_kv"], c["pe"], c["scales"], BF)])
+    for got, want in zip(outs[1], outs[0]):
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+    for k, v in stacked.items():
+        assert torch.equal(v[layer], alone[k])
+        for other in {0, 1, 2} - {layer}:
+            assert torch.equal(v[other].cpu(), before[k][other])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_attention_unrounded_rows_past_128_tokens(ext, monkeypatch, dt):
+    """MLA_CTX16=0: the attention's rows in float32 between the pass and 3d, two roundings (P and the
+    output) instead of three."""
+    g = torch.Generator().manual_seed(129)
+    lens = torch.randint(0, 400, (43,), generator=g).tolist()
+    lens[0], lens[1] = 3000, 0
+    qa, qr, w, cache, table = attention_case(lens, 4, 32, 64, DT[dt], 129)
+    rows = [torch.nan_to_num(r) for r in K.decode(cache)]
+    ref = K.attention(qa, qr, rows, table, lens, w, SCALE, True, 64, cache["c_kv"].size(0))
+    check_attention(attend(ext, qa, qr, w, cache, table, lens, True), ref, DT[dt], True)
+    monkeypatch.setenv("MLA_CTX16", "0")
+    check_attention(attend(ext, qa, qr, w, cache, table, lens, True), ref, DT[dt], True)
+
+
+def test_steps_on_two_streams(ext):
+    """Two servers with pools of their own, a step each at once on two streams: the bits of one after
+    the other."""
+    B, Sq, page = 5, 4, 64
+    cases = []
+    for seed, new in ((40, [4, 3, 0, 4, 1]), (41, [1, 4, 4, 2, 3])):
+        g, W, gain, cache = serving_state(BF, seed=seed)
+        x = torch.randn(B, Sq, 256, generator=g).to(BF).to(DEV)
+        cases.append((W.to(DEV), gain.to(DEV), cache, x, [t.to(DEV) for t in K.queries(B, Sq, 128, 128, g, BF)],
+                      i32(new).to(DEV)))
+
+    def state(case):
+        return {"W": case[0], "gain": case[1], **to_gpu(case[2]), "lens": i32([0] * B).to(DEV),
+                "state": i32([3, 14]).to(DEV), "table": torch.full((B, 4), -1, dtype=torch.int32, device=DEV),
+                "ring": torch.arange(14, dtype=torch.int32, device=DEV)}
+
+    def steps(case, st):
+        outs = []
+        for _ in range(6):
+            out = serve(ext, st, case[5], case[3], *case[4], Sq, page)
+            st["lens"], st["state"] = out[0], out[1]
+            outs.append(out)
+        return outs
+
+    want = [steps(c, state(c)) for c in cases]
+    states = [state(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            got[i] = steps(cases[i], states[i])
+    torch.cuda.synchronize()
+    for w, o in zip(want, got):
+        for a, b in zip(w, o):
+            for x, y in zip(a, b):
+                assert torch.equal(torch.nan_to_num(x), torch.nan_to_num(y))
