@@ -821,6 +821,9 @@ int check_fp8blk_attn(mla_dtype_t dtype, const mla_dims_t* d, int causal, int32_
     if ((int64_t)d->sq * d->heads * d->kv_rank * 2 >= 0x7fffffff)
         return fail(MLA_ERR_UNSUPPORTED, "Sq * heads * kv_rank * 2 must be below 2^31 bytes (Sq %d, "
                     "heads %d)", d->sq, d->heads);
+    // and 3d within 32 tokens' outputs
+    if ((int64_t)d->heads * d->v >= (int64_t)1 << 25)
+        return fail(MLA_ERR_UNSUPPORTED, "heads * v must be below 2^25 (heads %d, v %d)", d->heads, d->v);
     return MLA_OK;
 }
 
@@ -1659,9 +1662,10 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
     fp.block_table = block_table;
     fp.page_size = page_size;
     fp.num_pages = num_pages;
-    if (out_list_ok(fp, L.flash)) {   // decode: the chunks' merge inside 3d
+    if (out_list_ok(fp, L.flash)) {   // the chunks' merge inside 3d, or (many tokens) packed rows
         float* part = at<float>(workspace, L.off_part);
-        MLA_TRY_HIP(launch_flash(fp, L.flash, ctx, row_sum, part, stream, false),
+        const bool rows = out_rows_ok(fp, L.flash);
+        MLA_TRY_HIP(launch_flash(fp, L.flash, ctx, row_sum, part, stream, rows, rows ? ctx : nullptr),
                     "blocked fp8-cache attention launch");
         MLA_TRY_HIP(launch_out_list(fp, L.flash, ctx, row_sum, part, W_uv, out, dims->v, stream),
                     "3d launch");

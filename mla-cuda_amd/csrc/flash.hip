@@ -85,6 +85,8 @@ struct FlashArgs {
     // already normalised and rounded to the storage format, (o_scale O) (1 / l) -- what
     // 3d's A staging forms from ctx and row_sum -- at ctx16[row][R]
     void* ctx16;
+    // (flash16x8_kernel<.., true>: packed rows (pv_pack_rows) at ctx16 if this is set, their scales here)
+    float* row_scale;
     // block scales of an fp8 cache (flash16x8_kernel<.., true>): E8M0 bytes
     // [num_pages, page_size >> scale_shift, 2], 1 << scale_shift tokens a block
     const uint8_t* scales;
@@ -836,6 +838,78 @@ __global__ void __launch_bounds__(kFThreads, 1) flash16_kernel(FlashArgs a) {
 //   256 bytes, the two halves of a chunk swapped in rows with bit 4 set: the writes of 32 rows
 //   and the reads touch all banks evenly.
 constexpr uint32_t kPvOutBytes = 64 * 512;
+
+// Packed rows: the same normalised rows for 3d of many tokens (out_rows_kernel, out_terms_kernel), in the
+// bytes of 16-bit rows but nearly free of their rounding, which is a third of the outputs' (P, row, output).
+// Each 128 columns of a row have a float32 scale, their largest magnitude / 32767, and
+//   bf16: f16 numbers, off by 2^-12 of a value at most (bf16's by 2^-9), normal down to 2^-29 of the largest;
+//   f16: integers, off by 2^-16 of the largest.
+// In the 2-norm the outputs of a prefill chunk are 2.4e-3 off with them, 2.9e-3 with bf16 rows; rows in
+// float32 took 7% of the call's time.
+constexpr float kPackMax = 32767.f;
+// max(|a|, |b|, m), NaN if one of them is
+__device__ __forceinline__ float magnitude3(float a, float b, float m) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(a), fabsf(b)), m);   // one instruction
+}
+// What packed values are multiplied by (where nothing reaches 2^-110 they count as zeros; where one is
+// not finite the scale is not either).
+template <typename TL>
+__device__ __forceinline__ float pack_inverse(float most) {
+    return most < 0x1p-110f ? 0.f : (Half<TL>::kF16 ? 1.f : kPackMax) / most;
+}
+template <typename TL>
+__device__ __forceinline__ uint32_t pack2_row(float a, float b) {
+    if constexpr (Half<TL>::kF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(a, b));
+    else return pack_f16x2(a, b);
+}
+template <typename TL>
+__device__ __forceinline__ void pv_pack_rows(const FlashArgs& a, const FlashWork& work, uint8_t* mine,
+                                             const v16f (&O)[8], const float* xl, int r0, int rows_b,
+                                             int cq, int lane) {
+    const int l32 = lane & 31, hw = lane >> 5;
+    const int64_t slot0 = (int64_t)work.b * rows_b + r0;
+    const int rows = rows_b - r0;   // of the tile, if below 64
+    #pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int row = 32 * t + l32;
+        const float lsum = xl[t * 64 + l32] + xl[t * 64 + 32 + l32];
+        float tops[4];
+        #pragma unroll
+        for (int cb = 0; cb < 4; ++cb) {
+            tops[cb] = 0.f;
+            #pragma unroll
+            for (int i = 0; i < 16; i += 2)
+                tops[cb] = magnitude3(O[2 * cb + t][i], O[2 * cb + t][i + 1], tops[cb]);
+        }
+        float top = magnitude3(tops[0], tops[1], magnitude3(tops[2], tops[3], 0.f));
+        const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = magnitude3(__uint_as_float(other[0]), __uint_as_float(other[1]), 0.f);
+        const float inv = pack_inverse<TL>(top);
+        if (hw == 0 && row < rows)
+            a.row_scale[(slot0 + row) * 4 + cq] =
+                top * (lsum == 0.f ? 0.f : 1.f / lsum) * (1.f / kPackMax);
+        #pragma unroll
+        for (int cb = 0; cb < 4; ++cb)
+            #pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const v4f v = v4f{O[2 * cb + t][4 * q], O[2 * cb + t][4 * q + 1],
+                                  O[2 * cb + t][4 * q + 2], O[2 * cb + t][4 * q + 3]} * inv;
+                *reinterpret_cast<v2u*>(mine + row * 256 + 16 * ((4 * cb + q) ^ (row & 15)) +
+                                        8 * (hw ^ ((row >> 4) & 1))) =
+                    v2u{pack2_row<TL>(v[0], v[1]), pack2_row<TL>(v[2], v[3])};
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_wave_barrier();
+    uint16_t* const dst = static_cast<uint16_t*>(a.ctx16) + slot0 * kFR + 128 * cq + 8 * (lane & 15);
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = 4 * i + (lane >> 4);
+        const v4u v = *reinterpret_cast<const v4u*>(mine + row * 256 + 16 * ((lane & 15) ^ (row & 15)));
+        if (row < rows)
+            *reinterpret_cast<v4u*>(dst + (int64_t)row * kFR) = (i >> 2) & 1 ? v4u{v[2], v[3], v[0], v[1]} : v;
+    }
+}
 template <typename TL>
 __device__ __forceinline__ void pv_store_rows(const FlashArgs& a, const FlashWork& work,
                                               uint8_t* mine, const v16f (&O)[8], const float* xl,
@@ -1841,8 +1915,15 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         if (!again) break;
     }
     lds_barrier();       // F
+    if constexpr (BS) {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(O[i]));
+    }
     // an fp8 cache's values are its codes times kv_scale: ctx takes the factor here
-    pv_store_rows<TL>(a, work, smem + cq * kPvOutBytes, O, xl, xref, r0, rows_b, cq, lane, a.o_scale);
+    if (BS && a.row_scale && work.direct)
+        pv_pack_rows<TL>(a, work, smem + cq * kPvOutBytes, O, xl, r0, rows_b, cq, lane);
+    else
+        pv_store_rows<TL>(a, work, smem + cq * kPvOutBytes, O, xl, xref, r0, rows_b, cq, lane, a.o_scale);
 }
 
 // ------------------------------------------------------------------ fp32 variant
@@ -2772,6 +2853,8 @@ constexpr int kFStages = 4;   // LDS ring depth
 // Both orders are fixed, so the merge is deterministic.  The rows of a single-chunk batch cost
 // one list read per workgroup: one workgroup per row took 45 us to find the 170,496 rows of a
 // prefill chunk's four sequences already written.
+// kOutPackedBF16, kOutPackedF16: rows as pv_pack_rows packs them for that type, their scales in row_sum.
+constexpr int kOutPackedBF16 = 3, kOutPackedF16 = 4;
 constexpr int kMergeFew = 8;
 constexpr int kMergeManyRows = kNumCUs / 2;   // up to here flash_merge_many_kernel
 template <int OUT>
@@ -2800,6 +2883,21 @@ __global__ void __launch_bounds__(256) flash_merge_kernel(const float* __restric
             dst[0] = a0;
             dst[1] = a1;
             if (lane == 0) row_sum[r] = ls;
+        } else if constexpr (OUT >= kOutPackedBF16) {
+            using TL = std::conditional_t<OUT == kOutPackedF16, f16_t, bf16_t>;
+            float top = 0.f;
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) top = magnitude3(a0[k], a1[k], top);
+            #pragma unroll
+            for (int d = 8; d > 0; d >>= 1) top = magnitude3(__shfl_xor(top, d), 0.f, top);
+            const float inv = pack_inverse<TL>(top);
+            const v4f w0 = a0 * inv, w1 = a1 * inv;
+            reinterpret_cast<v4u*>(static_cast<uint16_t*>(ctx) + (int64_t)r * kFR)[lane] =
+                v4u{pack2_row<TL>(w0[0], w0[1]), pack2_row<TL>(w0[2], w0[3]), pack2_row<TL>(w1[0], w1[1]),
+                    pack2_row<TL>(w1[2], w1[3])};
+            if ((lane & 15) == 0)
+                row_sum[4 * (int64_t)r + (lane >> 4)] =
+                    top * (ls == 0.f ? 0.f : 1.f / ls) * (1.f / kPackMax);
         } else {
             using S = Store16<OUT>;
             const float f = ls == 0.f ? 0.f : 1.f / ls;
@@ -3136,9 +3234,9 @@ __global__ void __launch_bounds__(512) out_list_kernel(const float* __restrict__
 // What bounds it is the phases' order (rows, barrier, product: about 3 us a tile) and W_uv's first read.
 // Launches of their own against it, with the pass (us): 9 sequences up to 9,000 keys 38.3 / 37.2, 16 up
 // to 8,192 43.6 / 41.4, 61 up to 4,989 73.9 / 72.5, 64 of up to 300 30.5 / 29.8, 128 up to 8,192 184.5 /
-// 186.0, 32 of 4 queries 57.3 / 59.8; past 128 tokens it loses (200: 57.4 / 66.5) and is not taken.  A row
-// in 16 bits between the launches is the third of the outputs' roundings (P, the row, the output):
-// without it they are 2.4e-3 instead of 2.9e-3 off in bf16, relative, in the 2-norm.
+// 186.0, 32 of 4 queries 57.3 / 59.8; past 128 tokens it loses (200: 57.4 / 66.5) and packed rows take
+// over.  A bf16 row between the launches is the third of the outputs' roundings (P, the row, the output):
+// without it they are 2.4e-3 instead of 2.9e-3 off, relative, in the 2-norm.
 constexpr int kOutTile = 16;
 template <typename TL>
 __global__ void __launch_bounds__(512, 1) out_merge_kernel(const float* __restrict__ o,
@@ -3275,6 +3373,254 @@ __global__ void __launch_bounds__(512, 1) out_merge_kernel(const float* __restri
             *reinterpret_cast<v2u*>(out + ((int64_t)t * H + h) * V + v) =
                 v2u{Half<TL>::pack2(r[0], r[1]), Half<TL>::pack2(r[2], r[3])};
     }
+}
+
+// 3d of many tokens' packed rows: a workgroup takes a head and 128 output columns, keeps its W_uv rows (all
+// 512 depths) in registers and walks over its share of the tokens, kRowsTile at a time.  out_rows_kernel is
+// bf16's, out_terms_kernel f16's.
+// f16: wave w multiplies output columns 32 (w % 4) .. +31 by 16 of the tile's tokens.  Four rows a wave come
+// two tiles ahead and go to LDS as values in two f16 terms (hi in rows 0 .. 31, lo in 32 .. 63), two tiles'
+// in turn, so one barrier a tile is enough; between two barriers half of the waves multiply first and
+// half convert first, so that each SIMD does both at once.  1,332 tokens of 128 heads 60 us (the
+// large-tile GEMM on f16 rows 54, a call 831 against 825).
+constexpr int kRowsTile = 32;
+__global__ void __launch_bounds__(512, 1) out_terms_kernel(const uint16_t* __restrict__ rows,
+                                                          const float* __restrict__ scales,
+                                                          const uint16_t* __restrict__ W,
+                                                          uint16_t* __restrict__ out, int M, int H, int V,
+                                                          int share) {
+    constexpr int kTok = kRowsTile / 8;
+    __shared__ __attribute__((aligned(16))) uint8_t cols[2][2 * kRowsTile * kOutListPitch];
+    const int vb = (V + 127) / 128, tiles = (M + kRowsTile - 1) / kRowsTile;
+    const int wg = xcd_logical_block(blockIdx.x, gridDim.x);
+    const int q0 = wg % share, c0 = wg / share % vb * 128, h = wg / share / vb;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int vw = 32 * (wave & 3), tg = wave >> 2;
+    struct Rows { v4u x[kTok]; float s[kTok]; };
+    Rows set[2];
+    auto fetch = [&](Rows& r, int tile) __attribute__((always_inline)) {
+        #pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+            const int64_t row = (int64_t)min(kRowsTile * tile + wave + 8 * i, M - 1) * H + h;
+            r.x[i] = reinterpret_cast<const v4u*>(rows + row * kFR)[lane];
+            r.s[i] = scales[4 * row + g];
+        }
+    };
+    fetch(set[0], q0);
+    fetch(set[1], q0 + share);
+    v4u wr[2][kFR / 32];
+    #pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const v4u* src = reinterpret_cast<const v4u*>(
+            W + ((int64_t)h * V + min(c0 + vw + 16 * k + l16, V - 1)) * kFR) + g;
+        #pragma unroll
+        for (int s = 0; s < kFR / 32; ++s) wr[k][s] = src[4 * s];
+    }
+    // tile's rows, in set[which], to LDS; then the rows two tiles on
+    auto convert = [&](int tile, auto which) __attribute__((always_inline)) {
+        constexpr int buf = decltype(which)::value;
+        using S = Half<f16_t>;
+        #pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+            v4u hi, lo;
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t w = set[buf].x[i][k];
+                const float p = (float)(int16_t)(w & 0xffffu) * set[buf].s[i];
+                const float q = (float)((int32_t)w >> 16) * set[buf].s[i];
+                hi[k] = S::pack2(p, q);
+                lo[k] = S::pack2(p - S::to_f32(hi[k] & 0xffffu), q - S::to_f32(hi[k] >> 16));
+            }
+            *reinterpret_cast<v4u*>(cols[buf] + (wave + 8 * i) * kOutListPitch + 16 * lane) = hi;
+            *reinterpret_cast<v4u*>(cols[buf] + (kRowsTile + wave + 8 * i) * kOutListPitch + 16 * lane) = lo;
+        }
+        fetch(set[buf], tile + 2 * share);
+    };
+    auto multiply = [&](int tile, auto which) __attribute__((always_inline)) {
+        constexpr int buf = decltype(which)::value;
+        using S = Half<f16_t>;
+        v4f d[2][2];
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) d[k][0] = d[k][1] = v4f{0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int s = 0; s < kFR / 32; ++s)
+            #pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const v4u c = *reinterpret_cast<const v4u*>(cols[buf] + (kRowsTile * t + 16 * tg + l16) * kOutListPitch +
+                                                            64 * s + 16 * g);
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    d[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, wr[k][s]),
+                                                                     __builtin_bit_cast(v8h, c), d[k][t], 0, 0, 0);
+                }
+            }
+        const int t = kRowsTile * tile + 16 * tg + l16;
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const v4f r = d[k][0] + d[k][1];
+            const int v = c0 + vw + 16 * k + 4 * g;
+            if (v < V && t < M)
+                *reinterpret_cast<v2u*>(out + ((int64_t)t * H + h) * V + v) =
+                    v2u{S::pack2(r[0], r[1]), S::pack2(r[2], r[3])};
+        }
+    };
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    convert(q0, even);
+    lds_barrier();
+    auto step = [&](int tile, auto which, auto next) __attribute__((always_inline)) {
+        if (tg) {
+            convert(tile + share, next);
+            multiply(tile, which);
+        } else {
+            multiply(tile, which);
+            convert(tile + share, next);
+        }
+        lds_barrier();
+    };
+    for (int tile = q0;;) {
+        step(tile, even, odd);
+        if ((tile += share) >= tiles) break;
+        step(tile, odd, even);
+        if ((tile += share) >= tiles) break;
+    }
+}
+
+// bf16: rows are f16 numbers, and W_uv's are made so once (a power-of-two scale for each output column: all
+// eight bits of values down to 2^-29 of its largest), so the MFMAs take the rows as they come.  They go
+// from memory straight to LDS, three tiles of 32 KB in flight a CU; wave w multiplies output columns 16 w ..
+// +15 by the tile's 32 tokens, an accumulator for each of a row's four scales.
+// Bound by the rows' bytes: 1,332 tokens of 128 heads 41 us, 5.8 TB/s (they were just written: part of them
+// comes from the last-level cache), where the large-tile GEMM on bf16 rows takes 54; 200 tokens 15.5 / 13.6,
+// of which W_uv's load and conversion take 5.  With 32 columns a wave, for half of the tokens each, it was
+// 45 and 19.5: twice W_uv's registers to convert.
+constexpr int kRowsStage = kRowsTile * kFR * 2;   // 32 KB: chunk c (16 bytes) of row r at c ^ (r & 15)
+constexpr int kRowsAhead = 3;                     // tiles in flight
+constexpr int kRowsScales = (kRowsAhead + 1) * kRowsStage;   // the stages' scales, 1 KB each
+__global__ void __launch_bounds__(512, 1) out_rows_kernel(const uint16_t* __restrict__ rows,
+                                                          const float* __restrict__ scales,
+                                                          const uint16_t* __restrict__ W,
+                                                          uint16_t* __restrict__ out, int M, int H, int V,
+                                                          int share) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kRowsScales + (kRowsAhead + 1) * 1024];
+    const int vb = (V + 127) / 128, tiles = (M + kRowsTile - 1) / kRowsTile;
+    const int wg = xcd_logical_block(blockIdx.x, gridDim.x);
+    const int q0 = wg % share, c0 = wg / share % vb * 128, h = wg / share / vb;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mine = (tiles - q0 + share - 1) / share;   // tiles of this workgroup
+    v4u wr[kFR / 32];
+    {
+        const v4u* src = reinterpret_cast<const v4u*>(
+            W + ((int64_t)h * V + min(c0 + 16 * wave + l16, V - 1)) * kFR) + g;
+        #pragma unroll
+        for (int s = 0; s < kFR / 32; ++s) wr[s] = src[4 * s];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // the workgroup's j-th tile into stage j % 4, four rows a wave, and (wave 0) its rows' scales
+    const uint32_t lds0 = lds_addr(smem);
+    const uint32_t scale_voff = lane < kRowsTile ? (uint32_t)lane * H * 16 : kOob;
+    auto issue = [&](int j) __attribute__((always_inline)) {
+        const int tile = q0 + j * share, t0 = kRowsTile * tile;
+        const uint32_t st = lds0 + (uint32_t)(j & kRowsAhead) * kRowsStage;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 4 * wave + i;
+            const bool in = j < mine && t0 + r < M;
+            const uint64_t at = reinterpret_cast<uint64_t>(rows) + ((uint64_t)(in ? t0 + r : 0) * H + h) * (kFR * 2);
+            dma16(rsrc_span(at, 0, in ? kFR * 2 : 0), __builtin_amdgcn_readfirstlane(st + r * 1024),
+                  16u * (lane ^ (r & 15)));
+        }
+        if (wave == 0) {
+            const int n = j < mine ? min(kRowsTile, M - t0) : 0;
+            dma16(rsrc_span(reinterpret_cast<uint64_t>(scales) + ((uint64_t)(n ? t0 : 0) * H + h) * 16, 0,
+                            n ? (uint32_t)(n - 1) * H * 16 + 16 : 0),
+                  __builtin_amdgcn_readfirstlane(lds0 + kRowsScales + (j & kRowsAhead) * 1024), scale_voff);
+        }
+    };
+    static_assert(kRowsAhead == 3, "four stages");
+    for (int j = 0; j < kRowsAhead; ++j) issue(j);
+    // W_uv's values in f16: a row's largest exponent becomes f16's, 30, and those 30 below it zeros
+    float w_scale[4];
+    {
+        typedef uint16_t v2h_t __attribute__((ext_vector_type(2)));
+        auto two = [](uint32_t w) __attribute__((always_inline)) { return __builtin_bit_cast(v2h_t, w); };
+        v2h_t top = {0, 0};
+        #pragma unroll
+        for (int s = 0; s < kFR / 32; ++s)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, two(wr[s][i] & 0x7fff7fffu));
+        int most = max(top[0], top[1]);
+        most = max(most, __shfl_xor(most, 16));
+        most = max(most, __shfl_xor(most, 32));
+        const int down = max(min(most >> 7, 254) - 30, 0);   // off the exponents
+        const v2h_t sub = {(uint16_t)(down << 7), (uint16_t)(down << 7)};
+        #pragma unroll
+        for (int s = 0; s < kFR / 32; ++s)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = wr[s][i];
+                const v2h_t m = __builtin_elementwise_sub_sat(two(w & 0x7fff7fffu), sub);
+                wr[s][i] = (w & 0x80008000u) | __builtin_bit_cast(uint32_t, (v2h_t)(m << 3));
+            }
+        // f16 numbers with bf16's bits (three zeros behind) are 2^112 / 2^down times as large
+        const float back = __uint_as_float((uint32_t)(down + 15) << 23);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) w_scale[i] = __shfl(back, 4 * g + i);   // of the lane's results
+    }
+    const uint32_t out_row = (uint32_t)H * V * 2;   // bytes a token
+    const int v = c0 + 16 * wave + 4 * g;
+    const uint32_t out_voff = v < V ? (uint32_t)l16 * out_row + (uint32_t)(h * V + v) * 2 : kOob;
+    for (int j = 0; j < mine; ++j) {
+        // tile j has landed when at most the two behind it and the stores of three tiles are under way
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        auto landed = [&](auto stores) __attribute__((always_inline)) {
+            if (wave == 0) wait_vm<10 + decltype(stores)::value>();
+            else wait_vm<8 + decltype(stores)::value>();
+        };
+        if (j == 0) landed(std::integral_constant<int, 0>{});
+        else if (j == 1) landed(std::integral_constant<int, 2>{});
+        else if (j == 2) landed(std::integral_constant<int, 4>{});
+        else landed(std::integral_constant<int, 6>{});
+        lds_barrier();
+        issue(j + kRowsAhead);
+        const uint8_t* st = smem + (j & kRowsAhead) * kRowsStage + l16 * 1024;
+        v4f d[2][4];
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            d[0][q] = d[1][q] = v4f{0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int s = 4 * q; s < 4 * q + 4; ++s)
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const v4u c = *reinterpret_cast<const v4u*>(st + 16 * 1024 * k + 16 * ((4 * s + g) ^ l16));
+                    d[k][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, wr[s]),
+                                                                     __builtin_bit_cast(v8h, c), d[k][q], 0, 0, 0);
+                }
+        }
+        const int t0 = kRowsTile * (q0 + j * share);
+        const uint64_t at = reinterpret_cast<uint64_t>(out) + (uint64_t)t0 * out_row;
+        const uint32_t at_lo = __builtin_amdgcn_readfirstlane((uint32_t)at);
+        const uint32_t at_hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+        const __amdgpu_buffer_rsrc_t dst = __builtin_amdgcn_make_buffer_rsrc(
+            reinterpret_cast<void*>((uint64_t)at_hi << 32 | at_lo), 0,
+            __builtin_amdgcn_readfirstlane((int)(min(kRowsTile, M - t0) * out_row)), 0x00020000);
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const v4f sc = *reinterpret_cast<const v4f*>(smem + kRowsScales + (j & kRowsAhead) * 1024 +
+                                                         16 * (16 * k + l16));
+            v4f r = d[k][0] * sc[0];
+            #pragma unroll
+            for (int q = 1; q < 4; ++q) r += d[k][q] * sc[q];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] *= w_scale[i];
+            __builtin_amdgcn_raw_buffer_store_b64(v2u{pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3])}, dst,
+                                                  (int)(out_voff + 16 * k * out_row), 0, 0);
+        }
+    }
+    wait_vm<0>();   // the zero loads of the tiles past the end have landed
 }
 
 // Work list of a ragged batch (one workgroup; key counts are device data).  The chunk rule,
@@ -3546,22 +3892,41 @@ FlashPlan plan_flash(const FlashProblem& p) {
     return f;
 }
 
-// which of the kernels above: 0 neither, 1 out_list_kernel, 2 out_merge_kernel
+// which of the kernels above: 0 none, 1 out_list_kernel, 2 out_merge_kernel, 3 out_rows_kernel
 static int out_list_kind(const FlashProblem& p, const FlashPlan& f) {
     // MLA_OUT_SMALL=0: the merge and 3d launches of their own
     const char* env = std::getenv("MLA_OUT_SMALL");
     if (!p.scale_block || !f.balanced || p.R != kFR || (env && env[0] == '0')) return 0;
     const int64_t M = (int64_t)p.B * p.Sq;
     if (M <= kOutListTokens && p.Sq * f.max_items <= kOutListRows) return 1;
-    return M <= kOutMergeTokens ? 2 : 0;
+    return M <= kOutMergeTokens ? 2 : 3;
 }
 bool out_list_ok(const FlashProblem& p, const FlashPlan& f) { return out_list_kind(p, f) > 0; }
+bool out_rows_ok(const FlashProblem& p, const FlashPlan& f) { return out_list_kind(p, f) == 3; }
+// the packed rows' scales lie behind them in ctx
+static float* packed_scales(const FlashProblem& p, void* ctx) {
+    return reinterpret_cast<float*>(static_cast<uint16_t*>(ctx) + (size_t)p.B * p.Sq * p.H * kFR);
+}
 
-hipError_t launch_out_list(const FlashProblem& p, const FlashPlan& f, const float* ctx,
+hipError_t launch_out_list(const FlashProblem& p, const FlashPlan& f, float* ctx,
                            const float* row_sum, const float* partials, const void* W_uv, void* out,
                            int V, hipStream_t stream) {
     const int kind = out_list_kind(p, f);
     if (kind == 0 || V <= 0) return hipErrorInvalidValue;
+    if (kind == 3) {
+        const int M = p.B * p.Sq, heads = p.H * ((V + 127) / 128), tiles = (M + kRowsTile - 1) / kRowsTile;
+        const int share = std::max(1, std::min(tiles, kNumCUs / heads));
+        const dim3 grid((unsigned)(heads * share));
+        const uint16_t* rows = reinterpret_cast<const uint16_t*>(ctx);
+        const float* scales = packed_scales(p, ctx);
+        const uint16_t* W = static_cast<const uint16_t*>(W_uv);
+        uint16_t* dst = static_cast<uint16_t*>(out);
+        if (p.f16)
+            hipLaunchKernelGGL(out_terms_kernel, grid, dim3(512), 0, stream, rows, scales, W, dst, M, p.H, V, share);
+        else
+            hipLaunchKernelGGL(out_rows_kernel, grid, dim3(512), 0, stream, rows, scales, W, dst, M, p.H, V, share);
+        return hipGetLastError();
+    }
     const size_t rows_b = (size_t)p.Sq * p.H;
     const size_t wl_bytes = ((size_t)wl_ints(p.B, f.max_items) * sizeof(int) + 255) / 256 * 256;
     const float* o = reinterpret_cast<const float*>(reinterpret_cast<const char*>(partials) + wl_bytes);
@@ -3656,7 +4021,8 @@ static bool flash_spread(const FlashProblem& p, const FlashPlan& f) {
 
 hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, float* row_sum,
                         float* partials, hipStream_t stream, bool merge, void* ctx16) {
-    if (ctx16 && !flash_ctx16_ok(p, f)) return hipErrorInvalidValue;
+    const bool packed = ctx16 && out_rows_ok(p, f);
+    if (ctx16 && !packed && !flash_ctx16_ok(p, f)) return hipErrorInvalidValue;
     const int rows = p.B * p.Sq * p.H;
     const int rows_b = p.Sq * p.H;
     FlashArgs a;
@@ -3668,6 +4034,7 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
     a.o_direct = ctx;
     a.l_direct = row_sum;
     a.ctx16 = ctx16;
+    a.row_scale = packed ? packed_scales(p, ctx16) : nullptr;
     int grid;
     int* wl = nullptr;
     if (f.balanced) {
@@ -3776,7 +4143,7 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
     if (e != hipSuccess || (!f.balanced && f.n_split == 1)) return e;
     if (!merge) return e;   // the caller folds the merge in
     const int n = f.n_split;
-    if (rows <= kMergeManyRows) {
+    if (rows <= kMergeManyRows && !packed) {   // (packed rows are more)
         const dim3 grid2((unsigned)(2 * rows)), block2(512);
         if (!ctx16)
             hipLaunchKernelGGL(flash_merge_many_kernel<kOutF32>, grid2, block2, 0, stream, a.o, a.m, a.l,
@@ -3793,7 +4160,13 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
     // need no merge: 64, so that finding that out takes fewer workgroups
     const int rpw = rows <= 2048 ? 1 : f.balanced && rows >= 65536 ? 64 : 4;
     const dim3 mgrid((unsigned)((rows + rpw - 1) / rpw)), mblock(256);
-    if (!ctx16)
+    if (packed && p.f16)
+        hipLaunchKernelGGL(flash_merge_kernel<kOutPackedF16>, mgrid, mblock, 0, stream, a.o, a.m, a.l, ctx16,
+                           a.row_scale, p.B, rows, rows_b, n, rpw, a.wl);
+    else if (packed)
+        hipLaunchKernelGGL(flash_merge_kernel<kOutPackedBF16>, mgrid, mblock, 0, stream, a.o, a.m, a.l, ctx16,
+                           a.row_scale, p.B, rows, rows_b, n, rpw, a.wl);
+    else if (!ctx16)
         hipLaunchKernelGGL(flash_merge_kernel<kOutF32>, mgrid, mblock, 0, stream, a.o, a.m, a.l, ctx,
                            row_sum, p.B, rows, rows_b, n, rpw, a.wl);
     else if (p.f16)

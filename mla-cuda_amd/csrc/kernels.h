@@ -332,7 +332,10 @@ hipError_t launch_out_small(const FlashPartials& fp, const float* ctx, const flo
 // out_list_ok: by the shape and the plan.
 constexpr int kOutListTokens = 8, kOutMergeTokens = 128;
 bool out_list_ok(const FlashProblem& p, const FlashPlan& plan);
-hipError_t launch_out_list(const FlashProblem& p, const FlashPlan& plan, const float* ctx,
+// Past that the pass and the merge leave packed rows (merge = true and ctx16 = ctx, out_rows_ok), which
+// launch_out_list then takes from ctx.
+bool out_rows_ok(const FlashProblem& p, const FlashPlan& plan);
+hipError_t launch_out_list(const FlashProblem& p, const FlashPlan& plan, float* ctx,
                            const float* row_sum, const float* partials, const void* W_uv, void* out,
                            int V, hipStream_t stream);
 // The work list alone (plan.balanced, seq_lens given): wl receives flash_worklist_ints()

@@ -124,6 +124,7 @@ ATTEND = dict(dtype=BF16, dims=None, q_absorbed=P16, q_rope=P16, c_kv_pages=P16,
     (dict(dims=dims(kv_rank=256)), UNSUPPORTED, "kv_rank 512"), (dict(dims=dims(rope=128)), UNSUPPORTED, "rope 64"),
     (dict(dims=dims(sk=96)), INVALID, "page_size"), (dict(dims=dims(sq=300), causal=1), INVALID, "sk >= sq"),
     (dict(dims=dims(batch=1, sq=1 << 14)), UNSUPPORTED, "2^31"),
+    (dict(dims=dims(v=1 << 18)), UNSUPPORTED, "heads * v"),
     (dict(page_size=0), INVALID, "page_size"), (dict(num_pages=0), INVALID, "num_pages"),
     (dict(scale_block=1), UNSUPPORTED, "scale_block"), (dict(scale=ctypes.c_double(0.0)), INVALID, "scale"),
     *[({k: None}, INVALID, k) for k, v in ATTEND.items() if v is P16 and k != "workspace"],

@@ -503,7 +503,8 @@ def test_attention_fewer_keys_than_queries(ext, dt):
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("Sq,H,lens,at", [(4, 128, [300, 33, 4], 2), (4, 16, [64, 700, 4], 1), (40, 3, [40, 100, 2000], 17),
-                                          (33, 128, [500, 33, 64], 32), (7, 200, [90, 7, 4000], 0)])
+                                          (33, 128, [500, 33, 64], 32), (7, 200, [90, 7, 4000], 0),
+                                          (50, 3, [50, 100, 9000], 17), (64, 16, [900, 64, 2000], 63)])
 def test_attention_hidden_nan(ext, monkeypatch, dt, Sq, H, lens, at):
     """A NaN in a token's row (latent, or rope alone): the queries in front of it keep their bits, it
     and the ones behind it are NaN."""
@@ -848,14 +849,14 @@ def test_one_layer_of_layered_pools(ext, layer):
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 def test_attention_unrounded_rows_past_128_tokens(ext, monkeypatch, dt):
-    """MLA_CTX16=0: the attention's rows in float32 between the pass and 3d, two roundings (P and the
-    output) instead of three."""
+    """With MLA_OUT_SMALL=0 the large-tile GEMM is 3d, of rows in 16 bits or (MLA_CTX16=0) in float32."""
     g = torch.Generator().manual_seed(129)
     lens = torch.randint(0, 400, (43,), generator=g).tolist()
     lens[0], lens[1] = 3000, 0
     qa, qr, w, cache, table = attention_case(lens, 4, 32, 64, DT[dt], 129)
     rows = [torch.nan_to_num(r) for r in K.decode(cache)]
     ref = K.attention(qa, qr, rows, table, lens, w, SCALE, True, 64, cache["c_kv"].size(0))
+    monkeypatch.setenv("MLA_OUT_SMALL", "0")
     check_attention(attend(ext, qa, qr, w, cache, table, lens, True), ref, DT[dt], True)
     monkeypatch.setenv("MLA_CTX16", "0")
     check_attention(attend(ext, qa, qr, w, cache, table, lens, True), ref, DT[dt], True)
@@ -898,3 +899,40 @@ def test_steps_on_two_streams(ext):
         for a, b in zip(w, o):
             for x, y in zip(a, b):
                 assert torch.equal(torch.nan_to_num(x), torch.nan_to_num(y))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Sq,H,V,lens", [
+    (1, 129, 1, 4, [129]), (3, 100, 3, 132, [100, 1000, 101]), (130, 1, 5, 260, None), (2, 300, 16, 64, [7000, 300]),
+    (1, 1000, 2, 128, [1500]), (43, 4, 65, 128, None), (300, 1, 128, 128, None)])
+def test_attention_many_tokens(ext, dt, B, Sq, H, V, lens):
+    """Past 128 tokens the rows go to 3d packed: tiles of tokens that are not full, columns past a block of
+    128, sequences in one chunk and in several, empty ones."""
+    g = torch.Generator().manual_seed(B + Sq)
+    if lens is None:
+        lens = torch.randint(0, 300, (B,), generator=g).tolist()
+        lens[0], lens[1] = 2000, 0
+    qa, qr, w, cache, table = attention_case(lens, Sq, 32, 64, DT[dt], B, H=H, V=V)
+    rows = [torch.nan_to_num(r) for r in K.decode(cache)]
+    ref = K.attention(qa, qr, rows, table, lens, w, SCALE, True, 64, cache["c_kv"].size(0))
+    check_attention(attend(ext, qa, qr, w, cache, table, lens, True), ref, DT[dt], True)
+
+
+@pytest.mark.parametrize("up,w_up", [(60, 50), (-60, -40), (100, -90)])
+@pytest.mark.parametrize("Sq", [1, 70])
+def test_attention_powers_of_two(ext, up, w_up, Sq):
+    """Values times 2^up (the queries the less) and each output column's W_uv times a power of two of its
+    own: the outputs' bits but for the exponent, few tokens or many.  (bf16, whose range holds all of
+    them as normal numbers.)"""
+    lens = [70, 300, 1200]
+    g = torch.Generator().manual_seed(Sq)
+    qa, qr, w, cache, table = attention_case(lens, Sq, 32, 64, BF, 3, H=16)
+    cache["pe"].zero_()
+    base = attend(ext, qa, qr, w, cache, table, lens, True)
+    moved = {**cache, "scales": cache["scales"].clone()}
+    held = moved["scales"][..., 0] != 255
+    moved["scales"][..., 0][held] = (moved["scales"][..., 0][held].int() + up).to(torch.uint8)
+    e = torch.randint(min(0, w_up), max(0, w_up) + 1, (16, 128), generator=g).double()
+    out = attend(ext, (qa.double() * 2.0 ** -up).to(BF), qr, (w.double() * 2.0 ** e[..., None]).to(BF), moved, table,
+                 lens, True)
+    assert torch.equal(out.double(), base.double() * 2.0 ** (up + e))
