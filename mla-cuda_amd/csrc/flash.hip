@@ -1521,9 +1521,21 @@ __device__ __forceinline__ void f8_zero_nan(uint8_t* stage, int cq, int lane) {
 // zero-extended to a dword each, 256 bytes a stage past the flags; a wave reads its halves'
 // with its fragments.  Keys past the end take scale byte 0, whatever the page holds there (a
 // byte 255 would make their zero codes NaN).
+// BS's steps are one apart from the others': the softmax of block j - 1 runs between the score MFMAs of
+// block j, and P.V works on block j - 2, so a score wave's chain of MFMAs and its exponentials overlap.
+// What bounds a step is each wave's own stream of instructions (a score wave's 36 MFMAs and 72
+// conversions, a P.V wave's 16 and 32, at about 8 cycles an instruction), so the rest was cut: the next
+// block's descriptors behind the first P.V MFMAs, page entries in a register, addresses kept.  Measured
+// (us): descriptors in front of the step's barrier, with a division and a scalar load, a chunk of four
+// sequences' 333 queries 769, 128 sequences up to 8,192 keys 186, one of 65,536 39.9; behind the MFMAs
+// 704, 176, 38.4 (with the softmax behind its own block's MFMAs 733, 183); entries and addresses in
+// registers 699, 176, 38.4 (against 707).  Not kept: K's or V's first reads of the next block in
+// front of the barrier (763 and 740 against 725), P.V waves at a higher priority (723 to 764).
 template <typename TL, bool BS>
 __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     constexpr float kHeadroom = Half<TL>::kF16 ? 15.f : k2Headroom;
+    constexpr int kBehind = BS ? 2 : 1;                         // P.V works on block j - kBehind in step j
+    constexpr int kAhead = k8NS - 1 - kBehind;                  // blocks in flight past the one in work
     constexpr int kPBase = k8NS * k8Stage;                      // 144 KB: two P^T stages
     // the queries at the start: 64 rows of 1 KB (chunk c of row r at c ^ (r & 15)), then 64 rope
     // rows of 128 bytes (chunk c at c ^ ((r >> 1) & 7)), in the last four stages
@@ -1531,11 +1543,12 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     static_assert(kFRows * (kLatBytes + kPeBytes) == 4 * k8Stage, "the queries fill four stages");
     constexpr int kXBase = kPBase + 2 * kXPStage;               // references, sums, flags
     constexpr int kSBase = kXBase + 2 * 128 * 4 + 64;           // BS: the stages' scales
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kSBase + (BS ? k8NS * 256 : 0)];
+    constexpr int kTBase = kSBase + k8NS * 256;                 // BS: 64 table entries a P.V wave
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[BS ? kTBase + 4 * 256 : kSBase];
     float* xref = reinterpret_cast<float*>(smem + kXBase);      // [rt][kh][32 rows]
     float* xl = xref + 128;                                     // [rt][kh][32 rows]
     int* flags = reinterpret_cast<int*>(xl + 128);              // [score wave]
-    int* hidden_nan = flags + 8;                                // BS: [block & 1], the block + 1
+    int* hidden_nan = flags + 8;                                // BS: [block & 3], the block + 1
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4, l32 = lane & 31, hw = lane >> 5;
@@ -1588,8 +1601,14 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         uint32_t kb0 = kk * k8LatBytes + 8u * (g & 1) + 16u * ((g >> 1) ^ (x & 1)) + 32u * (x >> 1);
         uint32_t pb0 = k8LatStage + kk * k8PeBytes + 8u * (g & 1) + 16u * ((g >> 1) ^ (y & 1)) +
                              32u * (y >> 1);
+        // BS: 256 bytes (eight steps) on, only an immediate offset changes: ten registers of addresses
+        uint32_t kx[8], px[2];
+        #pragma unroll
+        for (int s = 0; s < 8; ++s) kx[s] = kb0 ^ (32u * s);
+        px[0] = pb0;
+        px[1] = pb0 ^ 32u;
         auto k_read = [&](uint32_t sbase, int s) __attribute__((always_inline)) {
-            const uint32_t off = s < kRSteps ? (kb0 ^ (32u * s)) : (pb0 ^ (32u * (s - kRSteps)));
+            const uint32_t off = BS ? (s < kRSteps ? kx[s & 7] + 256u * (s >> 3) : px[s & 1]) : s < kRSteps ? (kb0 ^ (32u * s)) : (pb0 ^ (32u * (s - kRSteps)));
             return *reinterpret_cast<const v2u*>(smem + sbase + off);
         };
         // P^T writes: rows 16h + l16 of the tile, keys 16kh + 4g .. +3 (8 bytes)
@@ -1601,29 +1620,22 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
             l_run[0] = l_run[1] = 0.f;
             bool overflow = false;
             if (nb == 0) break;
-            #pragma unroll 1
-            for (int j = 0; j <= nb; ++j) {
-                lds_barrier();        // A_j: block j is in LDS, P.V of block j-2 is done
-                v4f sc[2];
-                if (j < nb) {
+            if constexpr (BS) {
+                v4f sc[2], sp[2];   // the scores of block j, and of the one before
+                // block j's scores; `between(s)` runs behind step s's MFMAs
+                auto scores = [&](int j, auto between) __attribute__((always_inline)) {
                     constexpr int kWin = 4;
                     asm volatile("" : "+v"(kb0), "+v"(pb0));
                     const uint32_t sbase = (uint32_t)(j % k8NS) * k8Stage;
                     v2u kf[kWin];
-                    float s_lat = 1.f, s_pe = 1.f;
-                    if constexpr (BS) {
-                        const v2u w = *reinterpret_cast<const v2u*>(smem + kSBase + 256 * (j % k8NS) + 8 * kh);
-                        s_lat = __uint_as_float(w[0] << 23);
-                        s_pe = __uint_as_float(w[1] << 23);
-                    }
+                    const v2u w = *reinterpret_cast<const v2u*>(smem + kSBase + 256 * (j % k8NS) + 8 * kh);
                     #pragma unroll
                     for (int i = 0; i < kWin; ++i) kf[i] = k_read(sbase, i);
-                    // the compiler's own MFMA (not the asm form of the bf16 kernel): the K
-                    // operand is written by the conversions just before, a VALU-write ->
-                    // MFMA-read dependency whose wait states only the compiler inserts
+                    between(std::integral_constant<int, -1>{});
+                    const float s_lat = __uint_as_float(w[0] << 23), s_pe = __uint_as_float(w[1] << 23);
                     sc[0] = sc[1] = v4f{};
-                    #pragma unroll
-                    for (int s = 0; s < kQSteps; ++s) {
+                    auto step = [&](auto sv) __attribute__((always_inline)) {
+                        constexpr int s = decltype(sv)::value;
                         const v4u cur = fp8x8<TL>(kf[s % kWin], s < kRSteps ? s_lat : s_pe);
                         if (s + kWin < kQSteps) kf[s % kWin] = k_read(sbase, s + kWin);
                         #pragma unroll
@@ -1637,56 +1649,36 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                                     __builtin_bit_cast(v8bf, cur), __builtin_bit_cast(v8bf, qf[h][s]), sc[h],
                                     0, 0, 0);
                         }
-                    }
+                        between(sv);
+                    };
+                    [&]<int... S>(std::integer_sequence<int, S...>) __attribute__((always_inline)) {
+                        (step(std::integral_constant<int, S>{}), ...);
+                    }(std::make_integer_sequence<int, kQSteps>{});
                     __builtin_amdgcn_sched_barrier(0);
                     const int kq0 = k_lo + k2Keys * j + 16 * kh;
                     if (kq0 + 15 > lim_wave) {
                         const int kq = kq0 + 4 * g;
-                        if constexpr (BS) {
-                            // a hidden key with a NaN: the P.V waves take it out of the block's V
-                            bool nan = false;
-                            #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                nan |= (kq + i > lim0 && sc[0][i] != sc[0][i]) ||
-                                       (kq + i > lim1 && sc[1][i] != sc[1][i]);
-                            if (__builtin_amdgcn_ballot_w64(nan) && lane == 0) hidden_nan[j & 1] = j + 1;
-                        }
+                        // a hidden key with a NaN: the P.V waves take it out of the block's V
+                        bool nan = false;
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            nan |= (kq + i > lim0 && sc[0][i] != sc[0][i]) ||
+                                   (kq + i > lim1 && sc[1][i] != sc[1][i]);
+                        if (__builtin_amdgcn_ballot_w64(nan) && lane == 0) hidden_nan[j & 3] = j + 1;
                         #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             sc[0][i] = kq + i <= lim0 ? sc[0][i] : -INFINITY;
                             sc[1][i] = kq + i <= lim1 ? sc[1][i] : -INFINITY;
                         }
                     }
-                    if (j == 0) {
-                        // the pass's reference proposal of each row: the raised one of a
-                        // previous pass, else this block's maximum over the half's keys
-                        #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float mx = fmaxf(fmaxf(sc[h][0], sc[h][1]), fmaxf(sc[h][2], sc[h][3]));
-                            const float bm = row4_reduce(mx, OpMax{}) * a.c;
-                            const float prop = m_ref[h] == -INFINITY ? bm : m_ref[h];
-                            if (g == 0) xref[(rt * 2 + kh) * 32 + 16 * h + l16] = prop;
-                        }
-                    }
-                }
-                if (j == 0) {
-                    lds_barrier();    // X: both halves' proposals are in LDS
-                    #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int r = 16 * h + l16;
-                        const float ref = fmaxf(xref[(rt * 2) * 32 + r], xref[(rt * 2 + 1) * 32 + r]);
-                        m_ref[h] = ref;
-                        m_neg[h] = ref == -INFINITY ? 0.f : -ref;
-                        thr[h] = ref + kHeadroom;
-                    }
-                }
-                if (j < nb) {
+                };
+                // a row past its threshold raises its reference and flags a repeat (NaN scores come
+                // here too); rows without a reference have no visible key
+                auto check = [&]() __attribute__((always_inline)) {
                     float mx[2];
                     #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        mx[h] = fmaxf(fmaxf(sc[h][0], sc[h][1]), fmaxf(sc[h][2], sc[h][3]));
-                    // a row past its threshold raises its reference and flags a repeat (NaN
-                    // scores come here too); rows without a reference have no visible key
+                        mx[h] = fmaxf(fmaxf(sp[h][0], sp[h][1]), fmaxf(sp[h][2], sp[h][3]));
                     if (__builtin_amdgcn_ballot_w64(!(mx[0] * a.c <= thr[0]) || !(mx[1] * a.c <= thr[1]))) {
                         #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -1700,16 +1692,166 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                             }
                         }
                     }
-                    const uint32_t pws = pw0 + (uint32_t)(j & 1) * kXPStage;
+                };
+                // row half h's exponentials of block j - 1, its sums and P^T
+                auto exps = [&](int h, int j) __attribute__((always_inline)) {
+                    float e[4];
                     #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float e[4];
+                    for (int i = 0; i < 4; ++i)
+                        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sp[h][i], a.c, m_neg[h]));
+                    l_run[h] += (e[0] + e[1]) + (e[2] + e[3]);
+                    *reinterpret_cast<v2u*>(smem + pw0 + (uint32_t)((j - 1) & 1) * kXPStage + 16u * h * kXPPitch) =
+                        v2u{Half<TL>::pack2(e[0], e[1]), Half<TL>::pack2(e[2], e[3])};
+                };
+                lds_barrier();        // A_0: block 0 is in LDS
+                scores(0, [](auto) __attribute__((always_inline)) {});
+                // the pass's reference proposal of each row: the raised one of a previous pass,
+                // else this block's maximum over the half's keys
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float mx = fmaxf(fmaxf(sc[h][0], sc[h][1]), fmaxf(sc[h][2], sc[h][3]));
+                    const float bm = row4_reduce(mx, OpMax{}) * a.c;
+                    const float prop = m_ref[h] == -INFINITY ? bm : m_ref[h];
+                    if (g == 0) xref[(rt * 2 + kh) * 32 + 16 * h + l16] = prop;
+                }
+                lds_barrier();        // X: both halves' proposals are in LDS
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = 16 * h + l16;
+                    const float ref = fmaxf(xref[(rt * 2) * 32 + r], xref[(rt * 2 + 1) * 32 + r]);
+                    m_ref[h] = ref;
+                    m_neg[h] = ref == -INFINITY ? 0.f : -ref;
+                    thr[h] = ref + kHeadroom;
+                    sp[h] = sc[h];
+                }
+                #pragma unroll 1
+                for (int j = 1; j < nb; ++j) {
+                    lds_barrier();    // A_j: block j is in LDS, P.V of block j-3 is done
+                    scores(j, [&](auto sv) __attribute__((always_inline)) {
+                        constexpr int s = decltype(sv)::value;
+                        if constexpr (s == -1) check();
+                        if constexpr (s == 2) exps(0, j);
+                        if constexpr (s == 6) exps(1, j);
+                    });
+                    sp[0] = sc[0];
+                    sp[1] = sc[1];
+                }
+                lds_barrier();        // A_nb
+                check();
+                exps(0, nb);
+                exps(1, nb);
+                lds_barrier();        // A_nb+1: the last block's P^T
+            } else {
+                #pragma unroll 1
+                for (int j = 0; j <= nb; ++j) {
+                    lds_barrier();        // A_j: block j is in LDS, P.V of block j-2 is done
+                    v4f sc[2];
+                    if (j < nb) {
+                        constexpr int kWin = 4;
+                        asm volatile("" : "+v"(kb0), "+v"(pb0));
+                        const uint32_t sbase = (uint32_t)(j % k8NS) * k8Stage;
+                        v2u kf[kWin];
+                        float s_lat = 1.f, s_pe = 1.f;
+                        if constexpr (BS) {
+                            const v2u w = *reinterpret_cast<const v2u*>(smem + kSBase + 256 * (j % k8NS) + 8 * kh);
+                            s_lat = __uint_as_float(w[0] << 23);
+                            s_pe = __uint_as_float(w[1] << 23);
+                        }
                         #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][i], a.c, m_neg[h]));
-                        l_run[h] += (e[0] + e[1]) + (e[2] + e[3]);
-                        *reinterpret_cast<v2u*>(smem + pws + 16u * h * kXPPitch) =
-                            v2u{Half<TL>::pack2(e[0], e[1]), Half<TL>::pack2(e[2], e[3])};
+                        for (int i = 0; i < kWin; ++i) kf[i] = k_read(sbase, i);
+                        // the compiler's own MFMA (not the asm form of the bf16 kernel): the K
+                        // operand is written by the conversions just before, a VALU-write ->
+                        // MFMA-read dependency whose wait states only the compiler inserts
+                        sc[0] = sc[1] = v4f{};
+                        #pragma unroll
+                        for (int s = 0; s < kQSteps; ++s) {
+                            const v4u cur = fp8x8<TL>(kf[s % kWin], s < kRSteps ? s_lat : s_pe);
+                            if (s + kWin < kQSteps) kf[s % kWin] = k_read(sbase, s + kWin);
+                            #pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                if constexpr (Half<TL>::kF16)
+                                    sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                        __builtin_bit_cast(v8h, cur), __builtin_bit_cast(v8h, qf[h][s]), sc[h],
+                                        0, 0, 0);
+                                else
+                                    sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                        __builtin_bit_cast(v8bf, cur), __builtin_bit_cast(v8bf, qf[h][s]), sc[h],
+                                        0, 0, 0);
+                            }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                        const int kq0 = k_lo + k2Keys * j + 16 * kh;
+                        if (kq0 + 15 > lim_wave) {
+                            const int kq = kq0 + 4 * g;
+                            if constexpr (BS) {
+                                // a hidden key with a NaN: the P.V waves take it out of the block's V
+                                bool nan = false;
+                                #pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    nan |= (kq + i > lim0 && sc[0][i] != sc[0][i]) ||
+                                           (kq + i > lim1 && sc[1][i] != sc[1][i]);
+                                if (__builtin_amdgcn_ballot_w64(nan) && lane == 0) hidden_nan[j & 3] = j + 1;
+                            }
+                            #pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                sc[0][i] = kq + i <= lim0 ? sc[0][i] : -INFINITY;
+                                sc[1][i] = kq + i <= lim1 ? sc[1][i] : -INFINITY;
+                            }
+                        }
+                        if (j == 0) {
+                            // the pass's reference proposal of each row: the raised one of a
+                            // previous pass, else this block's maximum over the half's keys
+                            #pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float mx = fmaxf(fmaxf(sc[h][0], sc[h][1]), fmaxf(sc[h][2], sc[h][3]));
+                                const float bm = row4_reduce(mx, OpMax{}) * a.c;
+                                const float prop = m_ref[h] == -INFINITY ? bm : m_ref[h];
+                                if (g == 0) xref[(rt * 2 + kh) * 32 + 16 * h + l16] = prop;
+                            }
+                        }
+                    }
+                    if (j == 0) {
+                        lds_barrier();    // X: both halves' proposals are in LDS
+                        #pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int r = 16 * h + l16;
+                            const float ref = fmaxf(xref[(rt * 2) * 32 + r], xref[(rt * 2 + 1) * 32 + r]);
+                            m_ref[h] = ref;
+                            m_neg[h] = ref == -INFINITY ? 0.f : -ref;
+                            thr[h] = ref + kHeadroom;
+                        }
+                    }
+                    if (j < nb) {
+                        float mx[2];
+                        #pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            mx[h] = fmaxf(fmaxf(sc[h][0], sc[h][1]), fmaxf(sc[h][2], sc[h][3]));
+                        // a row past its threshold raises its reference and flags a repeat (NaN
+                        // scores come here too); rows without a reference have no visible key
+                        if (__builtin_amdgcn_ballot_w64(!(mx[0] * a.c <= thr[0]) || !(mx[1] * a.c <= thr[1]))) {
+                            #pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float bm = row4_reduce(mx[h], OpMax{}) * a.c;
+                                const bool over = pass < k2MaxPasses && m_ref[h] != -INFINITY && bm > thr[h];
+                                overflow |= __builtin_amdgcn_ballot_w64(over) != 0;
+                                if (over) {
+                                    m_ref[h] = bm;
+                                    m_neg[h] = -bm;
+                                    thr[h] = bm + kHeadroom;
+                                }
+                            }
+                        }
+                        const uint32_t pws = pw0 + (uint32_t)(j & 1) * kXPStage;
+                        #pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float e[4];
+                            #pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][i], a.c, m_neg[h]));
+                            l_run[h] += (e[0] + e[1]) + (e[2] + e[3]);
+                            *reinterpret_cast<v2u*>(smem + pws + 16u * h * kXPPitch) =
+                                v2u{Half<TL>::pack2(e[0], e[1]), Half<TL>::pack2(e[2], e[3])};
+                        }
                     }
                 }
             }
@@ -1746,10 +1888,14 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         const int x = swz(key & 15);
         vb0[ks] = key * k8LatBytes + 8u * h + 16u * ((G & 1) ^ (x & 1)) + 32u * (x >> 1);
     }
+    // BS: the addresses of its four column blocks in a register each (the key halves' are 16 rows apart)
+    uint32_t vx[4];
+    #pragma unroll
+    for (int c = 0; c < 4; ++c) vx[c] = vb0[0] ^ (32u * (4 * cq + c));
     typedef __attribute__((address_space(3))) v2i lds_v2i_t;
     auto v_read = [&](uint32_t sbase, int ks, int cb) __attribute__((always_inline)) {
-        const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (lds_v2i_t*)(smem + sbase + (vb0[ks] ^ (32u * cb))));
+        const uint32_t at = BS ? vx[cb & 3] + 16u * k8LatBytes * ks : vb0[ks] ^ (32u * cb);
+        const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t*)(smem + sbase + at));
         return __builtin_bit_cast(v2u, r);
     };
     // P^T of row tile t, key half ks in the B layout: row l32, keys 16ks + 8(l/32) .. +7
@@ -1776,28 +1922,6 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         const uint32_t sb = lds0 + (uint32_t)(j % k8NS) * k8Stage;
         const int kb = __builtin_amdgcn_readfirstlane(k_lo + k2Keys * j + 8 * wv);
         Loads d;
-        if constexpr (BS) {
-            // a 32-key block lies in one page (k_lo is a multiple of 32, a page of 64)
-            const int k0 = __builtin_amdgcn_readfirstlane(k_lo + k2Keys * j);
-            const int page = k0 < k_hi_s ? load_uniform(a.block_table + (int64_t)b * a.max_pages + k0 / a.page_size)
-                                         : -1;
-            const bool there = page >= 0 && page < a.num_pages;
-            const int64_t row = there ? (int64_t)page * a.page_size + k0 % a.page_size : 0;
-            const uint32_t left = there ? (uint32_t)max(0, min(8, k_hi_s - kb)) : 0u;
-            d.st = __builtin_amdgcn_readfirstlane(sb + 8 * wv * k8LatBytes);
-            d.rk = rsrc_span(ck_base + (uint64_t)(row + 8 * wv) * kFR, 0, left * kFR);
-            if (wv == 2) {   // the block's two scale bytes, or (blocks of 16) the two halves' four
-                const bool four = a.scale_shift == 4 && k_hi_s - k0 > 16;
-                d.rp = rsrc_span(reinterpret_cast<uint64_t>(a.scales) + 2 * (uint64_t)(row >> a.scale_shift), 0,
-                                 there ? (four ? 4u : 2u) : 0u);
-                d.st_pe = __builtin_amdgcn_readfirstlane(lds0 + kSBase + 256 * (uint32_t)(j % k8NS));
-            } else {
-                const uint32_t left_p = there ? (uint32_t)max(0, min(16, k_hi_s - k0 - 16 * (wv & 1))) : 0u;
-                d.st_pe = __builtin_amdgcn_readfirstlane(sb + k8LatStage + 16 * (wv & 1) * k8PeBytes);
-                d.rp = rsrc_span(pe_base + (uint64_t)(row + 16 * (wv & 1)) * kFD, 0, left_p * kFD);
-            }
-            return d;
-        }
         const uint32_t left = (uint32_t)max(0, min(8, k_hi_s - kb));
         d.st = __builtin_amdgcn_readfirstlane(sb + 8 * wv * k8LatBytes);
         d.rk = rsrc_span(ck_base + (uint64_t)flash_key_row(a, b, kb, k_hi_s) * kFR, 0, left * kFR);
@@ -1806,6 +1930,56 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         const uint32_t left_p = (uint32_t)max(0, min(16, k_hi_s - kp));
         d.st_pe = __builtin_amdgcn_readfirstlane(sb + k8LatStage + 16 * (wv & 1) * k8PeBytes);
         d.rp = rsrc_span(pe_base + (uint64_t)flash_key_row(a, b, kp, k_hi_s) * kFD, 0, left_p * kFD);
+        return d;
+    };
+    // BS: the blocks' loads in order.  A 32-key block lies in one page (k_lo is a multiple of 32, a page of
+    // 64), and its place in the page goes on from block to block.  The table's entries are in a register,
+    // one a lane, 64 pages at a time: a step waits for neither a division nor a scalar load (whose wait
+    // would be the LDS reads' too).
+    struct Walk { int left, at, entry, stage; };   // keys, row in the page, lane of the entry, ring stage
+    int first_entry = 0, entries = 0;              // of the 64 in the register; the lane's
+    const int last_entry = BS && nb > 0 ? (k_hi_s - 1) / a.page_size : 0;
+    auto issue_entries = [&](int first) __attribute__((always_inline)) {
+        first_entry = first;
+        dma_dword(rsrc_span(reinterpret_cast<uint64_t>(a.block_table + (int64_t)b * a.max_pages + first), 0,
+                            (uint32_t)max(0, min(64, last_entry + 1 - first)) * 4),
+                  __builtin_amdgcn_readfirstlane(lds0 + kTBase + 256 * wv), 4 * lane);
+    };
+    auto take_entries = [&]() __attribute__((always_inline)) {
+        entries = *reinterpret_cast<const int*>(smem + kTBase + 256 * wv + 4 * lane);
+    };
+    const uint32_t rp_off = wv == 2 ? 0u : 16u * (wv & 1) * kFD;
+    const uint64_t rp_base = wv == 2 ? reinterpret_cast<uint64_t>(a.scales) : pe_base + rp_off;
+    const int rp_down = wv == 2 ? a.scale_shift : 0, rp_up = wv == 2 ? 1 : 6;
+    static_assert(kFD == 64 && kFR == 512, "row shifts");
+    auto next_loads = [&](Walk& w) __attribute__((always_inline)) {
+        Loads d;
+        if (w.entry == 64) {
+            issue_entries(first_entry + 64);
+            wait_vm<0>();
+            take_entries();
+            w.entry = 0;
+        }
+        const int page = __builtin_amdgcn_readlane(entries, w.entry);
+        // (no bytes: the address does not matter)
+        const int n = (uint32_t)page < (uint32_t)a.num_pages ? max(0, min(k2Keys, w.left)) : 0;   // keys
+        const int64_t row = (int64_t)page * a.page_size + w.at;
+        d.st = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)w.stage * k8Stage + 8 * wv * k8LatBytes);
+        d.rk = rsrc_span(ck_base + (uint64_t)(row + 8 * wv) * kFR, 0, (uint32_t)max(0, min(8, n - 8 * wv)) * kFR);
+        // the rope rows; wave 2: the block's two scale bytes, or (blocks of 16) the two halves' four
+        d.rp = rsrc_span(rp_base + ((uint64_t)(row >> rp_down) << rp_up), 0,
+                         wv == 2 ? (n == 0 ? 0u : a.scale_shift == 4 && n > 16 ? 4u : 2u)
+                                 : (uint32_t)max(0, min(16, n - 16 * (wv & 1))) * kFD);
+        d.st_pe = __builtin_amdgcn_readfirstlane(wv == 2 ? lds0 + kSBase + 256 * (uint32_t)w.stage
+                                                         : lds0 + (uint32_t)w.stage * k8Stage + k8LatStage +
+                                                               16 * (wv & 1) * k8PeBytes);
+        w.left -= k2Keys;
+        w.at += k2Keys;
+        w.stage = (w.stage + 1) % k8NS;
+        if (w.at == a.page_size) {
+            w.at = 0;
+            ++w.entry;
+        }
         return d;
     };
     // the scale bytes' offsets: lane 2 half + part; the halves share a block unless it is 16 tokens
@@ -1829,7 +2003,9 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     };
     // The tile's queries into the last four stages, free until block 4 is issued after barrier
     // A_0: wave w loads rows 16w .. 16w+15.
+    const int entry0 = BS ? __builtin_amdgcn_readfirstlane(k_lo / a.page_size) : 0;
     if (nb > 0) {
+        if constexpr (BS) issue_entries(entry0);
         const uint32_t rows_q = (uint32_t)min(kFRows, rows_b - r0), row0 = 16 * wv;
         const v4i rq = rsrc_span(reinterpret_cast<uint64_t>(a.qa + ((int64_t)b * rows_b + r0) * kFR), 0,
                                  rows_q * kLatBytes);
@@ -1851,8 +2027,23 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         #pragma unroll
         for (int i = 0; i < 8; ++i) O[i] = v16f{};
         if (nb == 0) break;
+        Walk walk;
+        if constexpr (BS) {
+            walk = {__builtin_amdgcn_readfirstlane(k_hi - k_lo), __builtin_amdgcn_readfirstlane(k_lo % a.page_size), 0, 0};
+            if (pass > 1) {
+                issue_entries(entry0);
+                wait_vm<0>();
+            } else {
+                wait_vm<18>();   // all but the queries' loads
+            }
+            take_entries();
+        }
+        auto loads_at = [&](int j) __attribute__((always_inline)) {
+            if constexpr (BS) return next_loads(walk);
+            else return loads_of(j);
+        };
         #pragma unroll
-        for (int j = 0; j < 4; ++j) issue_block(loads_of(j));
+        for (int j = 0; j < 4; ++j) issue_block(loads_at(j));
         if (pass == 1) {
             wait_blocks(std::integral_constant<int, 4>{});   // the queries have landed
             lds_barrier();                 // Q
@@ -1860,20 +2051,28 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         wait_blocks(std::integral_constant<int, 3>{});       // block 0 has landed
         lds_barrier();                     // A_0
         #pragma unroll
-        for (int j = 4; j <= k8Ahead; ++j) issue_block(loads_of(j));   // their stages are free now
+        for (int j = 4; j <= kAhead; ++j) issue_block(loads_at(j));   // their stages are free now
         lds_barrier();                     // X
+        if constexpr (BS) {                // (P^T of block 0 is written in step 1)
+            const Loads next = loads_at(1 + kAhead);
+            wait_blocks(std::integral_constant<int, kAhead - 1>{});
+            lds_barrier();                 // A_1
+            issue_block(next);
+        }
         #pragma unroll 1
-        for (int j = 1; j <= nb; ++j) {
-            const Loads next = loads_of(j + k8Ahead);
-            // blocks 0 .. j+5 are issued: block j has landed when at most five are in flight
-            wait_blocks(std::integral_constant<int, k8Ahead - 1>{});
+        for (int j = kBehind; j < nb + kBehind; ++j) {
+            Loads next;
+            if constexpr (!BS) next = loads_of(j + kAhead);
+            // blocks 0 .. j + kAhead - 1 are issued: block j has landed when at most kAhead - 1 are in flight
+            wait_blocks(std::integral_constant<int, kAhead - 1>{});
             lds_barrier();                 // A_j
             {
+                const int jb = j - kBehind;   // the block
                 asm volatile("" : "+v"(vb0[0]), "+v"(vb0[1]));
-                const uint32_t sbase = (uint32_t)((j - 1) % k8NS) * k8Stage;
-                if (BS && a.causal && k_lo + k2Keys * j - 1 > lim_first && hidden_nan[(j - 1) & 1] == j)
+                const uint32_t sbase = (uint32_t)(jb % k8NS) * k8Stage;
+                if (BS && a.causal && k_lo + k2Keys * (jb + 1) - 1 > lim_first && hidden_nan[jb & 3] == jb + 1)
                     f8_zero_nan(smem + sbase, cq, lane);
-                const uint32_t prs = pr0 + (uint32_t)((j - 1) & 1) * kXPStage;
+                const uint32_t prs = pr0 + (uint32_t)(jb & 1) * kXPStage;
                 v4u pf[2][2];
                 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -1885,7 +2084,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                 constexpr int kVWin = 3;
                 float s_v[2] = {1.f, 1.f};   // the key halves' scales
                 if constexpr (BS) {
-                    const v4u w = *reinterpret_cast<const v4u*>(smem + kSBase + 256 * ((j - 1) % k8NS));
+                    const v4u w = *reinterpret_cast<const v4u*>(smem + kSBase + 256 * (jb % k8NS));
                     s_v[0] = __uint_as_float(w[0] << 23);
                     s_v[1] = __uint_as_float(w[2] << 23);
                 }
@@ -1901,8 +2100,13 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                         if (f + kVWin < 8) vf[f % kVWin] = v_read(sbase, (f + kVWin) >> 2, 4 * cq + ((f + kVWin) & 3));
                     }
                     O[t & 7] = mfma32h<TL>(cur, pf[t & 1][f >> 2], O[t & 7]);
-                    // block j+6 into stage (j+6) % 8, which block j-2 left at barrier A_j
-                    if (t % 3 == 0 && t / 3 < 4) issue_one(next, t / 3);
+                    // block j + kAhead into the stage that block jb - 1 left at barrier A_j
+                    if constexpr (BS) {
+                        if (t == 1) next = next_loads(walk);   // (behind the MFMAs)
+                        if (t >= 4 && t < 12 && t % 2 == 0) issue_one(next, (t - 4) / 2);
+                    } else {
+                        if (t % 3 == 0 && t / 3 < 4) issue_one(next, t / 3);
+                    }
                     if (t == 13 && five) issue_one(next, 4);
                 }
             }

@@ -59,6 +59,13 @@ __device__ __forceinline__ void dma16_imm(v4i rsrc, uint32_t lds, uint32_t voff)
                  : "s"(lds), "v"(voff), "s"(rsrc), "i"(OFF)
                  : "memory", "m0");
 }
+// A dword per lane: from buffer offset voff into LDS at lds + 4*lane.
+__device__ __forceinline__ void dma_dword(v4i rsrc, uint32_t lds, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(rsrc), "s"(0u)
+                 : "memory", "m0");
+}
 // One byte per lane, zero-extended to a dword: from buffer offset voff into LDS at lds + 4*lane.
 __device__ __forceinline__ void dma_byte(v4i rsrc, uint32_t lds, uint32_t voff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ubyte %1, %2, %3 offen lds"

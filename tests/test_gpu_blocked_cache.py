@@ -579,6 +579,26 @@ def test_attention_equals_one_scale(ext, monkeypatch):
         assert torch.equal(a, b) and torch.isfinite(a.float()).all()
 
 
+@pytest.mark.parametrize("B,Sq,H,Sk,page", [(1, 130, 128, 9000, 64), (2, 128, 64, 6000, 192), (300, 1, 64, 4500, 64)])
+def test_attention_long_walks(ext, monkeypatch, B, Sq, H, Sk, page):
+    """Workgroups that walk over more pages than a register holds entries of (64), from anywhere in the
+    table: again the bits of mla_attention_paged_fp8kv."""
+    monkeypatch.setenv("MLA_OUT_SMALL", "0")
+    g = torch.Generator().manual_seed(Sk)
+    P = 160
+    cache = to_gpu(K.new_pool(P, page, 64, g, 0.0))
+    cache["scales"].fill_(119)
+    table = torch.randint(0, P, (B, -(-Sk // page)), generator=g).int().to(DEV)
+    lens = torch.randint(Sk // 2, Sk + 1, (B,), generator=g)
+    lens[0] = Sk
+    qa, qr, w = (t.to(DEV) for t in K.queries(B, Sq, H, 128, g, BF))
+    a = ext.mla_attention_paged_fp8blk(qa, qr, cache["c_kv"], cache["pe"], cache["scales"], table,
+                                       lens.int().to(DEV), w, SCALE, Sq > 1)
+    b = ext.mla_attention_paged_fp8kv(qa, qr, cache["c_kv"], cache["pe"], table, lens.int().to(DEV), 2.0 ** -8, w,
+                                      SCALE, Sq > 1)
+    assert torch.equal(a, b) and torch.isfinite(a.float()).all()
+
+
 def test_attention_pages_outside_the_pool(ext):
     """A table entry that is no page, among a sequence's keys: rows of zeros, no access."""
     lens = [200, 130]
