@@ -1471,7 +1471,6 @@ constexpr int k8PeBytes = kFD;                         // 64 B per rope row
 constexpr int k8LatStage = 32 * k8LatBytes;            // 16 KB
 constexpr int k8Stage = k8LatStage + 32 * k8PeBytes;   // 18 KB per block
 constexpr int k8NS = 8;                                // ring stages
-constexpr int k8Ahead = k8NS - 2;                      // blocks in flight past the next one
 
 typedef int32_t v2i __attribute__((ext_vector_type(2)));
 
@@ -1512,6 +1511,12 @@ __device__ __forceinline__ void f8_zero_nan(uint8_t* stage, int cq, int lane) {
     }
 }
 
+// f(0), f(1), .. with constants
+template <int... S, typename F>
+__device__ __forceinline__ void unrolled(std::integer_sequence<int, S...>, F& f) {
+    (f(std::integral_constant<int, S>{}), ...);
+}
+
 // BS: a scale for each block of tokens and part (paged, bf16 or fp16 queries).  The conversions
 // take a power-of-two scale for nothing, and the 16 keys of a K fragment, or of a V^T fragment's
 // key half, share theirs (blocks are 16, 32 or 64 tokens), so the operands hold the values
@@ -1531,6 +1536,18 @@ __device__ __forceinline__ void f8_zero_nan(uint8_t* stage, int cq, int lane) {
 // 704, 176, 38.4 (with the softmax behind its own block's MFMAs 733, 183); entries and addresses in
 // registers 699, 176, 38.4 (against 707).  Not kept: K's or V's first reads of the next block in
 // front of the barrier (763 and 740 against 725), P.V waves at a higher priority (723 to 764).
+// fp16 (kRaise): its P ends at 2^16, so a row whose scores climb more than 15 powers of two above its
+// first block's raises its reference in the middle of a pass -- the 16-bit passes repeat the pass then, and
+// with scales that differ from block to block many sequences had a tile that did.  A score wave with
+// such a row raises all of its rows that have a new maximum, by whole powers of two, and their sums with
+// them, and leaves the references in LDS; a step later the other key half's wave follows, and the P.V waves
+// bring O and the lower half's P down.  O goes through memory for it (its chunk's place among the partial
+// rows, unused so far): kept, scaled, and added at the end, while the accumulators start again from zero;
+// scaled in place they were copied at every edge of the loop, and spilled.  128 sequences up to 8,192 keys
+// 281 -> 197 us, 60 up to 4,000 83 -> 66, 32 of 4 queries 143 -> 111, one of 65,536 49.5 -> 47.9, a chunk
+// 743 -> 742; where few rows rise the flags' price shows: four of up to 30,000 keys 46.7 -> 47.6, 2,048
+// queries over themselves 725 -> 759.  (With rows kept at their own places, 16 bytes an access, the four
+// took 50.8.)
 template <typename TL, bool BS>
 __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     constexpr float kHeadroom = Half<TL>::kF16 ? 15.f : k2Headroom;
@@ -1544,7 +1561,11 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     constexpr int kXBase = kPBase + 2 * kXPStage;               // references, sums, flags
     constexpr int kSBase = kXBase + 2 * 128 * 4 + 64;           // BS: the stages' scales
     constexpr int kTBase = kSBase + k8NS * 256;                 // BS: 64 table entries a P.V wave
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[BS ? kTBase + 4 * 256 : kSBase];
+    constexpr bool kRaise = BS && Half<TL>::kF16;               // references rise within a pass
+    constexpr int kRBase = kTBase + 4 * 256;                    // kRaise: raised references, then flags
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kRaise ? kRBase + 2 * 512 + 32 : BS ? kRBase : kSBase];
+    float* raised = reinterpret_cast<float*>(smem + kRBase);    // [block & 1][score wave][32 rows]
+    int* raised_by = reinterpret_cast<int*>(smem + kRBase + 2 * 512);   // [block & 1][score wave], the block + 1
     float* xref = reinterpret_cast<float*>(smem + kXBase);      // [rt][kh][32 rows]
     float* xl = xref + 128;                                     // [rt][kh][32 rows]
     int* flags = reinterpret_cast<int*>(xl + 128);              // [score wave]
@@ -1579,6 +1600,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         // Q^T fragments: step s of lane group g is depth 32s + 8g .. +7 (bf16: 16 bytes), chunk
         // 4s + g of the row (rope: 4 (s - 16) + g), from the ring's last four stages
         v4u qf[2][kQSteps];
+        if (kRaise && lane < 2) raised_by[4 * lane + wave] = -1;
         if (nb > 0) {
             lds_barrier();   // Q: the P.V waves' query loads have landed
             #pragma unroll
@@ -1651,9 +1673,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                         }
                         between(sv);
                     };
-                    [&]<int... S>(std::integer_sequence<int, S...>) __attribute__((always_inline)) {
-                        (step(std::integral_constant<int, S>{}), ...);
-                    }(std::make_integer_sequence<int, kQSteps>{});
+                    unrolled(std::make_integer_sequence<int, kQSteps>{}, step);
                     __builtin_amdgcn_sched_barrier(0);
                     const int kq0 = k_lo + k2Keys * j + 16 * kh;
                     if (kq0 + 15 > lim_wave) {
@@ -1674,8 +1694,29 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                 };
                 // a row past its threshold raises its reference and flags a repeat (NaN scores come
                 // here too); rows without a reference have no visible key
-                auto check = [&]() __attribute__((always_inline)) {
-                    float mx[2];
+                // kRaise: by a whole number of powers of two and at once, its sum with it; P.V and the other
+                // key half's wave take the row's higher reference over in the next step
+                auto raise_to = [&](int h, float ref) __attribute__((always_inline)) {
+                    l_run[h] *= __builtin_amdgcn_exp2f(m_ref[h] - ref);
+                    m_ref[h] = ref;
+                    m_neg[h] = -ref;
+                    thr[h] = ref + kHeadroom;
+                };
+                auto other_rise = [&](int j) __attribute__((always_inline)) {
+                    return raised_by[4 * (j & 1) + (wave ^ 1)];
+                };
+                auto follow = [&](int j, int by) __attribute__((always_inline)) {   // a rise at block j
+                    if (__builtin_amdgcn_readfirstlane(by) != j + 1) return;
+                    #pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float ref = raised[(j & 1) * 128 + (wave ^ 1) * 32 + 16 * h + l16];
+                        if (ref > m_ref[h]) raise_to(h, ref);
+                    }
+                };
+                auto check = [&](int j, int by) __attribute__((always_inline)) {   // block j - 1
+                    if constexpr (kRaise) follow(j - 2, by);
+                    bool rise = false;
+                    float mx[2], top[2] = {0.f, 0.f};
                     #pragma unroll
                     for (int h = 0; h < 2; ++h)
                         mx[h] = fmaxf(fmaxf(sp[h][0], sp[h][1]), fmaxf(sp[h][2], sp[h][3]));
@@ -1683,13 +1724,30 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                         #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float bm = row4_reduce(mx[h], OpMax{}) * a.c;
-                            const bool over = pass < k2MaxPasses && m_ref[h] != -INFINITY && bm > thr[h];
-                            overflow |= __builtin_amdgcn_ballot_w64(over) != 0;
-                            if (over) {
-                                m_ref[h] = bm;
-                                m_neg[h] = -bm;
-                                thr[h] = bm + kHeadroom;
+                            const bool over = (kRaise || pass < k2MaxPasses) && m_ref[h] != -INFINITY && bm > thr[h];
+                            if constexpr (kRaise) {
+                                rise |= __builtin_amdgcn_ballot_w64(over) != 0;
+                                top[h] = bm;
+                            } else {
+                                overflow |= __builtin_amdgcn_ballot_w64(over) != 0;
+                                if (over) {
+                                    m_ref[h] = bm;
+                                    m_neg[h] = -bm;
+                                    thr[h] = bm + kHeadroom;
+                                }
                             }
+                        }
+                        if (kRaise && rise) {
+                            // (every row that has a new maximum: one rise for P.V where there would be
+                            // several, block after block)
+                            #pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                if (m_ref[h] != -INFINITY && top[h] > m_ref[h])
+                                    raise_to(h, m_ref[h] + __builtin_ceilf(top[h] - m_ref[h]));
+                            #pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                if (g == 0) raised[((j - 1) & 1) * 128 + wave * 32 + 16 * h + l16] = m_ref[h];
+                            if (lane == 0) raised_by[4 * ((j - 1) & 1) + wave] = j;
                         }
                     }
                 };
@@ -1727,20 +1785,23 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                 #pragma unroll 1
                 for (int j = 1; j < nb; ++j) {
                     lds_barrier();    // A_j: block j is in LDS, P.V of block j-3 is done
+                    int by = -1;
                     scores(j, [&](auto sv) __attribute__((always_inline)) {
                         constexpr int s = decltype(sv)::value;
-                        if constexpr (s == -1) check();
-                        if constexpr (s == 2) exps(0, j);
-                        if constexpr (s == 6) exps(1, j);
+                        if constexpr (kRaise && s == -1) by = other_rise(j - 2);
+                        if constexpr (s == (kRaise ? 1 : -1)) check(j, by);
+                        if constexpr (s == (kRaise ? 4 : 2)) exps(0, j);
+                        if constexpr (s == (kRaise ? 8 : 6)) exps(1, j);
                     });
                     sp[0] = sc[0];
                     sp[1] = sc[1];
                 }
                 lds_barrier();        // A_nb
-                check();
+                check(nb, kRaise ? other_rise(nb - 2) : -1);
                 exps(0, nb);
                 exps(1, nb);
                 lds_barrier();        // A_nb+1: the last block's P^T
+                if constexpr (kRaise) follow(nb - 1, other_rise(nb - 1));
             } else {
                 #pragma unroll 1
                 for (int j = 0; j <= nb; ++j) {
@@ -2053,61 +2114,161 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         #pragma unroll
         for (int j = 4; j <= kAhead; ++j) issue_block(loads_at(j));   // their stages are free now
         lds_barrier();                     // X
+        float cur[2] = {0.f, 0.f}, before[2] = {0.f, 0.f};   // kRaise: the rows' references, and before a rise
+        if constexpr (kRaise) {
+            #pragma unroll
+            for (int t = 0; t < 2; ++t) cur[t] = fmaxf(xref[t * 64 + l32], xref[t * 64 + 32 + l32]);
+        }
         if constexpr (BS) {                // (P^T of block 0 is written in step 1)
             const Loads next = loads_at(1 + kAhead);
             wait_blocks(std::integral_constant<int, kAhead - 1>{});
             lds_barrier();                 // A_1
             issue_block(next);
         }
-        #pragma unroll 1
-        for (int j = kBehind; j < nb + kBehind; ++j) {
-            Loads next;
-            if constexpr (!BS) next = loads_of(j + kAhead);
-            // blocks 0 .. j + kAhead - 1 are issued: block j has landed when at most kAhead - 1 are in flight
-            wait_blocks(std::integral_constant<int, kAhead - 1>{});
-            lds_barrier();                 // A_j
-            {
-                const int jb = j - kBehind;   // the block
-                asm volatile("" : "+v"(vb0[0]), "+v"(vb0[1]));
-                const uint32_t sbase = (uint32_t)(jb % k8NS) * k8Stage;
-                if (BS && a.causal && k_lo + k2Keys * (jb + 1) - 1 > lim_first && hidden_nan[jb & 3] == jb + 1)
-                    f8_zero_nan(smem + sbase, cq, lane);
-                const uint32_t prs = pr0 + (uint32_t)(jb & 1) * kXPStage;
-                v4u pf[2][2];
+        // (kRaise: a step whose block raised references leaves the inner loop, has O kept, and comes in again
+        // past its barrier)
+        int j = kBehind;
+        bool again_j = false, kept = false;   // kRaise: step j's barrier is behind; O was kept
+        // the place that row tile t's O is kept at, in 16-byte units: 16 of each lane with a row of the tile's
+        // (of which there are n), `step` apart
+        auto kept_place = [&](int t, int* n, int* step) __attribute__((always_inline)) {
+            int tile_rows = min(kFRows, rows_b - r0);
+            asm volatile("" : "+s"(tile_rows));   // (not ahead of the loops: their registers are few)
+            *n = max(0, min(32, tile_rows - 32 * t));
+            *step = 2 * *n;
+            return reinterpret_cast<v4f*>(a.o + (work.slot * rows_b + r0) * kFR) + 32 * cq * tile_rows +
+                   t * 32 * 32 + hw * *n + l32;
+        };
+        for (;;) {
+            if constexpr (kRaise) {
                 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    #pragma unroll
-                    for (int ks = 0; ks < 2; ++ks)
-                        pf[t][ks] = *reinterpret_cast<const v4u*>(smem + prs + t * 32 * kXPPitch + 32u * ks);
-                // fragment f (one per two MFMAs, t = 2f and 2f + 1 for the two row tiles):
-                // key half f/4, column block 4cq + f%4
-                constexpr int kVWin = 3;
-                float s_v[2] = {1.f, 1.f};   // the key halves' scales
-                if constexpr (BS) {
-                    const v4u w = *reinterpret_cast<const v4u*>(smem + kSBase + 256 * (jb % k8NS));
-                    s_v[0] = __uint_as_float(w[0] << 23);
-                    s_v[1] = __uint_as_float(w[2] << 23);
+                for (int i = 0; i < 8; ++i) O[i] = v16f{};
+            }
+            #pragma unroll 1
+            for (; j < nb + kBehind; ++j) {
+                Loads next;
+                if (!kRaise || !again_j) {
+                    if constexpr (!BS) next = loads_of(j + kAhead);
+                    // blocks 0 .. j + kAhead - 1 are issued: block j has landed when at most kAhead - 1 are
+                    // in flight
+                    wait_blocks(std::integral_constant<int, kAhead - 1>{});
+                    lds_barrier();             // A_j
                 }
-                v2u vf[kVWin];
-                #pragma unroll
-                for (int f = 0; f < kVWin; ++f) vf[f] = v_read(sbase, f >> 2, 4 * cq + (f & 3));
-                v4u cur;
-                #pragma unroll
-                for (int t = 0; t < 16; ++t) {
-                    const int f = t >> 1;
-                    if ((t & 1) == 0) {
-                        cur = fp8x8<TL>(vf[f % kVWin], s_v[f >> 2]);
-                        if (f + kVWin < 8) vf[f % kVWin] = v_read(sbase, (f + kVWin) >> 2, 4 * cq + ((f + kVWin) & 3));
-                    }
-                    O[t & 7] = mfma32h<TL>(cur, pf[t & 1][f >> 2], O[t & 7]);
-                    // block j + kAhead into the stage that block jb - 1 left at barrier A_j
+                {
+                    const int jb = j - kBehind;   // the block
+                    asm volatile("" : "+v"(vb0[0]), "+v"(vb0[1]));
+                    const uint32_t sbase = (uint32_t)(jb % k8NS) * k8Stage;
+                    if (BS && a.causal && k_lo + k2Keys * (jb + 1) - 1 > lim_first && hidden_nan[jb & 3] == jb + 1)
+                        f8_zero_nan(smem + sbase, cq, lane);
+                    const uint32_t prs = pr0 + (uint32_t)(jb & 1) * kXPStage;
+                    v4u by = {};
+                    if constexpr (kRaise) by = *reinterpret_cast<const v4u*>(raised_by + 4 * (jb & 1));
+                    v4u pf[2][2];
+                    #pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        #pragma unroll
+                        for (int ks = 0; ks < 2; ++ks)
+                            pf[t][ks] = *reinterpret_cast<const v4u*>(smem + prs + t * 32 * kXPPitch + 32u * ks);
+                    // fragment f (one per two MFMAs, t = 2f and 2f + 1 for the two row tiles):
+                    // key half f/4, column block 4cq + f%4
+                    constexpr int kVWin = 3;
+                    float s_v[2] = {1.f, 1.f};   // the key halves' scales
                     if constexpr (BS) {
-                        if (t == 1) next = next_loads(walk);   // (behind the MFMAs)
-                        if (t >= 4 && t < 12 && t % 2 == 0) issue_one(next, (t - 4) / 2);
-                    } else {
-                        if (t % 3 == 0 && t / 3 < 4) issue_one(next, t / 3);
+                        const v4u w = *reinterpret_cast<const v4u*>(smem + kSBase + 256 * (jb % k8NS));
+                        s_v[0] = __uint_as_float(w[0] << 23);
+                        s_v[1] = __uint_as_float(w[2] << 23);
                     }
-                    if (t == 13 && five) issue_one(next, 4);
+                    v2u vf[kVWin];
+                    #pragma unroll
+                    for (int f = 0; f < kVWin; ++f) vf[f] = v_read(sbase, f >> 2, 4 * cq + (f & 3));
+                    if constexpr (kRaise) {
+                        if (!again_j) {
+                            const bool any = by[0] == jb + 1 || by[1] == jb + 1 || by[2] == jb + 1 || by[3] == jb + 1;
+                            if (__builtin_amdgcn_ballot_w64(any)) {
+                                again_j = true;
+                                break;
+                            }
+                        } else {
+                            // P of the half whose wave had the lower reference comes down to the higher one
+                            #pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                #pragma unroll
+                                for (int ks = 0; ks < 2; ++ks) {
+                                    const float ref = by[2 * t + ks] == jb + 1
+                                                          ? raised[(jb & 1) * 128 + (2 * t + ks) * 32 + l32] : before[t];
+                                    const float fp = ref == cur[t] ? 1.f : __builtin_amdgcn_exp2f(ref - cur[t]);
+                                    #pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        using S = Half<TL>;
+                                        pf[t][ks][i] = S::pack2(S::to_f32(pf[t][ks][i] & 0xffffu) * fp,
+                                                                S::to_f32(pf[t][ks][i] >> 16) * fp);
+                                    }
+                                }
+                            again_j = false;
+                        }
+                    }
+                    v4u frag;
+                    #pragma unroll
+                    for (int t = 0; t < 16; ++t) {
+                        const int f = t >> 1;
+                        if ((t & 1) == 0) {
+                            frag = fp8x8<TL>(vf[f % kVWin], s_v[f >> 2]);
+                            if (f + kVWin < 8) vf[f % kVWin] = v_read(sbase, (f + kVWin) >> 2, 4 * cq + ((f + kVWin) & 3));
+                        }
+                        O[t & 7] = mfma32h<TL>(frag, pf[t & 1][f >> 2], O[t & 7]);
+                        // block j + kAhead into the stage that block jb - 1 left at barrier A_j
+                        if constexpr (BS) {
+                            if (t == 1) next = next_loads(walk);   // (behind the MFMAs)
+                            if (t >= 4 && t < 12 && t % 2 == 0) issue_one(next, (t - 4) / 2);
+                        } else {
+                            if (t % 3 == 0 && t / 3 < 4) issue_one(next, t / 3);
+                        }
+                        if (t == 13 && five) issue_one(next, 4);
+                    }
+                }
+            }
+            if (!kRaise || !again_j) break;
+            const v4u by = *reinterpret_cast<const v4u*>(raised_by + 4 * ((j - kBehind) & 1));
+            #pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                before[t] = cur[t];
+                #pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+                    if ((int)by[2 * t + ks] == j - kBehind + 1)
+                        cur[t] = fmaxf(cur[t], raised[((j - kBehind) & 1) * 128 + (2 * t + ks) * 32 + l32]);
+                const float fo = before[t] == cur[t] ? 1.f : __builtin_amdgcn_exp2f(before[t] - cur[t]);
+                int n, step;
+                v4f* at = kept_place(t, &n, &step);
+                if (l32 < n) {
+                    #pragma unroll
+                    for (int cb = 0; cb < 4; ++cb)
+                        #pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const v16f& o = O[2 * cb + t];
+                            v4f v = {o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]};
+                            if (kept) v += *at;
+                            *at = v * fo;
+                            at += step;
+                        }
+                }
+            }
+            kept = true;
+        }
+        if (kRaise && kept) {
+            #pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                int n, step;
+                const v4f* at = kept_place(t, &n, &step);
+                if (l32 < n) {
+                    #pragma unroll
+                    for (int cb = 0; cb < 4; ++cb)
+                        #pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const v4f v = *at;
+                            at += step;
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) O[2 * cb + t][4 * q + e] += v[e];
+                        }
                 }
             }
         }

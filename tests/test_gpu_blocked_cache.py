@@ -956,3 +956,36 @@ def test_attention_powers_of_two(ext, up, w_up, Sq):
     out = attend(ext, (qa.double() * 2.0 ** -up).to(BF), qr, (w.double() * 2.0 ** e[..., None]).to(BF), moved, table,
                  lens, True)
     assert torch.equal(out.double(), base.double() * 2.0 ** (up + e))
+
+
+@pytest.mark.parametrize("B,Sq,H,Sk", [(1, 1, 128, 3000), (2, 1, 16, 700), (1, 70, 20, 900), (40, 4, 128, 300),
+                                       (1, 3, 3, 65), (130, 2, 128, 200)])
+@pytest.mark.parametrize("kind", ["ramp", "steps", "late", "halves"])
+def test_attention_scores_that_climb(ext, kind, B, Sq, H, Sk):
+    """fp16, whose P ends at 2^16: scores that climb past a row's first reference by hundreds of powers of
+    two, again and again, in one key half or the other, for some rows more than for others; few tokens and
+    many, in one chunk and in several."""
+    page, block = 64, 32
+    g = torch.Generator().manual_seed(B + Sk)
+    P = B * -(-Sk // page) + 2
+    table = K.tables([Sk] * B, page, P, g)
+    cache = K.new_pool(P, page, block, g, 0.0)
+    key = torch.arange(Sk)
+    level = {"ramp": key / Sk * 100, "steps": (key // 150) * 30.0, "late": (key >= Sk - 3) * 200.0,
+             "halves": ((key // 16) % 2) * (key // 40) * 9.0}[kind]          # powers of two
+    # a column of the rope key carries the level: q_r[0] = 1 (or less, by row) against it
+    lev = (level.double() * math.log(2) * SCALE).round()
+    e = max(0, math.ceil(math.log2(max(1.0, float(lev.max())) / 448)))
+    for b in range(B):
+        slots = K.slots_of(table, b, 0, Sk, page)
+        pe = cache["pe"].view(-1, 64)
+        pe[slots] = 0
+        pe[slots, 0] = (lev / 2.0 ** e).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    cache["scales"][..., 1] = 127 + e
+    qa, qr, w = K.queries(B, Sq, H, 128, g, H16)
+    qr.zero_()
+    qr[..., 0] = 1.0 - (torch.arange(H) % 3) * 0.25
+    lens = [Sk] * B
+    rows = [torch.nan_to_num(r) for r in K.decode(cache)]
+    ref = K.attention(qa, qr, rows, table, lens, w, SCALE, Sq > 1, page, P)
+    check_attention(attend(ext, qa, qr, w, cache, table, lens, Sq > 1), ref, H16, True)
