@@ -1563,9 +1563,9 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     constexpr int kTBase = kSBase + k8NS * 256;                 // BS: 64 table entries a P.V wave
     constexpr bool kRaise = BS && Half<TL>::kF16;               // references rise within a pass
     constexpr int kRBase = kTBase + 4 * 256;                    // kRaise: raised references, then flags
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kRaise ? kRBase + 2 * 512 + 32 : BS ? kRBase : kSBase];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kRaise ? kRBase + 2 * 512 + 40 : BS ? kRBase : kSBase];
     float* raised = reinterpret_cast<float*>(smem + kRBase);    // [block & 1][score wave][32 rows]
-    int* raised_by = reinterpret_cast<int*>(smem + kRBase + 2 * 512);   // [block & 1][score wave], the block + 1
+    int* raised_by = reinterpret_cast<int*>(smem + kRBase + 2 * 512);   // [block & 1][score wave], [block & 1] of any
     float* xref = reinterpret_cast<float*>(smem + kXBase);      // [rt][kh][32 rows]
     float* xl = xref + 128;                                     // [rt][kh][32 rows]
     int* flags = reinterpret_cast<int*>(xl + 128);              // [score wave]
@@ -1600,7 +1600,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         // Q^T fragments: step s of lane group g is depth 32s + 8g .. +7 (bf16: 16 bytes), chunk
         // 4s + g of the row (rope: 4 (s - 16) + g), from the ring's last four stages
         v4u qf[2][kQSteps];
-        if (kRaise && lane < 2) raised_by[4 * lane + wave] = -1;
+        if (kRaise && lane < 2) raised_by[4 * lane + wave] = raised_by[8 + lane] = -1;
         if (nb > 0) {
             lds_barrier();   // Q: the P.V waves' query loads have landed
             #pragma unroll
@@ -1747,7 +1747,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                             #pragma unroll
                             for (int h = 0; h < 2; ++h)
                                 if (g == 0) raised[((j - 1) & 1) * 128 + wave * 32 + 16 * h + l16] = m_ref[h];
-                            if (lane == 0) raised_by[4 * ((j - 1) & 1) + wave] = j;
+                            if (lane == 0) raised_by[4 * ((j - 1) & 1) + wave] = raised_by[8 + ((j - 1) & 1)] = j;
                         }
                     }
                 };
@@ -2161,8 +2161,8 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                     if (BS && a.causal && k_lo + k2Keys * (jb + 1) - 1 > lim_first && hidden_nan[jb & 3] == jb + 1)
                         f8_zero_nan(smem + sbase, cq, lane);
                     const uint32_t prs = pr0 + (uint32_t)(jb & 1) * kXPStage;
-                    v4u by = {};
-                    if constexpr (kRaise) by = *reinterpret_cast<const v4u*>(raised_by + 4 * (jb & 1));
+                    int rose = -1;
+                    if constexpr (kRaise) rose = raised_by[8 + (jb & 1)];
                     v4u pf[2][2];
                     #pragma unroll
                     for (int t = 0; t < 2; ++t)
@@ -2183,12 +2183,12 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                     for (int f = 0; f < kVWin; ++f) vf[f] = v_read(sbase, f >> 2, 4 * cq + (f & 3));
                     if constexpr (kRaise) {
                         if (!again_j) {
-                            const bool any = by[0] == jb + 1 || by[1] == jb + 1 || by[2] == jb + 1 || by[3] == jb + 1;
-                            if (__builtin_amdgcn_ballot_w64(any)) {
+                            if (__builtin_amdgcn_readfirstlane(rose) == jb + 1) {
                                 again_j = true;
                                 break;
                             }
                         } else {
+                            const v4u by = *reinterpret_cast<const v4u*>(raised_by + 4 * (jb & 1));
                             // P of the half whose wave had the lower reference comes down to the higher one
                             #pragma unroll
                             for (int t = 0; t < 2; ++t)
