@@ -1647,7 +1647,6 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                 // block j's scores; `between(s)` runs behind step s's MFMAs
                 auto scores = [&](int j, auto between) __attribute__((always_inline)) {
                     constexpr int kWin = 4;
-                    asm volatile("" : "+v"(kb0), "+v"(pb0));
                     const uint32_t sbase = (uint32_t)(j % k8NS) * k8Stage;
                     v2u kf[kWin];
                     const v2u w = *reinterpret_cast<const v2u*>(smem + kSBase + 256 * (j % k8NS) + 8 * kh);
@@ -1812,12 +1811,6 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                         asm volatile("" : "+v"(kb0), "+v"(pb0));
                         const uint32_t sbase = (uint32_t)(j % k8NS) * k8Stage;
                         v2u kf[kWin];
-                        float s_lat = 1.f, s_pe = 1.f;
-                        if constexpr (BS) {
-                            const v2u w = *reinterpret_cast<const v2u*>(smem + kSBase + 256 * (j % k8NS) + 8 * kh);
-                            s_lat = __uint_as_float(w[0] << 23);
-                            s_pe = __uint_as_float(w[1] << 23);
-                        }
                         #pragma unroll
                         for (int i = 0; i < kWin; ++i) kf[i] = k_read(sbase, i);
                         // the compiler's own MFMA (not the asm form of the bf16 kernel): the K
@@ -1826,7 +1819,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                         sc[0] = sc[1] = v4f{};
                         #pragma unroll
                         for (int s = 0; s < kQSteps; ++s) {
-                            const v4u cur = fp8x8<TL>(kf[s % kWin], s < kRSteps ? s_lat : s_pe);
+                            const v4u cur = fp8x8<TL>(kf[s % kWin], 1.f);
                             if (s + kWin < kQSteps) kf[s % kWin] = k_read(sbase, s + kWin);
                             #pragma unroll
                             for (int h = 0; h < 2; ++h) {
@@ -1844,15 +1837,6 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                         const int kq0 = k_lo + k2Keys * j + 16 * kh;
                         if (kq0 + 15 > lim_wave) {
                             const int kq = kq0 + 4 * g;
-                            if constexpr (BS) {
-                                // a hidden key with a NaN: the P.V waves take it out of the block's V
-                                bool nan = false;
-                                #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    nan |= (kq + i > lim0 && sc[0][i] != sc[0][i]) ||
-                                           (kq + i > lim1 && sc[1][i] != sc[1][i]);
-                                if (__builtin_amdgcn_ballot_w64(nan) && lane == 0) hidden_nan[j & 3] = j + 1;
-                            }
                             #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 sc[0][i] = kq + i <= lim0 ? sc[0][i] : -INFINITY;
