@@ -4210,7 +4210,7 @@ FlashPlan plan_flash(const FlashProblem& p) {
         // grid (flash_worklist_kernel); the partial slots, the list and its grid are sized
         // for its largest case
         f.balanced = true;
-        f.max_items = p.scale_block ? wl_max_items16(p.B, f.row_tiles) : wl_max_items(p.B, f.row_tiles);
+        f.max_items = p.scale_block ? wl_max_items16(p.B, f.row_tiles, p.Sk) : wl_max_items(p.B, f.row_tiles);
         // The workgroups work a small list out themselves where they run about once per CU: it costs
         // each of them more than reading one (launch against none, with 3d, us: one sequence, 512 keys
         // 24.8 / 21.7; 16 up to 8,192 50.2 / 43.3; 61 up to 4,989 78.4 / 73.4; 32 of 4 queries up to 1,000

@@ -44,14 +44,37 @@ MLA_HD int wl_max_items(int B, int row_tiles) {
     return (kWlPerCu * kNumCUs / row_tiles + B + 1 + kNumXCDs - 1) / kNumXCDs * kNumXCDs;
 }
 
+// The most splits that dense_keys_per_split (below, 16-bit) gives a sequence of up to Sk keys, from one
+// workgroup per CU up: those whose cost can be less than all fewer splits' (the rule's 3% for one), the cost of
+// s splits taken with blocks / s for its ceiling and the others' with (blocks + t - 1) / t for theirs.  The gain
+// grows with the blocks, so the longest sequence decides; past 33 rounds of CUs there is none.
+constexpr int kWlMostKeys = (1 << 21) - 1;   // Sk's own limit
+MLA_HD int wl_most_splits16(long long base, int Sk) {
+    const long long blocks = (Sk + 31) / 32;
+    for (int s = wl_min(4, (int)blocks); s > 1; --s) {
+        bool can = true;
+        for (int t = 1; t < s; ++t) {   // costs times 12
+            const long long least = (base * s + kNumCUs - 1) / kNumCUs * (blocks * 12 / s + 240) * 1000 +
+                                    12 * (64 * base * s * 2056 * 1000 / 4500000);
+            const long long most = (base * t + kNumCUs - 1) / kNumCUs * ((blocks + t - 1) * 12 / t + 240) * 1000 +
+                                   (t > 1 ? 12 * (64 * base * t * 2056 * 1000 / 4500000) : 0);
+            can &= least * 100 < most * (t == 1 ? 97 : 100);
+        }
+        if (can) return s;
+    }
+    return 1;
+}
+
 // The most items that a 16-bit list can have, by the rules below: pieces of at least an equal share
 // of the keys per CU (CUs / row_tiles of them, and a short one more per sequence); with equal lengths
-// the dense splits, one round of CUs below a CU's worth of tiles, past that up to four a sequence
+// the dense splits, one round of CUs below a CU's worth of tiles, past that wl_most_splits16 a sequence
 // (one where the tiles fill whole rounds).  A list's grid and partial slots are sized for it: the
-// workgroups past the list's end cost little, but there were up to five of them for each that works.
-MLA_HD int wl_max_items16(int B, int row_tiles) {
+// workgroups past the list's end cost little, but there were up to five of them for each that works, and
+// a prefill batch's slots are its memory (15 sequences of 4,000 queries of 128 heads: 16.8 GB with 16
+// items, 67 GB with four a sequence, of which it can use 15).
+MLA_HD int wl_max_items16(int B, int row_tiles, int Sk = kWlMostKeys) {
     const long long base = (long long)B * row_tiles;
-    const int equal = base < kNumCUs || base % kNumCUs == 0 ? B : 4 * B;
+    const int equal = base < kNumCUs || base % kNumCUs == 0 ? B : wl_most_splits16(base, Sk) * B;
     return (wl_max(kNumCUs / row_tiles + B, equal) + kNumXCDs - 1) / kNumXCDs * kNumXCDs;
 }
 
