@@ -279,6 +279,10 @@ __device__ __forceinline__ int scale_byte(float amax) {
     return max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u), kScaleMin);
 }
 __device__ __forceinline__ float scale_value(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+// 1 / scale_value(byte) for bytes 1 .. 254 (the last one's, 2^-127, is subnormal)
+__device__ __forceinline__ float scale_inverse(int byte) {
+    return __uint_as_float(byte < 254 ? (uint32_t)(254 - byte) << 23 : 0x00400000u);
+}
 __device__ __forceinline__ float code_input(float v, float inv) {
     return fabsf(v) < INFINITY ? v * inv : __uint_as_float(0x7fc00000u);
 }
@@ -465,7 +469,7 @@ __global__ void __launch_bounds__(kA8Threads) kv_append_blk_kernel(AppendBlkArgs
     }
     const int e_lat = max(scale_byte(top), old[0]), e_rot = max(scale_byte(top_r), old[1]);
     if (threadIdx.x == 0) { sc[0] = (uint8_t)e_lat; sc[1] = (uint8_t)e_rot; }
-    const float inv_l = scale_value(254 - min(e_lat, 254)), inv_r = scale_value(254 - min(e_rot, 254));
+    const float inv_l = scale_inverse(e_lat), inv_r = scale_inverse(e_rot);
     auto at_lat = [&](int r) __attribute__((always_inline)) { return a.c_kv + (row0 + r) * kA8R + 8 * lane; };
     auto at_rot = [&](int r) __attribute__((always_inline)) { return a.pe + (row0 + r) * kA8D + 2 * (lane & 31); };
     #pragma unroll
