@@ -3891,7 +3891,10 @@ __global__ void __launch_bounds__(512, 1) out_rows_kernel(const uint16_t* __rest
     static_assert(kRowsAhead == 3, "four stages");
     for (int j = 0; j < kRowsAhead; ++j) issue(j);
     // W_uv's values in f16: a row's largest exponent becomes f16's, 30, and those 30 below it zeros
-    float w_scale[4];
+    // d, a product of those by a row's, stays below 2^41; the row's scale times d need not stay in
+    // float32's range where the output does, so of W_uv's power of two as much of a negative exponent as
+    // brings d under 2 goes in front of the row's scale, the rest behind
+    float w_pre[4], w_post[4];
     {
         typedef uint16_t v2h_t __attribute__((ext_vector_type(2)));
         auto two = [](uint32_t w) __attribute__((always_inline)) { return __builtin_bit_cast(v2h_t, w); };
@@ -3914,9 +3917,13 @@ __global__ void __launch_bounds__(512, 1) out_rows_kernel(const uint16_t* __rest
                 wr[s][i] = (w & 0x80008000u) | __builtin_bit_cast(uint32_t, (v2h_t)(m << 3));
             }
         // f16 numbers with bf16's bits (three zeros behind) are 2^112 / 2^down times as large
-        const float back = __uint_as_float((uint32_t)(down + 15) << 23);
+        const int back = down - 112, pre = max(min(back, 0), -40);
         #pragma unroll
-        for (int i = 0; i < 4; ++i) w_scale[i] = __shfl(back, 4 * g + i);   // of the lane's results
+        for (int i = 0; i < 4; ++i) {   // of the lane's results
+            const int from = 4 * g + i;
+            w_pre[i] = __shfl(__builtin_ldexpf(1.f, pre), from);
+            w_post[i] = __shfl(__builtin_ldexpf(1.f, back - pre), from);
+        }
     }
     const uint32_t out_row = (uint32_t)H * V * 2;   // bytes a token
     const int v = c0 + 16 * wave + 4 * g;
@@ -3960,11 +3967,14 @@ __global__ void __launch_bounds__(512, 1) out_rows_kernel(const uint16_t* __rest
         for (int k = 0; k < 2; ++k) {
             const v4f sc = *reinterpret_cast<const v4f*>(smem + kRowsScales + (j & kRowsAhead) * 1024 +
                                                          16 * (16 * k + l16));
-            v4f r = d[k][0] * sc[0];
+            v4f r;
             #pragma unroll
-            for (int q = 1; q < 4; ++q) r += d[k][q] * sc[q];
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] *= w_scale[i];
+            for (int i = 0; i < 4; ++i) {
+                r[i] = d[k][0][i] * w_pre[i] * sc[0];
+                #pragma unroll
+                for (int q = 1; q < 4; ++q) r[i] += d[k][q][i] * w_pre[i] * sc[q];
+                r[i] *= w_post[i];
+            }
             __builtin_amdgcn_raw_buffer_store_b64(v2u{pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3])}, dst,
                                                   (int)(out_voff + 16 * k * out_row), 0, 0);
         }

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import blocked_cache as K
-from test_gpu_blocked_cache import DT, F32, append_inputs, check_append, ext, run_append  # noqa: F401
+from test_gpu_blocked_cache import (BF, DEV, DT, F32, SCALE, append_inputs, attention_case, check_append,  # noqa: F401
+                                    ext, i32, run_append)
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,31 @@ def test_append_under_the_largest_scales(ext, dt, block, byte):  # noqa: F811
     kept = want["touched"] & (want["e"][:, 0] == byte - 127)
     assert int(kept.sum()) >= 1
     check_append(cache, after, want, block)
+
+
+@pytest.mark.parametrize("up,w_up", [(114, -110), (114, 5), (-95, 100), (-60, -20)])
+@pytest.mark.parametrize("B,Sq", [(1, 1), (3, 20), (3, 70), (140, 1)])
+def test_attention_wide_powers_of_two(ext, up, w_up, B, Sq):  # noqa: F811
+    """bf16 values times 2^up and each output column's W_uv times a power of two of its own: the bits but
+    for the exponent, whatever the number of tokens -- nothing behind the softmax leaves float32's range
+    where the output does not.  (Queries of zeros: weights of 1, whose sums stay inside it.  Outputs down to
+    2^-100: what makes their last bit is normal too.)"""
+    g = torch.Generator().manual_seed(Sq)
+    lens = [70, 300, 1200] if B == 3 else [Sq + 200] * B
+    qa, qr, w, cache, table = attention_case(lens, Sq, 32, 64, BF, 3, H=16)
+    qa.zero_(), qr.zero_()
+    moved = {**cache, "scales": cache["scales"].clone()}
+    held = moved["scales"][..., 0] != 255
+    moved["scales"][..., 0][held] = (moved["scales"][..., 0][held].int() + up).to(torch.uint8)
+    e = torch.randint(min(0, w_up), max(0, w_up) + 1, (16, 128), generator=g).double()
+
+    def attend(c, w, scale):
+        return ext.mla_attention_paged_fp8blk(qa.to(DEV), qr.to(DEV), c["c_kv"].to(DEV), c["pe"].to(DEV),
+                                              c["scales"].to(DEV), table.to(DEV), i32(lens).to(DEV), w.to(DEV),
+                                              scale, True).cpu()
+
+    base = attend(cache, w, SCALE)
+    out = attend(moved, (w.double() * 2.0 ** e[..., None]).to(BF), SCALE * 2.0 ** up)
+    want = base.double() * 2.0 ** (up + e)
+    assert want.abs().max() < torch.finfo(BF).max
+    assert torch.equal(out.double(), want)
