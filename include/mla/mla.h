@@ -437,8 +437,9 @@ int mla_kv_read_fp8blk(mla_dtype_t dtype, const int64_t* slots, int64_t n,
 
 /* Attention over that cache: mla_attention_paged on its values, with bf16 or fp16 queries, W_uv
  * and output (values enter the products in that type: exact in bf16's normal range, and in
- * fp16's).  Same block_table, seq_lens and causal rule; a sequence or query that sees no key gives
- * zero rows, and rows of a page outside the pool count as zeros. */
+ * fp16's; a key with a NaN, or with a value past that type's range, which is infinite there,
+ * reaches only the queries that see it).  Same block_table, seq_lens and causal rule; a sequence or
+ * query that sees no key gives zero rows, and rows of a page outside the pool count as zeros. */
 size_t mla_attention_paged_fp8blk_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims,
                                                   int causal, int32_t page_size);
 int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_absorbed,

@@ -1490,13 +1490,19 @@ __device__ __forceinline__ v4u fp8x8(v2u r, float scale) {
     return v4u{two(r[0], lo), two(r[0], hi), two(r[1], lo), two(r[1], hi)};
 }
 
-// A NaN in a key that some of a tile's queries do not see would reach them through P.V, where their P
-// is 0: 0 * NaN.  Queries that do see it have it from their scores, since the latent row is key and
-// value, so V may do without: a P.V wave writes zeros over the NaN codes (0x7F, 0xFF) of its 128
-// columns of a block, whose K has been read by then.  (A causal block that ends past the first row's
-// last key, and in it a NaN score at a hidden place: the score waves note such blocks.)
-__device__ __forceinline__ void f8_zero_nan(uint8_t* stage, int cq, int lane) {
+// A value that is not finite, in a key that some of a tile's queries do not see, would reach them through
+// P.V, where their P is 0: 0 * NaN, or 0 * inf where code * scale is past TL's range.  Queries that do see
+// it have it from their scores, since the latent row is key and value, so V may do without: a P.V wave
+// writes zeros over such codes of its 128 columns of a block, whose K has been read by then: NaN (0x7F,
+// 0xFF), and magnitudes of at least 2^16 (fp16; bf16 2^128) over the scale of the key's 16, whose code
+// is a power of two's or a subnormal one.  (A causal block that ends past the first row's last key, and
+// in it a score that is not finite at a hidden place: the score waves note such blocks.)
+template <typename TL>
+__device__ __forceinline__ void f8_zero_hidden(uint8_t* stage, const uint32_t* scales, int cq, int lane) {
     const int key = lane >> 1;
+    const int e = (Half<TL>::kF16 ? 16 : 128) + 127 - (int)scales[2 * (key >> 4)];   // the code 2^e
+    const uint32_t least = e > 8 ? 0x7f : e >= -6 ? 8 * (e + 7) : e >= -9 ? 1 << (e + 9) : 1;
+    const uint32_t add = (0x80 - least) * 0x01010101u;
     uint8_t* row = stage + key * k8LatBytes + 256 * (cq >> 1);
     #pragma unroll
     for (int m = 0; m < 4; ++m) {
@@ -1504,7 +1510,7 @@ __device__ __forceinline__ void f8_zero_nan(uint8_t* stage, int cq, int lane) {
         v4u w = *p;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t top = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // bit 7 of each NaN
+            const uint32_t top = ((w[i] & 0x7f7f7f7fu) + add) & 0x80808080u;   // bit 7 of each from `least` up
             w[i] &= ~(top | (top - (top >> 7)));
         }
         *p = w;
@@ -1569,7 +1575,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     float* xref = reinterpret_cast<float*>(smem + kXBase);      // [rt][kh][32 rows]
     float* xl = xref + 128;                                     // [rt][kh][32 rows]
     int* flags = reinterpret_cast<int*>(xl + 128);              // [score wave]
-    int* hidden_nan = flags + 8;                                // BS: [block & 3], the block + 1
+    int* hidden_bad = flags + 8;                                // BS: [block & 3], the block + 1
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4, l32 = lane & 31, hw = lane >> 5;
@@ -1601,6 +1607,7 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
         // 4s + g of the row (rope: 4 (s - 16) + g), from the ring's last four stages
         v4u qf[2][kQSteps];
         if (kRaise && lane < 2) raised_by[4 * lane + wave] = raised_by[8 + lane] = -1;
+        if (BS && lane == 0) hidden_bad[wave] = 0;
         if (nb > 0) {
             lds_barrier();   // Q: the P.V waves' query loads have landed
             #pragma unroll
@@ -1677,13 +1684,13 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                     const int kq0 = k_lo + k2Keys * j + 16 * kh;
                     if (kq0 + 15 > lim_wave) {
                         const int kq = kq0 + 4 * g;
-                        // a hidden key with a NaN: the P.V waves take it out of the block's V
-                        bool nan = false;
+                        // a hidden key with a NaN or an infinity: the P.V waves take it out of the block's V
+                        bool bad = false;
                         #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            nan |= (kq + i > lim0 && sc[0][i] != sc[0][i]) ||
-                                   (kq + i > lim1 && sc[1][i] != sc[1][i]);
-                        if (__builtin_amdgcn_ballot_w64(nan) && lane == 0) hidden_nan[j & 3] = j + 1;
+                            bad |= (kq + i > lim0 && !(fabsf(sc[0][i]) < INFINITY)) ||
+                                   (kq + i > lim1 && !(fabsf(sc[1][i]) < INFINITY));
+                        if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) hidden_bad[j & 3] = j + 1;
                         #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             sc[0][i] = kq + i <= lim0 ? sc[0][i] : -INFINITY;
@@ -1723,7 +1730,10 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                         #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float bm = row4_reduce(mx[h], OpMax{}) * a.c;
-                            const bool over = (kRaise || pass < k2MaxPasses) && m_ref[h] != -INFINITY && bm > thr[h];
+                            // (kRaise: not for a score of infinity, whose row is NaN either way: a rise moves the
+                            // last bits of the other rows, which may not see that key)
+                            const bool over = (kRaise ? bm < INFINITY : pass < k2MaxPasses) &&
+                                              m_ref[h] != -INFINITY && bm > thr[h];
                             if constexpr (kRaise) {
                                 rise |= __builtin_amdgcn_ballot_w64(over) != 0;
                                 top[h] = bm;
@@ -2142,8 +2152,9 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                     const int jb = j - kBehind;   // the block
                     asm volatile("" : "+v"(vb0[0]), "+v"(vb0[1]));
                     const uint32_t sbase = (uint32_t)(jb % k8NS) * k8Stage;
-                    if (BS && a.causal && k_lo + k2Keys * (jb + 1) - 1 > lim_first && hidden_nan[jb & 3] == jb + 1)
-                        f8_zero_nan(smem + sbase, cq, lane);
+                    if (BS && a.causal && k_lo + k2Keys * (jb + 1) - 1 > lim_first && hidden_bad[jb & 3] == jb + 1)
+                        f8_zero_hidden<TL>(smem + sbase,
+                                           reinterpret_cast<const uint32_t*>(smem + kSBase + 256 * (jb % k8NS)), cq, lane);
                     const uint32_t prs = pr0 + (uint32_t)(jb & 1) * kXPStage;
                     int rose = -1;
                     if constexpr (kRaise) rose = raised_by[8 + (jb & 1)];

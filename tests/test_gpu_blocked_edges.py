@@ -58,3 +58,39 @@ def test_attention_wide_powers_of_two(ext, up, w_up, B, Sq):  # noqa: F811
     want = base.double() * 2.0 ** (up + e)
     assert want.abs().max() < torch.finfo(BF).max
     assert torch.equal(out.double(), want)
+
+
+@pytest.mark.parametrize("dt,up,code", [("f16", 13, 0x50), ("f16", 13, 0xFE), ("bf16", 120, 0x78), ("bf16", 120, 0xFE)])
+@pytest.mark.parametrize("Sq,H,lens,at", [(4, 16, [300, 33, 4], 2), (3, 3, [500, 17], 1), (20, 10, [500, 33, 64], 18),
+                                          (50, 16, [50, 100, 900], 17), (70, 3, [700, 70], 1)])
+def test_attention_hidden_values_past_the_range(ext, dt, up, code, Sq, H, lens, at):  # noqa: F811
+    """A value of 2^16 or more in fp16 (2^128 in bf16) in a token's latent row: the queries in front of it,
+    which do not see it, keep their bits, in its block and in the blocks beside it."""
+    dt, page, block = DT[dt], 64, 16
+    g = torch.Generator().manual_seed(Sq)
+    P = sum(-(-n // page) for n in lens) + 2
+    table = K.tables(lens, page, P, g)
+    # codes under 2^0 are values of unit spread (at most 7, so that 2^13 of them stay in fp16's range)
+    cache = {"c_kv": K.encode(torch.randn(P, 4, 16, K.KV, generator=g, dtype=K.F64).clamp(-7, 7),
+                              torch.zeros(P, 4)).view(P, page, K.KV),
+             "pe": K.encode(torch.randn(P, 4, 16, K.ROPE, generator=g, dtype=K.F64), torch.zeros(P, 4)).view(P, page, -1),
+             "scales": torch.full((P, page // block, 2), 127, dtype=torch.uint8)}
+    cache["scales"][..., 0] += up
+    qa, qr, w = K.queries(len(lens), Sq, H, 64, g, dt)
+    w = (w.double() * 2.0 ** -min(up, 100)).to(dt)
+
+    def attend(c):
+        return ext.mla_attention_paged_fp8blk(qa.to(DEV), qr.to(DEV), c["c_kv"].to(DEV), c["pe"].to(DEV),
+                                              c["scales"].to(DEV), table.to(DEV), i32(lens).to(DEV), w.to(DEV),
+                                              SCALE * 2.0 ** up, True).cpu()
+
+    clean = attend(cache)
+    assert torch.isfinite(clean).all()
+    for column in (3, 300):
+        bad = {k: v.clone() for k, v in cache.items()}
+        for b, n in enumerate(lens):
+            slot = int(K.slots_of(table, b, n - Sq + at, n - Sq + at + 1, page)[0])
+            bad["c_kv"].view(-1, K.KV)[slot, column] = code
+        out = attend(bad)
+        assert torch.equal(out[:, :at], clean[:, :at])
+        assert not torch.equal(out[:, at:], clean[:, at:])
