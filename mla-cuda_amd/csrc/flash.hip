@@ -3434,6 +3434,20 @@ __global__ void __launch_bounds__(512) flash_merge_many_kernel(const float* __re
     }
 }
 
+// Two values in two 16-bit terms each: hi, rounded to nearest, and lo, what that left, rounded: 16 significant
+// bits in bf16, 22 in f16 (of values below 2^-3 fewer: lo's steps end at 2^-24).  lo has to be formed from
+// hi's own bits: told that they are a conversion, the compiler makes it again for lo, in one instruction
+// with the product that the value comes from and so with one rounding where hi had two -- now and then f16's
+// other neighbour, and hi + lo a whole step off.
+template <typename TL>
+__device__ __forceinline__ void two_terms(float a, float b, uint32_t* hi, uint32_t* lo) {
+    using S = Half<TL>;
+    uint32_t h = S::pack2(a, b);
+    asm("" : "+v"(h));
+    *hi = h;
+    *lo = S::pack2(a - S::to_f32(h & 0xffffu), b - S::to_f32(h >> 16));
+}
+
 // 3d of a few tokens with the merge of their chunks in it: a workgroup takes a head and 64 output
 // columns.  Alone the merge writes a row per token and head that the product then waits a launch for,
 // and a GEMM tile is nearly empty at these token counts; here W_uv's rows are in flight while the
@@ -3444,8 +3458,8 @@ __global__ void __launch_bounds__(512) flash_merge_many_kernel(const float* __re
 //     in order.  The two workgroups of a head both read its rows (at most kOutListRows, 2 KB each), so
 //     they run on one XCD and the second read hits its L2: on two XCDs 65,536 keys' 33.5 MB of rows
 //     came twice from memory, 60.4 us with the pass against 58.6 for separate launches.
-//   product: 16x16x32 MFMAs, W_uv's rows by the tokens.  The merged row keeps fp32's precision in two
-//     16-bit terms, v = hi + lo: tokens' hi are columns 0-7, their lo 8-15, added at the end.  Wave w has
+//   product: 16x16x32 MFMAs, W_uv's rows by the tokens.  The merged row goes in as two
+//     16-bit terms (two_terms): tokens' hi are columns 0-7, their lo 8-15, added at the end.  Wave w has
 //     rows 16 (w % 4) and K half w / 4; the halves are added through LDS.
 constexpr int kOutListRows = 320;   // chunks' rows a head: Sq * wl_max_items16 at 8 tokens or fewer
 constexpr int kOutListPitch = kFR * 2 + 16;   // bytes of a column in LDS
@@ -3549,12 +3563,11 @@ __global__ void __launch_bounds__(512) out_list_kernel(const float* __restrict__
     for (int t = group; t < M; t += 4) {
         v4f v = sums[t * parts][c4];
         for (int q = 1; q < parts; ++q) v += sums[t * parts + q][c4];
-        using S = Half<TL>;
-        const v2u hi = {S::pack2(v[0], v[1]), S::pack2(v[2], v[3])};
-        const v2u lo = {S::pack2(v[0] - S::to_f32(hi[0] & 0xffffu), v[1] - S::to_f32(hi[0] >> 16)),
-                        S::pack2(v[2] - S::to_f32(hi[1] & 0xffffu), v[3] - S::to_f32(hi[1] >> 16))};
-        *reinterpret_cast<v2u*>(cols + t * kOutListPitch + 8 * c4) = hi;
-        *reinterpret_cast<v2u*>(cols + (t + kOutListTokens) * kOutListPitch + 8 * c4) = lo;
+        uint32_t hi[2], lo[2];
+        two_terms<TL>(v[0], v[1], &hi[0], &lo[0]);
+        two_terms<TL>(v[2], v[3], &hi[1], &lo[1]);
+        *reinterpret_cast<v2u*>(cols + t * kOutListPitch + 8 * c4) = v2u{hi[0], hi[1]};
+        *reinterpret_cast<v2u*>(cols + (t + kOutListTokens) * kOutListPitch + 8 * c4) = v2u{lo[0], lo[1]};
     }
     __syncthreads();
     // (a column without a token multiplies whatever is there into its own sums, which nobody reads)
@@ -3701,16 +3714,14 @@ __global__ void __launch_bounds__(512, 1) out_merge_kernel(const float* __restri
             }
             a *= inv;
             b *= inv;
-            using S = Half<TL>;
-            v4u hi, lo;
+            uint32_t hi[4], lo[4];
             #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float p = k < 2 ? a[2 * k] : b[2 * k - 4], q = k < 2 ? a[2 * k + 1] : b[2 * k - 3];
-                hi[k] = S::pack2(p, q);
-                lo[k] = S::pack2(p - S::to_f32(hi[k] & 0xffffu), q - S::to_f32(hi[k] >> 16));
-            }
-            *reinterpret_cast<v4u*>(cols[buf] + (wave + 8 * i) * kOutListPitch + 16 * lane) = hi;
-            *reinterpret_cast<v4u*>(cols[buf] + (kOutTile + wave + 8 * i) * kOutListPitch + 16 * lane) = lo;
+            for (int k = 0; k < 4; ++k)
+                two_terms<TL>(k < 2 ? a[2 * k] : b[2 * k - 4], k < 2 ? a[2 * k + 1] : b[2 * k - 3], &hi[k], &lo[k]);
+            *reinterpret_cast<v4u*>(cols[buf] + (wave + 8 * i) * kOutListPitch + 16 * lane) =
+                v4u{hi[0], hi[1], hi[2], hi[3]};
+            *reinterpret_cast<v4u*>(cols[buf] + (kOutTile + wave + 8 * i) * kOutListPitch + 16 * lane) =
+                v4u{lo[0], lo[1], lo[2], lo[3]};
         }
         if (tile + share < tiles) fetch(tile + share);
         lds_barrier();
@@ -3780,20 +3791,19 @@ __global__ void __launch_bounds__(512, 1) out_terms_kernel(const uint16_t* __res
     // tile's rows, in set[which], to LDS; then the rows two tiles on
     auto convert = [&](int tile, auto which) __attribute__((always_inline)) {
         constexpr int buf = decltype(which)::value;
-        using S = Half<f16_t>;
         #pragma unroll
         for (int i = 0; i < kTok; ++i) {
-            v4u hi, lo;
+            uint32_t hi[4], lo[4];
             #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t w = set[buf].x[i][k];
-                const float p = (float)(int16_t)(w & 0xffffu) * set[buf].s[i];
-                const float q = (float)((int32_t)w >> 16) * set[buf].s[i];
-                hi[k] = S::pack2(p, q);
-                lo[k] = S::pack2(p - S::to_f32(hi[k] & 0xffffu), q - S::to_f32(hi[k] >> 16));
+                two_terms<f16_t>((float)(int16_t)(w & 0xffffu) * set[buf].s[i], (float)((int32_t)w >> 16) * set[buf].s[i],
+                                 &hi[k], &lo[k]);
             }
-            *reinterpret_cast<v4u*>(cols[buf] + (wave + 8 * i) * kOutListPitch + 16 * lane) = hi;
-            *reinterpret_cast<v4u*>(cols[buf] + (kRowsTile + wave + 8 * i) * kOutListPitch + 16 * lane) = lo;
+            *reinterpret_cast<v4u*>(cols[buf] + (wave + 8 * i) * kOutListPitch + 16 * lane) =
+                v4u{hi[0], hi[1], hi[2], hi[3]};
+            *reinterpret_cast<v4u*>(cols[buf] + (kRowsTile + wave + 8 * i) * kOutListPitch + 16 * lane) =
+                v4u{lo[0], lo[1], lo[2], lo[3]};
         }
         fetch(set[buf], tile + 2 * share);
     };
