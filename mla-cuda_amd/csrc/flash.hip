@@ -1501,7 +1501,7 @@ template <typename TL>
 __device__ __forceinline__ void f8_zero_hidden(uint8_t* stage, const uint32_t* scales, int cq, int lane) {
     const int key = lane >> 1;
     const int e = (Half<TL>::kF16 ? 16 : 128) + 127 - (int)scales[2 * (key >> 4)];   // the code 2^e
-    const uint32_t least = e > 8 ? 0x7f : e >= -6 ? 8 * (e + 7) : e >= -9 ? 1 << (e + 9) : 1;
+    const uint32_t least = min(max(8 * (e + 7), 1 << min(max(e + 9, 0), 3)), 0x7f);
     const uint32_t add = (0x80 - least) * 0x01010101u;
     uint8_t* row = stage + key * k8LatBytes + 256 * (cq >> 1);
     #pragma unroll

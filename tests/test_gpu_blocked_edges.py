@@ -60,7 +60,8 @@ def test_attention_wide_powers_of_two(ext, up, w_up, B, Sq):  # noqa: F811
     assert torch.equal(out.double(), want)
 
 
-@pytest.mark.parametrize("dt,up,code", [("f16", 13, 0x50), ("f16", 13, 0xFE), ("bf16", 120, 0x78), ("bf16", 120, 0xFE)])
+@pytest.mark.parametrize("dt,up,code", [("f16", 13, 0x50), ("f16", 13, 0xFE), ("f16", 24, 0x02), ("bf16", 120, 0x78),
+                                        ("bf16", 120, 0xFE)])
 @pytest.mark.parametrize("Sq,H,lens,at", [(4, 16, [300, 33, 4], 2), (3, 3, [500, 17], 1), (20, 10, [500, 33, 64], 18),
                                           (50, 16, [50, 100, 900], 17), (70, 3, [700, 70], 1)])
 def test_attention_hidden_values_past_the_range(ext, dt, up, code, Sq, H, lens, at):  # noqa: F811
@@ -75,9 +76,11 @@ def test_attention_hidden_values_past_the_range(ext, dt, up, code, Sq, H, lens, 
                               torch.zeros(P, 4)).view(P, page, K.KV),
              "pe": K.encode(torch.randn(P, 4, 16, K.ROPE, generator=g, dtype=K.F64), torch.zeros(P, 4)).view(P, page, -1),
              "scales": torch.full((P, page // block, 2), 127, dtype=torch.uint8)}
+    if up == 24:   # under 2^24 the code 1 is 2^15, and 2 is past the range
+        cache["c_kv"] = torch.tensor([0, 1, 0x81], dtype=torch.uint8)[torch.randint(0, 3, cache["c_kv"].shape, generator=g)]
     cache["scales"][..., 0] += up
     qa, qr, w = K.queries(len(lens), Sq, H, 64, g, dt)
-    w = (w.double() * 2.0 ** -min(up, 100)).to(dt)
+    w = (w.double() * 2.0 ** -{13: 13, 24: 8, 120: 100}[up]).to(dt)
 
     def attend(c):
         return ext.mla_attention_paged_fp8blk(qa.to(DEV), qr.to(DEV), c["c_kv"].to(DEV), c["pe"].to(DEV),
