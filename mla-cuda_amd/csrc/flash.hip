@@ -1556,6 +1556,7 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, S...>, F& f)
 // took 50.8.)
 template <typename TL, bool BS>
 __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
+    static_assert(BS || !Half<TL>::kF16, "a cache of one scale is read with bf16 queries");
     constexpr float kHeadroom = Half<TL>::kF16 ? 15.f : k2Headroom;
     constexpr int kBehind = BS ? 2 : 1;                         // P.V works on block j - kBehind in step j
     constexpr int kAhead = k8NS - 1 - kBehind;                  // blocks in flight past the one in work
@@ -1832,16 +1833,10 @@ __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
                             const v4u cur = fp8x8<TL>(kf[s % kWin], 1.f);
                             if (s + kWin < kQSteps) kf[s % kWin] = k_read(sbase, s + kWin);
                             #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                if constexpr (Half<TL>::kF16)
-                                    sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                        __builtin_bit_cast(v8h, cur), __builtin_bit_cast(v8h, qf[h][s]), sc[h],
-                                        0, 0, 0);
-                                else
-                                    sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                        __builtin_bit_cast(v8bf, cur), __builtin_bit_cast(v8bf, qf[h][s]), sc[h],
-                                        0, 0, 0);
-                            }
+                            for (int h = 0; h < 2; ++h)
+                                sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    __builtin_bit_cast(v8bf, cur), __builtin_bit_cast(v8bf, qf[h][s]), sc[h],
+                                    0, 0, 0);
                         }
                         __builtin_amdgcn_sched_barrier(0);
                         const int kq0 = k_lo + k2Keys * j + 16 * kh;
@@ -3461,7 +3456,7 @@ __device__ __forceinline__ void two_terms(float a, float b, uint32_t* hi, uint32
 //   product: 16x16x32 MFMAs, W_uv's rows by the tokens.  The merged row goes in as two
 //     16-bit terms (two_terms): tokens' hi are columns 0-7, their lo 8-15, added at the end.  Wave w has
 //     rows 16 (w % 4) and K half w / 4; the halves are added through LDS.
-constexpr int kOutListRows = 320;   // chunks' rows a head: Sq * wl_max_items16 at 8 tokens or fewer
+constexpr int kOutListRows = 320;   // chunks' rows a head that fit (out_list_kind sends others to out_merge_kernel)
 constexpr int kOutListPitch = kFR * 2 + 16;   // bytes of a column in LDS
 template <typename TL>
 __global__ void __launch_bounds__(512) out_list_kernel(const float* __restrict__ o,
@@ -4523,7 +4518,8 @@ hipError_t launch_flash(const FlashProblem& p, const FlashPlan& f, float* ctx, f
     if (e != hipSuccess || (!f.balanced && f.n_split == 1)) return e;
     if (!merge) return e;   // the caller folds the merge in
     const int n = f.n_split;
-    if (rows <= kMergeManyRows && !packed) {   // (packed rows are more)
+    static_assert(kMergeManyRows <= kOutMergeTokens, "packed rows are more");
+    if (rows <= kMergeManyRows) {
         const dim3 grid2((unsigned)(2 * rows)), block2(512);
         if (!ctx16)
             hipLaunchKernelGGL(flash_merge_many_kernel<kOutF32>, grid2, block2, 0, stream, a.o, a.m, a.l,
