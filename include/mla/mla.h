@@ -436,10 +436,17 @@ int mla_kv_read_fp8blk(mla_dtype_t dtype, const int64_t* slots, int64_t n,
                        void* rope, hipStream_t stream);
 
 /* Attention over that cache: mla_attention_paged on its values, with bf16 or fp16 queries, W_uv
- * and output (values enter the products in that type: exact in bf16's normal range, and in
- * fp16's; a key with a NaN, or with a value past that type's range, which is infinite there,
- * reaches only the queries that see it).  Same block_table, seq_lens and causal rule; a sequence or
- * query that sees no key gives zero rows, and rows of a page outside the pool count as zeros. */
+ * and output.  Same block_table, seq_lens and causal rule; a sequence or query that sees no key gives
+ * zero rows, and rows of a page outside the pool count as zeros.
+ * Values enter the products in the queries' type: exact in bf16's normal range, and in fp16's.  A key
+ * with a NaN, or with a value past that type's range, which is infinite there, reaches only the
+ * queries that see it.  What is rounded on the way: each key's weight to that type, before the
+ * division by the row's sum (sums are float32, of weights up to 2^64 in bf16, 2^16 in fp16: values
+ * past about 2^40 in bf16 may leave its range where scores climb), the rows between the softmax and W_uv,
+ * and the output.  Those rows: up to 128 tokens (batch * sq) two terms of the type; past that 16 bits
+ * under a float32 scale for each 128 columns -- bf16: 11 significant bits down to 2^-29 of the largest
+ * (and W_uv's own bits down to 2^-29 of its row's largest), fp16: 2^-16 of the largest; columns that
+ * stay below 2^-110 are zeros there.  MLA_OUT_SMALL=0 keeps them in the type itself. */
 size_t mla_attention_paged_fp8blk_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims,
                                                   int causal, int32_t page_size);
 int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_absorbed,

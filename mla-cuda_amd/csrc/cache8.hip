@@ -58,7 +58,7 @@ constexpr int kExtendThreads = 1024;   // at most
 constexpr int kExtendWaves = kExtendThreads / 64;
 
 // x / d for 0 <= x < 2^31 and a d that the host knows (a division takes forty instructions, and each
-// request's plan has five): with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// request's plan has five), by the method of Granlund and Montgomery (1994): with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
 // x / d = (floor(m x / 2^32) + x) / 2^s, where the sum stays below 2^32.
 struct FastDiv {
     uint32_t d, m;

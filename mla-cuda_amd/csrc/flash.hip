@@ -842,10 +842,14 @@ constexpr uint32_t kPvOutBytes = 64 * 512;
 // Packed rows: the same normalised rows for 3d of many tokens (out_rows_kernel, out_terms_kernel), in the
 // bytes of 16-bit rows but nearly free of their rounding, which is a third of the outputs' (P, row, output).
 // Each 128 columns of a row have a float32 scale, their largest magnitude / 32767, and
-//   bf16: f16 numbers, off by 2^-12 of a value at most (bf16's by 2^-9), normal down to 2^-29 of the largest;
-//   f16: integers, off by 2^-16 of the largest.
-// In the 2-norm the outputs of a prefill chunk are 2.4e-3 off with them, 2.9e-3 with bf16 rows; rows in
-// float32 took 7% of the call's time.
+//   bf16: f16 numbers, off by 2^-11 of a value at most (bf16's by 2^-8), normal down to 2^-29 of the largest;
+//   f16: integers, off by 2^-16 of the largest (an f16 number by 2^-11 of itself: columns from 2^-5 of the
+//     largest up are held better, smaller ones less well).
+// They are kept for the outputs' accuracy, at any number of tokens past 128.  In the 2-norm, with them and with
+// rows in the type itself (their launches: the merge, the GEMM): bf16 2.3e-3 and 2.8e-3, f16 2.9e-4 and
+// 3.6e-4.  The calls (us, bf16; f16): 129 sequences up to 4,000 keys 112 and 112; 132 and 128, 200 up to 500 59 and
+// 58; 72 and 65, 43 of 4 queries up to 3,000 106 and 105; 122 and 117, four of 333 over 2,011 695 and 688; 732
+// and 732, one of 2,048 over itself 711 and 713; 769 and 765.  Rows in float32 took 7% of a chunk's time.
 constexpr float kPackMax = 32767.f;
 // max(|a|, |b|, m), NaN if one of them is
 __device__ __forceinline__ float magnitude3(float a, float b, float m) {
@@ -1534,9 +1538,12 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, S...>, F& f)
 // byte 255 would make their zero codes NaN).
 // BS's steps are one apart from the others': the softmax of block j - 1 runs between the score MFMAs of
 // block j, and P.V works on block j - 2, so a score wave's chain of MFMAs and its exponentials overlap.
-// What bounds a step is each wave's own stream of instructions (a score wave's 36 MFMAs and 72
-// conversions, a P.V wave's 16 and 32, at about 8 cycles an instruction), so the rest was cut: the next
-// block's descriptors behind the first P.V MFMAs, page entries in a register, addresses kept.  Measured
+// No unit is full: the counters of a prefill chunk give the matrix cores 46% of the cycles, and of a wave's time
+// 38% to issuing (1.29e8 VALU instructions, 2.7e7 of them MFMAs and 5.6e7 conversions), 28% to waiting for
+// its turn to issue and 34% to barriers and loads.  What a step takes is each wave's own stream of instructions
+// (a score wave's 36 MFMAs and 72 conversions, a P.V wave's 16 and 32) and the other waves' at the barrier, so
+// the rest was cut: the next block's descriptors behind the first P.V MFMAs, page entries in a register,
+// addresses kept.  Measured
 // (us): descriptors in front of the step's barrier, with a division and a scalar load, a chunk of four
 // sequences' 333 queries 769, 128 sequences up to 8,192 keys 186, one of 65,536 39.9; behind the MFMAs
 // 704, 176, 38.4 (with the softmax behind its own block's MFMAs 733, 183); entries and addresses in
@@ -1549,11 +1556,11 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, S...>, F& f)
 // them, and leaves the references in LDS; a step later the other key half's wave follows, and the P.V waves
 // bring O and the lower half's P down.  O goes through memory for it (its chunk's place among the partial
 // rows, unused so far): kept, scaled, and added at the end, while the accumulators start again from zero;
-// scaled in place they were copied at every edge of the loop, and spilled.  128 sequences up to 8,192 keys
-// 281 -> 197 us, 60 up to 4,000 83 -> 66, 32 of 4 queries 143 -> 111, one of 65,536 49.5 -> 47.9, a chunk
-// 743 -> 742; where few rows rise the flags' price shows: four of up to 30,000 keys 46.7 -> 47.6, 2,048
-// queries over themselves 725 -> 759.  (With rows kept at their own places, 16 bytes an access, the four
-// took 50.8.)
+// scaled in place they were copied at every edge of the loop, and spilled.  Against repeated passes, on one card
+// (us): 128 sequences up to 8,192 keys 279 -> 193, 60 up to 4,000 82 -> 66, 32 of 4 queries up to 1,000 69 -> 64, one of
+// 65,536 49.3 -> 47.8, a chunk 731 -> 730; where few rows rise the flags' price shows: four of up to 30,000
+// keys 46.7 -> 47.5, 2,048 queries over themselves 721 -> 750.  (With rows kept at their own places, 16 bytes
+// an access, the four took 3 us more.)
 template <typename TL, bool BS>
 __global__ void __launch_bounds__(kXThreads, 1) flash16x8_kernel(FlashArgs a) {
     static_assert(BS || !Half<TL>::kF16, "a cache of one scale is read with bf16 queries");
@@ -3600,11 +3607,13 @@ __global__ void __launch_bounds__(512) out_list_kernel(const float* __restrict__
 //     The rows go to LDS in two 16-bit terms, hi in columns 0 .. 15, lo in 16 .. 31, and each of
 //     these two blocks is one MFMA a step.  Two tiles' columns alternate, so one barrier a tile is enough.
 // What bounds it is the phases' order (rows, barrier, product: about 3 us a tile) and W_uv's first read.
-// Launches of their own against it, with the pass (us): 9 sequences up to 9,000 keys 38.3 / 37.2, 16 up
-// to 8,192 43.6 / 41.4, 61 up to 4,989 73.9 / 72.5, 64 of up to 300 30.5 / 29.8, 128 up to 8,192 184.5 /
-// 186.0, 32 of 4 queries 57.3 / 59.8; past 128 tokens it loses (200: 57.4 / 66.5) and packed rows take
-// over.  A bf16 row between the launches is the third of the outputs' roundings (P, the row, the output):
-// without it they are 2.4e-3 instead of 2.9e-3 off, relative, in the 2-norm.
+// Launches of their own against it, with the pass (us, bf16; f16): 9 sequences up to 9,000 keys 39.2 / 37.8;
+// 48.6 / 47.1, 16 up to 8,192 42.8 / 40.6; 53.5 / 50.9, 61 up to 4,989 72.9 / 72.0; 84.7 / 83.0, 64 of up to 300
+// 31.3 / 30.3; 41.1 / 39.7, 16 of 4 queries up to 4,989 72.7 / 70.7; 88.1 / 85.6, 128 up to 8,192 172.1 / 174.7;
+// 197.7 / 198.0, 32 of 4 up to 1,000 57.2 / 59.5; 64.0 / 65.2.  Towards 128 tokens it is the slower one by up to
+// 4%, and kept for the outputs' accuracy (the row between the launches in two terms and not in one: 2.3e-3 off
+// in bf16, not 2.8e-3, and 2.9e-4, not 3.6e-4, in f16); past 128 it loses 16% (200: 57.4 / 66.5), and packed rows
+// take over.
 constexpr int kOutTile = 16;
 template <typename TL>
 __global__ void __launch_bounds__(512, 1) out_merge_kernel(const float* __restrict__ o,
@@ -3748,7 +3757,7 @@ __global__ void __launch_bounds__(512, 1) out_merge_kernel(const float* __restri
 // two tiles ahead and go to LDS as values in two f16 terms (hi in rows 0 .. 31, lo in 32 .. 63), two tiles'
 // in turn, so one barrier a tile is enough; between two barriers half of the waves multiply first and
 // half convert first, so that each SIMD does both at once.  1,332 tokens of 128 heads 60 us (the
-// large-tile GEMM on f16 rows 54, a call 831 against 825).
+// large-tile GEMM on f16 rows 54; whole calls at pv_pack_rows).
 constexpr int kRowsTile = 32;
 __global__ void __launch_bounds__(512, 1) out_terms_kernel(const uint16_t* __restrict__ rows,
                                                           const float* __restrict__ scales,
@@ -3857,9 +3866,10 @@ __global__ void __launch_bounds__(512, 1) out_terms_kernel(const uint16_t* __res
 // from memory straight to LDS, three tiles of 32 KB in flight a CU; wave w multiplies output columns 16 w ..
 // +15 by the tile's 32 tokens, an accumulator for each of a row's four scales.
 // Bound by the rows' bytes: 1,332 tokens of 128 heads 41 us, 5.8 TB/s (they were just written: part of them
-// comes from the last-level cache), where the large-tile GEMM on bf16 rows takes 54; 200 tokens 15.5 / 13.6,
-// of which W_uv's load and conversion take 5.  With 32 columns a wave, for half of the tokens each, it was
-// 45 and 19.5: twice W_uv's registers to convert.
+// comes from the last-level cache), where the large-tile GEMM on bf16 rows takes 54 -- which the pass spends
+// again on packing them (whole calls at pv_pack_rows); 200 tokens 15.5 / 13.6, of which W_uv's load and
+// conversion take 5.  With 32 columns a wave, for half of the tokens each, it was 45 and 19.5: twice W_uv's
+// registers to convert.
 constexpr int kRowsStage = kRowsTile * kFR * 2;   // 32 KB: chunk c (16 bytes) of row r at c ^ (r & 15)
 constexpr int kRowsAhead = 3;                     // tiles in flight
 constexpr int kRowsScales = (kRowsAhead + 1) * kRowsStage;   // the stages' scales, 1 KB each
