@@ -1538,9 +1538,9 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, S...>, F& f)
 // byte 255 would make their zero codes NaN).
 // BS's steps are one apart from the others': the softmax of block j - 1 runs between the score MFMAs of
 // block j, and P.V works on block j - 2, so a score wave's chain of MFMAs and its exponentials overlap.
-// No unit is full: the counters of a prefill chunk give the matrix cores 46% of the cycles, and of a wave's time
-// 38% to issuing (1.29e8 VALU instructions, 2.7e7 of them MFMAs and 5.6e7 conversions), 28% to waiting for
-// its turn to issue and 34% to barriers and loads.  What a step takes is each wave's own stream of instructions
+// No unit is full: the counters of a prefill chunk give the matrix cores 48% of the cycles, and of a wave's time
+// 40% to issuing (1.29e8 VALU instructions, 2.7e7 of them MFMAs and 5.6e7 conversions), 29% to waiting for
+// its turn to issue and 31% to barriers and loads.  What a step takes is each wave's own stream of instructions
 // (a score wave's 36 MFMAs and 72 conversions, a P.V wave's 16 and 32) and the other waves' at the barrier, so
 // the rest was cut: the next block's descriptors behind the first P.V MFMAs, page entries in a register,
 // addresses kept.  Measured
