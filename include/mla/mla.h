@@ -457,6 +457,60 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
                                void* out, void* workspace, size_t workspace_bytes,
                                hipStream_t stream);
 
+/* ---- The expanded form (none in the reference), for chunks of many new tokens: keys and values per
+ * head from the latent rows,
+ *   k[j, h] = W_uk[h] c_kv[j],  v[j, h] = W_uv[h] c_kv[j],
+ *   out[b, i, h] = softmax_j((q_nope[b, i, h] . k[j, h] + q_rope[b, i, h] . pe[j]) / scale) . v[j, h],
+ * mla_attention's function of unabsorbed queries: 640 operations a pair and head instead of 2,176, and
+ * 262,144 a key and head once.  It pays from about 200 new tokens a sequence; below that mla_q_absorbed and the
+ * attention over the latents are faster.  bf16 or fp16 (queries, weights, output, and the cache where
+ * it is not in 8 bits), kv_rank 512, rope 64, nope and v 128 (MLA_ERR_UNSUPPORTED otherwise).
+ *   q_nope [B, Sq, H, 128], q_rope [B, Sq, H, 64]     mla_q_heads
+ *   W_uk [H, 128, 512], W_uv [H, 128, 512], out [B, Sq, H, 128]
+ * Causal rule and empty sequences as in mla_attention_paged.  new_lens [B] (or NULL: Sq of each): the
+ * last new_lens[b] (clamped to [0, Sq]) of sequence b's Sq rows are its queries, the rows in front of
+ * them padding, whose output is zeros.  Pages that sequences share at the same place behind a shared
+ * first page (mla_cache_fork) are expanded once.  Table entries outside the pool read as zero rows.
+ * Rounded on the way: keys, values and outputs to the type (fp16: those past its range to +-65504), each
+ * key's weight before the division by the row's sum; sums are float32.  A latent row
+ * with a NaN or an infinity makes the rows of the queries that see it NaN and reaches no other query.
+ * The workspace holds keys and values of as many heads at a time as 2 GiB take (one at least). */
+size_t mla_attention_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims, int causal);
+int mla_attention_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
+                           const void* q_rope, const void* c_kv, const void* pe_cache,
+                           const void* W_uk, const void* W_uv, double scale, int causal, void* out,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* over the paged cache: pools, block_table and seq_lens as mla_attention_paged, num_pages pages */
+size_t mla_attention_paged_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims,
+                                                    int causal, int32_t page_size);
+int mla_attention_paged_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
+                                 const void* q_rope, const void* c_kv_pages, const void* pe_pages,
+                                 const int32_t* block_table, const int32_t* seq_lens,
+                                 const int32_t* new_lens, int32_t page_size, int32_t num_pages,
+                                 const void* W_uk, const void* W_uv, double scale, int causal,
+                                 void* out, void* workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
+/* over the paged cache in 8 bits with block scales: as mla_attention_paged_fp8blk's; its values enter in
+ * the queries' type (in fp16 one past its range is infinite).  Workspace as the one above. */
+int mla_attention_paged_fp8blk_expanded(mla_dtype_t dtype, const mla_dims_t* dims,
+                                        const void* q_nope, const void* q_rope,
+                                        const void* c_kv_pages, const void* pe_pages,
+                                        const void* scales, const int32_t* block_table,
+                                        const int32_t* seq_lens, const int32_t* new_lens,
+                                        int32_t page_size, int32_t num_pages, int32_t scale_block,
+                                        const void* W_uk, const void* W_uv, double scale,
+                                        int causal, void* out, void* workspace,
+                                        size_t workspace_bytes, hipStream_t stream);
+
+/* Its queries: mla_q_absorbed without 2c.  q_nope [B, Sq, H, nope] is q_raw's nope part rounded to
+ * dtype (bf16 or fp16), q_rope as mla_q_absorbed's; positions [Sq], or with per_sequence [B, Sq].
+ * dims->kv_rank is not used; nope is a multiple of 8. */
+size_t mla_q_heads_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims);
+int mla_q_heads(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, const void* W_q_a,
+                const void* q_norm_w, const void* W_q_b, const int64_t* positions,
+                int per_sequence, const void* inv_freq, double eps, void* q_nope, void* q_rope,
+                void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* Output projection wo: out [B*Sq, hidden] = attn [B*Sq, H*v] @ W_o [H*v, hidden], all in
  * dtype (fp32 accumulation).  attn is mla_attention's output [B, Sq, H, v]. */
 size_t mla_o_proj_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims);

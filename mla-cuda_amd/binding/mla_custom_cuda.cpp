@@ -12,7 +12,9 @@
 // kv_append_paged for a ragged, paged cache (q_absorbed takes [B, Sq] positions for it);
 // mla_attention_fp8kv and mla_attention_paged_fp8kv for an e4m3 cache; cache_extend,
 // kv_append_paged_fp8blk, kv_read_fp8blk and mla_attention_paged_fp8blk for a paged e4m3 cache
-// with a scale for each block of tokens.  This file only
+// with a scale for each block of tokens; q_heads and the *_expanded attentions for chunks of
+// many tokens, cache_fork, cache_compact and cache_copy_pages for pages that requests share.
+// This file only
 // validates tensors, allocates outputs and workspace from torch's caching allocator and
 // passes raw pointers and the current HIP stream to the C ABI; all device work lives in
 // libmla_amd.so.
@@ -928,6 +930,212 @@ torch::Tensor op_mla_attention_paged_fp8blk(torch::Tensor q_absorbed, torch::Ten
     return out;
 }
 
+// ------------------------------------------------------------------ expanded form
+
+// Shapes that the three entry points share: queries per head, weights per head, scale.
+mla_dims_t expanded_dims(const torch::Tensor& qn, const torch::Tensor& qr, const torch::Tensor& W_uk,
+                         const torch::Tensor& W_uv) {
+    check_dim(qn, 4, "q_nope", "[B, Sq, H, nope]");
+    check_dim(qr, 4, "q_rope", "[B, Sq, H, rope]");
+    check_dim(W_uk, 3, "W_uk", "[H, nope, kv_rank]");
+    check_dim(W_uv, 3, "W_uv", "[H, v, kv_rank]");
+    const int64_t B = qn.size(0), Sq = qn.size(1), H = qn.size(2), nope = qn.size(3);
+    TORCH_CHECK(qr.size(0) == B && qr.size(1) == Sq && qr.size(2) == H,
+                "q_rope must be [B, Sq, H, rope] matching q_nope (got ", qr.sizes(), ")");
+    TORCH_CHECK(W_uk.size(0) == H && W_uk.size(1) == nope, "W_uk must be [H, nope, kv_rank] (got ",
+                W_uk.sizes(), ")");
+    TORCH_CHECK(W_uv.size(0) == H && W_uv.size(2) == W_uk.size(2),
+                "W_uv must be [H, v, kv_rank] (got ", W_uv.sizes(), ")");
+    TORCH_CHECK(B < INT32_MAX && Sq < INT32_MAX && H < INT32_MAX, "MLA: sizes must be below 2^31");
+    check_same_dtype(qn, qr, "q_rope");
+    check_same_dtype(qn, W_uk, "W_uk");
+    check_same_dtype(qn, W_uv, "W_uv");
+    mla_dims_t d{};
+    d.batch = (int32_t)B; d.sq = (int32_t)Sq; d.heads = (int32_t)H; d.nope = (int32_t)nope;
+    d.rope = (int32_t)qr.size(3); d.kv_rank = (int32_t)W_uk.size(2); d.v = (int32_t)W_uv.size(1);
+    return d;
+}
+
+// Attention in the expanded form over a dense cache.
+torch::Tensor op_mla_attention_expanded(torch::Tensor q_nope, torch::Tensor q_rope,
+                                        torch::Tensor c_kv, torch::Tensor pe_cache,
+                                        torch::Tensor W_uk, torch::Tensor W_uv, double scale,
+                                        bool causal) {
+    mla_dims_t d = expanded_dims(q_nope, q_rope, W_uk, W_uv);
+    check_dim(c_kv, 3, "c_kv", "[B, Sk, kv_rank]");
+    check_dim(pe_cache, 3, "pe_cache", "[B, Sk, rope]");
+    TORCH_CHECK(c_kv.size(0) == d.batch && c_kv.size(2) == d.kv_rank && c_kv.size(1) < INT32_MAX,
+                "c_kv must be [B, Sk, kv_rank] (got ", c_kv.sizes(), ")");
+    TORCH_CHECK(pe_cache.size(0) == d.batch && pe_cache.size(1) == c_kv.size(1) &&
+                    pe_cache.size(2) == d.rope,
+                "pe_cache must be [B, Sk, rope] (got ", pe_cache.sizes(), ")");
+    d.sk = (int32_t)c_kv.size(1);
+    const mla_dtype_t dt = to_mla_dtype(q_nope, "q_nope");
+    check_same_dtype(q_nope, c_kv, "c_kv");
+    check_same_dtype(q_nope, pe_cache, "pe_cache");
+    check_device({&q_nope, &q_rope, &c_kv, &pe_cache, &W_uk, &W_uv});
+
+    c10::DeviceGuard guard(q_nope.device());
+    auto qn = q_nope.contiguous();
+    auto qr = q_rope.contiguous();
+    auto ck = c_kv.contiguous();
+    auto pe = pe_cache.contiguous();
+    auto wuk = W_uk.contiguous();
+    auto wuv = W_uv.contiguous();
+    auto out = torch::empty({d.batch, d.sq, d.heads, d.v}, qn.options());
+    const size_t wsb = mla_attention_expanded_workspace_bytes(dt, &d, causal ? 1 : 0);
+    auto ws = workspace(wsb, qn);
+    check_status(mla_attention_expanded(dt, &d, qn.data_ptr(), qr.data_ptr(), ck.data_ptr(),
+                                        pe.data_ptr(), wuk.data_ptr(), wuv.data_ptr(), scale,
+                                        causal ? 1 : 0, out.data_ptr(), ws.data_ptr(), wsb,
+                                        current_stream()),
+                 "mla_attention_expanded");
+    return out;
+}
+
+// The same over a paged cache, in the queries' type (scales absent) or in 8 bits with block scales.
+torch::Tensor paged_expanded(const torch::Tensor& q_nope, const torch::Tensor& q_rope,
+                             const torch::Tensor& c_kv_pages, const torch::Tensor& pe_pages,
+                             const torch::Tensor* scales, const torch::Tensor& block_table,
+                             const torch::Tensor& seq_lens, const torch::Tensor& W_uk,
+                             const torch::Tensor& W_uv, double scale, bool causal,
+                             const c10::optional<torch::Tensor>& new_lens) {
+    mla_dims_t d = expanded_dims(q_nope, q_rope, W_uk, W_uv);
+    check_dim(c_kv_pages, 3, "c_kv_pages", "[num_pages, page_size, kv_rank]");
+    check_dim(pe_pages, 3, "pe_pages", "[num_pages, page_size, rope]");
+    check_dim(block_table, 2, "block_table", "[B, max_pages]");
+    const int64_t P = c_kv_pages.size(0), page = c_kv_pages.size(1);
+    TORCH_CHECK(c_kv_pages.size(2) == d.kv_rank,
+                "c_kv_pages must be [num_pages, page_size, kv_rank] (got ", c_kv_pages.sizes(), ")");
+    TORCH_CHECK(pe_pages.size(0) == P && pe_pages.size(1) == page && pe_pages.size(2) == d.rope,
+                "pe_pages must be [num_pages, page_size, rope] matching c_kv_pages (got ",
+                pe_pages.sizes(), ")");
+    TORCH_CHECK(block_table.size(0) == d.batch && block_table.scalar_type() == torch::kInt32,
+                "block_table must be an int32 [B, max_pages] tensor (got ", block_table.sizes(), ")");
+    check_int32(seq_lens, d.batch, "seq_lens");
+    if (new_lens) check_int32(*new_lens, d.batch, "new_lens");
+    TORCH_CHECK(P < INT32_MAX && page < INT32_MAX && block_table.size(1) < INT32_MAX &&
+                    block_table.size(1) * page < INT32_MAX,
+                "MLA: block_table spans too many keys");
+    d.sk = (int32_t)(block_table.size(1) * page);
+    const mla_dtype_t dt = to_mla_dtype(q_nope, "q_nope");
+    int32_t block = 0;
+    std::vector<const torch::Tensor*> all = {&q_nope, &q_rope, &c_kv_pages, &pe_pages, &block_table,
+                                             &seq_lens, &W_uk, &W_uv};
+    if (scales) {
+        block = check_blocked(c_kv_pages, pe_pages, *scales);
+        all.push_back(scales);
+    } else {
+        check_same_dtype(q_nope, c_kv_pages, "c_kv_pages");
+        check_same_dtype(q_nope, pe_pages, "pe_pages");
+    }
+    if (new_lens) all.push_back(&*new_lens);
+    check_device(all);
+
+    c10::DeviceGuard guard(q_nope.device());
+    auto qn = q_nope.contiguous();
+    auto qr = q_rope.contiguous();
+    auto ck = c_kv_pages.contiguous();
+    auto pe = pe_pages.contiguous();
+    auto tab = block_table.contiguous();
+    auto lens = seq_lens.contiguous();
+    auto wuk = W_uk.contiguous();
+    auto wuv = W_uv.contiguous();
+    torch::Tensor fresh, sc;
+    if (new_lens) fresh = new_lens->contiguous();
+    const int32_t* fresh_ptr = new_lens ? fresh.data_ptr<int32_t>() : nullptr;
+    auto out = torch::empty({d.batch, d.sq, d.heads, d.v}, qn.options());
+    const size_t wsb = mla_attention_paged_expanded_workspace_bytes(dt, &d, causal ? 1 : 0,
+                                                                    (int32_t)page);
+    auto ws = workspace(wsb, qn);
+    if (scales) {
+        sc = scales->contiguous();
+        check_status(mla_attention_paged_fp8blk_expanded(
+                         dt, &d, qn.data_ptr(), qr.data_ptr(), ck.data_ptr(), pe.data_ptr(),
+                         sc.data_ptr(), tab.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), fresh_ptr,
+                         (int32_t)page, (int32_t)P, block, wuk.data_ptr(), wuv.data_ptr(), scale,
+                         causal ? 1 : 0, out.data_ptr(), ws.data_ptr(), wsb, current_stream()),
+                     "mla_attention_paged_fp8blk_expanded");
+    } else {
+        check_status(mla_attention_paged_expanded(
+                         dt, &d, qn.data_ptr(), qr.data_ptr(), ck.data_ptr(), pe.data_ptr(),
+                         tab.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), fresh_ptr, (int32_t)page,
+                         (int32_t)P, wuk.data_ptr(), wuv.data_ptr(), scale, causal ? 1 : 0,
+                         out.data_ptr(), ws.data_ptr(), wsb, current_stream()),
+                     "mla_attention_paged_expanded");
+    }
+    return out;
+}
+torch::Tensor op_mla_attention_paged_expanded(torch::Tensor q_nope, torch::Tensor q_rope,
+                                              torch::Tensor c_kv_pages, torch::Tensor pe_pages,
+                                              torch::Tensor block_table, torch::Tensor seq_lens,
+                                              torch::Tensor W_uk, torch::Tensor W_uv, double scale,
+                                              bool causal, c10::optional<torch::Tensor> new_lens) {
+    return paged_expanded(q_nope, q_rope, c_kv_pages, pe_pages, nullptr, block_table, seq_lens, W_uk,
+                          W_uv, scale, causal, new_lens);
+}
+torch::Tensor op_mla_attention_paged_fp8blk_expanded(
+    torch::Tensor q_nope, torch::Tensor q_rope, torch::Tensor c_kv_pages, torch::Tensor pe_pages,
+    torch::Tensor scales, torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor W_uk,
+    torch::Tensor W_uv, double scale, bool causal, c10::optional<torch::Tensor> new_lens) {
+    return paged_expanded(q_nope, q_rope, c_kv_pages, pe_pages, &scales, block_table, seq_lens, W_uk,
+                          W_uv, scale, causal, new_lens);
+}
+
+// Queries per head for it: [q_nope [B, Sq, H, nope], q_rope [B, Sq, H, rope]].
+std::vector<torch::Tensor> op_q_heads(torch::Tensor x, torch::Tensor W_q_a, torch::Tensor q_norm_w,
+                                      torch::Tensor W_q_b, torch::Tensor positions,
+                                      int64_t nope_dim, int64_t rope_dim, double eps) {
+    check_dim(x, 3, "x", "[B, Sq, hidden]");
+    check_dim(W_q_a, 2, "W_q_a", "[hidden, q_lora]");
+    check_dim(W_q_b, 2, "W_q_b", "[q_lora, H*(nope+rope)]");
+    const int64_t B = x.size(0), Sq = x.size(1), hidden = x.size(2), q_lora = W_q_a.size(1);
+    TORCH_CHECK(nope_dim > 0 && rope_dim > 0 && nope_dim < INT32_MAX && rope_dim < INT32_MAX,
+                "MLA: nope_dim and rope_dim must be positive");
+    TORCH_CHECK(W_q_a.size(0) == hidden, "W_q_a must be [hidden, q_lora]");
+    TORCH_CHECK(W_q_b.size(0) == q_lora && W_q_b.size(1) > 0 && W_q_b.size(1) % (nope_dim + rope_dim) == 0,
+                "W_q_b must be [q_lora, H*(nope+rope)] (got ", W_q_b.sizes(), ")");
+    const int64_t H = W_q_b.size(1) / (nope_dim + rope_dim);
+    TORCH_CHECK(q_norm_w.dim() == 1 && q_norm_w.size(0) == q_lora,
+                "q_norm_w must be a 1-D tensor of length q_lora (got ", q_norm_w.sizes(), ")");
+    const bool per_seq = positions.dim() == 2;
+    TORCH_CHECK((positions.dim() == 1 && positions.size(0) == Sq) ||
+                    (per_seq && positions.size(0) == B && positions.size(1) == Sq),
+                "positions must be [Sq] (shared by the batch) or [B, Sq] (per sequence) (got ",
+                positions.sizes(), ")");
+    TORCH_CHECK(!positions.is_floating_point() && !positions.is_complex(),
+                "positions must be an integer tensor");
+    TORCH_CHECK(B < INT32_MAX && Sq < INT32_MAX && hidden < INT32_MAX && q_lora < INT32_MAX &&
+                    H < INT32_MAX, "MLA: sizes must be below 2^31");
+    TORCH_CHECK(rope_dim % 2 == 0, "MLA: rope_dim must be positive and even");
+    const mla_dtype_t dt = to_mla_dtype(x, "x");
+    check_same_dtype(x, W_q_a, "W_q_a");
+    check_same_dtype(x, q_norm_w, "q_norm_w");
+    check_same_dtype(x, W_q_b, "W_q_b");
+    check_device({&x, &W_q_a, &q_norm_w, &W_q_b, &positions});
+
+    c10::DeviceGuard guard(x.device());
+    auto xc = x.contiguous();
+    auto wa = W_q_a.contiguous();
+    auto g = q_norm_w.contiguous();
+    auto wb = W_q_b.contiguous();
+    auto pos = positions.to(torch::kLong).contiguous();
+    auto inv_freq = device_inv_freq(rope_dim, x.device());
+    mla_dims_t d{};
+    d.batch = (int32_t)B; d.sq = (int32_t)Sq; d.hidden = (int32_t)hidden;
+    d.q_lora = (int32_t)q_lora; d.heads = (int32_t)H; d.nope = (int32_t)nope_dim;
+    d.rope = (int32_t)rope_dim;
+    auto qn = torch::empty({B, Sq, H, nope_dim}, x.options());
+    auto qr = torch::empty({B, Sq, H, rope_dim}, x.options());
+    const size_t wsb = mla_q_heads_workspace_bytes(dt, &d);
+    auto ws = workspace(wsb, x);
+    check_status(mla_q_heads(dt, &d, xc.data_ptr(), wa.data_ptr(), g.data_ptr(), wb.data_ptr(),
+                             pos.data_ptr<int64_t>(), per_seq ? 1 : 0, inv_freq.data_ptr(), eps,
+                             qn.data_ptr(), qr.data_ptr(), ws.data_ptr(), wsb, current_stream()),
+                 "q_heads");
+    return {qn, qr};
+}
+
 // ------------------------------------------------------------------ neighbours of the path
 
 // Weight prep once at load: the W_uk / W_uv halves of wkv_b as contiguous tensors.
@@ -1127,4 +1335,26 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("q_absorbed"), py::arg("q_rope"), py::arg("c_kv_pages"), py::arg("pe_pages"),
           py::arg("scales"), py::arg("block_table"), py::arg("seq_lens"), py::arg("W_uv"),
           py::arg("scale"), py::arg("causal") = false);
+    m.def("q_heads", &op_q_heads,
+          "Queries per head for the expanded form (bf16 or fp16): returns [q_nope [B, Sq, H, nope], "
+          "q_rope [B, Sq, H, rope]]",
+          py::arg("x"), py::arg("W_q_a"), py::arg("q_norm_w"), py::arg("W_q_b"), py::arg("positions"),
+          py::arg("nope_dim"), py::arg("rope_dim"), py::arg("eps"));
+    m.def("mla_attention_expanded", &op_mla_attention_expanded,
+          "Attention in the expanded form (keys and values per head made from the latent rows; bf16 "
+          "or fp16): returns out [B, Sq, H, v]",
+          py::arg("q_nope"), py::arg("q_rope"), py::arg("c_kv"), py::arg("pe_cache"), py::arg("W_uk"),
+          py::arg("W_uv"), py::arg("scale"), py::arg("causal") = false);
+    m.def("mla_attention_paged_expanded", &op_mla_attention_paged_expanded,
+          "The same over a paged, ragged cache; of each sequence's Sq rows the last new_lens[b] are "
+          "queries (all without it)",
+          py::arg("q_nope"), py::arg("q_rope"), py::arg("c_kv_pages"), py::arg("pe_pages"),
+          py::arg("block_table"), py::arg("seq_lens"), py::arg("W_uk"), py::arg("W_uv"),
+          py::arg("scale"), py::arg("causal") = false, py::arg("new_lens") = py::none());
+    m.def("mla_attention_paged_fp8blk_expanded", &op_mla_attention_paged_fp8blk_expanded,
+          "The same over a paged cache of e4m3 codes with a power-of-two scale for each block of tokens",
+          py::arg("q_nope"), py::arg("q_rope"), py::arg("c_kv_pages"), py::arg("pe_pages"),
+          py::arg("scales"), py::arg("block_table"), py::arg("seq_lens"), py::arg("W_uk"),
+          py::arg("W_uv"), py::arg("scale"), py::arg("causal") = false,
+          py::arg("new_lens") = py::none());
 }

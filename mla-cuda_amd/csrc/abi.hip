@@ -633,8 +633,9 @@ int q_absorbed_impl(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, co
                    const void* q_norm_w, const void* W_q_b, const void* W_uk,
                    const int64_t* positions, const void* inv_freq_tab, double eps,
                    void* q_absorbed, void* q_rope, void* workspace, size_t workspace_bytes,
-                   hipStream_t stream, bool pos_per_batch) {
-    if (dtype == MLA_DTYPE_F64)
+                   hipStream_t stream, bool pos_per_batch, void* q_heads = nullptr) {
+    // q_heads: the queries per head (mla_q_heads) -- 16 bits, no 2c, q_nope into q_heads
+    if (dtype == MLA_DTYPE_F64 && !q_heads)
         return q_absorbed_f64(dims, x, W_q_a, q_norm_w, W_q_b, W_uk, positions, inv_freq_tab,
                               eps, q_absorbed, q_rope, workspace, workspace_bytes, stream,
                               pos_per_batch);
@@ -645,10 +646,10 @@ int q_absorbed_impl(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, co
     MLA_CHECK(check_ptr(W_q_a, "W_q_a"));
     MLA_CHECK(check_ptr(q_norm_w, "q_norm_w"));
     MLA_CHECK(check_ptr(W_q_b, "W_q_b"));
-    MLA_CHECK(check_ptr(W_uk, "W_uk"));
+    if (!q_heads) MLA_CHECK(check_ptr(W_uk, "W_uk"));
     MLA_CHECK(check_ptr(positions, "positions"));
     MLA_CHECK(check_ptr(inv_freq, "inv_freq"));
-    MLA_CHECK(check_ptr(q_absorbed, "q_absorbed"));
+    MLA_CHECK(check_ptr(q_heads ? q_heads : q_absorbed, q_heads ? "q_nope" : "q_absorbed"));
     MLA_CHECK(check_ptr(q_rope, "q_rope"));
     if (!(eps >= 0.0) || !std::isfinite(eps))
         return fail(MLA_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
@@ -689,11 +690,11 @@ int q_absorbed_impl(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, co
     GemmProblem up = q_up_problem(dtype, dims, lat, W_q_b, raw);
     if (L.fused) {
         QUpEpilogue qe;
-        qe.q_nope = raw; qe.q_rope = q_rope; qe.cos_sin = rt.cos_sin;
+        qe.q_nope = q_heads ? q_heads : raw; qe.q_rope = q_rope; qe.cos_sin = rt.cos_sin;
         qe.H = dims->heads; qe.nope = dims->nope; qe.rope = dims->rope;
         up.qup = &qe;
         up.C = nullptr;
-        if (L.fused_2c && (reinterpret_cast<uintptr_t>(W_uk) & 15) == 0 &&
+        if (L.fused_2c && !q_heads && (reinterpret_cast<uintptr_t>(W_uk) & 15) == 0 &&
             (reinterpret_cast<uintptr_t>(q_absorbed) & 3) == 0) {
             qe.w_uk = W_uk; qe.q_abs = q_absorbed; qe.kv = dims->kv_rank;
             MLA_TRY_HIP(launch_gemm(up, L.up, at<void>(workspace, L.off_up_ws), stream),
@@ -702,6 +703,7 @@ int q_absorbed_impl(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, co
         }
         MLA_TRY_HIP(launch_gemm(up, L.up, at<void>(workspace, L.off_up_ws), stream),
                     "2a2 + 2b launch");
+        if (q_heads) return ok();
         GemmProblem ab = absorb_problem(dtype, dims, raw, W_uk, q_absorbed, true);
         MLA_TRY_HIP(launch_gemm(ab, L.absorb, at<void>(workspace, L.off_abs_ws), stream),
                     "2c launch");
@@ -749,6 +751,12 @@ int q_absorbed_impl(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, co
                                 dims->sq, dims->heads, dims->nope, dims->rope, stream,
                                 pos_per_batch),
                     "2b launch");
+    }
+    if (q_heads) {
+        MLA_TRY_HIP(launch_q_nope(raw, q_heads, is_f16(dtype), (int64_t)bq * dims->heads, dims->nope,
+                                  dims->nope + dims->rope, stream),
+                    "q_nope launch");
+        return ok();
     }
     // 2c
     GemmProblem ab = absorb_problem(dtype, dims, raw, W_uk, q_absorbed);
@@ -825,6 +833,63 @@ int check_fp8blk_attn(mla_dtype_t dtype, const mla_dims_t* d, int causal, int32_
     if ((int64_t)d->heads * d->v >= (int64_t)1 << 25)
         return fail(MLA_ERR_UNSUPPORTED, "heads * v must be below 2^25 (heads %d, v %d)", d->heads, d->v);
     return MLA_OK;
+}
+
+// The expanded form: 16 bits and the DeepSeek-V3 widths; counts that its kernels form in 32 bits.
+int check_expanded(mla_dtype_t dtype, const mla_dims_t* d, int causal) {
+    MLA_CHECK(check_dtype(dtype));
+    if (!is_half(dtype))
+        return fail(MLA_ERR_UNSUPPORTED, "expanded attention takes bf16 or fp16 (dtype %d)", (int)dtype);
+    MLA_CHECK(check_attn_dims(dtype, d, causal));
+    if (d->kv_rank != 512 || d->rope != 64 || d->nope != 128 || d->v != 128)
+        return fail(MLA_ERR_UNSUPPORTED, "expanded attention needs kv_rank 512, rope 64, nope 128 and v 128 "
+                    "(got %d, %d, %d, %d)", d->kv_rank, d->rope, d->nope, d->v);
+    const int64_t units = ((int64_t)d->sk + kExpandUnit - 1) / kExpandUnit;
+    if (d->batch > 65535 || units * kExpandUnit * d->batch > kMaxI32 / 2)
+        return fail(MLA_ERR_UNSUPPORTED, "expanded attention takes at most 65535 sequences and 2^30 keys "
+                    "in all (batch %d, sk %d)", d->batch, d->sk);
+    return MLA_OK;
+}
+int set_expanded_pages(ExpandProblem* p, const void* c_kv_pages, const void* pe_pages,
+                       const int32_t* block_table, const int32_t* seq_lens, const int32_t* new_lens,
+                       int32_t page_size, int32_t num_pages) {
+    MLA_CHECK(check_ptr(c_kv_pages, "c_kv_pages"));
+    MLA_CHECK(check_ptr(pe_pages, "pe_pages"));
+    MLA_CHECK(check_ptr(block_table, "block_table"));
+    MLA_CHECK(check_ptr(seq_lens, "seq_lens"));
+    if (new_lens) MLA_CHECK(check_ptr(new_lens, "new_lens"));
+    p->c_kv = c_kv_pages; p->pe = pe_pages; p->block_table = block_table;
+    p->seq_lens = seq_lens; p->new_lens = new_lens;
+    p->page_size = page_size; p->num_pages = num_pages;
+    return MLA_OK;
+}
+int run_expanded(ExpandProblem p, mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
+                 const void* q_rope, const void* W_uk, const void* W_uv, double scale, int causal,
+                 void* out, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    MLA_CHECK(check_scale(scale));
+    MLA_CHECK(check_ptr(q_nope, "q_nope"));
+    MLA_CHECK(check_ptr(q_rope, "q_rope"));
+    MLA_CHECK(check_ptr(W_uk, "W_uk"));
+    MLA_CHECK(check_ptr(W_uv, "W_uv"));
+    MLA_CHECK(check_ptr(out, "out"));
+    const ExpandPlan plan = plan_expand(dims->batch, dims->sk, dims->heads, p.block_table != nullptr);
+    MLA_CHECK(check_ws(workspace, workspace_bytes, plan.total));
+    p.f16 = is_f16(dtype);
+    p.q_nope = q_nope; p.q_rope = q_rope; p.W_uk = W_uk; p.W_uv = W_uv; p.out = out;
+    p.B = dims->batch; p.Sq = dims->sq; p.Sk = dims->sk; p.H = dims->heads;
+    p.scale = scale; p.causal = causal != 0;
+    MLA_TRY_HIP(launch_expand(p, plan, workspace, stream), "expanded attention launch");
+    return ok();
+}
+// mla_q_heads: the Q path's dims, with a kv_rank for the layout that 2c would use (it does not run)
+int check_q_heads(mla_dtype_t dtype, const mla_dims_t* dims, mla_dims_t* d) {
+    MLA_CHECK(check_dtype(dtype));
+    if (!is_half(dtype))
+        return fail(MLA_ERR_UNSUPPORTED, "queries per head are made in bf16 or fp16 (dtype %d)", (int)dtype);
+    if (!dims) return fail(MLA_ERR_INVALID_ARGUMENT, "dims must not be NULL");
+    *d = *dims;
+    d->kv_rank = 8;
+    return check_q_dims(dtype, d);
 }
 
 // KV append: x @ W_kv_a into the workspace, then the fused norm / RoPE / scatter kernel.
@@ -1678,6 +1743,87 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
                              : out_problem(dtype, dims, ctx, row_sum, W_uv, out);
     MLA_TRY_HIP(launch_gemm(op, L.out, at<void>(workspace, L.off_out_ws), stream), "3d launch");
     return ok();
+}
+
+// ------------------------------------------------------------------ expanded form
+
+size_t mla_attention_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims, int causal) {
+    if (check_expanded(dtype, dims, causal) != MLA_OK) return 0;
+    return plan_expand(dims->batch, dims->sk, dims->heads, false).total;
+}
+
+int mla_attention_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
+                           const void* q_rope, const void* c_kv, const void* pe_cache,
+                           const void* W_uk, const void* W_uv, double scale, int causal, void* out,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    MLA_CHECK(check_expanded(dtype, dims, causal));
+    MLA_CHECK(check_ptr(c_kv, "c_kv"));
+    MLA_CHECK(check_ptr(pe_cache, "pe_cache"));
+    ExpandProblem p;
+    p.c_kv = c_kv; p.pe = pe_cache;
+    return run_expanded(p, dtype, dims, q_nope, q_rope, W_uk, W_uv, scale, causal, out, workspace,
+                        workspace_bytes, stream);
+}
+
+size_t mla_attention_paged_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims,
+                                                    int causal, int32_t page_size) {
+    if (check_expanded(dtype, dims, causal) != MLA_OK || check_pages(dims, page_size) != MLA_OK) return 0;
+    return plan_expand(dims->batch, dims->sk, dims->heads, true).total;
+}
+
+int mla_attention_paged_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
+                                 const void* q_rope, const void* c_kv_pages, const void* pe_pages,
+                                 const int32_t* block_table, const int32_t* seq_lens,
+                                 const int32_t* new_lens, int32_t page_size, int32_t num_pages,
+                                 const void* W_uk, const void* W_uv, double scale, int causal,
+                                 void* out, void* workspace, size_t workspace_bytes,
+                                 hipStream_t stream) {
+    MLA_CHECK(check_expanded(dtype, dims, causal));
+    MLA_CHECK(check_pages(dims, page_size));
+    MLA_CHECK(check_pos(num_pages, "num_pages"));
+    ExpandProblem p;
+    MLA_CHECK(set_expanded_pages(&p, c_kv_pages, pe_pages, block_table, seq_lens, new_lens, page_size,
+                                 num_pages));
+    return run_expanded(p, dtype, dims, q_nope, q_rope, W_uk, W_uv, scale, causal, out, workspace,
+                        workspace_bytes, stream);
+}
+
+int mla_attention_paged_fp8blk_expanded(mla_dtype_t dtype, const mla_dims_t* dims,
+                                        const void* q_nope, const void* q_rope,
+                                        const void* c_kv_pages, const void* pe_pages,
+                                        const void* scales, const int32_t* block_table,
+                                        const int32_t* seq_lens, const int32_t* new_lens,
+                                        int32_t page_size, int32_t num_pages, int32_t scale_block,
+                                        const void* W_uk, const void* W_uv, double scale,
+                                        int causal, void* out, void* workspace,
+                                        size_t workspace_bytes, hipStream_t stream) {
+    MLA_CHECK(check_expanded(dtype, dims, causal));
+    MLA_CHECK(check_fp8blk(dims, page_size, num_pages, scale_block));
+    MLA_CHECK(check_scale_ptr(scales));
+    ExpandProblem p;
+    p.scales = scales; p.scale_block = scale_block;
+    MLA_CHECK(set_expanded_pages(&p, c_kv_pages, pe_pages, block_table, seq_lens, new_lens, page_size,
+                                 num_pages));
+    return run_expanded(p, dtype, dims, q_nope, q_rope, W_uk, W_uv, scale, causal, out, workspace,
+                        workspace_bytes, stream);
+}
+
+size_t mla_q_heads_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims) {
+    mla_dims_t d;
+    if (check_q_heads(dtype, dims, &d) != MLA_OK) return 0;
+    return q_layout(dtype, &d).total;
+}
+
+int mla_q_heads(mla_dtype_t dtype, const mla_dims_t* dims, const void* x, const void* W_q_a,
+                const void* q_norm_w, const void* W_q_b, const int64_t* positions,
+                int per_sequence, const void* inv_freq, double eps, void* q_nope, void* q_rope,
+                void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    mla_dims_t d;
+    MLA_CHECK(check_q_heads(dtype, dims, &d));
+    MLA_CHECK(check_ptr(q_nope, "q_nope"));
+    return q_absorbed_impl(dtype, &d, x, W_q_a, q_norm_w, W_q_b, nullptr, positions, inv_freq, eps,
+                           nullptr, q_rope, workspace, workspace_bytes, stream, per_sequence != 0,
+                           q_nope);
 }
 
 // ------------------------------------------------------------------ fp8 KV cache

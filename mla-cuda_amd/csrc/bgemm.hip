@@ -57,11 +57,21 @@ struct BArgs {
     float* ws; int64_t ws_split;                 // split > 1: partials [split][G][M][N]
     int M, N, K, G, split, k_chunk, tiles_m, tiles_n;
     QUpEpilogue q;                               // QUP kernels: 2a2 with 2b
+    const int* rows;                             // EXPAND kernels: M, on the device
+    int64_t b_hi;                                // and what B's rows past 128 of a group lie further on
 };
 
-template <typename TL, int BM, int BN, int NS, int MINB, bool NT, bool QUP>
+// EXPAND: the keys and values of the expanded attention (expand.hip).  The groups are heads, all of
+// them over the same A: their columns are walked like further N tiles.  A group's 256 columns are two
+// weights of 128 rows each, and how many rows A has is known on the device alone.
+template <typename TL, int BM, int BN, int NS, int MINB, bool NT, bool QUP, bool EXPAND = false>
 __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
     static_assert(!NT || !QUP, "2a2 reads N-contiguous W");
+    static_assert(!EXPAND || NT, "the heads' weights are K-contiguous");
+    if constexpr (EXPAND) {
+        a.M = load_uniform(a.rows);
+        a.tiles_m = (a.M + BM - 1) / BM;
+    }
     constexpr int RB = BM / 64, CB = BN / 128;         // 32x32 blocks per wave
     constexpr int kAStage = BM * 2 * kBKS, kBStage = BN * 2 * kBKS;
     constexpr int kStage = kAStage + kBStage;
@@ -104,22 +114,24 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
     auto job_at = [&](int t) __attribute__((always_inline)) {
         int tm, tn;
         Job j;
-        if (a.G > 1) {   // split == 1
+        if (!EXPAND && a.G > 1) {   // split == 1
             tn = t % a.tiles_n;
             const int tg = t / a.tiles_n;
             tm = tg / a.G;
             j.g = (tg % a.G + tm * kNumXCDs / a.tiles_m * (a.G / kNumXCDs)) % a.G;
             j.sp = 0;
         } else {
-            const int plane = a.tiles_m * a.tiles_n;
-            j.sp = t / plane;
+            const int tiles_n = EXPAND ? a.tiles_n * a.G : a.tiles_n;
+            const int plane = a.tiles_m * tiles_n;
+            j.sp = EXPAND ? 0 : t / plane;
             const int p = t - j.sp * plane;
-            const int grp = p / (kBGroupM * a.tiles_n);
+            const int grp = p / (kBGroupM * tiles_n);
             const int gm = min(kBGroupM, a.tiles_m - grp * kBGroupM);
-            const int q = p - grp * kBGroupM * a.tiles_n;
+            const int q = p - grp * kBGroupM * tiles_n;
             tm = grp * kBGroupM + q % gm;
             tn = q / gm;
-            j.g = 0;
+            j.g = EXPAND ? tn / a.tiles_n : 0;
+            if (EXPAND) tn -= j.g * a.tiles_n;
         }
         j.m0 = tm * BM;
         j.n0 = tn * BN;
@@ -128,6 +140,8 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
         j.a_base = reinterpret_cast<uint64_t>(a.A + j.g * a.sAg + (int64_t)j.m0 * a.lda + k0);
         j.b_base = reinterpret_cast<uint64_t>(
             a.B + j.g * a.sBg + (NT ? (int64_t)j.n0 * a.ldb + k0 : (int64_t)k0 * a.ldb + j.n0));
+        if constexpr (EXPAND)
+            if (j.n0 + (BN / 8) * wave >= 128) j.b_base += 2 * (uint64_t)a.b_hi;   // this wave's rows
         const int rows = min(BM, a.M - j.m0), cols = min(BN, a.N - j.n0);
         j.a_bytes = (uint32_t)(rows - 1) * (uint32_t)a.lda * 2u + 2u * kBKS;
         j.b_bytes = NT ? (uint32_t)(cols - 1) * (uint32_t)a.ldb * 2u + 2u * kBKS
@@ -376,6 +390,19 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
             }
             const __amdgpu_buffer_rsrc_t rc = make_rsrc(a.C16 + (int64_t)job.g * a.sCg + (int64_t)job.m0 * a.ldc);
             const uint32_t cmask = oob_mask(col, a.N);
+            // past fp16's range a key or value stays at its end: an infinite value would reach queries
+            // that its key is hidden from, as 0 * inf (a NaN stays one)
+            if constexpr (EXPAND && Half<TL>::kF16) {
+                #pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+                    #pragma unroll
+                    for (int cb = 0; cb < CB; ++cb)
+                        #pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float x = acc[rb][cb][e];
+                            acc[rb][cb][e] = fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
+                        }
+            }
             #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 #pragma unroll
@@ -510,6 +537,37 @@ hipError_t launch_bgemm(const GemmProblem& p, const GemmPlan& plan, float* parti
                      : launch_bgemm_t<bf16_t, true, false>(a, plan, grid, stream);
     return p.f16 ? launch_bgemm_t<f16_t, false, false>(a, plan, grid, stream)
                  : launch_bgemm_t<bf16_t, false, false>(a, plan, grid, stream);
+}
+
+// Keys and values of the expanded attention: kv[h][row][0..127] = lat[row] W_uk[h]^T, [128..255] =
+// lat[row] W_uv[h]^T, for the rows that *rows says (at most rows_cap).
+hipError_t launch_kv_expand(const KvExpand& p, hipStream_t stream) {
+    constexpr int kR = 512, kN = 128;
+    BArgs a = {};
+    a.A = p.lat; a.lda = kR; a.sAg = 0;
+    a.B = p.W_uk; a.ldb = kR; a.sBg = (int64_t)kN * kR;
+    a.b_hi = (int64_t)((reinterpret_cast<uintptr_t>(p.W_uv) - reinterpret_cast<uintptr_t>(p.W_uk)) / 2) -
+             (int64_t)kN * kR;
+    a.C16 = p.kv; a.ldc = 2 * kN; a.sCg = p.rows_cap * 2 * kN;
+    a.N = 2 * kN; a.K = kR; a.G = p.heads; a.split = 1; a.k_chunk = kR;
+    a.rows = p.rows;
+    // tiles of 128 x 128 (two workgroups a CU) while those of 256 x 256 are fewer than the CUs
+    const bool small = (p.rows_cap + 255) / 256 * p.heads < kNumCUs;
+    const int bm = small ? 128 : 256;
+    a.tiles_n = 2 * kN / bm;
+    const int64_t tiles = (p.rows_cap + bm - 1) / bm * a.tiles_n * p.heads;
+    if (tiles <= 0 || tiles > 0x3fffffff) return hipErrorInvalidValue;
+    const int64_t resident = (int64_t)kNumCUs * (small ? 2 : 1);
+    const dim3 grid((unsigned)(std::min(tiles, resident) + kNumXCDs - 1) / kNumXCDs * kNumXCDs), block(kBThreads);
+    if (small && p.f16)
+        hipLaunchKernelGGL((bgemm_kernel<f16_t, 128, 128, 4, 4, true, false, true>), grid, block, 0, stream, a);
+    else if (small)
+        hipLaunchKernelGGL((bgemm_kernel<bf16_t, 128, 128, 4, 4, true, false, true>), grid, block, 0, stream, a);
+    else if (p.f16)
+        hipLaunchKernelGGL((bgemm_kernel<f16_t, 256, 256, 4, 2, true, false, true>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((bgemm_kernel<bf16_t, 256, 256, 4, 2, true, false, true>), grid, block, 0, stream, a);
+    return hipGetLastError();
 }
 
 }  // namespace mla

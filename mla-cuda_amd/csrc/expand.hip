@@ -1,0 +1,606 @@
+// Attention in the expanded form, for chunks of many new tokens: every head has keys and values of
+// its own, made from the cache's latent rows,
+//   k[h] = W_uk[h] c (128),  v[h] = W_uv[h] c (128),
+//   out[h] = softmax((q_nope[h] . k[h] + q_rope[h] . pe) / scale) v[h],
+// the same function as the absorbed pass (flash.hip) at 2 * 320 operations a pair and head instead of
+// 2 * 1,088, for 2 * 256 * 512 a key and head once.  In launches:
+//   expand_plan_kernel    which 64-row units of the cache the batch holds, shared pages once
+//   expand_gather_kernel  their rows side by side in 16 bits: latent [rows, 512], rope [rows, 64]
+//   bgemm_kernel<EXPAND>  the heads' keys and values [heads][rows][128 | 128] (bgemm.hip)
+//   heads_kernel          the attention
+// the last two for as many heads at a time as the workspace holds.
+
+#include <algorithm>
+
+#include "kernels.h"
+#include "mma.h"
+#include "stage.h"
+
+namespace mla {
+
+namespace {
+
+typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
+typedef float v2f_t __attribute__((ext_vector_type(2)));
+
+constexpr int kUnit = kExpandUnit;            // rows a unit (and keys a step of the attention)
+constexpr int kR = 512, kD = 64, kN = 128;    // latent, rope, nope / value widths
+
+// ---- units ----------------------------------------------------------------------------------
+// Unit j of sequence b is its keys [64 j, 64 j + 64).  Sequences that continue one prompt hold the
+// same page there; such a unit is expanded once, for the lowest of them (only where it is full in
+// both: the rows past a sequence's end are zeros, and the others' are not).  A sequence is only
+// compared with those that share its first page, which is what a shared prefix begins with.
+struct PlanArgs {
+    const int* seq_lens;     // null, with the table: a dense cache, nothing to plan
+    const int* table;
+    int* owner;      // [B][units] the sequence that the unit is made for
+    int* rank;       // [B][units] how many own units it has in front
+    int* count;      // [B] own units
+    int* any_bad;
+    int B, Sk, units, max_pages, per_page;   // per_page: units a page
+};
+
+constexpr int kPlanThreads = 256, kPlanList = 1024;
+
+__global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
+    __shared__ int list[kPlanList], n_list, w_own[kPlanThreads / 64];
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (b == 0 && tid == 0) *a.any_bad = 0;
+    if (!a.table) return;
+    const int len = min(max(a.seq_lens[b], 0), a.Sk);
+    const int* row = a.table + (int64_t)b * a.max_pages;
+    // sequences in front of this one with the same first page, in order
+    if (tid == 0) n_list = 0;
+    __syncthreads();
+    if (len >= kUnit && wave == 0) {
+        const int page = row[0];
+        int n = 0;
+        for (int c0 = 0; c0 < b && n < kPlanList; c0 += 64) {
+            const int c = min(c0 + lane, b);
+            const bool same = c < b && a.table[(int64_t)c * a.max_pages] == page && a.seq_lens[c] >= kUnit;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(same);
+            const int at = n + __popcll(m & ((1ull << lane) - 1));
+            if (same && at < kPlanList) list[at] = c;
+            n += __popcll(m);
+        }
+        if (lane == 0) n_list = min(n, kPlanList);
+    }
+    __syncthreads();
+    const int units = (len + kUnit - 1) / kUnit;
+    int base = 0;
+    for (int j0 = 0; j0 < units; j0 += kPlanThreads) {
+        const int j = j0 + tid;
+        int own = b;
+        if (j < units && (j + 1) * kUnit <= len) {
+            const int pg = j / a.per_page, page = row[pg];
+            for (int i = 0; i < n_list; ++i) {
+                const int c = list[i];
+                if (a.table[(int64_t)c * a.max_pages + pg] == page && a.seq_lens[c] >= (j + 1) * kUnit) {
+                    own = c;
+                    break;
+                }
+            }
+        }
+        const bool mine = j < units && own == b;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(mine);
+        if (lane == 0) w_own[wave] = __popcll(m);
+        __syncthreads();
+        int before = base;
+        for (int w = 0; w < kPlanThreads / 64; ++w) {
+            if (w < wave) before += w_own[w];
+            base += w_own[w];
+        }
+        if (j < units) {
+            a.owner[(int64_t)b * a.units + j] = own;
+            a.rank[(int64_t)b * a.units + j] = before + __popcll(m & ((1ull << lane) - 1));
+        }
+        __syncthreads();
+    }
+    if (tid == 0) a.count[b] = base;
+}
+
+// ---- gather ---------------------------------------------------------------------------------
+// A workgroup copies a unit's rows, or only notes where its owner's are.  A latent row with a value
+// that is not finite makes every key and value of it NaN or infinite, and with it every output of a
+// query that sees it NaN (also under a weight of 0); the row is written as zeros, so that queries
+// in front of it are not touched by 0 * NaN, and the unit's first such row is noted for the queries
+// behind it.  Rope values need no such care: they only reach their own key's scores.
+struct GatherArgs {
+    const void* c_kv;
+    const void* pe;
+    const uint8_t* scales;
+    const int* seq_lens;     // null: every sequence has Sk keys
+    const int* table;        // null: [B, Sk] rows
+    const int* owner;
+    const int* rank;
+    const int* count;
+    int* unit;               // [B][units] the unit's place in lat / rot
+    int* bad;                // [places] first row that is not finite, or 64
+    int* any_bad;
+    int* rows;               // rows in all
+    uint16_t* lat;
+    uint16_t* rot;
+    int B, Sk, units, max_pages, page_size, num_pages, block_shift;
+};
+
+template <typename TL>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+    constexpr uint32_t e = Half<TL>::kF16 ? 0x7c00u : 0x7f80u;
+    return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// four e4m3 codes under a power of two, in the 16-bit type
+template <typename TL>
+__device__ __forceinline__ v2u_t decode_half4(uint32_t w, float scale) {
+    const v2f_t lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false);
+    const v2f_t hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
+    return v2u_t{Half<TL>::pack2(lo[0], lo[1]), Half<TL>::pack2(hi[0], hi[1])};
+}
+
+template <typename TL, bool F8>
+__global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
+    __shared__ int part[4], w_bad[4];
+    const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.Sk) : a.Sk;
+    const bool first = j == 0 && b == 0;
+    const bool here = j * kUnit < len;
+    if (!here && !first) return;
+    int place = b * a.units + j, own = b;
+    if (a.table) {
+        const int at = place;
+        own = here ? a.owner[at] : 0;
+        // units of the sequences in front of the owner; the first workgroup also adds up all of them
+        int sum = 0, all = 0;
+        for (int c = tid; c < (first ? a.B : own); c += 256) {
+            const int n = a.count[c];
+            all += n;
+            sum += c < own ? n : 0;
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) part[wave] = sum;
+        __syncthreads();
+        sum = part[0] + part[1] + part[2] + part[3];
+        if (first) {
+            __syncthreads();
+            all = wave_sum(all);
+            if (lane == 0) part[wave] = all;
+            __syncthreads();
+            if (tid == 0) *a.rows = kUnit * (part[0] + part[1] + part[2] + part[3]);
+        }
+        if (!here) return;
+        place = sum + a.rank[(int64_t)own * a.units + j];
+        if (tid == 0) a.unit[at] = place;
+        if (own != b) return;
+    } else if (tid == 0) {
+        a.unit[place] = place;
+        if (first) *a.rows = kUnit * a.B * a.units;
+    }
+
+    // where the unit's rows lie (a page is a whole number of units)
+    const int k0 = j * kUnit;
+    int64_t r0 = (int64_t)b * a.Sk + k0;
+    bool in = true;
+    if (a.table) {
+        const int page = a.table[(int64_t)b * a.max_pages + k0 / a.page_size];
+        in = page >= 0 && page < a.num_pages;
+        r0 = (int64_t)page * a.page_size + k0 % a.page_size;
+    }
+    const int n = in ? min(kUnit, len - k0) : 0;
+    uint16_t* lat = a.lat + (int64_t)place * kUnit * kR;
+    uint16_t* rot = a.rot + (int64_t)place * kUnit * kD;
+    // latent rows: 16 a wave, 8 columns a lane
+    int worst = kUnit;
+    #pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        v4u x[8];
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 16 * wave + 8 * half + i;
+            x[i] = v4u{0, 0, 0, 0};
+            if (r >= n) continue;
+            if constexpr (F8) {
+                const v2u_t c = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.c_kv) + (r0 + r) * kR)[lane];
+                const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift)] << 23);
+                const v2u_t lo = decode_half4<TL>(c[0], f), hi = decode_half4<TL>(c[1], f);
+                x[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
+            } else {
+                x[i] = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.c_kv) + (r0 + r) * kR)[lane];
+            }
+        }
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 16 * wave + 8 * half + i;
+            bool odd = not_finite2<TL>(x[i][0]) || not_finite2<TL>(x[i][1]) ||
+                       not_finite2<TL>(x[i][2]) || not_finite2<TL>(x[i][3]);
+            odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+            if (odd) {
+                worst = min(worst, r);
+                x[i] = v4u{0, 0, 0, 0};
+            }
+            reinterpret_cast<v4u*>(lat + r * kR)[lane] = x[i];
+        }
+    }
+    // rope rows: 8 lanes a row
+    #pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = 32 * half + (tid >> 3), c = tid & 7;
+        v4u x = {0, 0, 0, 0};
+        if (r < n) {
+            if constexpr (F8) {
+                const v2u_t w = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.pe) + (r0 + r) * kD)[c];
+                const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift) + 1] << 23);
+                const v2u_t lo = decode_half4<TL>(w[0], f), hi = decode_half4<TL>(w[1], f);
+                x = v4u{lo[0], lo[1], hi[0], hi[1]};
+            } else {
+                x = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.pe) + (r0 + r) * kD)[c];
+            }
+        }
+        reinterpret_cast<v4u*>(rot + r * kD)[c] = x;
+    }
+    if (lane == 0) w_bad[wave] = worst;
+    __syncthreads();
+    if (tid == 0) {
+        worst = min(min(w_bad[0], w_bad[1]), min(w_bad[2], w_bad[3]));
+        a.bad[place] = worst;
+        if (worst < kUnit) *a.any_bad = 1;   // cleared by the plan; every writer writes the same
+    }
+}
+
+// ---- attention ------------------------------------------------------------------------------
+// A workgroup has 128 query rows of one head, a wave 32 of them, and walks the keys in steps of a
+// unit: its keys (nope 16 KB, rope 8 KB) and values (16 KB) go global -> LDS with direct loads, two
+// stages of them, and two workgroups share a CU.
+// A wave's scores are S^T = K Q^T, 32 keys x 32 queries an accumulator: a lane has one query's
+// scores (the other half-wave the other half of them), so that maxima, sums and rescaling are a
+// lane's own business, and the exponentials, packed as they lie, are the B operand of O^T = V^T P^T:
+// a lane's eight of a 16-key step are keys 4h + 0..3 and 8 + 4h + 0..3 (h: its half), and V's
+// transposing reads take the rows in that order.
+// The reference of a row's exponentials moves only when a score passes it by kRise powers of two (few
+// do after the first step), and what is in the accumulators is scaled then.
+struct HeadsArgs {
+    const uint16_t* qn;      // [B, Sq, H, 128]
+    const uint16_t* qr;      // [B, Sq, H, 64]
+    const uint16_t* kv;      // [heads][rows_cap][256]
+    const uint16_t* rot;     // [rows_cap][64]
+    const int* unit;
+    const int* bad;
+    const int* any_bad;
+    const int* seq_lens;
+    const int* new_lens;
+    uint16_t* out;           // [B, Sq, H, 128]
+    int B, Sq, Sk, H, h0, units, tiles, causal;
+    int64_t head_stride;     // elements of kv a head
+    float c;                 // log2(e) / scale
+};
+
+constexpr int kHRows = 128, kHThreads = 256;
+constexpr int kKBytes = kUnit * 2 * kN, kRBytes = kUnit * 2 * kD;       // a stage's parts
+constexpr int kStageBytes = 2 * kKBytes + kRBytes;
+constexpr int kVAt = kKBytes, kRAt = 2 * kKBytes;
+
+template <typename TL>
+__global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStageBytes];
+    // fp16 weights start at 2^kBias and may rise to 2^(kBias + kRise) < 65504: small ones keep more
+    // bits above its subnormals; bf16 has the exponent range of the sums
+    constexpr float kRise = Half<TL>::kF16 ? 6.f : 8.f, kBias = Half<TL>::kF16 ? 8.f : 0.f;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hi = lane >> 5, q = lane & 31;
+    const uint32_t lds0 = lds_addr(smem);
+
+    // heads outermost, a contiguous run of them an XCD; within a head the longest tiles first
+    const int item = xcd_logical_block(blockIdx.x, gridDim.x);
+    const int per_head = a.B * a.tiles;
+    const int hl = item / per_head, rest = item - hl * per_head;
+    const int t = a.tiles - 1 - rest / a.B, b = rest % a.B;
+    const int h = a.h0 + hl;
+    const int len = a.seq_lens ? min(max(load_uniform(a.seq_lens + b), 0), a.Sk) : a.Sk;
+    const int fresh = a.new_lens ? min(max(load_uniform(a.new_lens + b), 0), a.Sq) : a.Sq;
+    const int pad = a.Sq - fresh;
+    const int64_t row_stride = (int64_t)a.H * kN;
+    uint16_t* const out = a.out + (int64_t)b * a.Sq * row_stride + (int64_t)h * kN;
+
+    // rows in front of the new ones
+    for (int r = kHRows * t + (tid >> 4); r < min(pad, kHRows * (t + 1)); r += kHThreads / 16)
+        reinterpret_cast<v4u*>(out + r * row_stride)[tid & 15] = v4u{0, 0, 0, 0};
+    const int r0 = pad + kHRows * t;
+    if (r0 >= a.Sq) return;
+
+    // row i sees keys up to lim(i)
+    auto lim_of = [&](int row) __attribute__((always_inline)) {
+        return a.causal ? min(len - a.Sq + row, len - 1) : len - 1;
+    };
+    const int w0 = r0 + 32 * wave;
+    const int row = min(w0 + q, a.Sq - 1);
+    const int lim = lim_of(row);
+    const int wave_first = w0 < a.Sq ? lim_of(w0) : -1, wave_last = w0 < a.Sq ? lim_of(min(w0 + 31, a.Sq - 1)) : -1;
+    const int n_tiles = (lim_of(min(r0 + kHRows, a.Sq) - 1) + kUnit) / kUnit;   // lim -1: 0
+
+    v4u qf[12];
+    {
+        const uint16_t* p = a.qn + ((int64_t)b * a.Sq + row) * row_stride + (int64_t)h * kN + 8 * hi;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) qf[i] = *reinterpret_cast<const v4u*>(p + 16 * i);
+        const uint16_t* r = a.qr + (((int64_t)b * a.Sq + row) * a.H + h) * kD + 8 * hi;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) qf[8 + i] = *reinterpret_cast<const v4u*>(r + 16 * i);
+    }
+
+    // ---- staging.  Key rows of 256 bytes, 16-byte chunk c of row r at c ^ (r & 15); value rows of
+    // 256, chunk c at c ^ 4 (r & 3); rope rows of 128, chunk c at c ^ ((r >> 1) & 7).
+    const uint64_t kv = reinterpret_cast<uint64_t>(a.kv + hl * a.head_stride);
+    const uint64_t rot = reinterpret_cast<uint64_t>(a.rot);
+    const int* units = a.unit + (int64_t)b * a.units;
+    const uint32_t l4 = lane >> 4, l15 = lane & 15;
+    const uint32_t voff_k = (16 * wave + l4) * 512 + 16 * (l15 ^ l4);
+    const uint32_t voff_v = (16 * wave + l4) * 512 + 256 + 16 * (l15 ^ (4 * l4));
+    const uint32_t voff_r = (16 * wave + (lane >> 3)) * 128 + 16 * ((lane & 7) ^ l4);
+    auto issue = [&](int place, uint32_t st) __attribute__((always_inline)) {
+        const v4i rk = rsrc_span(kv + (uint64_t)place * (kUnit * 512), 0, kUnit * 512);
+        const v4i rr = rsrc_span(rot + (uint64_t)place * (kUnit * 128), 0, kUnit * 128);
+        const uint32_t base = __builtin_amdgcn_readfirstlane(lds0 + st + 16 * wave * 256);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            dma16(rk, base + 1024 * i, (voff_k + 2048 * i) ^ (64 * i));
+            dma16(rk, base + kVAt + 1024 * i, voff_v + 2048 * i);
+        }
+        const uint32_t rbase = __builtin_amdgcn_readfirstlane(lds0 + st + kRAt + 16 * wave * 128);
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) dma16(rr, rbase + 1024 * i, (voff_r + 1024 * i) ^ (64 * i));
+    };
+
+    // ---- fragments
+    const uint32_t k_rd = (uint32_t)q * 256 + 16 * (hi ^ (q & 15));
+    const uint32_t r_rd = kRAt + (uint32_t)q * 128 + 16 * (hi ^ ((q >> 1) & 7));
+    const int G4 = lane >> 4, q4 = (lane >> 2) & 3, i4 = lane & 3;
+    const uint32_t v_rd = kVAt + (uint32_t)(4 * (G4 >> 1) + q4) * 256 +
+                          16 * ((2 * (G4 & 1) + (i4 >> 1)) ^ (4 * q4)) + 8 * (i4 & 1);
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+    v16f o[4];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = v16f{};
+    float m_ref = -INFINITY, l = 0.f;
+
+    int next = n_tiles > 0 ? load_uniform(units) : 0;
+    if (n_tiles > 0) issue(next, 0);
+    next = n_tiles > 1 ? load_uniform(units + 1) : 0;
+    #pragma unroll 1
+    for (int j = 0; j < n_tiles; ++j) {
+        const uint32_t st = (j & 1) * kStageBytes;
+        wait_vm<0>();
+        lds_barrier();      // step j has landed; every wave is done with step j - 1
+        if (j + 1 < n_tiles) {
+            issue(next, kStageBytes - st);
+            next = j + 2 < n_tiles ? load_uniform(units + j + 2) : 0;
+        }
+        if (j * kUnit > wave_last) continue;
+        v16f s[2] = {v16f{}, v16f{}};
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
+            #pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                s[kb] = Mma<TL>::sub(*reinterpret_cast<const v4u*>(smem + st + 8192 * kb + (k_rd ^ (32 * i))),
+                                     qf[i], 0, s[kb]);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i)
+            #pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                s[kb] = Mma<TL>::sub(*reinterpret_cast<const v4u*>(smem + st + 4096 * kb + (r_rd ^ (32 * i))),
+                                     qf[8 + i], 0, s[kb]);
+        if (j * kUnit + kUnit - 1 > wave_first) {
+            #pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                #pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[kb][i] = j * kUnit + 32 * kb + acc_row(i, lane) <= lim ? s[kb][i] : -INFINITY;
+        }
+        float top = s[0][0];
+        #pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.c;
+        }
+        // (only those rows: a row's bits do not depend on the others of its wave)
+        const bool over = top > m_ref + kRise;
+        if (__builtin_amdgcn_ballot_w64(over)) {
+            const float m = over ? top : m_ref;
+            const float f = over ? __builtin_amdgcn_exp2f(m_ref - m) : 1.f;
+            m_ref = m;
+            l *= f;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                #pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= f;
+        }
+        const float neg = m_ref == -INFINITY ? 0.f : kBias - m_ref;
+        #pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.c, neg));
+                l += s[kb][i];
+            }
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {       // 16 keys
+            v4u p;
+            #pragma unroll
+            for (int e = 0; e < 4; ++e)
+                p[e] = Half<TL>::pack2(s[i >> 1][8 * (i & 1) + 2 * e], s[i >> 1][8 * (i & 1) + 2 * e + 1]);
+            #pragma unroll
+            for (int vb = 0; vb < 4; ++vb) {
+                const uint8_t* at = smem + st + 4096 * i + (v_rd ^ (64 * vb));
+                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 2048));
+                o[vb] = Mma<TL>::sub(__builtin_bit_cast(v4u, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)),
+                                     p, 0, o[vb]);
+            }
+        }
+    }
+
+    {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    float f = l == 0.f ? 0.f : 1.f / l;
+    if (load_uniform(a.any_bad)) {
+        int worst = 0x7fffffff;
+        for (int j = lane; j < n_tiles; j += 64) {
+            const int r = a.bad[units[j]];
+            if (r < kUnit) worst = min(worst, j * kUnit + r);
+        }
+        #pragma unroll
+        for (int i = 1; i < 64; i *= 2) worst = min(worst, __shfl_xor(worst, i));
+        if (worst <= lim) f = __uint_as_float(0x7fc00000u);
+    }
+    // an average of values up to 65504 stays there, also where its weights are rounded up (NaN is NaN)
+    if constexpr (Half<TL>::kF16) {
+        #pragma unroll
+        for (int vb = 0; vb < 4; ++vb)
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = o[vb][i] * f;
+                o[vb][i] = fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
+            }
+        f = 1.f;
+    }
+    if (w0 + q < a.Sq) {
+        uint16_t* const dst = out + row * row_stride + 4 * hi;
+        #pragma unroll
+        for (int vb = 0; vb < 4; ++vb)
+            #pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<v2u_t*>(dst + 32 * vb + 2 * i) =
+                    v2u_t{Half<TL>::pack2(o[vb][i] * f, o[vb][i + 1] * f),
+                          Half<TL>::pack2(o[vb][i + 2] * f, o[vb][i + 3] * f)};
+    }
+}
+
+// ---- queries per head -----------------------------------------------------------------------
+// The nope columns of q_raw (fp32 [rows, H (nope + rope)]) in 16 bits, [rows, H, nope].
+template <typename TL>
+__global__ void __launch_bounds__(256) q_nope_kernel(const float* __restrict__ raw, uint16_t* __restrict__ out,
+                                                     int64_t chunks, int nope, int qk) {
+    const int per = nope / 8;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < chunks; i += gridDim.x * 256ll) {
+        const int64_t r = i / per;
+        const float* p = raw + r * qk + 8 * (i - r * per);
+        const v4f x = *reinterpret_cast<const v4f*>(p), y = *reinterpret_cast<const v4f*>(p + 4);
+        reinterpret_cast<v4u*>(out)[i] = v4u{Half<TL>::pack2(x[0], x[1]), Half<TL>::pack2(x[2], x[3]),
+                                             Half<TL>::pack2(y[0], y[1]), Half<TL>::pack2(y[2], y[3])};
+    }
+}
+
+// Keys and values of this many bytes at a time at most, in groups of heads (one head at least).
+constexpr int64_t kExpandBytes = (int64_t)2 << 30;
+
+}  // namespace
+
+ExpandPlan plan_expand(int B, int Sk, int H, bool paged) {
+    ExpandPlan p;
+    p.units = (Sk + kUnit - 1) / kUnit;
+    const int64_t places = (int64_t)B * p.units;
+    p.rows_cap = places * kUnit;
+    p.heads = (int)std::max<int64_t>(1, std::min<int64_t>(H, kExpandBytes / (p.rows_cap * 512)));
+    size_t o = 0;
+    auto take = [&](size_t bytes) {
+        const size_t at = o;
+        o = (o + bytes + 255) / 256 * 256;
+        return at;
+    };
+    p.off_owner = take(paged ? places * 4 : 0);
+    p.off_rank = take(paged ? places * 4 : 0);
+    p.off_count = take(paged ? (size_t)B * 4 : 0);
+    p.off_unit = take(places * 4);
+    p.off_bad = take(places * 4);
+    p.off_any = take(8);                      // any_bad, rows
+    p.off_lat = take((size_t)p.rows_cap * kR * 2);
+    p.off_rot = take((size_t)p.rows_cap * kD * 2);
+    p.off_kv = take((size_t)p.heads * p.rows_cap * 512);
+    p.total = o;
+    return p;
+}
+
+hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* workspace, hipStream_t stream) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    auto ints = [&](size_t off) { return reinterpret_cast<int*>(ws + off); };
+    auto half = [&](size_t off) { return reinterpret_cast<uint16_t*>(ws + off); };
+    const int64_t tiles = (p.Sq + kHRows - 1) / kHRows;
+    if (p.B > 65535 || plan.rows_cap > 0x7fffffff || tiles * p.B * plan.heads > 0x7fffffff)
+        return hipErrorInvalidValue;
+    int* any_bad = ints(plan.off_any);
+    PlanArgs u;
+    u.seq_lens = p.seq_lens; u.table = p.block_table;
+    u.owner = ints(plan.off_owner); u.rank = ints(plan.off_rank); u.count = ints(plan.off_count);
+    u.any_bad = any_bad;
+    u.B = p.B; u.Sk = p.Sk; u.units = plan.units;
+    u.max_pages = p.block_table ? p.Sk / p.page_size : 0;
+    u.per_page = p.block_table ? p.page_size / kUnit : 1;
+    hipLaunchKernelGGL(expand_plan_kernel, dim3(p.block_table ? p.B : 1), dim3(kPlanThreads), 0, stream, u);
+    GatherArgs g;
+    g.c_kv = p.c_kv; g.pe = p.pe; g.scales = static_cast<const uint8_t*>(p.scales);
+    g.seq_lens = p.seq_lens; g.table = p.block_table;
+    g.owner = u.owner; g.rank = u.rank; g.count = u.count;
+    g.unit = ints(plan.off_unit); g.bad = ints(plan.off_bad); g.any_bad = any_bad; g.rows = any_bad + 1;
+    g.lat = half(plan.off_lat); g.rot = half(plan.off_rot);
+    g.B = p.B; g.Sk = p.Sk; g.units = plan.units;
+    g.page_size = p.page_size; g.max_pages = u.max_pages; g.num_pages = p.num_pages;
+    g.block_shift = p.scale_block == 16 ? 4 : p.scale_block == 32 ? 5 : 6;
+    const dim3 gather((unsigned)plan.units, (unsigned)p.B);
+    if (p.scales) {
+        if (p.f16) hipLaunchKernelGGL((expand_gather_kernel<f16_t, true>), gather, dim3(256), 0, stream, g);
+        else hipLaunchKernelGGL((expand_gather_kernel<bf16_t, true>), gather, dim3(256), 0, stream, g);
+    } else {
+        if (p.f16) hipLaunchKernelGGL((expand_gather_kernel<f16_t, false>), gather, dim3(256), 0, stream, g);
+        else hipLaunchKernelGGL((expand_gather_kernel<bf16_t, false>), gather, dim3(256), 0, stream, g);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+
+    HeadsArgs a;
+    a.qn = static_cast<const uint16_t*>(p.q_nope); a.qr = static_cast<const uint16_t*>(p.q_rope);
+    a.kv = half(plan.off_kv); a.rot = g.rot;
+    a.unit = g.unit; a.bad = g.bad; a.any_bad = any_bad;
+    a.seq_lens = p.seq_lens; a.new_lens = p.new_lens;
+    a.out = static_cast<uint16_t*>(p.out);
+    a.B = p.B; a.Sq = p.Sq; a.Sk = p.Sk; a.H = p.H; a.units = plan.units;
+    a.tiles = (int)tiles; a.causal = p.causal;
+    a.head_stride = plan.rows_cap * 256;
+    a.c = (float)(1.4426950408889634 / p.scale);
+    for (int h0 = 0; h0 < p.H; h0 += plan.heads) {
+        const int heads = std::min(plan.heads, p.H - h0);
+        KvExpand k;
+        k.f16 = p.f16;
+        k.lat = g.lat; k.kv = half(plan.off_kv);
+        k.W_uk = static_cast<const uint16_t*>(p.W_uk) + (int64_t)h0 * kN * kR;
+        k.W_uv = static_cast<const uint16_t*>(p.W_uv) + (int64_t)h0 * kN * kR;
+        k.rows = g.rows; k.rows_cap = plan.rows_cap; k.heads = heads;
+        e = launch_kv_expand(k, stream);
+        if (e != hipSuccess) return e;
+        a.h0 = h0;
+        const dim3 grid((unsigned)(tiles * p.B * heads));
+        if (p.f16) hipLaunchKernelGGL(heads_kernel<f16_t>, grid, dim3(kHThreads), 0, stream, a);
+        else hipLaunchKernelGGL(heads_kernel<bf16_t>, grid, dim3(kHThreads), 0, stream, a);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_q_nope(const float* raw, void* out, bool f16, int64_t rows, int nope, int qk,
+                         hipStream_t stream) {
+    const int64_t chunks = rows * (nope / 8);
+    const dim3 grid((unsigned)std::min<int64_t>((chunks + 255) / 256, 16 * kNumCUs));
+    uint16_t* o = static_cast<uint16_t*>(out);
+    if (f16) hipLaunchKernelGGL(q_nope_kernel<f16_t>, grid, dim3(256), 0, stream, raw, o, chunks, nope, qk);
+    else hipLaunchKernelGGL(q_nope_kernel<bf16_t>, grid, dim3(256), 0, stream, raw, o, chunks, nope, qk);
+    return hipGetLastError();
+}
+
+}  // namespace mla

@@ -344,6 +344,51 @@ int flash_worklist_ints(const FlashProblem& p, const FlashPlan& plan);
 hipError_t launch_flash_worklist(const FlashProblem& p, const FlashPlan& plan, int* wl,
                                  hipStream_t stream);
 
+// ---------------------------------------------------------------- expanded form (expand.hip)
+// out[b, i, h] = softmax((q_nope . W_uk[h] c + q_rope . pe) / scale) W_uv[h] c over the keys that
+// query i sees; 16 bits, kv_rank 512, rope 64, nope and v 128.
+constexpr int kExpandUnit = 64;      // keys that are expanded, and shared, together
+struct ExpandProblem {
+    bool f16 = false;
+    const void* q_nope = nullptr;    // [B, Sq, H, 128]
+    const void* q_rope = nullptr;    // [B, Sq, H, 64]
+    const void* c_kv = nullptr;      // [B, Sk, 512], or pools of pages (e4m3 codes with scales)
+    const void* pe = nullptr;
+    const void* scales = nullptr;    // as FlashProblem's
+    const void* W_uk = nullptr;      // [H, 128, 512]
+    const void* W_uv = nullptr;
+    void* out = nullptr;             // [B, Sq, H, 128]
+    const int32_t* seq_lens = nullptr;     // paged
+    const int32_t* block_table = nullptr;  // paged
+    const int32_t* new_lens = nullptr;     // or null: Sq of each
+    int B = 0, Sq = 0, Sk = 0, H = 0, page_size = 0, num_pages = 0, scale_block = 0;
+    double scale = 1.0;
+    bool causal = false;
+};
+struct ExpandPlan {
+    int units = 0;                   // of a sequence, at most
+    int64_t rows_cap = 0;            // rows of all of them
+    int heads = 0;                   // expanded and attended to at a time
+    size_t off_owner, off_rank, off_count, off_unit, off_bad, off_any, off_lat, off_rot, off_kv, total;
+};
+ExpandPlan plan_expand(int B, int Sk, int H, bool paged);
+hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* workspace, hipStream_t stream);
+// its product (bgemm.hip): kv [heads][rows_cap][256] from lat [rows][512]; *rows on the device
+struct KvExpand {
+    bool f16 = false;
+    const uint16_t* lat = nullptr;
+    const uint16_t* W_uk = nullptr;
+    const uint16_t* W_uv = nullptr;
+    uint16_t* kv = nullptr;
+    const int* rows = nullptr;
+    int64_t rows_cap = 0;
+    int heads = 0;
+};
+hipError_t launch_kv_expand(const KvExpand& p, hipStream_t stream);
+// q_raw's nope columns in 16 bits: raw [rows][qk] -> out [rows][nope], nope a multiple of 8
+hipError_t launch_q_nope(const float* raw, void* out, bool f16, int64_t rows, int nope, int qk,
+                         hipStream_t stream);
+
 // ---------------------------------------------------------------- float64 path (f64.hip)
 // C[g] = alpha * A[g] . op(B[g]) + beta * C[g] in double on the double MFMA (beta 0: C is
 // not read):  A[g][m][k] at A + g*sA + m*lda + k;  B (NN) at B + g*sB + k*ldb + n,

@@ -1,0 +1,377 @@
+"""GPU checks of the expanded attention (dense, paged, paged in 8 bits) and of the queries per head
+that it takes, against 64-bit plain forms (tests/expanded_ref.py, which derives the tolerances)."""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+import blocked_cache as K
+import expanded_ref as E
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF, H16 = torch.bfloat16, torch.float16
+DT = {"bf16": BF, "f16": H16}
+R, D, N = 512, 64, 128
+SCALE = math.sqrt(N + D)
+NAN, INF = math.nan, math.inf
+
+
+@pytest.fixture(scope="module")
+def ext():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a ROCm GPU")
+    import mla_custom_cuda
+    return mla_custom_cuda
+
+
+def normal(g, *shape, dtype, std=1.0):
+    return (torch.randn(*shape, generator=g, device=DEV) * std).to(dtype)
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def make(seed, B, Sq, lens, H, dtype, page=64, spare=3, shared=None, spread=1.0):
+    """Queries, weights and a paged cache of random pages; rows that no sequence holds are NaN.
+    shared: {b: (c, pages)} makes the first pages of b those of c."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    max_pages = max(1, -(-max(max(lens), Sq) // page))
+    need = [-(-n // page) for n in lens]
+    P = sum(need) + spare
+    order = torch.randperm(P, generator=g, device=DEV).tolist()
+    table = torch.zeros(B, max_pages, dtype=torch.int32)
+    for b in range(B):
+        for j in range(need[b]):
+            table[b, j] = order.pop()
+        if shared and b in shared:
+            c, k = shared[b]
+            table[b, :k] = table[c, :k]
+    t = {"c_kv": torch.full((P, page, R), NAN, dtype=dtype, device=DEV),
+         "pe": torch.full((P, page, D), NAN, dtype=dtype, device=DEV)}
+    for b in range(B):
+        for j in range(need[b]):
+            n = min(page, lens[b] - j * page)
+            if shared and b in shared and j < shared[b][1]:
+                continue
+            t["c_kv"][table[b, j], :n] = normal(g, n, R, dtype=dtype)
+            t["pe"][table[b, j], :n] = normal(g, n, D, dtype=dtype)
+    t["table"], t["lens"] = table.to(DEV), i32(lens)
+    t["q_nope"] = normal(g, B, Sq, H, N, dtype=dtype, std=spread)
+    t["q_rope"] = normal(g, B, Sq, H, D, dtype=dtype, std=spread)
+    t["W_uk"] = normal(g, H, N, R, dtype=dtype, std=R ** -0.5)
+    t["W_uv"] = normal(g, H, N, R, dtype=dtype, std=R ** -0.5)
+    return t
+
+
+def rows_of(t, b, n):
+    page = t["c_kv"].size(1)
+    j = torch.arange(n, device=DEV)
+    p = t["table"][b].long()[j // page]
+    return t["c_kv"][p, j % page], t["pe"][p, j % page]
+
+
+def run_paged(ext, t, causal, new=None):
+    return ext.mla_attention_paged_expanded(
+        t["q_nope"], t["q_rope"], t["c_kv"], t["pe"], t["table"], t["lens"], t["W_uk"], t["W_uv"],
+        SCALE, causal=causal, new_lens=None if new is None else i32(new))
+
+
+def check_all(t, got, lens, causal, new=None, rows=rows_of):
+    B, Sq = t["q_nope"].shape[:2]
+    parts = [[], [], [], []]
+    for b in range(B):
+        k = Sq if new is None else max(0, min(Sq, new[b]))
+        assert not got[b, :Sq - k].any(), f"padding rows of sequence {b}"
+        lat, rot = rows(t, b, lens[b])
+        ref = E.attention(t["q_nope"][b, Sq - k:], t["q_rope"][b, Sq - k:], lat, rot, t["W_uk"], t["W_uv"],
+                          SCALE, E.limits(Sq, lens[b], k, causal), got.dtype)
+        for p, x in zip(parts, (got[b, Sq - k:],) + ref):
+            p.append(x)
+    E.check(*(torch.cat(p) for p in parts))
+
+
+# Sq around a wave's 32 rows, a workgroup's 128 and past two of those; keys around the 64-key step;
+# odd heads and head counts that do not divide by the XCDs
+PAGED = [
+    (1, 1, [1], 1), (1, 1, [64], 3), (2, 1, [65, 200], 8), (1, 2, [2], 5), (3, 31, [31, 64, 130], 2),
+    (2, 33, [33, 63], 16), (1, 127, [500], 3), (1, 128, [128], 8), (2, 129, [129, 700], 2),
+    (1, 257, [1000], 4), (4, 64, [64, 1000, 64, 127], 3), (1, 300, [2300], 9), (5, 70, [70, 71, 90, 128, 333], 1),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Sq,lens,H", PAGED)
+def test_paged_causal(ext, dtype, B, Sq, lens, H):
+    t = make(Sq + sum(lens), B, Sq, lens, H, DT[dtype])
+    check_all(t, run_paged(ext, t, True), lens, True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Sq,lens,H,page", [(2, 40, [3, 300], 2, 64), (1, 5, [1], 3, 128), (3, 140, [0, 64, 257], 2, 192)])
+def test_paged_full(ext, dtype, B, Sq, lens, H, page):
+    """Not causal: every key visible; a sequence without keys gives zeros; larger pages."""
+    t = make(7 + Sq, B, Sq, lens, H, DT[dtype], page=page)
+    check_all(t, run_paged(ext, t, False), lens, False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_ragged_new_tokens(ext, dtype, causal):
+    """Fewer new tokens than Sq, none, more than Sq and below zero (clamped); rows in front are zeros;
+    queries that see no key give zeros."""
+    lens, new, Sq = [400, 64, 10, 200, 150, 3], [150, 0, 10, 999, -5, 20], 150
+    t = make(3, 6, Sq, lens, 3, DT[dtype])
+    got = run_paged(ext, t, causal, new)
+    check_all(t, got, lens, causal, new)
+    if causal:      # sequence 5 has 3 keys: of its 20 queries the first 17 see none
+        assert not got[5, Sq - 20:Sq - 3].any() and got[5, Sq - 3:].any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_lengths_past_the_table(ext, dtype):
+    """Lengths are clamped to the table's span."""
+    t = make(4, 2, 16, [128, 128], 2, DT[dtype])
+    want = run_paged(ext, t, True)
+    t["lens"] = i32([2 ** 31 - 1, 128])
+    assert torch.equal(run_paged(ext, t, True), want)
+    t["lens"] = i32([-7, 128])
+    got = run_paged(ext, t, True)
+    assert not got[0].any() and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("page", [64, 128])
+def test_shared_pages(ext, dtype, page):
+    """Pages shared with another sequence, whole, partly past one's end, or with different lengths."""
+    k = page // 64
+    lens = [700, 650, 300, 20, 700, 128]
+    shared = {1: (0, 10 // k), 2: (0, 4 // k), 4: (2, 2 // k), 5: (0, 2 // k)}
+    t = make(9, 6, 130, lens, 2, DT[dtype], page=page, shared=shared)
+    check_all(t, run_paged(ext, t, True), lens, True)
+
+
+def test_same_page_past_one_end(ext):
+    """A page that one sequence holds in part and another whole is not taken for a shared unit."""
+    t = make(11, 2, 8, [64, 40], 2, BF)
+    t["table"][1, 0] = t["table"][0, 0]
+    check_all(t, run_paged(ext, t, True), [64, 40], True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_pages_outside_the_pool(ext, dtype):
+    """Entries outside the pool read as zero rows and are never followed."""
+    t = make(12, 2, 20, [200, 64], 2, DT[dtype])
+    t["table"][0, 1], t["table"][1, 0] = -1, t["c_kv"].size(0)
+
+    def rows(t, b, n):
+        u = dict(t, table=t["table"].clamp(0, t["c_kv"].size(0) - 1))
+        lat, rot = (x.clone() for x in rows_of(u, b, n))
+        if b == 0:
+            lat[64:128], rot[64:128] = 0, 0
+        else:
+            lat.zero_(), rot.zero_()
+        return lat, rot
+    check_all(t, run_paged(ext, t, True), [200, 64], True, rows=rows)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+def test_rows_that_are_not_finite(ext, dtype, bad):
+    """A latent value that is not finite makes the rows that see it NaN and touches no other; so
+    does a rope value of NaN; an infinite rope value gives NaN or a weight of zero."""
+    Sq, lens = 140, [300, 140]
+    t = make(13, 2, Sq, lens, 2, DT[dtype])
+    want = run_paged(ext, t, True)
+    page, at = t["table"][0, 250 // 64].item(), 250 % 64
+    t["c_kv"][page, at, 17] = bad
+    got = run_paged(ext, t, True)
+    first = 250 - (300 - Sq)                  # the query whose own key is 250
+    assert torch.equal(got[0, :first], want[0, :first]) and torch.equal(got[1], want[1])
+    assert got[0, first:].isnan().all()
+    t["c_kv"][page, at, 17] = 0
+    t["pe"][page, at, 5] = bad
+    got = run_paged(ext, t, True)
+    assert torch.equal(got[0, :first], want[0, :first]) and torch.equal(got[1], want[1])
+    if math.isnan(bad):
+        assert got[0, first:].isnan().all()
+    else:
+        down = t["q_rope"][0, first:, :, 5].double() * bad < 0
+        assert torch.equal(got[0, first:].isnan().any(-1), ~down)
+        assert torch.equal(got[0, first:].isnan().all(-1), ~down)
+
+
+def test_values_past_fp16(ext):
+    """An expanded value past fp16's range stays finite and hidden from queries in front of it."""
+    t = make(14, 1, 70, [70], 2, H16)
+    want = run_paged(ext, t, True)
+    t["c_kv"][t["table"][0, 0], 40] = 60000.0 * torch.sign(t["W_uv"][0, 0].float()).to(H16)
+    got = run_paged(ext, t, True)
+    assert torch.equal(got[0, :40], want[0, :40])
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("spread", [8.0, 30.0])
+def test_large_scores(ext, dtype, spread):
+    """Scores that climb far from one key step to the next: references move, sums stay."""
+    t = make(15, 1, 130, [900], 2, DT[dtype], spread=spread)
+    check_all(t, run_paged(ext, t, True), [900], True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Sq,Sk,H,causal", [(1, 1, 1, 1, False), (2, 50, 77, 3, True), (1, 200, 641, 8, True), (2, 130, 64, 2, False)])
+def test_dense(ext, dtype, B, Sq, Sk, H, causal):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(Sk)
+    dt = DT[dtype]
+    t = make(16, B, Sq, [Sk] * B, H, dt)
+    ckv, pe = normal(g, B, Sk, R, dtype=dt), normal(g, B, Sk, D, dtype=dt)
+    got = ext.mla_attention_expanded(t["q_nope"], t["q_rope"], ckv, pe, t["W_uk"], t["W_uv"], SCALE, causal)
+    check_all(t, got, [Sk] * B, causal, rows=lambda _, b, n: (ckv[b], pe[b]))
+    absorbed = torch.einsum("bshn,hnr->bshr", t["q_nope"].float(), t["W_uk"].float()).to(dt)
+    other = ext.mla_attention(absorbed.contiguous(), t["q_rope"], ckv, pe, t["W_uv"], SCALE, causal)
+    # the two forms round different things: keys and values here, absorbed queries and ctx there
+    assert (got.double() - other.double()).norm() <= 8 * torch.finfo(dt).eps * other.double().norm()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("page", [64, 128])
+def test_blocked_cache(ext, dtype, block, page):
+    """Over the 8-bit cache: its decoded values, exact in the queries' type."""
+    dt, Sq, lens, new = DT[dtype], 75, [200, 64, 129], [75, 3, 40]
+    t = make(17, 3, Sq, lens, 3, dt, page=page)
+    P = t["c_kv"].size(0)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(block)
+    scales = torch.randint(119, 127, (P, page // block, 2), generator=g, device=DEV).to(torch.uint8)
+    codes = {n: torch.nan_to_num(t[n].float()).mul(40).to(torch.float8_e4m3fn) for n in ("c_kv", "pe")}
+
+    def value(n, part):
+        f = torch.exp2(scales[..., part].double() - 127).repeat_interleave(block, 1)[..., None]
+        return codes[n].float().double() * f
+    plain = dict(t, c_kv=value("c_kv", 0), pe=value("pe", 1))
+    got = ext.mla_attention_paged_fp8blk_expanded(
+        t["q_nope"], t["q_rope"], codes["c_kv"], codes["pe"], scales, t["table"], t["lens"], t["W_uk"],
+        t["W_uv"], SCALE, True, i32(new))
+    check_all(dict(t), got, lens, True, new, rows=lambda _, b, n: rows_of(plain, b, n))
+    same = ext.mla_attention_paged_expanded(
+        t["q_nope"], t["q_rope"], plain["c_kv"].to(dt), plain["pe"].to(dt), t["table"], t["lens"],
+        t["W_uk"], t["W_uv"], SCALE, True, i32(new))
+    assert torch.equal(got, same)
+    # a NaN code reaches only the queries that see it
+    codes["c_kv"].view(torch.uint8)[t["table"][0, 190 // page], 190 % page, 3] = 0x7F
+    hurt = ext.mla_attention_paged_fp8blk_expanded(
+        t["q_nope"], t["q_rope"], codes["c_kv"], codes["pe"], scales, t["table"], t["lens"], t["W_uk"],
+        t["W_uv"], SCALE, True, i32(new))
+    first = 190 - (200 - Sq)
+    assert torch.equal(hurt[0, :first], got[0, :first]) and hurt[0, first:].isnan().all()
+    assert torch.equal(hurt[1:], got[1:])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,H,ragged", [(1, 4, False), (3, 128, True), (128, 6, False), (300, 16, True), (2050, 2, False)])
+def test_q_heads(ext, dtype, rows, H, ragged):
+    """q_rope has q_absorbed's bits, and q_nope times W_uk is what q_absorbed makes of it: with W_uk
+    an identity, q_nope itself."""
+    dt = DT[dtype]
+    g = torch.Generator(device=DEV)
+    g.manual_seed(rows + H)
+    B, Sq = (3, rows // 3) if ragged and rows >= 3 else (1, rows)
+    x = normal(g, B, Sq, 1024, dtype=dt)
+    wa, wb = normal(g, 1024, 256, dtype=dt, std=1 / 32), normal(g, 256, H * 192, dtype=dt, std=1 / 16)
+    gain = (1 + 0.1 * torch.randn(256, generator=g, device=DEV)).to(dt)
+    pos = torch.randint(-1, 30000, (B, Sq) if ragged else (Sq,), generator=g, device=DEV)
+    eye = torch.eye(N, dtype=dt, device=DEV).expand(H, N, N).contiguous()
+    qa, qr = ext.q_absorbed(x, wa, gain, wb, eye, pos, N, D, 1e-6)
+    qn, qr2 = ext.q_heads(x, wa, gain, wb, pos, N, D, 1e-6)
+    assert qn.shape == (B, Sq, H, N) and qr2.shape == (B, Sq, H, D)
+    assert torch.equal(qr, qr2) and torch.equal(qa, qn)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_head_groups(ext, dtype):
+    """A span whose keys and values need several groups of heads."""
+    H, Sq, n = 5, 130, 1000
+    t = make(18, 1, Sq, [n], H, DT[dtype])
+    want = run_paged(ext, t, True)
+    span = 1400000          # 2 GiB hold three heads of that many keys
+    table = torch.zeros(1, span // 64, dtype=torch.int32, device=DEV)
+    table[:, :t["table"].size(1)] = t["table"]
+    t["table"] = table
+    assert torch.equal(run_paged(ext, t, True), want)
+
+
+def test_strided_and_other_stream(ext):
+    """Non-contiguous queries, and a call on a stream of its own."""
+    t = make(19, 2, 40, [100, 70], 4, BF)
+    want = run_paged(ext, t, True)
+    wide = torch.empty(2, 40, 4, N + D, dtype=BF, device=DEV)
+    wide[..., :N], wide[..., N:] = t["q_nope"], t["q_rope"]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ext.mla_attention_paged_expanded(wide[..., :N], wide[..., N:], t["c_kv"], t["pe"], t["table"],
+                                               t["lens"], t["W_uk"], t["W_uv"], SCALE, causal=True)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_graph_replay(ext, dtype):
+    """Captured once, replayed with other lengths, rows and queries in the same tensors, beside eager
+    calls; each replay equals the eager call."""
+    lens, new = [300, 129], [100, 60]
+    t = make(20, 2, 100, lens, 4, DT[dtype])
+    fresh = i32(new)
+
+    def call():
+        return ext.mla_attention_paged_expanded(t["q_nope"], t["q_rope"], t["c_kv"], t["pe"], t["table"],
+                                                t["lens"], t["W_uk"], t["W_uv"], SCALE, True, fresh)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        if i:
+            t["q_nope"].mul_(-1.0)
+            t["lens"].copy_(i32([300 - 40 * i, 129 - i]))
+            fresh.copy_(i32([100 - i, 60 + i]))
+        if i == 2:
+            t["c_kv"][t["table"][0, 2], 3, 3] = NAN        # key 131 of sequence 0
+        if i == 3:
+            t["c_kv"][t["table"][0, 2], 3, 3] = 0.5
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+        assert bool(got.isnan().any()) == (i == 2)
+
+
+def test_same_result_twice(ext):
+    t = make(21, 3, 200, [700, 200, 333], 6, BF)
+    a, b = run_paged(ext, t, True), run_paged(ext, t, True)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_batches(ext, seed):
+    r = random.Random(seed)
+    B, Sq, H = r.randint(1, 5), r.randint(1, 280), r.choice([1, 2, 3, 7])
+    lens = [r.randint(0, 900) for _ in range(B)]
+    new = [r.randint(0, Sq) for _ in range(B)]
+    page = r.choice([64, 128, 256])
+    t = make(seed, B, Sq, lens, H, r.choice([BF, H16]), page=page)
+    causal = r.random() < 0.7
+    check_all(t, run_paged(ext, t, causal, new), lens, causal, new)
