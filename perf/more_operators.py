@@ -498,7 +498,7 @@ def run(s):
             s["new_lens"], out["seq_lens"], out["block_table"], s["free_pages"], out["free_state"],
             c["Sq"], PAGE)
         table = out["block_table"]
-        mla.kv_append_paged(s["x"], s["W_kv_a"], s["kv_norm_w"], pos, s["c_kv"], s["pe"], table, EPS)
+        mla.kv_append_paged(s["x"], s["W_kv_a"], s["kv_norm_w"], pos, table, s["c_kv"], s["pe"], EPS)
         q_nope, q_rope = mla.q_heads(s["x"], s["W_q_a"], s["q_norm_w"], s["W_q_b"], pos, NOPE, D, EPS)
         attn = mla.mla_attention_paged_expanded(q_nope, q_rope, s["c_kv"], s["pe"], table, lens,
                                                 s["W_uk"], s["W_uv"], SCALE, causal=True, new_lens=new)
