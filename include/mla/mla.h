@@ -457,6 +457,64 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
                                void* out, void* workspace, size_t workspace_bytes,
                                hipStream_t stream);
 
+/* ---- Pages that requests share (none in the reference; any cache format).  Every row of block_table
+ * that names a page among its request's ceil(seq_lens[b] / page_size) first entries holds it; nothing
+ * else is kept about pages.  Between calls of mla_cache_fork the last, partly filled page of a request is
+ * its own and only whole pages are shared, so that mla_cache_extend may let requests grow (new_lens
+ * > 0) and appends may write; while rows share pages, tokens are dropped and requests ended by
+ * mla_cache_fork (mla_cache_extend would give a shared page back).  Tables, ring, sizes and limits as
+ * in mla_cache_extend; batch is at most 2^24.
+ *
+ * Fork: request b becomes the first n = min(max(keep_lens[b], 0), L) tokens of request parents[b] as
+ * it was before the call, of L tokens (clamped as there; n = 0 if parents[b] is outside [0, batch)).
+ * parents[b] = b keeps, cuts back or ends (keep_lens 0) request b itself.
+ *   - The whole pages of those tokens, n / page_size of them, are shared.
+ *   - A page that is partly filled then ("open") stays with the lowest request that has it open, unless
+ *     some request holds it whole; the others get a copy: they take a free page, in request order,
+ *     and copies [batch, 2] says {old page, free page} ({-1, -1} for requests without).  Where the free
+ *     pages run out a request is cut back to its whole pages.
+ *   - Pages that no request holds any more go behind the ring's tail, in the order of their numbers,
+ *     for later calls.
+ *   block_table_out [batch, max_pages], seq_lens_out [batch], free_state_out [2]   the state after the
+ *                call; entries that hold nothing are 0.  Other memory than the inputs.
+ *   free_pages   in place
+ * A table entry outside [0, num_pages) stays as it is and counts for no page.  The pages' contents are
+ * copied by mla_cache_copy_pages(copies, batch, ..), before the next call that writes the cache. */
+size_t mla_cache_fork_workspace_bytes(int32_t batch, int32_t num_pages);   /* 0 for a small pool */
+int mla_cache_fork(int32_t batch, int32_t page_size, int32_t max_pages, int32_t num_pages,
+                   const int32_t* parents, const int32_t* keep_lens, const int32_t* seq_lens,
+                   const int32_t* block_table, const int32_t* free_state, int32_t* free_pages,
+                   int32_t* seq_lens_out, int32_t* block_table_out, int32_t* free_state_out,
+                   int32_t* copies, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Compact: with U pages held, the lowest U of the held and the free pages are the held ones after the
+ * call.  The i-th held page past them moves to the i-th free one among them: copies
+ * [max(1, num_pages / 2), 2] lists {from, to} of all moves, then {-1, -1}; no page is in two of them.
+ *   block_table_out [batch, max_pages]   the table through the moves (0 where it holds nothing)
+ *   free_pages_out  [num_pages], free_state_out {0, count}   the other pages in order, then -1
+ * Outputs are other memory than the inputs.  Pages that are neither held nor in the ring stay out of it;
+ * a page that is both counts as held. */
+size_t mla_cache_compact_workspace_bytes(int32_t num_pages);   /* 0 for a small pool */
+int mla_cache_compact(int32_t batch, int32_t page_size, int32_t max_pages, int32_t num_pages,
+                      const int32_t* seq_lens, const int32_t* block_table,
+                      const int32_t* free_pages, const int32_t* free_state,
+                      int32_t* block_table_out, int32_t* free_pages_out, int32_t* free_state_out,
+                      int32_t* copies, void* workspace, size_t workspace_bytes,
+                      hipStream_t stream);
+
+/* Copy pages within pools: for each of n pairs {from, to} (int32 [n, 2], device memory) page `to` becomes
+ * page `from`, in every layer of up to 8 pools (an array in host memory, read by the call).  Pairs
+ * with a page outside [0, num_pages) are skipped.  A page that is a destination is in no other pair. */
+typedef struct mla_page_pool {
+    void* data;            /* page i of layer j at data + j * layer_bytes + i * page_bytes */
+    int64_t page_bytes;
+    int64_t layer_bytes;   /* at least num_pages * page_bytes where layers > 1 */
+    int32_t layers;
+} mla_page_pool_t;
+#define MLA_MAX_PAGE_POOLS 8
+int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
+                         const mla_page_pool_t* pools, int32_t n_pools, hipStream_t stream);
+
 /* ---- The expanded form (none in the reference), for chunks of many new tokens: keys and values per
  * head from the latent rows,
  *   k[j, h] = W_uk[h] c_kv[j],  v[j, h] = W_uv[h] c_kv[j],

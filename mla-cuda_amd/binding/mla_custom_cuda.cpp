@@ -26,6 +26,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -801,6 +802,127 @@ std::vector<torch::Tensor> op_cache_extend(torch::Tensor new_lens, torch::Tensor
     return {lens_out, state_out, granted, positions, slots};
 }
 
+void check_page_tables(const torch::Tensor& seq_lens, const torch::Tensor& block_table,
+                       const torch::Tensor& free_pages, const torch::Tensor& free_state,
+                       int64_t page_size) {
+    check_dim(block_table, 2, "block_table", "[B, max_pages]");
+    TORCH_CHECK(block_table.scalar_type() == torch::kInt32, "block_table must be int32");
+    const int64_t B = block_table.size(0), max_pages = block_table.size(1);
+    TORCH_CHECK(B > 0 && max_pages > 0, "block_table must be [B, max_pages] (got ",
+                block_table.sizes(), ")");
+    check_int32(seq_lens, B, "seq_lens");
+    check_int32(free_state, 2, "free_state");
+    TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) > 0 &&
+                    free_pages.scalar_type() == torch::kInt32,
+                "free_pages must be a 1-D int32 tensor with a place for each page of the pool (got ",
+                free_pages.sizes(), ")");
+    TORCH_CHECK(page_size > 0 && page_size < INT32_MAX && B < INT32_MAX && max_pages < INT32_MAX &&
+                    free_pages.size(0) < INT32_MAX,
+                "MLA: page_size must be positive, and the sizes below 2^31");
+}
+
+// Requests become prefixes of requests, whole pages shared; free_pages in place, the rest comes back:
+// [seq_lens, block_table, free_state, copies [B, 2]].
+std::vector<torch::Tensor> op_cache_fork(torch::Tensor parents, torch::Tensor keep_lens,
+                                         torch::Tensor seq_lens, torch::Tensor block_table,
+                                         torch::Tensor free_pages, torch::Tensor free_state,
+                                         int64_t page_size) {
+    check_page_tables(seq_lens, block_table, free_pages, free_state, page_size);
+    const int64_t B = block_table.size(0);
+    check_int32(parents, B, "parents");
+    check_int32(keep_lens, B, "keep_lens");
+    TORCH_CHECK(free_pages.is_contiguous(), "MLA: free_pages is updated in place and must be contiguous");
+    check_device({&parents, &keep_lens, &seq_lens, &block_table, &free_pages, &free_state});
+
+    c10::DeviceGuard guard(block_table.device());
+    auto from = parents.contiguous();
+    auto keep = keep_lens.contiguous();
+    auto lens = seq_lens.contiguous();
+    auto tab = block_table.contiguous();
+    auto state = free_state.contiguous();
+    auto lens_out = torch::empty({B}, lens.options());
+    auto tab_out = torch::empty({B, block_table.size(1)}, lens.options());
+    auto state_out = torch::empty({2}, lens.options());
+    auto copies = torch::empty({B, 2}, lens.options());
+    const int32_t P = (int32_t)free_pages.size(0);
+    const size_t wsb = mla_cache_fork_workspace_bytes((int32_t)B, P);
+    torch::Tensor ws;
+    if (wsb > 0) ws = workspace(wsb, lens);
+    check_status(mla_cache_fork((int32_t)B, (int32_t)page_size, (int32_t)block_table.size(1), P,
+                                from.data_ptr<int32_t>(), keep.data_ptr<int32_t>(),
+                                lens.data_ptr<int32_t>(), tab.data_ptr<int32_t>(),
+                                state.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(),
+                                lens_out.data_ptr<int32_t>(), tab_out.data_ptr<int32_t>(),
+                                state_out.data_ptr<int32_t>(), copies.data_ptr<int32_t>(),
+                                wsb > 0 ? ws.data_ptr() : nullptr, wsb, current_stream()),
+                 "cache_fork");
+    return {lens_out, tab_out, state_out, copies};
+}
+
+// Held pages to the low end of the pool: [block_table, free_pages, free_state, copies].
+std::vector<torch::Tensor> op_cache_compact(torch::Tensor seq_lens, torch::Tensor block_table,
+                                            torch::Tensor free_pages, torch::Tensor free_state,
+                                            int64_t page_size) {
+    check_page_tables(seq_lens, block_table, free_pages, free_state, page_size);
+    check_device({&seq_lens, &block_table, &free_pages, &free_state});
+
+    c10::DeviceGuard guard(block_table.device());
+    const int64_t B = block_table.size(0), P = free_pages.size(0);
+    auto lens = seq_lens.contiguous();
+    auto tab = block_table.contiguous();
+    auto ring = free_pages.contiguous();
+    auto state = free_state.contiguous();
+    auto tab_out = torch::empty({B, block_table.size(1)}, lens.options());
+    auto ring_out = torch::empty({P}, lens.options());
+    auto state_out = torch::empty({2}, lens.options());
+    auto copies = torch::empty({std::max<int64_t>(1, P / 2), 2}, lens.options());
+    const size_t wsb = mla_cache_compact_workspace_bytes((int32_t)P);
+    torch::Tensor ws;
+    if (wsb > 0) ws = workspace(wsb, lens);
+    check_status(mla_cache_compact((int32_t)B, (int32_t)page_size, (int32_t)block_table.size(1),
+                                   (int32_t)P, lens.data_ptr<int32_t>(), tab.data_ptr<int32_t>(),
+                                   ring.data_ptr<int32_t>(), state.data_ptr<int32_t>(),
+                                   tab_out.data_ptr<int32_t>(), ring_out.data_ptr<int32_t>(),
+                                   state_out.data_ptr<int32_t>(), copies.data_ptr<int32_t>(),
+                                   wsb > 0 ? ws.data_ptr() : nullptr, wsb, current_stream()),
+                 "cache_compact");
+    return {tab_out, ring_out, state_out, copies};
+}
+
+// Pages copied within pools [num_pages, ..], or with `layered` [layers, num_pages, ..], in place.
+void op_cache_copy_pages(torch::Tensor copies, std::vector<torch::Tensor> pools, bool layered) {
+    check_dim(copies, 2, "copies", "[n, 2]");
+    TORCH_CHECK(copies.size(1) == 2 && copies.scalar_type() == torch::kInt32,
+                "copies must be an int32 [n, 2] tensor (got ", copies.sizes(), ")");
+    TORCH_CHECK(!pools.empty() && pools.size() <= MLA_MAX_PAGE_POOLS, "MLA: from 1 to ",
+                MLA_MAX_PAGE_POOLS, " pools at a time (got ", pools.size(), ")");
+    const int at = layered ? 1 : 0;
+    std::vector<const torch::Tensor*> all = {&copies};
+    std::vector<mla_page_pool_t> desc;
+    for (const auto& t : pools) {
+        TORCH_CHECK(t.dim() > at && t.size(at) == pools[0].size(at) && t.size(at) < INT32_MAX &&
+                        t.numel() > 0,
+                    "pools must be ", layered ? "[layers, num_pages, ..]" : "[num_pages, ..]",
+                    " of one num_pages (got ", t.sizes(), ")");
+        const auto layer = layered ? t.select(0, 0) : t;
+        TORCH_CHECK(layer.is_contiguous(), "MLA: pools are updated in place and their layers must be contiguous");
+        mla_page_pool_t p{};
+        p.data = t.data_ptr();
+        p.page_bytes = layer.numel() / layer.size(0) * t.element_size();
+        p.layers = layered ? (int32_t)std::min<int64_t>(t.size(0), INT32_MAX) : 1;
+        p.layer_bytes = layered ? t.stride(0) * t.element_size() : 0;
+        desc.push_back(p);
+        all.push_back(&t);
+    }
+    check_device(all);
+    c10::DeviceGuard guard(copies.device());
+    auto pairs = copies.contiguous();
+    check_status(mla_cache_copy_pages(pairs.data_ptr<int32_t>(), pairs.size(0),
+                                      (int32_t)pools[0].size(at), desc.data(), (int32_t)desc.size(),
+                                      current_stream()),
+                 "cache_copy_pages");
+}
+
 // KV-cache append into the blocked 8-bit cache, in place: the last new_lens[b] rows of x[b] become
 // the last tokens of sequence b, which has seq_lens[b] with them.
 void op_kv_append_paged_fp8blk(torch::Tensor x, torch::Tensor W_kv_a, torch::Tensor kv_norm_w,
@@ -1335,6 +1457,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("q_absorbed"), py::arg("q_rope"), py::arg("c_kv_pages"), py::arg("pe_pages"),
           py::arg("scales"), py::arg("block_table"), py::arg("seq_lens"), py::arg("W_uv"),
           py::arg("scale"), py::arg("causal") = false);
+    m.def("cache_fork", &op_cache_fork,
+          "Requests become the first keep_lens[b] tokens of requests parents[b]: whole pages shared, "
+          "partly filled ones copied where two would write them, pages that nobody holds freed; "
+          "free_pages in place, returns [seq_lens, block_table, free_state, copies [B, 2]]",
+          py::arg("parents"), py::arg("keep_lens"), py::arg("seq_lens"), py::arg("block_table"),
+          py::arg("free_pages"), py::arg("free_state"), py::arg("page_size"));
+    m.def("cache_compact", &op_cache_compact,
+          "Held pages to the low end of the pool: returns [block_table, free_pages, free_state, "
+          "copies [num_pages / 2, 2]]",
+          py::arg("seq_lens"), py::arg("block_table"), py::arg("free_pages"), py::arg("free_state"),
+          py::arg("page_size"));
+    m.def("cache_copy_pages", &op_cache_copy_pages,
+          "Pages copied within pools [num_pages, ..] (layered: [layers, num_pages, ..]) in place: "
+          "for each pair of copies (int32 [n, 2]; skipped where one is no page) page copies[i, 1] "
+          "becomes page copies[i, 0]",
+          py::arg("copies"), py::arg("pools"), py::arg("layered") = false);
     m.def("q_heads", &op_q_heads,
           "Queries per head for the expanded form (bf16 or fp16): returns [q_nope [B, Sq, H, nope], "
           "q_rope [B, Sq, H, rope]]",

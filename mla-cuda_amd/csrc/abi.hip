@@ -835,6 +835,35 @@ int check_fp8blk_attn(mla_dtype_t dtype, const mla_dims_t* d, int causal, int32_
     return MLA_OK;
 }
 
+// Tables of requests that share pages: mla_cache_extend's limits, and a batch that a word per page can name.
+int check_page_tables(int32_t batch, int32_t page_size, int32_t max_pages, int32_t num_pages) {
+    MLA_CHECK(check_pos(batch, "batch"));
+    MLA_CHECK(check_pos(max_pages, "max_pages"));
+    MLA_CHECK(check_pos(num_pages, "num_pages"));
+    if (page_size <= 0 || page_size % 64 != 0)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "page_size must be a positive multiple of 64 (got %d)",
+                    page_size);
+    if (batch > (1 << 24) || num_pages > (1 << 30))
+        return fail(MLA_ERR_INVALID_ARGUMENT, "batch must be at most 2^24 and num_pages at most 2^30");
+    if ((int64_t)max_pages * page_size > kMaxI32 || (int64_t)batch * max_pages > kMaxI32)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "max_pages * page_size and batch * max_pages must be "
+                    "below 2^31");
+    return MLA_OK;
+}
+// int32 arrays: no output overlaps an input or another output.
+struct Span { const int32_t* p; int64_t n; };
+int check_apart(const Span* in, int n_in, const Span* out, int n_out) {
+    auto meet = [](const Span& a, const Span& b) { return a.p < b.p + b.n && b.p < a.p + a.n; };
+    for (int o = 0; o < n_out; ++o) {
+        for (int i = 0; i < n_in; ++i)
+            if (meet(out[o], in[i]))
+                return fail(MLA_ERR_INVALID_ARGUMENT, "outputs must not overlap the inputs");
+        for (int i = 0; i < o; ++i)
+            if (meet(out[o], out[i])) return fail(MLA_ERR_INVALID_ARGUMENT, "outputs must not overlap");
+    }
+    return MLA_OK;
+}
+
 // The expanded form: 16 bits and the DeepSeek-V3 widths; counts that its kernels form in 32 bits.
 int check_expanded(mla_dtype_t dtype, const mla_dims_t* d, int causal) {
     MLA_CHECK(check_dtype(dtype));
@@ -1628,6 +1657,112 @@ int mla_cache_extend(int32_t batch, int32_t sq, int32_t page_size, int32_t max_p
     p.seq_lens_out = seq_lens_out; p.free_state_out = free_state_out; p.granted = granted;
     p.positions = positions; p.slots = slots;
     MLA_TRY_HIP(launch_cache_extend(p, workspace, stream), "cache extend launch");
+    return ok();
+}
+
+size_t mla_cache_fork_workspace_bytes(int32_t batch, int32_t num_pages) {
+    return batch > 0 && num_pages > 0 ? align_up(cache_fork_workspace(batch, num_pages)) : 0;
+}
+
+int mla_cache_fork(int32_t batch, int32_t page_size, int32_t max_pages, int32_t num_pages,
+                   const int32_t* parents, const int32_t* keep_lens, const int32_t* seq_lens,
+                   const int32_t* block_table, const int32_t* free_state, int32_t* free_pages,
+                   int32_t* seq_lens_out, int32_t* block_table_out, int32_t* free_state_out,
+                   int32_t* copies, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    MLA_CHECK(check_page_tables(batch, page_size, max_pages, num_pages));
+    MLA_CHECK(check_ptr(parents, "parents"));
+    MLA_CHECK(check_ptr(keep_lens, "keep_lens"));
+    MLA_CHECK(check_ptr(seq_lens, "seq_lens"));
+    MLA_CHECK(check_ptr(block_table, "block_table"));
+    MLA_CHECK(check_ptr(free_state, "free_state"));
+    MLA_CHECK(check_ptr(free_pages, "free_pages"));
+    MLA_CHECK(check_ptr(seq_lens_out, "seq_lens_out"));
+    MLA_CHECK(check_ptr(block_table_out, "block_table_out"));
+    MLA_CHECK(check_ptr(free_state_out, "free_state_out"));
+    MLA_CHECK(check_ptr(copies, "copies"));
+    const int64_t table = (int64_t)batch * max_pages;
+    const Span in[] = {{parents, batch}, {keep_lens, batch}, {seq_lens, batch}, {block_table, table},
+                       {free_state, 2}, {free_pages, num_pages}};
+    const Span out[] = {{seq_lens_out, batch}, {block_table_out, table}, {free_state_out, 2},
+                        {copies, 2 * (int64_t)batch}};
+    MLA_CHECK(check_apart(in, 6, out, 4));
+    MLA_CHECK(check_ws(workspace, workspace_bytes, mla_cache_fork_workspace_bytes(batch, num_pages)));
+    CacheFork p;
+    p.B = batch; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
+    p.parents = parents; p.keep_lens = keep_lens; p.seq_lens = seq_lens; p.block_table = block_table;
+    p.free_state = free_state; p.free_pages = free_pages;
+    p.seq_lens_out = seq_lens_out; p.block_table_out = block_table_out;
+    p.free_state_out = free_state_out; p.copies = copies;
+    MLA_TRY_HIP(launch_cache_fork(p, workspace, stream), "cache fork launch");
+    return ok();
+}
+
+size_t mla_cache_compact_workspace_bytes(int32_t num_pages) {
+    return num_pages > 0 ? align_up(cache_compact_workspace(num_pages)) : 0;
+}
+
+int mla_cache_compact(int32_t batch, int32_t page_size, int32_t max_pages, int32_t num_pages,
+                      const int32_t* seq_lens, const int32_t* block_table,
+                      const int32_t* free_pages, const int32_t* free_state,
+                      int32_t* block_table_out, int32_t* free_pages_out, int32_t* free_state_out,
+                      int32_t* copies, void* workspace, size_t workspace_bytes,
+                      hipStream_t stream) {
+    MLA_CHECK(check_page_tables(batch, page_size, max_pages, num_pages));
+    MLA_CHECK(check_ptr(seq_lens, "seq_lens"));
+    MLA_CHECK(check_ptr(block_table, "block_table"));
+    MLA_CHECK(check_ptr(free_pages, "free_pages"));
+    MLA_CHECK(check_ptr(free_state, "free_state"));
+    MLA_CHECK(check_ptr(block_table_out, "block_table_out"));
+    MLA_CHECK(check_ptr(free_pages_out, "free_pages_out"));
+    MLA_CHECK(check_ptr(free_state_out, "free_state_out"));
+    MLA_CHECK(check_ptr(copies, "copies"));
+    const int64_t table = (int64_t)batch * max_pages;
+    const Span in[] = {{seq_lens, batch}, {block_table, table}, {free_pages, num_pages}, {free_state, 2}};
+    const Span out[] = {{block_table_out, table}, {free_pages_out, num_pages}, {free_state_out, 2},
+                        {copies, 2 * (int64_t)std::max(1, num_pages / 2)}};
+    MLA_CHECK(check_apart(in, 4, out, 4));
+    MLA_CHECK(check_ws(workspace, workspace_bytes, mla_cache_compact_workspace_bytes(num_pages)));
+    CacheCompact p;
+    p.B = batch; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
+    p.seq_lens = seq_lens; p.block_table = block_table; p.free_pages = free_pages;
+    p.free_state = free_state; p.block_table_out = block_table_out;
+    p.free_pages_out = free_pages_out; p.free_state_out = free_state_out; p.copies = copies;
+    MLA_TRY_HIP(launch_cache_compact(p, workspace, stream), "cache compact launch");
+    return ok();
+}
+
+int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
+                         const mla_page_pool_t* pools, int32_t n_pools, hipStream_t stream) {
+    static_assert(kMaxPools == MLA_MAX_PAGE_POOLS, "as mla.h says");
+    if (n < 0 || n > kMaxI32)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "n must be in [0, 2^31) (got %lld)", (long long)n);
+    MLA_CHECK(check_pos(num_pages, "num_pages"));
+    if (!pools) return fail(MLA_ERR_INVALID_ARGUMENT, "pools must not be NULL");
+    if (n_pools < 1 || n_pools > kMaxPools)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "n_pools must be in [1, %d] (got %d)", kMaxPools, n_pools);
+    CopyPages p;
+    int64_t parts = 0;
+    constexpr int64_t kMost = (int64_t)1 << 46;   // bytes of a layer, and of a pool
+    for (int i = 0; i < n_pools; ++i) {
+        const mla_page_pool_t& q = pools[i];
+        if (!q.data) return fail(MLA_ERR_INVALID_ARGUMENT, "pool %d: data must not be NULL", i);
+        if (q.layers < 1) return fail(MLA_ERR_INVALID_ARGUMENT, "pool %d: layers must be positive (got %d)", i, q.layers);
+        if (q.page_bytes < 1 || q.page_bytes > kMost / num_pages)
+            return fail(MLA_ERR_INVALID_ARGUMENT, "pool %d: page_bytes must be positive, and a layer below 2^46 "
+                        "bytes (got %lld)", i, (long long)q.page_bytes);
+        if (q.layers > 1 && (q.layer_bytes < q.page_bytes * num_pages || q.layer_bytes > kMost / q.layers))
+            return fail(MLA_ERR_INVALID_ARGUMENT, "pool %d: layer_bytes must hold num_pages pages, and the pool "
+                        "lie below 2^46 bytes (got %lld)", i, (long long)q.layer_bytes);
+        parts += q.layers;
+        p.pool[i].data = q.data; p.pool[i].page_bytes = q.page_bytes; p.pool[i].layers = q.layers;
+        p.pool[i].layer_bytes = q.layers > 1 ? q.layer_bytes : 0;
+    }
+    if (parts > 65535)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "at most 65535 layers of all pools (got %lld)", (long long)parts);
+    if (n == 0) return ok();
+    MLA_CHECK(check_ptr(copies, "copies"));
+    p.copies = copies; p.n = n; p.num_pages = num_pages; p.pools = n_pools;
+    MLA_TRY_HIP(launch_copy_pages(p, stream), "page copy launch");
     return ok();
 }
 

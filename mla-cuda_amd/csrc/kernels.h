@@ -344,6 +344,45 @@ int flash_worklist_ints(const FlashProblem& p, const FlashPlan& plan);
 hipError_t launch_flash_worklist(const FlashProblem& p, const FlashPlan& plan, int* wl,
                                  hipStream_t stream);
 
+// ---------------------------------------------------------------- shared pages (pages.hip)
+constexpr int kPageRange = 16384;    // pages of a pool that one workgroup keeps in LDS
+struct CacheFork {
+    int B = 0, page_size = 0, max_pages = 0, num_pages = 0;
+    const int* parents = nullptr;      // [B]
+    const int* keep_lens = nullptr;    // [B]
+    const int* seq_lens = nullptr;     // [B]
+    const int* block_table = nullptr;  // [B, max_pages]
+    const int* free_state = nullptr;   // {head, count}
+    int* free_pages = nullptr;         // [num_pages] ring
+    int* seq_lens_out = nullptr;
+    int* block_table_out = nullptr;
+    int* free_state_out = nullptr;
+    int* copies = nullptr;             // [B, 2]
+};
+size_t cache_fork_workspace(int B, int num_pages);      // 0 where one launch does it all
+hipError_t launch_cache_fork(const CacheFork& p, void* workspace, hipStream_t stream);
+struct CacheCompact {
+    int B = 0, page_size = 0, max_pages = 0, num_pages = 0;
+    const int* seq_lens = nullptr;
+    const int* block_table = nullptr;
+    const int* free_pages = nullptr;
+    const int* free_state = nullptr;
+    int* block_table_out = nullptr;
+    int* free_pages_out = nullptr;
+    int* free_state_out = nullptr;
+    int* copies = nullptr;             // [max(1, num_pages / 2), 2]
+};
+size_t cache_compact_workspace(int num_pages);
+hipError_t launch_cache_compact(const CacheCompact& p, void* workspace, hipStream_t stream);
+constexpr int kMaxPools = 8;
+struct CopyPages {
+    const int* copies = nullptr;       // [n, 2]
+    int64_t n = 0;
+    int num_pages = 0, pools = 0;
+    struct { void* data; int64_t page_bytes, layer_bytes; int layers; } pool[kMaxPools];
+};
+hipError_t launch_copy_pages(const CopyPages& p, hipStream_t stream);
+
 // ---------------------------------------------------------------- expanded form (expand.hip)
 // out[b, i, h] = softmax((q_nope . W_uk[h] c + q_rope . pe) / scale) W_uv[h] c over the keys that
 // query i sees; 16 bits, kv_rank 512, rope 64, nope and v 128.

@@ -1,0 +1,637 @@
+// Pages of a cache that requests share: forking requests (their tables, and which pages need a copy),
+// making a pool dense again, and the copies themselves.  Tables and the ring of free pages are those
+// of cache8.hip's extend; a page is held by every table row that names it among its request's pages,
+// so that who holds what follows from the tables alone and nothing is counted between calls.
+//
+// What follows from all holders of a page is made by the workgroup that owns the page's range of the
+// pool: it reads the whole table and keeps a word a page in LDS, so that no memory has to be cleared
+// and no order of atomics shows in a result.  Past one range (a large pool) the next step is a launch
+// of its own; a small pool is done in one.
+
+#include <algorithm>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace mla {
+
+namespace {
+
+typedef uint32_t v4u_t __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kRange = kPageRange;            // pages a workgroup owns
+constexpr int kPer = kRange / kThreads;       // consecutive ones a thread
+
+// Sum over the threads in front of this one; *total that over all.
+__device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+    s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xF, 0xF, true);    // row_shr:1, 2, 4, 8
+    s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xF, 0xF, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xF, 0xF, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x118, 0xF, 0xF, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x142, 0xA, 0xF, false);   // row_bcast:15, 31
+    s += __builtin_amdgcn_update_dpp(0, s, 0x143, 0xC, 0xF, false);
+    __syncthreads();                          // the last use of `waves` is over
+    if (lane == 63) waves[wave] = s;
+    __syncthreads();
+    int before = s - v, all = 0;
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before += waves[w];
+        all += waves[w];
+    }
+    *total = all;
+    return before;
+}
+
+__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((int64_t)tokens + page - 1) / page); }
+__device__ __forceinline__ int ring_at(int head, int64_t i, int n) { return (int)((head + i) % n); }
+
+// ---- fork -----------------------------------------------------------------------------------
+// Request b continues the first n = min(keep_lens[b], L[p]) tokens of request p = parents[b].  A
+// page's word says how it is held: not (0), before the call only (1), as the open page of request b
+// and of none in front (kOpen - b), as a whole page (kWhole).  A larger word wins, so that the word
+// does not depend on the order of its holders.  An open page stays with the request that its word
+// names; the others that would write it, all of them if it is somebody's whole page, take a copy.
+constexpr uint32_t kHeld = 1u, kOpen = 0x7fffffffu, kWhole = 0xffffffffu;
+constexpr int kNoCopy = -0x7fffffff - 1;      // no free page (whatever a ring may hold)
+
+struct ForkArgs {
+    const int* parents;
+    const int* keep;
+    const int* lens;
+    const int* table;
+    const int* state;        // {head, count}
+    int* ring;
+    int* lens_out;
+    int* table_out;
+    int* state_out;
+    int* copies;             // [B][2]
+    uint32_t* words;         // [num_pages] (past one range)
+    int* freed;              // [ranges]
+    int B, page, max_pages, num_pages, ranges;
+};
+
+struct ForkRow { int src, n; };
+__device__ __forceinline__ int fork_len(const ForkArgs& a, int b) {
+    return (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
+}
+__device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int b) {
+    const int p = a.parents[b];
+    if (p < 0 || p >= a.B) return {0, 0};
+    return {p, min(max(a.keep[b], 0), fork_len(a, p))};
+}
+
+// The words of pages [lo, lo + kRange), and how many of them nobody holds any more.
+__device__ __forceinline__ int fork_words(const ForkArgs& a, int lo, uint32_t* words, int* waves) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int pages = min(kRange, a.num_pages - lo);
+    for (int i = tid; i < kRange; i += kThreads) words[i] = 0;
+    __syncthreads();
+    auto mark = [&](int page, uint32_t w) __attribute__((always_inline)) {
+        const uint32_t i = (uint32_t)(page - lo);
+        if (page >= lo && i < (uint32_t)pages) atomicMax(&words[i], w);
+    };
+    for (int b = wave; b < a.B; b += kWaves) {
+        const ForkRow r = fork_row(a, b);
+        const int have = pages_of(fork_len(a, b), a.page);
+        const int whole = r.n / a.page, open = r.n % a.page != 0;
+        const int* own = a.table + (int64_t)b * a.max_pages;
+        const int* from = a.table + (int64_t)r.src * a.max_pages;
+        for (int j = lane; j < max(have, whole + open); j += 64) {
+            if (j < have) mark(own[j], kHeld);
+            if (j < whole + open) mark(from[j], j < whole ? kWhole : kOpen - (uint32_t)b);
+        }
+    }
+    __syncthreads();
+    int n = 0, total;
+    for (int i = 0; i < kPer; ++i) n += words[tid * kPer + i] == kHeld;
+    block_scan(n, waves, &total);
+    return total;
+}
+
+// The plan of all requests: each one's copy, if it needs one and a free page is left for it.
+// put(b, row, old page, fresh page or kNoCopy, whether it is cut back to its whole pages)
+template <class Word, class Put>
+__device__ __forceinline__ int fork_plan(const ForkArgs& a, int head, int count, int* waves, Word word, Put put) {
+    const int per = (a.B + kThreads - 1) / kThreads;
+    const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+    auto needs = [&](int b, ForkRow r, int* old) __attribute__((always_inline)) {
+        if (r.n % a.page == 0) return false;
+        *old = a.table[(int64_t)r.src * a.max_pages + r.n / a.page];
+        return *old >= 0 && *old < a.num_pages && word(*old) != kOpen - (uint32_t)b;
+    };
+    int n = 0, old = -1, total;
+    for (int b = b0; b < b1; ++b) n += needs(b, fork_row(a, b), &old);
+    int order = block_scan(n, waves, &total);
+    for (int b = b0; b < b1; ++b) {
+        const ForkRow r = fork_row(a, b);
+        const bool need = needs(b, r, &old), given = need && order < count;
+        put(b, r, old, given ? a.ring[ring_at(head, order, a.num_pages)] : kNoCopy, need && !given);
+        order += need;
+    }
+    return min(total, count);
+}
+
+// This request's new table row, by a wave.
+__device__ __forceinline__ void fork_write(const ForkArgs& a, int b, int src, int n, int fresh) {
+    const int whole = n / a.page, held = pages_of(n, a.page);
+    const int* from = a.table + (int64_t)src * a.max_pages;
+    int* to = a.table_out + (int64_t)b * a.max_pages;
+    for (int j = threadIdx.x & 63; j < a.max_pages; j += 64)
+        to[j] = j >= held ? 0 : j < whole || fresh == kNoCopy ? from[j] : fresh;
+}
+
+// The pages of a range that nobody holds any more, behind the ring's tail: `before` of them come first.
+__device__ __forceinline__ void fork_free(const ForkArgs& a, int lo, const uint32_t* words, int before,
+                                          int head, int count, int* waves) {
+    const int at = threadIdx.x * kPer;
+    int n = 0, total;
+    for (int i = 0; i < kPer; ++i) n += words[at + i] == kHeld;
+    int k = before + block_scan(n, waves, &total);
+    for (int i = 0; i < kPer; ++i)
+        if (words[at + i] == kHeld) {
+            if (k < a.num_pages - count) a.ring[ring_at(head, (int64_t)count + k, a.num_pages)] = lo + at + i;
+            ++k;
+        }
+}
+
+__device__ __forceinline__ void ring_state(const int* state, int n, int* head, int* count) {
+    *head = state[0] % n;
+    if (*head < 0) *head += n;
+    *count = min(max(state[1], 0), n);
+}
+
+struct ForkInfo { int src, n, fresh; };
+
+// ONE: one range and at most kThreads requests, all of it here.  Else the words and how many pages each
+// range frees.
+template <bool ONE>
+__global__ void __launch_bounds__(kThreads) fork_words_kernel(ForkArgs a) {
+    __shared__ uint32_t words[kRange];
+    __shared__ int waves[kWaves];
+    __shared__ ForkInfo info[ONE ? kThreads : 1];
+    const int tid = threadIdx.x, lo = blockIdx.x * kRange;
+    const int freed = fork_words(a, lo, words, waves);
+    if (!ONE) {
+        if (tid == 0) a.freed[blockIdx.x] = freed;
+        for (int i = tid; i < min(kRange, a.num_pages - lo); i += kThreads) a.words[lo + i] = words[i];
+        return;
+    }
+    int head, count;
+    ring_state(a.state, a.num_pages, &head, &count);
+    const int taken = fork_plan(a, head, count, waves, [&](int page) { return words[page]; },
+                                [&](int b, ForkRow r, int old, int fresh, bool cut) __attribute__((always_inline)) {
+        const int n = cut ? r.n / a.page * a.page : r.n;
+        info[b] = {r.src, n, fresh};
+        a.lens_out[b] = n;
+        a.copies[2 * b] = fresh == kNoCopy ? -1 : old;
+        a.copies[2 * b + 1] = fresh == kNoCopy ? -1 : fresh;
+    });
+    if (tid == 0) {
+        a.state_out[0] = ring_at(head, taken, a.num_pages);
+        a.state_out[1] = min(count - taken + freed, a.num_pages);
+    }
+    fork_free(a, lo, words, 0, head, count, waves);
+    __syncthreads();
+    for (int b = tid >> 6; b < a.B; b += kWaves) fork_write(a, b, info[b].src, info[b].n, info[b].fresh);
+}
+
+// Workgroups [0, ranges) free pages, the others write kWaves rows each.
+__global__ void __launch_bounds__(kThreads) fork_emit_kernel(ForkArgs a) {
+    __shared__ uint32_t words[kRange];
+    __shared__ int waves[kWaves];
+    __shared__ ForkInfo info[kWaves];
+    const int tid = threadIdx.x;
+    int head, count;
+    ring_state(a.state, a.num_pages, &head, &count);
+    if ((int)blockIdx.x < a.ranges) {
+        const int lo = blockIdx.x * kRange;
+        for (int i = tid; i < kRange; i += kThreads) words[i] = lo + i < a.num_pages ? a.words[lo + i] : 0;
+        int n = 0, before;
+        for (int r = tid; r < (int)blockIdx.x; r += kThreads) n += a.freed[r];
+        block_scan(n, waves, &before);
+        fork_free(a, lo, words, before, head, count, waves);
+        return;
+    }
+    const int r0 = (blockIdx.x - a.ranges) * kWaves;
+    const int taken = fork_plan(a, head, count, waves, [&](int page) { return a.words[page]; },
+                                [&](int b, ForkRow r, int old, int fresh, bool cut) __attribute__((always_inline)) {
+        if (b < r0 || b >= r0 + kWaves) return;
+        const int n = cut ? r.n / a.page * a.page : r.n;
+        info[b - r0] = {r.src, n, fresh};
+        a.lens_out[b] = n;
+        a.copies[2 * b] = fresh == kNoCopy ? -1 : old;
+        a.copies[2 * b + 1] = fresh == kNoCopy ? -1 : fresh;
+    });
+    if (r0 == 0) {
+        int n = 0, freed;
+        for (int r = tid; r < a.ranges; r += kThreads) n += a.freed[r];
+        block_scan(n, waves, &freed);
+        if (tid == 0) {
+            a.state_out[0] = ring_at(head, taken, a.num_pages);
+            a.state_out[1] = (int)min((int64_t)count - taken + freed, (int64_t)a.num_pages);
+        }
+    }
+    __syncthreads();
+    const int b = r0 + (tid >> 6);
+    if (b < a.B) fork_write(a, b, info[tid >> 6].src, info[tid >> 6].n, info[tid >> 6].fresh);
+}
+
+// ---- compact --------------------------------------------------------------------------------
+// The pages that tables hold (U of them) and the free ones of the ring, in the order of their
+// numbers: the first U are to be held, the others free.  A held page past the first U moves to a free
+// one among them, both in order.  Pages that are neither (a program's own) stay out of it.
+constexpr uint32_t kUsed = 1u, kFree = 2u;   // a page's word
+
+struct CompactArgs {
+    const int* lens;
+    const int* table;
+    const int* ring;
+    const int* state;
+    int* table_out;
+    int* ring_out;
+    int* state_out;
+    int* copies;             // [room][2]
+    uint8_t* words;          // [ranges * kRange] (past one range)
+    int2* sums;              // [ranges] {used, free}
+    int* to;                 // [num_pages] which move a page is
+    int* cut;                // the first page that is not among the first U
+    int B, page, max_pages, num_pages, ranges, room;
+};
+
+__device__ __forceinline__ int2 compact_words(const CompactArgs& a, int lo, uint32_t* words, int* waves) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int pages = min(kRange, a.num_pages - lo);
+    for (int i = tid; i < kRange; i += kThreads) words[i] = 0;
+    int head, count;
+    ring_state(a.state, a.num_pages, &head, &count);
+    __syncthreads();
+    auto mark = [&](int page, uint32_t w) __attribute__((always_inline)) {
+        const uint32_t i = (uint32_t)(page - lo);
+        if (page >= lo && i < (uint32_t)pages) atomicOr(&words[i], w);
+    };
+    for (int b = wave; b < a.B; b += kWaves) {
+        const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
+        const int have = pages_of(len, a.page);
+        for (int j = lane; j < have; j += 64) mark(a.table[(int64_t)b * a.max_pages + j], kUsed);
+    }
+    for (int i = tid; i < count; i += kThreads) mark(a.ring[ring_at(head, i, a.num_pages)], kFree);
+    __syncthreads();
+    int used = 0, free = 0, all_used, all_free;
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t w = words[tid * kPer + i];
+        used += (w & kUsed) != 0;
+        free += w == kFree;
+    }
+    block_scan(used, waves, &all_used);
+    block_scan(free, waves, &all_free);
+    return make_int2(all_used, all_free);
+}
+
+struct CompactSums { int U, all, used, free; };   // held, held or free; held and free in front of a range
+
+// The cut, in the range whose words these are, with `s` its sums: the page, and the held pages in front
+// of it.  False in the threads that do not have it.
+template <class Word>
+__device__ __forceinline__ bool compact_cut(const CompactSums& s, int lo, int pages, Word word, int* waves,
+                                            int* page, int* used) {
+    const int at = threadIdx.x * kPer;
+    int n = 0, m = 0, total;
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t w = at + i < pages ? word(at + i) : 0;
+        n += w != 0;
+        m += (w & kUsed) != 0;
+    }
+    int rank = s.used + s.free + block_scan(n, waves, &total);
+    int held = s.used + block_scan(m, waves, &total);
+    if (rank > s.U || rank + n <= s.U) return false;
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t w = at + i < pages ? word(at + i) : 0;
+        if (w == 0) continue;
+        if (rank == s.U) {
+            *page = lo + at + i;
+            *used = held;
+            return true;
+        }
+        ++rank;
+        held += (w & kUsed) != 0;
+    }
+    return false;
+}
+
+// Moves and free pages of one range: hold(page, move) for a page that moves, hole(page, move) for one
+// that is moved to.
+template <class Word, class Hold, class Hole>
+__device__ __forceinline__ void compact_emit(const CompactArgs& a, const CompactSums& s, int lo, int pages,
+                                             int used_below, Word word, int* waves, Hold hold, Hole hole) {
+    const int at = threadIdx.x * kPer;
+    int n = 0, m = 0, total;
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t w = at + i < pages ? word(at + i) : 0;
+        n += (w & kUsed) != 0;
+        m += w == kFree;
+    }
+    int used = s.used + block_scan(n, waves, &total);
+    int free = s.free + block_scan(m, waves, &total);
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t w = at + i < pages ? word(at + i) : 0;
+        if (w == 0) continue;
+        const int rank = used + free, p = lo + at + i;
+        if (rank >= s.U) a.ring_out[rank - s.U] = p;     // free after the call
+        if (w & kUsed) {
+            if (rank >= s.U) hold(p, used - used_below);
+            ++used;
+        } else {
+            if (rank < s.U) hole(p, free);
+            ++free;
+        }
+    }
+}
+
+// A row's entries through the moves, by a wave.
+template <class To>
+__device__ __forceinline__ void compact_row(const CompactArgs& a, int b, int cut, To to) {
+    const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
+    const int have = pages_of(len, a.page);
+    for (int j = threadIdx.x & 63; j < a.max_pages; j += 64) {
+        int p = 0;
+        if (j < have) {
+            p = a.table[(int64_t)b * a.max_pages + j];
+            if (p >= cut && p < a.num_pages) p = to(p);
+        }
+        a.table_out[(int64_t)b * a.max_pages + j] = p;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) compact_words_kernel(CompactArgs a) {
+    __shared__ uint32_t words[kRange];
+    __shared__ int waves[kWaves];
+    const int lo = blockIdx.x * kRange;
+    const int2 s = compact_words(a, lo, words, waves);
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
+    for (int i = threadIdx.x; i < kRange / 4; i += kThreads)
+        reinterpret_cast<uint32_t*>(a.words + (int64_t)lo)[i] =
+            words[4 * i] | words[4 * i + 1] << 8 | words[4 * i + 2] << 16 | words[4 * i + 3] << 24;
+}
+
+__global__ void __launch_bounds__(kThreads) compact_emit_kernel(CompactArgs a) {
+    __shared__ int waves[kWaves];
+    __shared__ int cut_at[3];    // range of the cut, page, held pages in front of it
+    const int tid = threadIdx.x, g = blockIdx.x;
+    // sums in front of this range and in all, and the range of the cut
+    CompactSums s = {0, 0, 0, 0}, c = {0, 0, 0, 0};
+    int u = 0, f = 0, uu = 0, ff = 0;
+    for (int r = tid; r < a.ranges; r += kThreads) {
+        const int2 x = a.sums[r];
+        uu += x.x;
+        ff += x.y;
+        if (r < g) { u += x.x; f += x.y; }
+    }
+    int total;
+    block_scan(u, waves, &s.used);
+    block_scan(f, waves, &s.free);
+    block_scan(uu, waves, &s.U);
+    block_scan(ff, waves, &total);
+    s.all = s.U + total;
+    if (tid == 0) cut_at[0] = -1;
+    int base = 0, used = 0;      // by one wave, 64 ranges at a time
+    __syncthreads();
+    if (tid < 64)
+        for (int r0 = 0; r0 < a.ranges; r0 += 64) {
+            const int2 x = r0 + tid < a.ranges ? a.sums[r0 + tid] : make_int2(0, 0);
+            int both = x.x + x.y, held = x.x;
+            for (int i = 1; i < 64; i *= 2) {
+                const int p = __shfl_up(both, i), q = __shfl_up(held, i);
+                if (tid >= i) { both += p; held += q; }
+            }
+            const int before = base + both - x.x - x.y;
+            if (before <= s.U && s.U < before + x.x + x.y) {
+                cut_at[0] = r0 + tid;
+                cut_at[1] = before;
+                cut_at[2] = used + held - x.x;
+            }
+            base += __shfl(both, 63);
+            used += __shfl(held, 63);
+        }
+    __syncthreads();
+    const int at = cut_at[0];
+    int cut = a.num_pages, used_below = s.U;     // without a free page nothing is past the first U
+    if (at >= 0) {
+        c.U = s.U;
+        c.used = cut_at[2];
+        c.free = cut_at[1] - cut_at[2];
+        __syncthreads();
+        int p, held;
+        const uint8_t* w = a.words + (int64_t)at * kRange;
+        if (compact_cut(c, at * kRange, kRange, [&](int i) { return (uint32_t)w[i]; }, waves, &p, &held)) {
+            cut_at[1] = p;
+            cut_at[2] = held;
+        }
+        __syncthreads();
+        cut = cut_at[1];
+        used_below = cut_at[2];
+    }
+    const uint8_t* w = a.words + (int64_t)g * kRange;
+    compact_emit(a, s, g * kRange, kRange, used_below, [&](int i) { return (uint32_t)w[i]; }, waves,
+                 [&](int p, int k) { a.to[p] = k; if (k < a.room) a.copies[2 * k] = p; },
+                 [&](int p, int k) { if (k < a.room) a.copies[2 * k + 1] = p; });
+    // what is past the moves and the free pages
+    const int moves = s.U - used_below, left = s.all - s.U;
+    for (int64_t k = moves + (int64_t)g * kThreads + tid; k < a.room; k += (int64_t)a.ranges * kThreads)
+        a.copies[2 * k] = a.copies[2 * k + 1] = -1;
+    for (int64_t k = left + (int64_t)g * kThreads + tid; k < a.num_pages; k += (int64_t)a.ranges * kThreads)
+        a.ring_out[k] = -1;
+    if (g == 0 && tid == 0) {
+        a.state_out[0] = 0;
+        a.state_out[1] = left;
+        *a.cut = cut;
+    }
+}
+
+__global__ void __launch_bounds__(256) compact_table_kernel(CompactArgs a) {
+    const int cut = *a.cut;
+    for (int b = blockIdx.x * 4 + (threadIdx.x >> 6); b < a.B; b += gridDim.x * 4)
+        compact_row(a, b, cut, [&](int p) { return a.copies[2 * a.to[p] + 1]; });
+}
+
+// One range: all of it here, the moves in LDS.
+__global__ void __launch_bounds__(kThreads) compact_one_kernel(CompactArgs a) {
+    __shared__ uint32_t words[kRange];
+    __shared__ int waves[kWaves], cut_at[2], holes[kRange / 2];
+    const int tid = threadIdx.x;
+    const int2 x = compact_words(a, 0, words, waves);
+    const CompactSums s = {x.x, x.x + x.y, 0, 0};
+    if (tid == 0) {
+        cut_at[0] = a.num_pages;
+        cut_at[1] = s.U;
+    }
+    __syncthreads();
+    int p, held;
+    if (compact_cut(s, 0, a.num_pages, [&](int i) { return words[i]; }, waves, &p, &held)) {
+        cut_at[0] = p;
+        cut_at[1] = held;
+    }
+    __syncthreads();
+    const int cut = cut_at[0], used_below = cut_at[1];
+    // a page that moves keeps its move's number in its word, above the two bits
+    compact_emit(a, s, 0, a.num_pages, used_below, [&](int i) { return words[i] & 3u; }, waves,
+                 [&](int p, int k) { words[p] |= (uint32_t)k << 2; a.copies[2 * k] = p; },
+                 [&](int p, int k) { holes[k] = p; a.copies[2 * k + 1] = p; });
+    for (int k = s.U - used_below + tid; k < a.room; k += kThreads) a.copies[2 * k] = a.copies[2 * k + 1] = -1;
+    for (int k = s.all - s.U + tid; k < a.num_pages; k += kThreads) a.ring_out[k] = -1;
+    if (tid == 0) {
+        a.state_out[0] = 0;
+        a.state_out[1] = s.all - s.U;
+    }
+    __syncthreads();
+    for (int b = tid >> 6; b < a.B; b += kWaves) compact_row(a, b, cut, [&](int q) { return holes[words[q] >> 2]; });
+}
+
+// ---- copies ---------------------------------------------------------------------------------
+// Workgroup (x, y) copies pairs [x per, (x + 1) per) in part y, a layer of a pool.  Bound by the bytes.
+constexpr int kCopyThreads = 256;
+
+struct CopyArgs {
+    const int* copies;       // [n][2] {source, destination}
+    int64_t n;
+    int num_pages, per, pools;
+    int first[kMaxPools + 1];    // part that a pool begins with
+    uint8_t* data[kMaxPools];
+    int64_t page_bytes[kMaxPools], layer_bytes[kMaxPools];
+    int width[kMaxPools];    // bytes a lane: 16, 4 or 1
+};
+
+template <typename T>
+__device__ __forceinline__ void copy_page(uint8_t* dst, const uint8_t* src, int64_t bytes) {
+    const int64_t n = bytes / (int64_t)sizeof(T);
+    const T* s = reinterpret_cast<const T*>(src);
+    T* d = reinterpret_cast<T*>(dst);
+    constexpr int kRun = 8;
+    for (int64_t i = threadIdx.x; i < n; i += kRun * kCopyThreads) {
+        T x[kRun];
+        #pragma unroll
+        for (int k = 0; k < kRun; ++k) x[k] = s[min(i + k * kCopyThreads, n - 1)];
+        #pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            if (i + k * kCopyThreads < n) d[i + k * kCopyThreads] = x[k];
+    }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(CopyArgs a) {
+    int pool = 0;
+    while (pool + 1 < a.pools && (int)blockIdx.y >= a.first[pool + 1]) ++pool;
+    uint8_t* base = a.data[pool] + ((int)blockIdx.y - a.first[pool]) * a.layer_bytes[pool];
+    const int64_t bytes = a.page_bytes[pool];
+    const int64_t i0 = (int64_t)blockIdx.x * a.per;
+    const int lane = threadIdx.x & 63;
+    // up to 64 pairs, a lane each; the same in every wave
+    const int64_t i = i0 + lane;
+    int2 mine = make_int2(-1, -1);
+    if (lane < a.per && i < a.n) mine = reinterpret_cast<const int2*>(a.copies)[i];
+    const bool in = mine.x >= 0 && mine.x < a.num_pages && mine.y >= 0 && mine.y < a.num_pages && mine.x != mine.y;
+    uint64_t todo = __builtin_amdgcn_ballot_w64(in);
+    while (todo) {
+        const int k = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const uint8_t* src = base + (int64_t)__builtin_amdgcn_readlane(mine.x, k) * bytes;
+        uint8_t* dst = base + (int64_t)__builtin_amdgcn_readlane(mine.y, k) * bytes;
+        if (a.width[pool] == 16) copy_page<v4u_t>(dst, src, bytes);
+        else if (a.width[pool] == 4) copy_page<uint32_t>(dst, src, bytes);
+        else copy_page<uint8_t>(dst, src, bytes);
+    }
+}
+
+int ranges_of(int num_pages) { return (int)(((int64_t)num_pages + kRange - 1) / kRange); }
+bool fork_in_one(int B, int num_pages) { return B <= kThreads && num_pages <= kRange; }
+
+}  // namespace
+
+size_t cache_fork_workspace(int B, int num_pages) {
+    if (fork_in_one(B, num_pages)) return 0;
+    return ((size_t)num_pages + ranges_of(num_pages)) * 4;
+}
+
+hipError_t launch_cache_fork(const CacheFork& p, void* workspace, hipStream_t stream) {
+    ForkArgs a;
+    a.parents = p.parents; a.keep = p.keep_lens; a.lens = p.seq_lens; a.table = p.block_table;
+    a.state = p.free_state; a.ring = p.free_pages;
+    a.lens_out = p.seq_lens_out; a.table_out = p.block_table_out; a.state_out = p.free_state_out;
+    a.copies = p.copies;
+    a.words = static_cast<uint32_t*>(workspace);
+    a.freed = static_cast<int*>(workspace) + p.num_pages;
+    a.B = p.B; a.page = p.page_size; a.max_pages = p.max_pages; a.num_pages = p.num_pages;
+    a.ranges = ranges_of(p.num_pages);
+    if (fork_in_one(p.B, p.num_pages)) {
+        hipLaunchKernelGGL(fork_words_kernel<true>, dim3(1), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(fork_words_kernel<false>, dim3((unsigned)a.ranges), dim3(kThreads), 0, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(fork_emit_kernel, dim3((unsigned)(a.ranges + (p.B + kWaves - 1) / kWaves)), dim3(kThreads), 0,
+                       stream, a);
+    return hipGetLastError();
+}
+
+size_t cache_compact_workspace(int num_pages) {
+    if (num_pages <= kRange) return 0;
+    const size_t r = ranges_of(num_pages);
+    return r * kRange + r * 8 + (size_t)num_pages * 4 + 4;
+}
+
+hipError_t launch_cache_compact(const CacheCompact& p, void* workspace, hipStream_t stream) {
+    CompactArgs a;
+    a.lens = p.seq_lens; a.table = p.block_table; a.ring = p.free_pages; a.state = p.free_state;
+    a.table_out = p.block_table_out; a.ring_out = p.free_pages_out; a.state_out = p.free_state_out;
+    a.copies = p.copies;
+    a.B = p.B; a.page = p.page_size; a.max_pages = p.max_pages; a.num_pages = p.num_pages;
+    a.ranges = ranges_of(p.num_pages);
+    a.room = std::max(1, p.num_pages / 2);
+    a.words = static_cast<uint8_t*>(workspace);
+    a.sums = reinterpret_cast<int2*>(a.words + (size_t)a.ranges * kRange);
+    a.to = reinterpret_cast<int*>(a.sums + a.ranges);
+    a.cut = a.to + p.num_pages;
+    if (p.num_pages <= kRange) {
+        hipLaunchKernelGGL(compact_one_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(compact_words_kernel, dim3((unsigned)a.ranges), dim3(kThreads), 0, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(compact_emit_kernel, dim3((unsigned)a.ranges), dim3(kThreads), 0, stream, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(compact_table_kernel, dim3((unsigned)std::min((p.B + 3) / 4, 8 * kNumCUs)), dim3(256), 0,
+                       stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_copy_pages(const CopyPages& p, hipStream_t stream) {
+    if (p.n <= 0) return hipSuccess;
+    CopyArgs a;
+    a.copies = p.copies; a.n = p.n; a.num_pages = p.num_pages; a.pools = p.pools;
+    int parts = 0;
+    for (int i = 0; i < p.pools; ++i) {
+        a.first[i] = parts;
+        parts += p.pool[i].layers;
+        a.data[i] = static_cast<uint8_t*>(p.pool[i].data);
+        a.page_bytes[i] = p.pool[i].page_bytes;
+        a.layer_bytes[i] = p.pool[i].layer_bytes;
+        const uint64_t low = reinterpret_cast<uintptr_t>(p.pool[i].data) | (uint64_t)a.page_bytes[i] |
+                             (p.pool[i].layers > 1 ? (uint64_t)a.layer_bytes[i] : 0);
+        a.width[i] = low % 16 == 0 ? 16 : low % 4 == 0 ? 4 : 1;
+    }
+    a.first[p.pools] = parts;
+    // about 4,096 workgroups: of a long list, whose places may be empty, each takes several pairs
+    int per = 1;
+    while (per < 64 && p.n * parts / per > 4096) per *= 2;
+    a.per = per;
+    const int64_t groups = (p.n + per - 1) / per;
+    if (groups > 0x7fffffff || parts > 65535) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)groups, (unsigned)parts), dim3(kCopyThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace mla
