@@ -529,9 +529,12 @@ int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
  * last new_lens[b] (clamped to [0, Sq]) of sequence b's Sq rows are its queries, the rows in front of
  * them padding, whose output is zeros.  Pages that sequences share at the same place behind a shared
  * first page (mla_cache_fork) are expanded once.  Table entries outside the pool read as zero rows.
- * Rounded on the way: keys, values and outputs to the type (fp16: those past its range to +-65504), each
- * key's weight before the division by the row's sum; sums are float32.  A latent row
- * with a NaN or an infinity makes the rows of the queries that see it NaN and reaches no other query.
+ * Rounded on the way, in both types: keys, values and each key's weight (before the division by the
+ * row's sum) to 11 bits as fp16 numbers, in bf16 under a power of two for each 64 keys that brings
+ * their largest latent or rope value to [64, 128); weights down to 2^-22 of the row's largest; bf16
+ * queries to 11 bits down to 2^-14 of the row's largest; the output to its type.  Sums are float32.  A key
+ * or value past fp16's range (65504, in bf16 times that power of two) stays there.  A latent row with a
+ * NaN or an infinity makes the rows of the queries that see it NaN and reaches no other query.
  * The workspace holds keys and values of as many heads at a time as 2 GiB take (one at least). */
 size_t mla_attention_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims, int causal);
 int mla_attention_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,

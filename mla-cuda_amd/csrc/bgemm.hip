@@ -390,9 +390,10 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
             }
             const __amdgpu_buffer_rsrc_t rc = make_rsrc(a.C16 + (int64_t)job.g * a.sCg + (int64_t)job.m0 * a.ldc);
             const uint32_t cmask = oob_mask(col, a.N);
-            // past fp16's range a key or value stays at its end: an infinite value would reach queries
-            // that its key is hidden from, as 0 * inf (a NaN stays one)
-            if constexpr (EXPAND && Half<TL>::kF16) {
+            // keys and values are fp16 whatever the operands are; one past its range stays at its end: an
+            // infinite value would reach queries that its key is hidden from, as 0 * inf (a NaN is NaN)
+            typedef std::conditional_t<EXPAND, f16_t, TL> TO;
+            if constexpr (EXPAND) {
                 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb)
                     #pragma unroll
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
                         const float x0 = acc[rb][cb][e], x1 = acc[rb][cb][e + 1];
                         const float p0 = dpp_move<0xB1>(x0), p1 = dpp_move<0xB1>(x1);
                         const int row = acc_row(odd ? e + 1 : e, lane);
-                        const uint32_t w = odd ? Half<TL>::pack2(p1, x1) : Half<TL>::pack2(x0, p0);
+                        const uint32_t w = odd ? Half<TO>::pack2(p1, x1) : Half<TO>::pack2(x0, p0);
                         *reinterpret_cast<uint32_t*>(mine + row * kRowB + 16 * ((c2 >> 3) ^ (row & kSw)) +
                                                      2 * (c2 & 7)) = w;
                     }

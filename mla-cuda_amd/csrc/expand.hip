@@ -25,6 +25,7 @@ typedef float v2f_t __attribute__((ext_vector_type(2)));
 
 constexpr int kUnit = kExpandUnit;            // rows a unit (and keys a step of the attention)
 constexpr int kR = 512, kD = 64, kN = 128;    // latent, rope, nope / value widths
+constexpr int kHead = 6;                      // log2 of a bf16 unit's largest value as it is stored
 
 // ---- units ----------------------------------------------------------------------------------
 // Unit j of sequence b is its keys [64 j, 64 j + 64).  Sequences that continue one prompt hold the
@@ -101,11 +102,20 @@ __global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
 }
 
 // ---- gather ---------------------------------------------------------------------------------
-// A workgroup copies a unit's rows, or only notes where its owner's are.  A latent row with a value
-// that is not finite makes every key and value of it NaN or infinite, and with it every output of a
-// query that sees it NaN (also under a weight of 0); the row is written as zeros, so that queries
-// in front of it are not touched by 0 * NaN, and the unit's first such row is noted for the queries
-// behind it.  Rope values need no such care: they only reach their own key's scores.
+// A workgroup copies a unit's rows, or only notes where its owner's are.
+// Keys, values and weights are fp16 from here on, in bf16 too: 11 bits instead of 8 bring the outputs'
+// distance from the exact ones from 1.6 to 2.3 times that of their own rounding down to about it (bf16).
+// A bf16 cache is fitted into fp16's range by a power of two for each unit, 2^e: its rows are stored
+// under it, the largest value in [2^kHead, 2^(kHead+1)), and the attention puts it back.  kHead leaves
+// 2^9 above for keys and values, sums of 512 products with weights (below 1 they cannot reach fp16's
+// end), and 2^20 below down to its subnormals, so that neither large rows nor weights cost the other rows
+// bits.  An fp16 cache is as it is (e = 0).  The latent rows keep the type of W_uk and W_uv, which they
+// are multiplied with; the rope rows are fp16.
+// A latent row with a value that is not finite makes every key and value of it NaN or infinite, and
+// with it every output of a query that sees it NaN (also under a weight of 0); the row is written as
+// zeros, so that queries in front of it are not touched by 0 * NaN, and the unit's first such row is
+// noted for the queries behind it.  Rope values need no such care: they only reach their own key's
+// scores.
 struct GatherArgs {
     const void* c_kv;
     const void* pe;
@@ -117,6 +127,7 @@ struct GatherArgs {
     const int* count;
     int* unit;               // [B][units] the unit's place in lat / rot
     int* bad;                // [places] first row that is not finite, or 64
+    int* exps;               // [places] e
     int* any_bad;
     int* rows;               // rows in all
     uint16_t* lat;
@@ -130,17 +141,32 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
     return (w & e) == e || ((w >> 16) & e) == e;
 }
 
-// four e4m3 codes under a power of two, in the 16-bit type
+// 2^k, for k in [-126, 127]
+__device__ __forceinline__ float two_to(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
+// the exponent of a positive float; zero and what is below 2^-100 count as 2^-100 (so that values under
+// 2^-e, and outputs under 2^e, stay in float32's range)
+__device__ __forceinline__ int exponent_of(float x) { return max((int)(__float_as_uint(x) >> 23) - 127, -100); }
+
+// two 16-bit values, or two of four e4m3 codes under a power of two in the 16-bit type
+template <typename TL>
+__device__ __forceinline__ v2f_t halves(uint32_t w) {
+    return v2f_t{Half<TL>::to_f32(w & 0xffffu), Half<TL>::to_f32(w >> 16)};
+}
 template <typename TL>
 __device__ __forceinline__ v2u_t decode_half4(uint32_t w, float scale) {
     const v2f_t lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false);
     const v2f_t hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
     return v2u_t{Half<TL>::pack2(lo[0], lo[1]), Half<TL>::pack2(hi[0], hi[1])};
 }
+__device__ __forceinline__ float finite_max(float m, float x) {
+    x = fabsf(x);
+    return x < INFINITY ? fmaxf(m, x) : m;
+}
 
 template <typename TL, bool F8>
 __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
     __shared__ int part[4], w_bad[4];
+    __shared__ float w_top[4];
     const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.Sk) : a.Sk;
@@ -190,61 +216,89 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
     const int n = in ? min(kUnit, len - k0) : 0;
     uint16_t* lat = a.lat + (int64_t)place * kUnit * kR;
     uint16_t* rot = a.rot + (int64_t)place * kUnit * kD;
-    // latent rows: 16 a wave, 8 columns a lane
+    // latent rows: 16 a wave, 8 columns a lane; rope rows: 8 lanes a row, 2 of 8 columns a thread
+    v4u x[16], y[2];
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = 16 * wave + i;
+        x[i] = v4u{0, 0, 0, 0};
+        if (r >= n) continue;
+        if constexpr (F8) {
+            const v2u_t c = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.c_kv) + (r0 + r) * kR)[lane];
+            const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift)] << 23);
+            const v2u_t lo = decode_half4<TL>(c[0], f), hi = decode_half4<TL>(c[1], f);
+            x[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
+        } else {
+            x[i] = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.c_kv) + (r0 + r) * kR)[lane];
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = 32 * i + (tid >> 3), c = tid & 7;
+        y[i] = v4u{0, 0, 0, 0};
+        if (r >= n) continue;
+        if constexpr (F8) {
+            const v2u_t w = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.pe) + (r0 + r) * kD)[c];
+            const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift) + 1] << 23);
+            const v2u_t lo = decode_half4<TL>(w[0], f), hi = decode_half4<TL>(w[1], f);
+            y[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
+        } else {
+            y[i] = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.pe) + (r0 + r) * kD)[c];
+        }
+    }
     int worst = kUnit;
+    float top = 0.f;
     #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        v4u x[8];
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = 16 * wave + 8 * half + i;
+    for (int i = 0; i < 16; ++i) {
+        const bool odd = not_finite2<TL>(x[i][0]) || not_finite2<TL>(x[i][1]) || not_finite2<TL>(x[i][2]) ||
+                         not_finite2<TL>(x[i][3]);
+        if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+            worst = min(worst, 16 * wave + i);
             x[i] = v4u{0, 0, 0, 0};
-            if (r >= n) continue;
-            if constexpr (F8) {
-                const v2u_t c = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.c_kv) + (r0 + r) * kR)[lane];
-                const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift)] << 23);
-                const v2u_t lo = decode_half4<TL>(c[0], f), hi = decode_half4<TL>(c[1], f);
-                x[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
-            } else {
-                x[i] = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.c_kv) + (r0 + r) * kR)[lane];
-            }
         }
         #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = 16 * wave + 8 * half + i;
-            bool odd = not_finite2<TL>(x[i][0]) || not_finite2<TL>(x[i][1]) ||
-                       not_finite2<TL>(x[i][2]) || not_finite2<TL>(x[i][3]);
-            odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-            if (odd) {
-                worst = min(worst, r);
-                x[i] = v4u{0, 0, 0, 0};
-            }
-            reinterpret_cast<v4u*>(lat + r * kR)[lane] = x[i];
+        for (int k = 0; k < 4; ++k) {
+            const v2f_t v = halves<TL>(x[i][k]);
+            top = fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1])));
         }
     }
-    // rope rows: 8 lanes a row
     #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int r = 32 * half + (tid >> 3), c = tid & 7;
-        v4u x = {0, 0, 0, 0};
-        if (r < n) {
-            if constexpr (F8) {
-                const v2u_t w = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.pe) + (r0 + r) * kD)[c];
-                const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift) + 1] << 23);
-                const v2u_t lo = decode_half4<TL>(w[0], f), hi = decode_half4<TL>(w[1], f);
-                x = v4u{lo[0], lo[1], hi[0], hi[1]};
-            } else {
-                x = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.pe) + (r0 + r) * kD)[c];
-            }
+    for (int i = 0; i < 2; ++i)
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const v2f_t v = halves<TL>(y[i][k]);
+            top = finite_max(finite_max(top, v[0]), v[1]);
         }
-        reinterpret_cast<v4u*>(rot + r * kD)[c] = x;
-    }
-    if (lane == 0) w_bad[wave] = worst;
+    top = wave_reduce(top, OpMax());
+    if (lane == 0) { w_bad[wave] = worst; w_top[wave] = top; }
     __syncthreads();
+    worst = min(min(w_bad[0], w_bad[1]), min(w_bad[2], w_bad[3]));
+    const int e = Half<TL>::kF16 ? 0 : exponent_of(fmaxf(fmaxf(w_top[0], w_top[1]), fmaxf(w_top[2], w_top[3]))) - kHead;
+    const float f = two_to(-e);
     if (tid == 0) {
-        worst = min(min(w_bad[0], w_bad[1]), min(w_bad[2], w_bad[3]));
+        a.exps[place] = e;
         a.bad[place] = worst;
         if (worst < kUnit) *a.any_bad = 1;   // cleared by the plan; every writer writes the same
+    }
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        v4u o;
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const v2f_t v = halves<TL>(x[i][k]);
+            o[k] = Half<TL>::pack2(v[0] * f, v[1] * f);
+        }
+        reinterpret_cast<v4u*>(lat + (16 * wave + i) * kR)[lane] = o;
+    }
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        v4u o;
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const v2f_t v = halves<TL>(y[i][k]);
+            o[k] = pack_f16x2(v[0] * f, v[1] * f);
+        }
+        reinterpret_cast<v4u*>(rot + (32 * i + (tid >> 3)) * kD)[tid & 7] = o;
     }
 }
 
@@ -258,7 +312,13 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
 // a lane's eight of a 16-key step are keys 4h + 0..3 and 8 + 4h + 0..3 (h: its half), and V's
 // transposing reads take the rows in that order.
 // The reference of a row's exponentials moves only when a score passes it by kRise powers of two (few
-// do after the first step), and what is in the accumulators is scaled then.
+// do after the first step), and what is in the accumulators is scaled then.  They are fp16, as keys and
+// values are (the gather's comment): they start at 2^kBias, so that small ones keep more bits above
+// fp16's subnormals, and rise to 2^(kBias + kRise) < 65504.
+// A unit's power of two is one number a step: its keys' goes into the factor of the scores, its values'
+// into the exponentials, as d = e - E <= 0 with the largest e so far in E (what is in the accumulators
+// is scaled when that grows); the sum takes it out again.  bf16 queries are made fp16 under a power of
+// two of their own.
 struct HeadsArgs {
     const uint16_t* qn;      // [B, Sq, H, 128]
     const uint16_t* qr;      // [B, Sq, H, 64]
@@ -266,6 +326,7 @@ struct HeadsArgs {
     const uint16_t* rot;     // [rows_cap][64]
     const int* unit;
     const int* bad;
+    const int* exps;
     const int* any_bad;
     const int* seq_lens;
     const int* new_lens;
@@ -283,9 +344,7 @@ constexpr int kVAt = kKBytes, kRAt = 2 * kKBytes;
 template <typename TL>
 __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStageBytes];
-    // fp16 weights start at 2^kBias and may rise to 2^(kBias + kRise) < 65504: small ones keep more
-    // bits above its subnormals; bf16 has the exponent range of the sums
-    constexpr float kRise = Half<TL>::kF16 ? 6.f : 8.f, kBias = Half<TL>::kF16 ? 8.f : 0.f;
+    constexpr float kRise = 6.f, kBias = 8.f;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, q = lane & 31;
     const uint32_t lds0 = lds_addr(smem);
@@ -327,6 +386,28 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         #pragma unroll
         for (int i = 0; i < 4; ++i) qf[8 + i] = *reinterpret_cast<const v4u*>(r + 16 * i);
     }
+    float c = a.c;
+    if constexpr (!Half<TL>::kF16) {
+        float top = 0.f;
+        #pragma unroll
+        for (int i = 0; i < 12; ++i)
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(qf[i][k]);
+                top = finite_max(finite_max(top, v[0]), v[1]);
+            }
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        const int e = min(exponent_of(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]))), 126);
+        const float f = two_to(-e);
+        c *= two_to(e);
+        #pragma unroll
+        for (int i = 0; i < 12; ++i)
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(qf[i][k]);
+                qf[i][k] = pack_f16x2(v[0] * f, v[1] * f);
+            }
+    }
 
     // ---- staging.  Key rows of 256 bytes, 16-byte chunk c of row r at c ^ (r & 15); value rows of
     // 256, chunk c at c ^ 4 (r & 3); rope rows of 128, chunk c at c ^ ((r >> 1) & 7).
@@ -366,15 +447,19 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     float m_ref = -INFINITY, l = 0.f;
 
     int next = n_tiles > 0 ? load_uniform(units) : 0;
+    int e_next = n_tiles > 0 ? load_uniform(a.exps + next) : 0;
     if (n_tiles > 0) issue(next, 0);
     next = n_tiles > 1 ? load_uniform(units + 1) : 0;
+    int E = e_next;
     #pragma unroll 1
     for (int j = 0; j < n_tiles; ++j) {
         const uint32_t st = (j & 1) * kStageBytes;
         wait_vm<0>();
         lds_barrier();      // step j has landed; every wave is done with step j - 1
+        const int e = e_next;
         if (j + 1 < n_tiles) {
             issue(next, kStageBytes - st);
+            e_next = load_uniform(a.exps + next);
             next = j + 2 < n_tiles ? load_uniform(units + j + 2) : 0;
         }
         if (j * kUnit > wave_last) continue;
@@ -383,13 +468,13 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         for (int i = 0; i < 8; ++i)
             #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                s[kb] = Mma<TL>::sub(*reinterpret_cast<const v4u*>(smem + st + 8192 * kb + (k_rd ^ (32 * i))),
+                s[kb] = Mma<f16_t>::sub(*reinterpret_cast<const v4u*>(smem + st + 8192 * kb + (k_rd ^ (32 * i))),
                                      qf[i], 0, s[kb]);
         #pragma unroll
         for (int i = 0; i < 4; ++i)
             #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                s[kb] = Mma<TL>::sub(*reinterpret_cast<const v4u*>(smem + st + 4096 * kb + (r_rd ^ (32 * i))),
+                s[kb] = Mma<f16_t>::sub(*reinterpret_cast<const v4u*>(smem + st + 4096 * kb + (r_rd ^ (32 * i))),
                                      qf[8 + i], 0, s[kb]);
         if (j * kUnit + kUnit - 1 > wave_first) {
             #pragma unroll
@@ -398,6 +483,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                 for (int i = 0; i < 16; ++i)
                     s[kb][i] = j * kUnit + 32 * kb + acc_row(i, lane) <= lim ? s[kb][i] : -INFINITY;
         }
+        const float ct = c * two_to(e);
         float top = s[0][0];
         #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
@@ -405,7 +491,15 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
         {
             const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.c;
+            top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * ct;
+        }
+        if (e > E) {
+            const float f = e - E > 126 ? 0.f : two_to(E - e);
+            E = e;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                #pragma unroll
+                for (int k = 0; k < 16; ++k) o[i][k] *= f;
         }
         // (only those rows: a row's bits do not depend on the others of its wave)
         const bool over = top > m_ref + kRise;
@@ -419,26 +513,29 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[i][e] *= f;
         }
-        const float neg = m_ref == -INFINITY ? 0.f : kBias - m_ref;
+        const int d = max(e - E, -100);
+        const float neg = (m_ref == -INFINITY ? 0.f : kBias - m_ref) + (float)d;
+        float sum = 0.f;
         #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
             #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.c, neg));
-                l += s[kb][i];
+                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], ct, neg));
+                sum += s[kb][i];
             }
+        l += sum * two_to(-d);
         #pragma unroll
         for (int i = 0; i < 4; ++i) {       // 16 keys
             v4u p;
             #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                p[e] = Half<TL>::pack2(s[i >> 1][8 * (i & 1) + 2 * e], s[i >> 1][8 * (i & 1) + 2 * e + 1]);
+            for (int k = 0; k < 4; ++k)
+                p[k] = pack_f16x2(s[i >> 1][8 * (i & 1) + 2 * k], s[i >> 1][8 * (i & 1) + 2 * k + 1]);
             #pragma unroll
             for (int vb = 0; vb < 4; ++vb) {
                 const uint8_t* at = smem + st + 4096 * i + (v_rd ^ (64 * vb));
                 const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
                 const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 2048));
-                o[vb] = Mma<TL>::sub(__builtin_bit_cast(v4u, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)),
+                o[vb] = Mma<f16_t>::sub(__builtin_bit_cast(v4u, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)),
                                      p, 0, o[vb]);
             }
         }
@@ -448,7 +545,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
         l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     }
-    float f = l == 0.f ? 0.f : 1.f / l;
+    float f = l == 0.f ? 0.f : two_to(E) / l;
     if (load_uniform(a.any_bad)) {
         int worst = 0x7fffffff;
         for (int j = lane; j < n_tiles; j += 64) {
@@ -519,6 +616,7 @@ ExpandPlan plan_expand(int B, int Sk, int H, bool paged) {
     p.off_count = take(paged ? (size_t)B * 4 : 0);
     p.off_unit = take(places * 4);
     p.off_bad = take(places * 4);
+    p.off_exps = take(places * 4);
     p.off_any = take(8);                      // any_bad, rows
     p.off_lat = take((size_t)p.rows_cap * kR * 2);
     p.off_rot = take((size_t)p.rows_cap * kD * 2);
@@ -547,7 +645,7 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     g.c_kv = p.c_kv; g.pe = p.pe; g.scales = static_cast<const uint8_t*>(p.scales);
     g.seq_lens = p.seq_lens; g.table = p.block_table;
     g.owner = u.owner; g.rank = u.rank; g.count = u.count;
-    g.unit = ints(plan.off_unit); g.bad = ints(plan.off_bad); g.any_bad = any_bad; g.rows = any_bad + 1;
+    g.unit = ints(plan.off_unit); g.bad = ints(plan.off_bad); g.exps = ints(plan.off_exps); g.any_bad = any_bad; g.rows = any_bad + 1;
     g.lat = half(plan.off_lat); g.rot = half(plan.off_rot);
     g.B = p.B; g.Sk = p.Sk; g.units = plan.units;
     g.page_size = p.page_size; g.max_pages = u.max_pages; g.num_pages = p.num_pages;
@@ -566,7 +664,7 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     HeadsArgs a;
     a.qn = static_cast<const uint16_t*>(p.q_nope); a.qr = static_cast<const uint16_t*>(p.q_rope);
     a.kv = half(plan.off_kv); a.rot = g.rot;
-    a.unit = g.unit; a.bad = g.bad; a.any_bad = any_bad;
+    a.unit = g.unit; a.bad = g.bad; a.exps = g.exps; a.any_bad = any_bad;
     a.seq_lens = p.seq_lens; a.new_lens = p.new_lens;
     a.out = static_cast<uint16_t*>(p.out);
     a.B = p.B; a.Sq = p.Sq; a.Sk = p.Sk; a.H = p.H; a.units = plan.units;

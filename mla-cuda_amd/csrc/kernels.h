@@ -408,7 +408,7 @@ struct ExpandPlan {
     int units = 0;                   // of a sequence, at most
     int64_t rows_cap = 0;            // rows of all of them
     int heads = 0;                   // expanded and attended to at a time
-    size_t off_owner, off_rank, off_count, off_unit, off_bad, off_any, off_lat, off_rot, off_kv, total;
+    size_t off_owner, off_rank, off_count, off_unit, off_bad, off_exps, off_any, off_lat, off_rot, off_kv, total;
 };
 ExpandPlan plan_expand(int B, int Sk, int H, bool paged);
 hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* workspace, hipStream_t stream);
