@@ -45,6 +45,7 @@ namespace mla {
 namespace {
 
 typedef float v2f __attribute__((ext_vector_type(2)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBThreads = 512;
 constexpr int kBKS = 32;          // K per slice
@@ -63,12 +64,18 @@ struct BArgs {
 
 // EXPAND: the keys and values of the expanded attention (expand.hip).  The groups are heads, all of
 // them over the same A: their columns are walked like further N tiles.  A group's 256 columns are two
-// weights of 128 rows each, and how many rows A has is known on the device alone.
+// weights of 128 rows each, and how many rows A has is known on the device alone.  Its results are fp16
+// whatever the operands are, and one past fp16's range stays at its end (an infinite value would reach
+// queries that its key is hidden from, as 0 * inf; a NaN is NaN): the MODE register's FP16_OVFL bit, which
+// lasts for the wave.  With K at 512 a tile's way out is a third of its time: the MFMAs' operands are
+// swapped, which leaves four columns of a row in a lane (4,096 rows and 128 heads 198 -> 155 us; 16-byte
+// stores from there, without LDS, are half lines: 187).
 template <typename TL, int BM, int BN, int NS, int MINB, bool NT, bool QUP, bool EXPAND = false>
 __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
     static_assert(!NT || !QUP, "2a2 reads N-contiguous W");
     static_assert(!EXPAND || NT, "the heads' weights are K-contiguous");
     if constexpr (EXPAND) {
+        __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, 1);   // hwreg(MODE, bit 23, 1 bit)
         a.M = load_uniform(a.rows);
         a.tiles_m = (a.M + BM - 1) / BM;
     }
@@ -273,7 +280,8 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
             }
             #pragma unroll
             for (int cb = 0; cb < CB; ++cb)
-                acc[rb][cb] = Mma<TL>::sub(af[cur][rb], bf[cur][cb], 0, acc[rb][cb]);
+                acc[rb][cb] = EXPAND ? Mma<TL>::sub(bf[cur][cb], af[cur][rb], 0, acc[rb][cb])
+                                     : Mma<TL>::sub(af[cur][rb], bf[cur][cb], 0, acc[rb][cb]);
             if (d) {
                 constexpr int n = (kLoads + RB - 1) / RB;
                 #pragma unroll
@@ -390,31 +398,29 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
             }
             const __amdgpu_buffer_rsrc_t rc = make_rsrc(a.C16 + (int64_t)job.g * a.sCg + (int64_t)job.m0 * a.ldc);
             const uint32_t cmask = oob_mask(col, a.N);
-            // keys and values are fp16 whatever the operands are; one past its range stays at its end: an
-            // infinite value would reach queries that its key is hidden from, as 0 * inf (a NaN is NaN)
-            typedef std::conditional_t<EXPAND, f16_t, TL> TO;
-            if constexpr (EXPAND) {
-                #pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-                    #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb)
-                        #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float x = acc[rb][cb][e];
-                            acc[rb][cb][e] = fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
-                        }
-            }
             #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
+                    if constexpr (EXPAND) {
+                        // the transposed accumulators: four columns of one row a lane, no exchange
+                        const int row = lane & 31;
+                        #pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            const v2u v = {pack_f16x2(acc[rb][cb][e], acc[rb][cb][e + 1]),
+                                           pack_f16x2(acc[rb][cb][e + 2], acc[rb][cb][e + 3])};
+                            *reinterpret_cast<v2u*>(mine + row * kRowB + 16 * ((4 * cb + (e >> 2)) ^ (row & kSw)) +
+                                                    8 * (lane >> 5)) = v;
+                        }
+                        continue;
+                    }
                     const int c2 = 32 * cb + ((lane & 31) & ~1);
                     #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         const float x0 = acc[rb][cb][e], x1 = acc[rb][cb][e + 1];
                         const float p0 = dpp_move<0xB1>(x0), p1 = dpp_move<0xB1>(x1);
                         const int row = acc_row(odd ? e + 1 : e, lane);
-                        const uint32_t w = odd ? Half<TO>::pack2(p1, x1) : Half<TO>::pack2(x0, p0);
+                        const uint32_t w = odd ? Half<TL>::pack2(p1, x1) : Half<TL>::pack2(x0, p0);
                         *reinterpret_cast<uint32_t*>(mine + row * kRowB + 16 * ((c2 >> 3) ^ (row & kSw)) +
                                                      2 * (c2 & 7)) = w;
                     }

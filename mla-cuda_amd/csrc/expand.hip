@@ -11,6 +11,7 @@
 // the last two for as many heads at a time as the workspace holds.
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "kernels.h"
 #include "mma.h"
@@ -38,6 +39,7 @@ struct PlanArgs {
     int* owner;      // [B][units] the sequence that the unit is made for
     int* rank;       // [B][units] how many own units it has in front
     int* count;      // [B] own units
+    int* order;      // [B] the sequences, longest first
     int* any_bad;
     int B, Sk, units, max_pages, per_page;   // per_page: units a page
 };
@@ -51,9 +53,18 @@ __global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
     if (!a.table) return;
     const int len = min(max(a.seq_lens[b], 0), a.Sk);
     const int* row = a.table + (int64_t)b * a.max_pages;
+    // longer sequences, and those as long in front of this one
+    int longer = 0;
+    for (int c = tid; c < a.B; c += kPlanThreads) {
+        const int n = min(max(a.seq_lens[c], 0), a.Sk);
+        longer += n > len || (n == len && c < b);
+    }
+    longer = wave_sum(longer);
+    if (lane == 0) w_own[wave] = longer;
     // sequences in front of this one with the same first page, in order
     if (tid == 0) n_list = 0;
     __syncthreads();
+    if (tid == 0) a.order[w_own[0] + w_own[1] + w_own[2] + w_own[3]] = b;
     if (len >= kUnit && wave == 0) {
         const int page = row[0];
         int n = 0;
@@ -330,8 +341,11 @@ struct HeadsArgs {
     const int* any_bad;
     const int* seq_lens;
     const int* new_lens;
+    const int* order;        // null: as they come
     uint16_t* out;           // [B, Sq, H, 128]
-    int B, Sq, Sk, H, h0, units, tiles, causal;
+    float* part;             // SPLIT: [splits][B, Sq, heads][128] rows of a split, divided by its sums,
+    float2* state;           // [splits][B, Sq, heads] {reference, sum}
+    int B, Sq, Sk, H, h0, heads, units, tiles, causal, splits;
     int64_t head_stride;     // elements of kv a head
     float c;                 // log2(e) / scale
 };
@@ -341,7 +355,18 @@ constexpr int kKBytes = kUnit * 2 * kN, kRBytes = kUnit * 2 * kD;       // a sta
 constexpr int kStageBytes = 2 * kKBytes + kRBytes;
 constexpr int kVAt = kKBytes, kRAt = 2 * kKBytes;
 
+// Two outputs in their type.  An average of fp16 values up to 65504 stays there, also where its weights
+// are rounded up (a NaN is NaN).
 template <typename TL>
+__device__ __forceinline__ uint32_t to_half2(float x, float y) {
+    if constexpr (Half<TL>::kF16) {
+        x = fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
+        y = fabsf(y) > 65504.f ? copysignf(65504.f, y) : y;
+    }
+    return Half<TL>::pack2(x, y);
+}
+
+template <typename TL, bool SPLIT>
 __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStageBytes];
     constexpr float kRise = 6.f, kBias = 8.f;
@@ -349,11 +374,18 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     const int hi = lane >> 5, q = lane & 31;
     const uint32_t lds0 = lds_addr(smem);
 
-    // heads outermost, a contiguous run of them an XCD; within a head the longest tiles first
-    const int item = xcd_logical_block(blockIdx.x, gridDim.x);
-    const int per_head = a.B * a.tiles;
-    const int hl = item / per_head, rest = item - hl * per_head;
-    const int t = a.tiles - 1 - rest / a.B, b = rest % a.B;
+    // The longest sequences first, and in them the tiles that see most; an XCD has heads of its own (one
+    // in eight; where that does not divide, a contiguous run of all items), whose tiles follow one
+    // another and find each other's keys in its L2.
+    const bool eighth = a.heads % kNumXCDs == 0;
+    int item = eighth ? blockIdx.x / kNumXCDs : xcd_logical_block(blockIdx.x, gridDim.x);
+    int sp = 0;
+    if constexpr (SPLIT) { sp = item % a.splits; item /= a.splits; }
+    const int t = a.tiles - 1 - item % a.tiles;
+    item /= a.tiles;
+    const int some = eighth ? a.heads / kNumXCDs : a.heads;
+    const int hl = eighth ? item % some * kNumXCDs + blockIdx.x % kNumXCDs : item % some;
+    const int b = a.order ? load_uniform(a.order + item / some) : item / some;
     const int h = a.h0 + hl;
     const int len = a.seq_lens ? min(max(load_uniform(a.seq_lens + b), 0), a.Sk) : a.Sk;
     const int fresh = a.new_lens ? min(max(load_uniform(a.new_lens + b), 0), a.Sq) : a.Sq;
@@ -362,7 +394,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     uint16_t* const out = a.out + (int64_t)b * a.Sq * row_stride + (int64_t)h * kN;
 
     // rows in front of the new ones
-    for (int r = kHRows * t + (tid >> 4); r < min(pad, kHRows * (t + 1)); r += kHThreads / 16)
+    for (int r = kHRows * t + (tid >> 4); sp == 0 && r < min(pad, kHRows * (t + 1)); r += kHThreads / 16)
         reinterpret_cast<v4u*>(out + r * row_stride)[tid & 15] = v4u{0, 0, 0, 0};
     const int r0 = pad + kHRows * t;
     if (r0 >= a.Sq) return;
@@ -375,7 +407,13 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     const int row = min(w0 + q, a.Sq - 1);
     const int lim = lim_of(row);
     const int wave_first = w0 < a.Sq ? lim_of(w0) : -1, wave_last = w0 < a.Sq ? lim_of(min(w0 + 31, a.Sq - 1)) : -1;
-    const int n_tiles = (lim_of(min(r0 + kHRows, a.Sq) - 1) + kUnit) / kUnit;   // lim -1: 0
+    int n_tiles = (lim_of(min(r0 + kHRows, a.Sq) - 1) + kUnit) / kUnit;   // lim -1: 0
+    int first = 0;               // SPLIT: a share of them
+    if constexpr (SPLIT) {
+        const int share = (n_tiles + a.splits - 1) / a.splits;
+        first = sp * share;
+        n_tiles = min(n_tiles, first + share);
+    }
 
     v4u qf[12];
     {
@@ -446,14 +484,14 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     for (int i = 0; i < 4; ++i) o[i] = v16f{};
     float m_ref = -INFINITY, l = 0.f;
 
-    int next = n_tiles > 0 ? load_uniform(units) : 0;
-    int e_next = n_tiles > 0 ? load_uniform(a.exps + next) : 0;
-    if (n_tiles > 0) issue(next, 0);
-    next = n_tiles > 1 ? load_uniform(units + 1) : 0;
+    int next = n_tiles > first ? load_uniform(units + first) : 0;
+    int e_next = n_tiles > first ? load_uniform(a.exps + next) : 0;
+    if (n_tiles > first) issue(next, 0);
+    next = n_tiles > first + 1 ? load_uniform(units + first + 1) : 0;
     int E = e_next;
     #pragma unroll 1
-    for (int j = 0; j < n_tiles; ++j) {
-        const uint32_t st = (j & 1) * kStageBytes;
+    for (int j = first; j < n_tiles; ++j) {
+        const uint32_t st = ((j - first) & 1) * kStageBytes;
         wait_vm<0>();
         lds_barrier();      // step j has landed; every wave is done with step j - 1
         const int e = e_next;
@@ -548,24 +586,26 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     float f = l == 0.f ? 0.f : two_to(E) / l;
     if (load_uniform(a.any_bad)) {
         int worst = 0x7fffffff;
-        for (int j = lane; j < n_tiles; j += 64) {
+        for (int j = first + lane; j < n_tiles; j += 64) {
             const int r = a.bad[units[j]];
             if (r < kUnit) worst = min(worst, j * kUnit + r);
         }
         #pragma unroll
         for (int i = 1; i < 64; i *= 2) worst = min(worst, __shfl_xor(worst, i));
-        if (worst <= lim) f = __uint_as_float(0x7fc00000u);
+        if (worst <= lim) l = f = __uint_as_float(0x7fc00000u);
     }
-    // an average of values up to 65504 stays there, also where its weights are rounded up (NaN is NaN)
-    if constexpr (Half<TL>::kF16) {
+    if constexpr (SPLIT) {
+        if (w0 + q >= a.Sq) return;
+        const int64_t at = ((int64_t)(sp * a.B + b) * a.Sq + row) * a.heads + hl;
+        if (hi == 0) a.state[at] = make_float2(m_ref, l);
+        float* const dst = a.part + at * kN + 4 * hi;
         #pragma unroll
         for (int vb = 0; vb < 4; ++vb)
             #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = o[vb][i] * f;
-                o[vb][i] = fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
-            }
-        f = 1.f;
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<v4f*>(dst + 32 * vb + 2 * i) =
+                    v4f{o[vb][i] * f, o[vb][i + 1] * f, o[vb][i + 2] * f, o[vb][i + 3] * f};
+        return;
     }
     if (w0 + q < a.Sq) {
         uint16_t* const dst = out + row * row_stride + 4 * hi;
@@ -574,9 +614,37 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             #pragma unroll
             for (int i = 0; i < 16; i += 4)
                 *reinterpret_cast<v2u_t*>(dst + 32 * vb + 2 * i) =
-                    v2u_t{Half<TL>::pack2(o[vb][i] * f, o[vb][i + 1] * f),
-                          Half<TL>::pack2(o[vb][i + 2] * f, o[vb][i + 3] * f)};
+                    v2u_t{to_half2<TL>(o[vb][i] * f, o[vb][i + 1] * f),
+                          to_half2<TL>(o[vb][i + 2] * f, o[vb][i + 3] * f)};
     }
+}
+
+// Rows from their splits' (averages of values, each with the reference and sum of its weights): half a wave
+// a row.
+template <typename TL>
+__global__ void __launch_bounds__(256) heads_merge_kernel(HeadsArgs a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = (int64_t)a.B * a.Sq * a.heads;
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const int64_t bi = r / a.heads;
+    const int hl = (int)(r - bi * a.heads), b = (int)(bi / a.Sq), i = (int)(bi - (int64_t)b * a.Sq);
+    const int fresh = a.new_lens ? min(max(a.new_lens[b], 0), a.Sq) : a.Sq;
+    if (i < a.Sq - fresh) return;        // padding has its zeros
+    float M = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.state[s * rows + r].x);
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 x = a.state[s * rows + r];
+        if (x.y == 0.f) continue;        // no key seen there
+        const float w = x.y * __builtin_amdgcn_exp2f(x.x - M);
+        total += w;
+        o += *reinterpret_cast<const v4f*>(a.part + (s * rows + r) * kN + 4 * lane) * w;
+    }
+    const float f = total == 0.f ? 0.f : 1.f / total;
+    uint16_t* const dst = a.out + (bi * a.H + a.h0 + hl) * kN;
+    reinterpret_cast<v2u_t*>(dst)[lane] = v2u_t{to_half2<TL>(o[0] * f, o[1] * f), to_half2<TL>(o[2] * f, o[3] * f)};
 }
 
 // ---- queries per head -----------------------------------------------------------------------
@@ -599,7 +667,19 @@ constexpr int64_t kExpandBytes = (int64_t)2 << 30;
 
 }  // namespace
 
-ExpandPlan plan_expand(int B, int Sk, int H, bool paged) {
+// Key splits of the attention: two workgroups a CU share the matrix cores' and the VALU's time, and a few
+// short ones wait for their first keys (kSplitTo below); MLA_EXPAND_SPLITS overrides the rule.
+int expand_splits(int64_t items, int units) {
+    if (const char* e = std::getenv("MLA_EXPAND_SPLITS")) {
+        const int n = std::atoi(e);
+        if (n >= 1) return std::min(n, 64);
+    }
+    constexpr int64_t kSplitTo = 4 * kNumCUs;
+    if (items > 2 * kNumCUs) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kSplitTo / items, 16), units / 2));
+}
+
+ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged) {
     ExpandPlan p;
     p.units = (Sk + kUnit - 1) / kUnit;
     const int64_t places = (int64_t)B * p.units;
@@ -614,6 +694,7 @@ ExpandPlan plan_expand(int B, int Sk, int H, bool paged) {
     p.off_owner = take(paged ? places * 4 : 0);
     p.off_rank = take(paged ? places * 4 : 0);
     p.off_count = take(paged ? (size_t)B * 4 : 0);
+    p.off_order = take(paged ? (size_t)B * 4 : 0);
     p.off_unit = take(places * 4);
     p.off_bad = take(places * 4);
     p.off_exps = take(places * 4);
@@ -621,6 +702,11 @@ ExpandPlan plan_expand(int B, int Sk, int H, bool paged) {
     p.off_lat = take((size_t)p.rows_cap * kR * 2);
     p.off_rot = take((size_t)p.rows_cap * kD * 2);
     p.off_kv = take((size_t)p.heads * p.rows_cap * 512);
+    const int64_t tiles = (Sq + kHRows - 1) / kHRows;
+    p.splits = expand_splits(tiles * B * p.heads, p.units);
+    const size_t rows = p.splits > 1 ? (size_t)p.splits * B * Sq * p.heads : 0;
+    p.off_part = take(rows * kN * 4);
+    p.off_state = take(rows * 8);
     p.total = o;
     return p;
 }
@@ -630,13 +716,13 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     auto ints = [&](size_t off) { return reinterpret_cast<int*>(ws + off); };
     auto half = [&](size_t off) { return reinterpret_cast<uint16_t*>(ws + off); };
     const int64_t tiles = (p.Sq + kHRows - 1) / kHRows;
-    if (p.B > 65535 || plan.rows_cap > 0x7fffffff || tiles * p.B * plan.heads > 0x7fffffff)
+    if (p.B > 65535 || plan.rows_cap > 0x7fffffff || tiles * p.B * plan.heads * plan.splits > 0x7fffffff)
         return hipErrorInvalidValue;
     int* any_bad = ints(plan.off_any);
     PlanArgs u;
     u.seq_lens = p.seq_lens; u.table = p.block_table;
     u.owner = ints(plan.off_owner); u.rank = ints(plan.off_rank); u.count = ints(plan.off_count);
-    u.any_bad = any_bad;
+    u.order = ints(plan.off_order); u.any_bad = any_bad;
     u.B = p.B; u.Sk = p.Sk; u.units = plan.units;
     u.max_pages = p.block_table ? p.Sk / p.page_size : 0;
     u.per_page = p.block_table ? p.page_size / kUnit : 1;
@@ -666,6 +752,10 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     a.kv = half(plan.off_kv); a.rot = g.rot;
     a.unit = g.unit; a.bad = g.bad; a.exps = g.exps; a.any_bad = any_bad;
     a.seq_lens = p.seq_lens; a.new_lens = p.new_lens;
+    a.order = p.block_table ? u.order : nullptr;
+    a.part = reinterpret_cast<float*>(ws + plan.off_part);
+    a.state = reinterpret_cast<float2*>(ws + plan.off_state);
+    a.splits = plan.splits;
     a.out = static_cast<uint16_t*>(p.out);
     a.B = p.B; a.Sq = p.Sq; a.Sk = p.Sk; a.H = p.H; a.units = plan.units;
     a.tiles = (int)tiles; a.causal = p.causal;
@@ -681,10 +771,20 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
         k.rows = g.rows; k.rows_cap = plan.rows_cap; k.heads = heads;
         e = launch_kv_expand(k, stream);
         if (e != hipSuccess) return e;
-        a.h0 = h0;
-        const dim3 grid((unsigned)(tiles * p.B * heads));
-        if (p.f16) hipLaunchKernelGGL(heads_kernel<f16_t>, grid, dim3(kHThreads), 0, stream, a);
-        else hipLaunchKernelGGL(heads_kernel<bf16_t>, grid, dim3(kHThreads), 0, stream, a);
+        a.h0 = h0; a.heads = heads;
+        const dim3 grid((unsigned)(tiles * p.B * heads * plan.splits)), block(kHThreads);
+        if (plan.splits > 1) {
+            if (p.f16) hipLaunchKernelGGL((heads_kernel<f16_t, true>), grid, block, 0, stream, a);
+            else hipLaunchKernelGGL((heads_kernel<bf16_t, true>), grid, block, 0, stream, a);
+            e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            const dim3 merge((unsigned)(((int64_t)p.B * p.Sq * heads + 7) / 8));
+            if (p.f16) hipLaunchKernelGGL(heads_merge_kernel<f16_t>, merge, dim3(256), 0, stream, a);
+            else hipLaunchKernelGGL(heads_merge_kernel<bf16_t>, merge, dim3(256), 0, stream, a);
+        } else {
+            if (p.f16) hipLaunchKernelGGL((heads_kernel<f16_t, false>), grid, block, 0, stream, a);
+            else hipLaunchKernelGGL((heads_kernel<bf16_t, false>), grid, block, 0, stream, a);
+        }
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

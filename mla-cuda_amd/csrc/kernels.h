@@ -408,9 +408,11 @@ struct ExpandPlan {
     int units = 0;                   // of a sequence, at most
     int64_t rows_cap = 0;            // rows of all of them
     int heads = 0;                   // expanded and attended to at a time
-    size_t off_owner, off_rank, off_count, off_unit, off_bad, off_exps, off_any, off_lat, off_rot, off_kv, total;
+    int splits = 1;                  // of the keys
+    size_t off_owner, off_rank, off_count, off_order, off_unit, off_bad, off_exps, off_any, off_lat, off_rot, off_kv,
+        off_part, off_state, total;
 };
-ExpandPlan plan_expand(int B, int Sk, int H, bool paged);
+ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged);
 hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* workspace, hipStream_t stream);
 // its product (bgemm.hip): kv [heads][rows_cap][256] from lat [rows][512]; *rows on the device
 struct KvExpand {

@@ -46,7 +46,23 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
 }
 
 __device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((int64_t)tokens + page - 1) / page); }
-__device__ __forceinline__ int ring_at(int head, int64_t i, int n) { return (int)((head + i) % n); }
+// place i past the ring's head, for head < n and i < n (or i = n: head again)
+__device__ __forceinline__ int ring_at(int head, int i, int n) {
+    const uint32_t p = (uint32_t)head + (uint32_t)i;
+    return (int)(p >= (uint32_t)n ? p - (uint32_t)n : p);
+}
+// this thread's kPer consecutive words of a range, in LDS
+struct Words { uint32_t w[kPer]; };
+__device__ __forceinline__ Words own_words(const uint32_t* words) {
+    Words x;
+    #pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+        const v4u_t v = *reinterpret_cast<const v4u_t*>(words + threadIdx.x * kPer + i);
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) x.w[i + k] = v[k];
+    }
+    return x;
+}
 
 // ---- fork -----------------------------------------------------------------------------------
 // Request b continues the first n = min(keep_lens[b], L[p]) tokens of request p = parents[b].  A
@@ -83,30 +99,59 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int b) {
     return {p, min(max(a.keep[b], 0), fork_len(a, p))};
 }
 
-// The words of pages [lo, lo + kRange), and how many of them nobody holds any more.
-__device__ __forceinline__ int fork_words(const ForkArgs& a, int lo, uint32_t* words, int* waves) {
+// The words of pages [lo, lo + kRange), and how many of them nobody holds any more.  A wave reads kRows
+// rows at a time, 128 entries of each, all loads before the first mark; rows[kThreads] is scratch.
+struct ForkMark { int src, have, whole, held; };
+__device__ __forceinline__ int fork_words(const ForkArgs& a, int lo, uint32_t* words, ForkMark* rows, int* waves) {
+    constexpr int kRows = 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int pages = min(kRange, a.num_pages - lo);
-    for (int i = tid; i < kRange; i += kThreads) words[i] = 0;
-    __syncthreads();
+    for (int i = tid; i < kRange / 4; i += kThreads) reinterpret_cast<v4u_t*>(words)[i] = v4u_t{0, 0, 0, 0};
     auto mark = [&](int page, uint32_t w) __attribute__((always_inline)) {
-        const uint32_t i = (uint32_t)(page - lo);
+        const uint32_t i = (uint32_t)page - (uint32_t)lo;
         if (page >= lo && i < (uint32_t)pages) atomicMax(&words[i], w);
     };
-    for (int b = wave; b < a.B; b += kWaves) {
-        const ForkRow r = fork_row(a, b);
-        const int have = pages_of(fork_len(a, b), a.page);
-        const int whole = r.n / a.page, open = r.n % a.page != 0;
-        const int* own = a.table + (int64_t)b * a.max_pages;
-        const int* from = a.table + (int64_t)r.src * a.max_pages;
-        for (int j = lane; j < max(have, whole + open); j += 64) {
-            if (j < have) mark(own[j], kHeld);
-            if (j < whole + open) mark(from[j], j < whole ? kWhole : kOpen - (uint32_t)b);
+    for (int c0 = 0; c0 < a.B; c0 += kThreads) {
+        const int nb = min(kThreads, a.B - c0);
+        __syncthreads();
+        if (tid < nb) {
+            const ForkRow r = fork_row(a, c0 + tid);
+            rows[tid] = {r.src, pages_of(fork_len(a, c0 + tid), a.page), r.n / a.page, pages_of(r.n, a.page)};
+        }
+        __syncthreads();
+        for (int r0 = wave; r0 < nb; r0 += kRows * kWaves) {
+            ForkMark m[kRows];
+            int most = 0;
+            #pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                m[k] = r0 + k * kWaves < nb ? rows[r0 + k * kWaves] : ForkMark{0, 0, 0, 0};
+                most = max(most, max(m[k].have, m[k].held));
+            }
+            for (int j0 = lane; j0 < most; j0 += 128) {
+                int own[kRows][2], from[kRows][2];
+                #pragma unroll
+                for (int k = 0; k < kRows; ++k)
+                    #pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = j0 + 64 * i;
+                        own[k][i] = j < m[k].have ? a.table[(int64_t)(c0 + r0 + k * kWaves) * a.max_pages + j] : -1;
+                        from[k][i] = j < m[k].held ? a.table[(int64_t)m[k].src * a.max_pages + j] : -1;
+                    }
+                #pragma unroll
+                for (int k = 0; k < kRows; ++k)
+                    #pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        mark(own[k][i], kHeld);
+                        mark(from[k][i], j0 + 64 * i < m[k].whole ? kWhole : kOpen - (uint32_t)(c0 + r0 + k * kWaves));
+                    }
+            }
         }
     }
     __syncthreads();
+    const Words x = own_words(words);
     int n = 0, total;
-    for (int i = 0; i < kPer; ++i) n += words[tid * kPer + i] == kHeld;
+    #pragma unroll
+    for (int i = 0; i < kPer; ++i) n += x.w[i] == kHeld;
     block_scan(n, waves, &total);
     return total;
 }
@@ -146,13 +191,16 @@ __device__ __forceinline__ void fork_write(const ForkArgs& a, int b, int src, in
 // The pages of a range that nobody holds any more, behind the ring's tail: `before` of them come first.
 __device__ __forceinline__ void fork_free(const ForkArgs& a, int lo, const uint32_t* words, int before,
                                           int head, int count, int* waves) {
-    const int at = threadIdx.x * kPer;
+    const Words x = own_words(words);
     int n = 0, total;
-    for (int i = 0; i < kPer; ++i) n += words[at + i] == kHeld;
+    #pragma unroll
+    for (int i = 0; i < kPer; ++i) n += x.w[i] == kHeld;
     int k = before + block_scan(n, waves, &total);
+    if (n == 0) return;
+    #pragma unroll
     for (int i = 0; i < kPer; ++i)
-        if (words[at + i] == kHeld) {
-            if (k < a.num_pages - count) a.ring[ring_at(head, (int64_t)count + k, a.num_pages)] = lo + at + i;
+        if (x.w[i] == kHeld) {
+            if (k < a.num_pages - count) a.ring[ring_at(head, count + k, a.num_pages)] = lo + threadIdx.x * kPer + i;
             ++k;
         }
 }
@@ -169,11 +217,12 @@ struct ForkInfo { int src, n, fresh; };
 // range frees.
 template <bool ONE>
 __global__ void __launch_bounds__(kThreads) fork_words_kernel(ForkArgs a) {
-    __shared__ uint32_t words[kRange];
+    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
     __shared__ int waves[kWaves];
+    __shared__ ForkMark rows[kThreads];
     __shared__ ForkInfo info[ONE ? kThreads : 1];
     const int tid = threadIdx.x, lo = blockIdx.x * kRange;
-    const int freed = fork_words(a, lo, words, waves);
+    const int freed = fork_words(a, lo, words, rows, waves);
     if (!ONE) {
         if (tid == 0) a.freed[blockIdx.x] = freed;
         for (int i = tid; i < min(kRange, a.num_pages - lo); i += kThreads) a.words[lo + i] = words[i];
@@ -200,7 +249,7 @@ __global__ void __launch_bounds__(kThreads) fork_words_kernel(ForkArgs a) {
 
 // Workgroups [0, ranges) free pages, the others write kWaves rows each.
 __global__ void __launch_bounds__(kThreads) fork_emit_kernel(ForkArgs a) {
-    __shared__ uint32_t words[kRange];
+    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
     __shared__ int waves[kWaves];
     __shared__ ForkInfo info[kWaves];
     const int tid = threadIdx.x;
@@ -272,18 +321,42 @@ __device__ __forceinline__ int2 compact_words(const CompactArgs& a, int lo, uint
         const uint32_t i = (uint32_t)(page - lo);
         if (page >= lo && i < (uint32_t)pages) atomicOr(&words[i], w);
     };
-    for (int b = wave; b < a.B; b += kWaves) {
-        const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
-        const int have = pages_of(len, a.page);
-        for (int j = lane; j < have; j += 64) mark(a.table[(int64_t)b * a.max_pages + j], kUsed);
+    constexpr int kRun = 8;
+    for (int b0 = wave; b0 < a.B; b0 += 4 * kWaves) {     // four rows at a time, 128 entries of each
+        int have[4], most = 0;
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int b = min(b0 + k * kWaves, a.B - 1);
+            const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
+            have[k] = b0 + k * kWaves < a.B ? pages_of(len, a.page) : 0;
+            most = max(most, have[k]);
+        }
+        for (int j0 = lane; j0 < most; j0 += 128) {
+            int p[kRun];
+            #pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                const int j = j0 + 64 * (k & 1);
+                p[k] = j < have[k >> 1] ? a.table[(int64_t)(b0 + (k >> 1) * kWaves) * a.max_pages + j] : -1;
+            }
+            #pragma unroll
+            for (int k = 0; k < kRun; ++k) mark(p[k], kUsed);
+        }
     }
-    for (int i = tid; i < count; i += kThreads) mark(a.ring[ring_at(head, i, a.num_pages)], kFree);
+    for (int i = tid; i < count; i += kRun * kThreads) {
+        int p[kRun];
+        #pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            p[k] = i + k * kThreads < count ? a.ring[ring_at(head, i + k * kThreads, a.num_pages)] : -1;
+        #pragma unroll
+        for (int k = 0; k < kRun; ++k) mark(p[k], kFree);
+    }
     __syncthreads();
+    const Words x = own_words(words);
     int used = 0, free = 0, all_used, all_free;
+    #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const uint32_t w = words[tid * kPer + i];
-        used += (w & kUsed) != 0;
-        free += w == kFree;
+        used += (x.w[i] & kUsed) != 0;
+        free += x.w[i] == kFree;
     }
     block_scan(used, waves, &all_used);
     block_scan(free, waves, &all_free);
@@ -294,53 +367,49 @@ struct CompactSums { int U, all, used, free; };   // held, held or free; held an
 
 // The cut, in the range whose words these are, with `s` its sums: the page, and the held pages in front
 // of it.  False in the threads that do not have it.
-template <class Word>
-__device__ __forceinline__ bool compact_cut(const CompactSums& s, int lo, int pages, Word word, int* waves,
+__device__ __forceinline__ bool compact_cut(const CompactSums& s, int lo, const Words& x, int* waves,
                                             int* page, int* used) {
-    const int at = threadIdx.x * kPer;
     int n = 0, m = 0, total;
+    #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const uint32_t w = at + i < pages ? word(at + i) : 0;
-        n += w != 0;
-        m += (w & kUsed) != 0;
+        n += x.w[i] != 0;
+        m += (x.w[i] & kUsed) != 0;
     }
     int rank = s.used + s.free + block_scan(n, waves, &total);
     int held = s.used + block_scan(m, waves, &total);
     if (rank > s.U || rank + n <= s.U) return false;
+    #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const uint32_t w = at + i < pages ? word(at + i) : 0;
-        if (w == 0) continue;
+        if (x.w[i] == 0) continue;
         if (rank == s.U) {
-            *page = lo + at + i;
+            *page = lo + threadIdx.x * kPer + i;
             *used = held;
-            return true;
         }
         ++rank;
-        held += (w & kUsed) != 0;
+        held += (x.w[i] & kUsed) != 0;
     }
-    return false;
+    return true;
 }
 
 // Moves and free pages of one range: hold(page, move) for a page that moves, hole(page, move) for one
 // that is moved to.
-template <class Word, class Hold, class Hole>
-__device__ __forceinline__ void compact_emit(const CompactArgs& a, const CompactSums& s, int lo, int pages,
-                                             int used_below, Word word, int* waves, Hold hold, Hole hole) {
-    const int at = threadIdx.x * kPer;
+template <class Hold, class Hole>
+__device__ __forceinline__ void compact_emit(const CompactArgs& a, const CompactSums& s, int lo, const Words& x,
+                                             int used_below, int* waves, Hold hold, Hole hole) {
     int n = 0, m = 0, total;
+    #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const uint32_t w = at + i < pages ? word(at + i) : 0;
-        n += (w & kUsed) != 0;
-        m += w == kFree;
+        n += (x.w[i] & kUsed) != 0;
+        m += x.w[i] == kFree;
     }
     int used = s.used + block_scan(n, waves, &total);
     int free = s.free + block_scan(m, waves, &total);
+    #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const uint32_t w = at + i < pages ? word(at + i) : 0;
-        if (w == 0) continue;
-        const int rank = used + free, p = lo + at + i;
+        if (x.w[i] == 0) continue;
+        const int rank = used + free, p = lo + threadIdx.x * kPer + i;
         if (rank >= s.U) a.ring_out[rank - s.U] = p;     // free after the call
-        if (w & kUsed) {
+        if (x.w[i] & kUsed) {
             if (rank >= s.U) hold(p, used - used_below);
             ++used;
         } else {
@@ -348,6 +417,15 @@ __device__ __forceinline__ void compact_emit(const CompactArgs& a, const Compact
             ++free;
         }
     }
+}
+// this thread's words of a range that compact_words_kernel left in memory
+__device__ __forceinline__ Words bytes_words(const uint8_t* w) {
+    static_assert(kPer == 16, "16 bytes a thread");
+    const v4u_t v = reinterpret_cast<const v4u_t*>(w)[threadIdx.x];
+    Words x;
+    #pragma unroll
+    for (int i = 0; i < kPer; ++i) x.w[i] = v[i >> 2] >> (8 * (i & 3)) & 0xffu;
+    return x;
 }
 
 // A row's entries through the moves, by a wave.
@@ -366,7 +444,7 @@ __device__ __forceinline__ void compact_row(const CompactArgs& a, int b, int cut
 }
 
 __global__ void __launch_bounds__(kThreads) compact_words_kernel(CompactArgs a) {
-    __shared__ uint32_t words[kRange];
+    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
     __shared__ int waves[kWaves];
     const int lo = blockIdx.x * kRange;
     const int2 s = compact_words(a, lo, words, waves);
@@ -380,6 +458,7 @@ __global__ void __launch_bounds__(kThreads) compact_emit_kernel(CompactArgs a) {
     __shared__ int waves[kWaves];
     __shared__ int cut_at[3];    // range of the cut, page, held pages in front of it
     const int tid = threadIdx.x, g = blockIdx.x;
+    const Words own = bytes_words(a.words + (int64_t)g * kRange);
     // sums in front of this range and in all, and the range of the cut
     CompactSums s = {0, 0, 0, 0}, c = {0, 0, 0, 0};
     int u = 0, f = 0, uu = 0, ff = 0;
@@ -424,8 +503,7 @@ __global__ void __launch_bounds__(kThreads) compact_emit_kernel(CompactArgs a) {
         c.free = cut_at[1] - cut_at[2];
         __syncthreads();
         int p, held;
-        const uint8_t* w = a.words + (int64_t)at * kRange;
-        if (compact_cut(c, at * kRange, kRange, [&](int i) { return (uint32_t)w[i]; }, waves, &p, &held)) {
+        if (compact_cut(c, at * kRange, bytes_words(a.words + (int64_t)at * kRange), waves, &p, &held)) {
             cut_at[1] = p;
             cut_at[2] = held;
         }
@@ -433,8 +511,7 @@ __global__ void __launch_bounds__(kThreads) compact_emit_kernel(CompactArgs a) {
         cut = cut_at[1];
         used_below = cut_at[2];
     }
-    const uint8_t* w = a.words + (int64_t)g * kRange;
-    compact_emit(a, s, g * kRange, kRange, used_below, [&](int i) { return (uint32_t)w[i]; }, waves,
+    compact_emit(a, s, g * kRange, own, used_below, waves,
                  [&](int p, int k) { a.to[p] = k; if (k < a.room) a.copies[2 * k] = p; },
                  [&](int p, int k) { if (k < a.room) a.copies[2 * k + 1] = p; });
     // what is past the moves and the free pages
@@ -458,7 +535,7 @@ __global__ void __launch_bounds__(256) compact_table_kernel(CompactArgs a) {
 
 // One range: all of it here, the moves in LDS.
 __global__ void __launch_bounds__(kThreads) compact_one_kernel(CompactArgs a) {
-    __shared__ uint32_t words[kRange];
+    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
     __shared__ int waves[kWaves], cut_at[2], holes[kRange / 2];
     const int tid = threadIdx.x;
     const int2 x = compact_words(a, 0, words, waves);
@@ -469,14 +546,15 @@ __global__ void __launch_bounds__(kThreads) compact_one_kernel(CompactArgs a) {
     }
     __syncthreads();
     int p, held;
-    if (compact_cut(s, 0, a.num_pages, [&](int i) { return words[i]; }, waves, &p, &held)) {
+    const Words own = own_words(words);
+    if (compact_cut(s, 0, own, waves, &p, &held)) {
         cut_at[0] = p;
         cut_at[1] = held;
     }
     __syncthreads();
     const int cut = cut_at[0], used_below = cut_at[1];
     // a page that moves keeps its move's number in its word, above the two bits
-    compact_emit(a, s, 0, a.num_pages, used_below, [&](int i) { return words[i] & 3u; }, waves,
+    compact_emit(a, s, 0, own, used_below, waves,
                  [&](int p, int k) { words[p] |= (uint32_t)k << 2; a.copies[2 * k] = p; },
                  [&](int p, int k) { holes[k] = p; a.copies[2 * k + 1] = p; });
     for (int k = s.U - used_below + tid; k < a.room; k += kThreads) a.copies[2 * k] = a.copies[2 * k + 1] = -1;

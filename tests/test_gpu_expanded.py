@@ -302,12 +302,26 @@ def test_head_groups(ext, dtype):
     """A span whose keys and values need several groups of heads."""
     H, Sq, n = 5, 130, 1000
     t = make(18, 1, Sq, [n], H, DT[dtype])
-    want = run_paged(ext, t, True)
     span = 1400000          # 2 GiB hold three heads of that many keys
     table = torch.zeros(1, span // 64, dtype=torch.int32, device=DEV)
     table[:, :t["table"].size(1)] = t["table"]
     t["table"] = table
-    assert torch.equal(run_paged(ext, t, True), want)
+    check_all(t, run_paged(ext, t, True), [n], True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("splits", [1, 2, 5, 64])
+def test_key_splits(ext, dtype, splits, monkeypatch):
+    """Any number of key splits, empty ones among them; NaN and padding rows through the merge."""
+    monkeypatch.setenv("MLA_EXPAND_SPLITS", str(splits))
+    lens, new, Sq = [700, 64, 10, 330], [150, 64, 0, 150], 150
+    t = make(22, 4, Sq, lens, 3, DT[dtype])
+    t["new"] = new
+    got = run_paged(ext, t, True, new)
+    check_all(t, got, lens, True, new)
+    t["c_kv"][t["table"][0, 10], 0] = NAN           # key 640: seen by queries from 90 on
+    hurt = run_paged(ext, t, True, new)
+    assert torch.equal(hurt[0, :90], got[0, :90]) and hurt[0, 90:].isnan().all() and torch.equal(hurt[1:], got[1:])
 
 
 def test_strided_and_other_stream(ext):
