@@ -23,6 +23,7 @@ namespace {
 
 typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
 typedef float v2f_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kUnit = kExpandUnit;            // rows a unit (and keys a step of the attention)
 constexpr int kR = 512, kD = 64, kN = 128;    // latent, rope, nope / value widths
@@ -325,11 +326,18 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
 // The reference of a row's exponentials moves only when a score passes it by kRise powers of two (few
 // do after the first step), and what is in the accumulators is scaled then.  They are fp16, as keys and
 // values are (the gather's comment): they start at 2^kBias, so that small ones keep more bits above
-// fp16's subnormals, and rise to 2^(kBias + kRise) < 65504.
+// fp16's subnormals, and rise to 2^(kBias + kRise) < 65504; their sum is of what is packed.
 // A unit's power of two is one number a step: its keys' goes into the factor of the scores, its values'
 // into the exponentials, as d = e - E <= 0 with the largest e so far in E (what is in the accumulators
 // is scaled when that grows); the sum takes it out again.  bf16 queries are made fp16 under a power of
 // two of their own.
+// What bounds it: the matrix cores' power and the order of two waves on a SIMD.  4,096 causal rows of 128 heads
+// 725 us, 948 TFLOP/s (a large fp16 library product 1,318); the cores are busy 0.46 of the cycles, and
+// with operands of zeros a fifth faster.  A step without the exponentials takes 6% less, without its loads
+// 10%.  Other structures, each on one card against this one: the next step's scores and the last one's
+// values between the exponentials of a step (+6%), the same with 64 rows a wave in 512 registers (+60%) or
+// eight waves a workgroup (+10%), loads between the score MFMAs (+12%), the MFMAs at a higher wave priority
+// (+1%), windows of 3 and 4 fragments (+0.3%, +1.5%), left to the compiler's order (+5%).
 struct HeadsArgs {
     const uint16_t* qn;      // [B, Sq, H, 128]
     const uint16_t* qr;      // [B, Sq, H, 64]
@@ -351,9 +359,11 @@ struct HeadsArgs {
 };
 
 constexpr int kHRows = 128, kHThreads = 256;
+constexpr int kWinK = 2, kWinV = 3;          // fragments read ahead (keys by pairs)
 constexpr int kKBytes = kUnit * 2 * kN, kRBytes = kUnit * 2 * kD;       // a stage's parts
-constexpr int kStageBytes = 2 * kKBytes + kRBytes;
-constexpr int kVAt = kKBytes, kRAt = 2 * kKBytes;
+constexpr int kKeyBytes = kKBytes + kRBytes;                            // keys: nope and rope columns
+constexpr int kSlice = kUnit * 64;
+constexpr int kStageBytes = kKeyBytes + kKBytes, kVAt = kKeyBytes;      // then values
 
 // Two outputs in their type.  An average of fp16 values up to 65504 stays there, also where its weights
 // are rounded up (a NaN is NaN).
@@ -447,42 +457,47 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             }
     }
 
-    // ---- staging.  Key rows of 256 bytes, 16-byte chunk c of row r at c ^ (r & 15); value rows of
-    // 256, chunk c at c ^ 4 (r & 3); rope rows of 128, chunk c at c ^ ((r >> 1) & 7).
+    // ---- staging, in slices of 64 bytes a row: a load is 16 rows of one, lane l chunk l % 4 of row
+    // l / 4.  Chunk c of a key or rope row r lies at c ^ ((r >> 2) & 3) (the 16 lanes of a ds_read_b128 cycle
+    // touch 16 different places of 256 bytes), values as they come (four rows of a transposing read are
+    // 256 bytes).  So a step's reads differ by constants, but for one bit in keys.
     const uint64_t kv = reinterpret_cast<uint64_t>(a.kv + hl * a.head_stride);
     const uint64_t rot = reinterpret_cast<uint64_t>(a.rot);
     const int* units = a.unit + (int64_t)b * a.units;
-    const uint32_t l4 = lane >> 4, l15 = lane & 15;
-    const uint32_t voff_k = (16 * wave + l4) * 512 + 16 * (l15 ^ l4);
-    const uint32_t voff_v = (16 * wave + l4) * 512 + 256 + 16 * (l15 ^ (4 * l4));
-    const uint32_t voff_r = (16 * wave + (lane >> 3)) * 128 + 16 * ((lane & 7) ^ l4);
+    const uint32_t r16 = 16 * wave + (lane >> 2), c_sw = 16 * ((lane & 3) ^ (lane >> 4));
+    const uint32_t voff_k = r16 * 512 + c_sw, voff_r = r16 * 128 + c_sw;
+    const uint32_t voff_v = r16 * 512 + 256 + 16 * (lane & 3);
     auto issue = [&](int place, uint32_t st) __attribute__((always_inline)) {
         const v4i rk = rsrc_span(kv + (uint64_t)place * (kUnit * 512), 0, kUnit * 512);
         const v4i rr = rsrc_span(rot + (uint64_t)place * (kUnit * 128), 0, kUnit * 128);
-        const uint32_t base = __builtin_amdgcn_readfirstlane(lds0 + st + 16 * wave * 256);
+        const uint32_t base = __builtin_amdgcn_readfirstlane(lds0 + st + 1024 * wave);
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            dma16(rk, base + 1024 * i, (voff_k + 2048 * i) ^ (64 * i));
-            dma16(rk, base + kVAt + 1024 * i, voff_v + 2048 * i);
-        }
-        const uint32_t rbase = __builtin_amdgcn_readfirstlane(lds0 + st + kRAt + 16 * wave * 128);
+        for (int i = 0; i < 6; ++i) dma16(i < 4 ? rk : rr, base + kSlice * i, i < 4 ? voff_k + 64 * i : voff_r + 64 * (i - 4));
         #pragma unroll
-        for (int i = 0; i < 2; ++i) dma16(rr, rbase + 1024 * i, (voff_r + 1024 * i) ^ (64 * i));
+        for (int i = 0; i < 4; ++i) dma16(rk, base + kVAt + kSlice * i, voff_v + 64 * i);
     };
 
     // ---- fragments
-    const uint32_t k_rd = (uint32_t)q * 256 + 16 * (hi ^ (q & 15));
-    const uint32_t r_rd = kRAt + (uint32_t)q * 128 + 16 * (hi ^ ((q >> 1) & 7));
+    const uint32_t k_rd = (uint32_t)q * 64 + 16 * (hi ^ ((q >> 2) & 3));
     const int G4 = lane >> 4, q4 = (lane >> 2) & 3, i4 = lane & 3;
-    const uint32_t v_rd = kVAt + (uint32_t)(4 * (G4 >> 1) + q4) * 256 +
-                          16 * ((2 * (G4 & 1) + (i4 >> 1)) ^ (4 * q4)) + 8 * (i4 & 1);
+    const uint32_t v_rd = (uint32_t)(4 * (G4 >> 1) + q4) * 64 + 32 * (G4 & 1) + 8 * i4;
     typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
+    auto k_frag = [&](uint32_t st, int kb, int i) __attribute__((always_inline)) {   // i: 16 of 192 columns
+        return *reinterpret_cast<const v4u*>(smem + st + kSlice * (i >> 1) + 2048 * kb + (k_rd ^ (32 * (i & 1))));
+    };
+    auto v_frag = [&](uint32_t st, int i) __attribute__((always_inline)) {   // i: 4 * (16 keys) + columns
+        const uint8_t* at = smem + st + kVAt + kSlice * (i & 3) + 1024 * (i >> 2) + v_rd;
+        const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 512));
+        return __builtin_bit_cast(v4u, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
 
     v16f o[4];
     #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = v16f{};
     float m_ref = -INFINITY, l = 0.f;
+    const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
 
     int next = n_tiles > first ? load_uniform(units + first) : 0;
     int e_next = n_tiles > first ? load_uniform(a.exps + next) : 0;
@@ -501,36 +516,30 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             next = j + 2 < n_tiles ? load_uniform(units + j + 2) : 0;
         }
         if (j * kUnit > wave_last) continue;
+        // scores; a fragment's place is read again as soon as it is used
         v16f s[2] = {v16f{}, v16f{}};
+        v4u kf[kWinK][2];
         #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                s[kb] = Mma<f16_t>::sub(*reinterpret_cast<const v4u*>(smem + st + 8192 * kb + (k_rd ^ (32 * i))),
-                                     qf[i], 0, s[kb]);
+        for (int i = 0; i < kWinK; ++i) { kf[i][0] = k_frag(st, 0, i); kf[i][1] = k_frag(st, 1, i); }
         #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 12; ++i) {
             #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                s[kb] = Mma<f16_t>::sub(*reinterpret_cast<const v4u*>(smem + st + 4096 * kb + (r_rd ^ (32 * i))),
-                                     qf[8 + i], 0, s[kb]);
-        if (j * kUnit + kUnit - 1 > wave_first) {
+            for (int kb = 0; kb < 2; ++kb) {
+                s[kb] = Mma<f16_t>::sub(kf[i % kWinK][kb], qf[i], 0, s[kb]);
+                if (i + kWinK < 12) kf[i % kWinK][kb] = k_frag(st, kb, i + kWinK);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (j * kUnit + kUnit - 1 > wave_first) {     // (opaque: 32 differences are not to stay in registers)
+            int past = lim - j * kUnit - 4 * hi;
+            asm volatile("" : "+v"(past));
             #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[kb][i] = j * kUnit + 32 * kb + acc_row(i, lane) <= lim ? s[kb][i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + acc_row(i, 0) <= past ? s[kb][i] : -INFINITY;
         }
+        // weights
         const float ct = c * two_to(e);
-        float top = s[0][0];
-        #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
-        #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
-        {
-            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * ct;
-        }
         if (e > E) {
             const float f = e - E > 126 ? 0.f : two_to(E - e);
             E = e;
@@ -539,9 +548,16 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[i][k] *= f;
         }
-        // (only those rows: a row's bits do not depend on the others of its wave)
-        const bool over = top > m_ref + kRise;
-        if (__builtin_amdgcn_ballot_w64(over)) {
+        float top = fmaxf(s[0][0], s[0][1]);
+        #pragma unroll
+        for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(s[0][i], s[0][i + 1]), top);
+        #pragma unroll
+        for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(s[1][i], s[1][i + 1]), top);
+        // (rows whose scores passed their reference only: a row's bits do not depend on the others of its wave)
+        if (__builtin_amdgcn_ballot_w64(top * ct > m_ref + kRise)) {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * ct;
+            const bool over = top > m_ref + kRise;
             const float m = over ? top : m_ref;
             const float f = over ? __builtin_amdgcn_exp2f(m_ref - m) : 1.f;
             m_ref = m;
@@ -549,33 +565,39 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             #pragma unroll
             for (int i = 0; i < 4; ++i)
                 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[i][e] *= f;
+                for (int k = 0; k < 16; ++k) o[i][k] *= f;
         }
         const int d = max(e - E, -100);
         const float neg = (m_ref == -INFINITY ? 0.f : kBias - m_ref) + (float)d;
+        v4u vf[kWinV];
+        #pragma unroll
+        for (int i = 0; i < kWinV; ++i) vf[i] = v_frag(st, i);
+        v4u p[4];
         float sum = 0.f;
         #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int i = 0; i < 16; ++i) {
+            const int kb = i >> 3, k = 2 * (i & 7);
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k], ct, neg));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k + 1], ct, neg));
+            s[kb][k] = x; s[kb][k + 1] = y;
+            const uint32_t w = pack_f16x2(x, y);
+            p[i >> 2][i & 3] = w;
+            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, w), ones, sum, false);
+        }
+        if (d < -8) {        // a unit of far smaller values: its weights' sum is not to go under fp16's end
+            sum = 0.f;
             #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], ct, neg));
-                sum += s[kb][i];
-            }
+            for (int kb = 0; kb < 2; ++kb)
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) sum += s[kb][i];
+        }
         l += sum * two_to(-d);
+        // values
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {       // 16 keys
-            v4u p;
-            #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                p[k] = pack_f16x2(s[i >> 1][8 * (i & 1) + 2 * k], s[i >> 1][8 * (i & 1) + 2 * k + 1]);
-            #pragma unroll
-            for (int vb = 0; vb < 4; ++vb) {
-                const uint8_t* at = smem + st + 4096 * i + (v_rd ^ (64 * vb));
-                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
-                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 2048));
-                o[vb] = Mma<f16_t>::sub(__builtin_bit_cast(v4u, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)),
-                                     p, 0, o[vb]);
-            }
+        for (int i = 0; i < 16; ++i) {
+            o[i & 3] = Mma<f16_t>::sub(vf[i % kWinV], p[i >> 2], 0, o[i & 3]);
+            if (i + kWinV < 16) vf[i % kWinV] = v_frag(st, i + kWinV);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
