@@ -134,6 +134,7 @@ struct GatherArgs {
     const uint8_t* scales;
     const int* seq_lens;     // null: every sequence has Sk keys
     const int* table;        // null: [B, Sk] rows
+    int planned;             // whether the plan ran (else every sequence has its units in its own places)
     const int* owner;
     const int* rank;
     const int* count;
@@ -184,9 +185,9 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
     const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.Sk) : a.Sk;
     const bool first = j == 0 && b == 0;
     const bool here = j * kUnit < len;
-    if (!here && !first) return;
+    if (!here && !first) return;     // the first workgroup leaves the number of rows, whatever it has
     int place = b * a.units + j, own = b;
-    if (a.table) {
+    if (a.planned) {
         const int at = place;
         own = here ? a.owner[at] : 0;
         // units of the sequences in front of the owner; the first workgroup also adds up all of them
@@ -212,9 +213,11 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
         if (tid == 0) a.unit[at] = place;
         if (own != b) return;
     } else if (tid == 0) {
-        a.unit[place] = place;
-        if (first) *a.rows = kUnit * a.B * a.units;
+        if (here) a.unit[place] = place;
+        if (first) *a.rows = a.B == 1 ? (len + kUnit - 1) / kUnit * kUnit : kUnit * a.B * a.units;
     }
+
+    if (!here) return;
 
     // where the unit's rows lie (a page is a whole number of units)
     const int k0 = j * kUnit;
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
     if (tid == 0) {
         a.exps[place] = e;
         a.bad[place] = worst;
-        if (worst < kUnit) *a.any_bad = 1;   // cleared by the plan; every writer writes the same
+        if (a.any_bad && worst < kUnit) *a.any_bad = 1;   // cleared by the plan; every writer writes the same
     }
     #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -346,7 +349,7 @@ struct HeadsArgs {
     const int* unit;
     const int* bad;
     const int* exps;
-    const int* any_bad;
+    const int* any_bad;      // null: look for yourself
     const int* seq_lens;
     const int* new_lens;
     const int* order;        // null: as they come
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     }
     float f = l == 0.f ? 0.f : two_to(E) / l;
-    if (load_uniform(a.any_bad)) {
+    if (!a.any_bad || load_uniform(a.any_bad)) {
         int worst = 0x7fffffff;
         for (int j = first + lane; j < n_tiles; j += 64) {
             const int r = a.bad[units[j]];
@@ -689,16 +692,16 @@ constexpr int64_t kExpandBytes = (int64_t)2 << 30;
 
 }  // namespace
 
-// Key splits of the attention: two workgroups a CU share the matrix cores' and the VALU's time, and a few
-// short ones wait for their first keys (kSplitTo below); MLA_EXPAND_SPLITS overrides the rule.
+// Key splits of the attention, where its workgroups are fewer than two a CU (which share the matrix cores' and
+// the VALU's time): 256 of them over 512 units 1,023 us unsplit, 836 in 2, 871 in 3, 836 in 4.  A
+// share is at least 8 units: 128 workgroups over 8 units 51.1 us unsplit, 52.0 in 2, 54.8 in 4.
+// MLA_EXPAND_SPLITS overrides the rule.
 int expand_splits(int64_t items, int units) {
     if (const char* e = std::getenv("MLA_EXPAND_SPLITS")) {
         const int n = std::atoi(e);
         if (n >= 1) return std::min(n, 64);
     }
-    constexpr int64_t kSplitTo = 4 * kNumCUs;
-    if (items > 2 * kNumCUs) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kSplitTo / items, 16), units / 2));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * kNumCUs / items, 16), units / 8));
 }
 
 ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged) {
@@ -748,12 +751,15 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     u.B = p.B; u.Sk = p.Sk; u.units = plan.units;
     u.max_pages = p.block_table ? p.Sk / p.page_size : 0;
     u.per_page = p.block_table ? p.page_size / kUnit : 1;
-    hipLaunchKernelGGL(expand_plan_kernel, dim3(p.block_table ? p.B : 1), dim3(kPlanThreads), 0, stream, u);
+    // one sequence shares nothing; of up to 64 units a lane of the attention looks each up for itself
+    const bool alone = p.B == 1 && plan.units <= kWave;
+    if (!alone) hipLaunchKernelGGL(expand_plan_kernel, dim3(p.block_table ? p.B : 1), dim3(kPlanThreads), 0, stream, u);
     GatherArgs g;
     g.c_kv = p.c_kv; g.pe = p.pe; g.scales = static_cast<const uint8_t*>(p.scales);
     g.seq_lens = p.seq_lens; g.table = p.block_table;
     g.owner = u.owner; g.rank = u.rank; g.count = u.count;
-    g.unit = ints(plan.off_unit); g.bad = ints(plan.off_bad); g.exps = ints(plan.off_exps); g.any_bad = any_bad; g.rows = any_bad + 1;
+    g.unit = ints(plan.off_unit); g.bad = ints(plan.off_bad); g.exps = ints(plan.off_exps); g.rows = any_bad + 1;
+    g.any_bad = alone ? nullptr : any_bad; g.planned = p.block_table && p.B > 1;
     g.lat = half(plan.off_lat); g.rot = half(plan.off_rot);
     g.B = p.B; g.Sk = p.Sk; g.units = plan.units;
     g.page_size = p.page_size; g.max_pages = u.max_pages; g.num_pages = p.num_pages;
@@ -772,9 +778,9 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     HeadsArgs a;
     a.qn = static_cast<const uint16_t*>(p.q_nope); a.qr = static_cast<const uint16_t*>(p.q_rope);
     a.kv = half(plan.off_kv); a.rot = g.rot;
-    a.unit = g.unit; a.bad = g.bad; a.exps = g.exps; a.any_bad = any_bad;
+    a.unit = g.unit; a.bad = g.bad; a.exps = g.exps; a.any_bad = g.any_bad;
     a.seq_lens = p.seq_lens; a.new_lens = p.new_lens;
-    a.order = p.block_table ? u.order : nullptr;
+    a.order = p.block_table && p.B > 1 ? u.order : nullptr;
     a.part = reinterpret_cast<float*>(ws + plan.off_part);
     a.state = reinterpret_cast<float2*>(ws + plan.off_state);
     a.splits = plan.splits;

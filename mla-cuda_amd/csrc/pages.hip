@@ -23,7 +23,8 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kRange = kPageRange;            // pages a workgroup owns
 constexpr int kPer = kRange / kThreads;       // consecutive ones a thread
 
-// Sum over the threads in front of this one; *total that over all.
+// Sum over the threads in front of this one of a workgroup of W waves; *total that over all.
+template <int W = kWaves>
 __device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int s = v;
@@ -37,7 +38,8 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
     if (lane == 63) waves[wave] = s;
     __syncthreads();
     int before = s - v, all = 0;
-    for (int w = 0; w < kWaves; ++w) {
+    #pragma unroll
+    for (int w = 0; w < W; ++w) {
         if (w < wave) before += waves[w];
         all += waves[w];
     }
@@ -303,8 +305,9 @@ struct CompactArgs {
     int* ring_out;
     int* state_out;
     int* copies;             // [room][2]
-    uint8_t* words;          // [ranges * kRange] (past one range)
-    int2* sums;              // [ranges] {used, free}
+    uint8_t* used;           // [ranges * kPart] past one workgroup's range: whether a page is held,
+    uint8_t* free;           // and whether the ring has it
+    int2* sums;              // [ranges] {held, free} pages of each kPart
     int* to;                 // [num_pages] which move a page is
     int* cut;                // the first page that is not among the first U
     int B, page, max_pages, num_pages, ranges, room;
@@ -367,6 +370,7 @@ struct CompactSums { int U, all, used, free; };   // held, held or free; held an
 
 // The cut, in the range whose words these are, with `s` its sums: the page, and the held pages in front
 // of it.  False in the threads that do not have it.
+template <int W>
 __device__ __forceinline__ bool compact_cut(const CompactSums& s, int lo, const Words& x, int* waves,
                                             int* page, int* used) {
     int n = 0, m = 0, total;
@@ -375,8 +379,8 @@ __device__ __forceinline__ bool compact_cut(const CompactSums& s, int lo, const 
         n += x.w[i] != 0;
         m += (x.w[i] & kUsed) != 0;
     }
-    int rank = s.used + s.free + block_scan(n, waves, &total);
-    int held = s.used + block_scan(m, waves, &total);
+    int rank = s.used + s.free + block_scan<W>(n, waves, &total);
+    int held = s.used + block_scan<W>(m, waves, &total);
     if (rank > s.U || rank + n <= s.U) return false;
     #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -393,7 +397,7 @@ __device__ __forceinline__ bool compact_cut(const CompactSums& s, int lo, const 
 
 // Moves and free pages of one range: hold(page, move) for a page that moves, hole(page, move) for one
 // that is moved to.
-template <class Hold, class Hole>
+template <int W, class Hold, class Hole>
 __device__ __forceinline__ void compact_emit(const CompactArgs& a, const CompactSums& s, int lo, const Words& x,
                                              int used_below, int* waves, Hold hold, Hole hole) {
     int n = 0, m = 0, total;
@@ -402,8 +406,8 @@ __device__ __forceinline__ void compact_emit(const CompactArgs& a, const Compact
         n += (x.w[i] & kUsed) != 0;
         m += x.w[i] == kFree;
     }
-    int used = s.used + block_scan(n, waves, &total);
-    int free = s.free + block_scan(m, waves, &total);
+    int used = s.used + block_scan<W>(n, waves, &total);
+    int free = s.free + block_scan<W>(m, waves, &total);
     #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         if (x.w[i] == 0) continue;
@@ -418,16 +422,6 @@ __device__ __forceinline__ void compact_emit(const CompactArgs& a, const Compact
         }
     }
 }
-// this thread's words of a range that compact_words_kernel left in memory
-__device__ __forceinline__ Words bytes_words(const uint8_t* w) {
-    static_assert(kPer == 16, "16 bytes a thread");
-    const v4u_t v = reinterpret_cast<const v4u_t*>(w)[threadIdx.x];
-    Words x;
-    #pragma unroll
-    for (int i = 0; i < kPer; ++i) x.w[i] = v[i >> 2] >> (8 * (i & 3)) & 0xffu;
-    return x;
-}
-
 // A row's entries through the moves, by a wave.
 template <class To>
 __device__ __forceinline__ void compact_row(const CompactArgs& a, int b, int cut, To to) {
@@ -443,36 +437,85 @@ __device__ __forceinline__ void compact_row(const CompactArgs& a, int b, int cut
     }
 }
 
-__global__ void __launch_bounds__(kThreads) compact_words_kernel(CompactArgs a) {
-    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
-    __shared__ int waves[kWaves];
-    const int lo = blockIdx.x * kRange;
-    const int2 s = compact_words(a, lo, words, waves);
-    if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
-    for (int i = threadIdx.x; i < kRange / 4; i += kThreads)
-        reinterpret_cast<uint32_t*>(a.words + (int64_t)lo)[i] =
-            words[4 * i] | words[4 * i + 1] << 8 | words[4 * i + 2] << 16 | words[4 * i + 3] << 24;
+// A large pool, in parts of kPart pages: bytes a page, written plainly (all writers write 1), then sums,
+// then the moves.
+constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64, kPart = kPartThreads * kPer;
+
+__global__ void __launch_bounds__(256) compact_clear_kernel(v4u_t* p, int64_t n) {
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = v4u_t{0, 0, 0, 0};
 }
 
-__global__ void __launch_bounds__(kThreads) compact_emit_kernel(CompactArgs a) {
-    __shared__ int waves[kWaves];
+// A wave marks a row of the table, and a workgroup its share of the ring.
+__global__ void __launch_bounds__(256) compact_mark_kernel(CompactArgs a) {
+    const int lane = threadIdx.x & 63;
+    constexpr int kRun = 8;
+    for (int b = blockIdx.x * 4 + (threadIdx.x >> 6); b < a.B; b += gridDim.x * 4) {
+        const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
+        const int have = pages_of(len, a.page);
+        for (int j = lane; j < have; j += kRun * 64) {
+            int p[kRun];
+            #pragma unroll
+            for (int k = 0; k < kRun; ++k) p[k] = j + 64 * k < have ? a.table[(int64_t)b * a.max_pages + j + 64 * k] : -1;
+            #pragma unroll
+            for (int k = 0; k < kRun; ++k)
+                if (p[k] >= 0 && p[k] < a.num_pages) a.used[p[k]] = 1;
+        }
+    }
+    int head, count;
+    ring_state(a.state, a.num_pages, &head, &count);
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) {
+        const int p = a.ring[ring_at(head, i, a.num_pages)];
+        if (p >= 0 && p < a.num_pages) a.free[p] = 1;
+    }
+}
+
+// this thread's words of part g
+__device__ __forceinline__ Words part_words(const CompactArgs& a, int g) {
+    static_assert(kPer == 16, "16 bytes a thread");
+    const int64_t at = (int64_t)g * kPartThreads + threadIdx.x;
+    const v4u_t u = reinterpret_cast<const v4u_t*>(a.used)[at], f = reinterpret_cast<const v4u_t*>(a.free)[at];
+    Words x;
+    #pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t held = u[i >> 2] >> (8 * (i & 3)) & 1u;
+        x.w[i] = held ? kUsed : (f[i >> 2] >> (8 * (i & 3)) & 1u) * kFree;
+    }
+    return x;
+}
+
+__global__ void __launch_bounds__(kPartThreads) compact_sums_kernel(CompactArgs a) {
+    __shared__ int waves[kPartWaves];
+    const Words x = part_words(a, blockIdx.x);
+    int used = 0, free = 0, all_used, all_free;
+    #pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        used += x.w[i] == kUsed;
+        free += x.w[i] == kFree;
+    }
+    block_scan<kPartWaves>(used, waves, &all_used);
+    block_scan<kPartWaves>(free, waves, &all_free);
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = make_int2(all_used, all_free);
+}
+
+__global__ void __launch_bounds__(kPartThreads) compact_emit_kernel(CompactArgs a) {
+    __shared__ int waves[kPartWaves];
     __shared__ int cut_at[3];    // range of the cut, page, held pages in front of it
     const int tid = threadIdx.x, g = blockIdx.x;
-    const Words own = bytes_words(a.words + (int64_t)g * kRange);
+    const Words own = part_words(a, g);
     // sums in front of this range and in all, and the range of the cut
     CompactSums s = {0, 0, 0, 0}, c = {0, 0, 0, 0};
     int u = 0, f = 0, uu = 0, ff = 0;
-    for (int r = tid; r < a.ranges; r += kThreads) {
+    for (int r = tid; r < a.ranges; r += kPartThreads) {
         const int2 x = a.sums[r];
         uu += x.x;
         ff += x.y;
         if (r < g) { u += x.x; f += x.y; }
     }
     int total;
-    block_scan(u, waves, &s.used);
-    block_scan(f, waves, &s.free);
-    block_scan(uu, waves, &s.U);
-    block_scan(ff, waves, &total);
+    block_scan<kPartWaves>(u, waves, &s.used);
+    block_scan<kPartWaves>(f, waves, &s.free);
+    block_scan<kPartWaves>(uu, waves, &s.U);
+    block_scan<kPartWaves>(ff, waves, &total);
     s.all = s.U + total;
     if (tid == 0) cut_at[0] = -1;
     int base = 0, used = 0;      // by one wave, 64 ranges at a time
@@ -503,7 +546,7 @@ __global__ void __launch_bounds__(kThreads) compact_emit_kernel(CompactArgs a) {
         c.free = cut_at[1] - cut_at[2];
         __syncthreads();
         int p, held;
-        if (compact_cut(c, at * kRange, bytes_words(a.words + (int64_t)at * kRange), waves, &p, &held)) {
+        if (compact_cut<kPartWaves>(c, at * kPart, part_words(a, at), waves, &p, &held)) {
             cut_at[1] = p;
             cut_at[2] = held;
         }
@@ -511,14 +554,14 @@ __global__ void __launch_bounds__(kThreads) compact_emit_kernel(CompactArgs a) {
         cut = cut_at[1];
         used_below = cut_at[2];
     }
-    compact_emit(a, s, g * kRange, own, used_below, waves,
+    compact_emit<kPartWaves>(a, s, g * kPart, own, used_below, waves,
                  [&](int p, int k) { a.to[p] = k; if (k < a.room) a.copies[2 * k] = p; },
                  [&](int p, int k) { if (k < a.room) a.copies[2 * k + 1] = p; });
     // what is past the moves and the free pages
     const int moves = s.U - used_below, left = s.all - s.U;
-    for (int64_t k = moves + (int64_t)g * kThreads + tid; k < a.room; k += (int64_t)a.ranges * kThreads)
+    for (int64_t k = moves + (int64_t)g * kPartThreads + tid; k < a.room; k += (int64_t)a.ranges * kPartThreads)
         a.copies[2 * k] = a.copies[2 * k + 1] = -1;
-    for (int64_t k = left + (int64_t)g * kThreads + tid; k < a.num_pages; k += (int64_t)a.ranges * kThreads)
+    for (int64_t k = left + (int64_t)g * kPartThreads + tid; k < a.num_pages; k += (int64_t)a.ranges * kPartThreads)
         a.ring_out[k] = -1;
     if (g == 0 && tid == 0) {
         a.state_out[0] = 0;
@@ -547,14 +590,14 @@ __global__ void __launch_bounds__(kThreads) compact_one_kernel(CompactArgs a) {
     __syncthreads();
     int p, held;
     const Words own = own_words(words);
-    if (compact_cut(s, 0, own, waves, &p, &held)) {
+    if (compact_cut<kWaves>(s, 0, own, waves, &p, &held)) {
         cut_at[0] = p;
         cut_at[1] = held;
     }
     __syncthreads();
     const int cut = cut_at[0], used_below = cut_at[1];
     // a page that moves keeps its move's number in its word, above the two bits
-    compact_emit(a, s, 0, own, used_below, waves,
+    compact_emit<kWaves>(a, s, 0, own, used_below, waves,
                  [&](int p, int k) { words[p] |= (uint32_t)k << 2; a.copies[2 * k] = p; },
                  [&](int p, int k) { holes[k] = p; a.copies[2 * k + 1] = p; });
     for (int k = s.U - used_below + tid; k < a.room; k += kThreads) a.copies[2 * k] = a.copies[2 * k + 1] = -1;
@@ -655,8 +698,8 @@ hipError_t launch_cache_fork(const CacheFork& p, void* workspace, hipStream_t st
 
 size_t cache_compact_workspace(int num_pages) {
     if (num_pages <= kRange) return 0;
-    const size_t r = ranges_of(num_pages);
-    return r * kRange + r * 8 + (size_t)num_pages * 4 + 4;
+    const size_t parts = ((size_t)num_pages + kPart - 1) / kPart;
+    return 2 * parts * kPart + parts * 8 + (size_t)num_pages * 4 + 4;
 }
 
 hipError_t launch_cache_compact(const CacheCompact& p, void* workspace, hipStream_t stream) {
@@ -665,24 +708,27 @@ hipError_t launch_cache_compact(const CacheCompact& p, void* workspace, hipStrea
     a.table_out = p.block_table_out; a.ring_out = p.free_pages_out; a.state_out = p.free_state_out;
     a.copies = p.copies;
     a.B = p.B; a.page = p.page_size; a.max_pages = p.max_pages; a.num_pages = p.num_pages;
-    a.ranges = ranges_of(p.num_pages);
     a.room = std::max(1, p.num_pages / 2);
-    a.words = static_cast<uint8_t*>(workspace);
-    a.sums = reinterpret_cast<int2*>(a.words + (size_t)a.ranges * kRange);
+    a.ranges = (int)(((int64_t)p.num_pages + kPart - 1) / kPart);
+    const size_t bytes = (size_t)a.ranges * kPart;
+    a.used = static_cast<uint8_t*>(workspace);
+    a.free = a.used + bytes;
+    a.sums = reinterpret_cast<int2*>(a.free + bytes);
     a.to = reinterpret_cast<int*>(a.sums + a.ranges);
     a.cut = a.to + p.num_pages;
     if (p.num_pages <= kRange) {
         hipLaunchKernelGGL(compact_one_kernel, dim3(1), dim3(kThreads), 0, stream, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(compact_words_kernel, dim3((unsigned)a.ranges), dim3(kThreads), 0, stream, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(compact_emit_kernel, dim3((unsigned)a.ranges), dim3(kThreads), 0, stream, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(compact_table_kernel, dim3((unsigned)std::min((p.B + 3) / 4, 8 * kNumCUs)), dim3(256), 0,
-                       stream, a);
+    const int64_t chunks = (int64_t)(2 * bytes / 16);
+    const unsigned rows = (unsigned)std::min((p.B + 3) / 4, 8 * kNumCUs);
+    const unsigned ring = (unsigned)std::min<int64_t>(((int64_t)p.num_pages + 1023) / 1024, 8 * kNumCUs);
+    hipLaunchKernelGGL(compact_clear_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 8 * kNumCUs)), dim3(256),
+                       0, stream, reinterpret_cast<v4u_t*>(workspace), chunks);
+    hipLaunchKernelGGL(compact_mark_kernel, dim3(std::max(rows, ring)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(compact_sums_kernel, dim3((unsigned)a.ranges), dim3(kPartThreads), 0, stream, a);
+    hipLaunchKernelGGL(compact_emit_kernel, dim3((unsigned)a.ranges), dim3(kPartThreads), 0, stream, a);
+    hipLaunchKernelGGL(compact_table_kernel, dim3(rows), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
