@@ -463,7 +463,7 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
  * its own and only whole pages are shared, so that mla_cache_extend may let requests grow (new_lens
  * > 0) and appends may write; while rows share pages, tokens are dropped and requests ended by
  * mla_cache_fork (mla_cache_extend would give a shared page back).  Tables, ring, sizes and limits as
- * in mla_cache_extend; batch is at most 2^24.
+ * in mla_cache_extend; batch is at most 2^16.
  *
  * Fork: request b becomes the first n = min(max(keep_lens[b], 0), L) tokens of request parents[b] as
  * it was before the call, of L tokens (clamped as there; n = 0 if parents[b] is outside [0, batch)).

@@ -835,7 +835,7 @@ int check_fp8blk_attn(mla_dtype_t dtype, const mla_dims_t* d, int causal, int32_
     return MLA_OK;
 }
 
-// Tables of requests that share pages: mla_cache_extend's limits, and a batch that a word per page can name.
+// Tables of requests that share pages: mla_cache_extend's limits, and those of the batch and the pool.
 int check_page_tables(int32_t batch, int32_t page_size, int32_t max_pages, int32_t num_pages) {
     MLA_CHECK(check_pos(batch, "batch"));
     MLA_CHECK(check_pos(max_pages, "max_pages"));
@@ -843,8 +843,8 @@ int check_page_tables(int32_t batch, int32_t page_size, int32_t max_pages, int32
     if (page_size <= 0 || page_size % 64 != 0)
         return fail(MLA_ERR_INVALID_ARGUMENT, "page_size must be a positive multiple of 64 (got %d)",
                     page_size);
-    if (batch > (1 << 24) || num_pages > (1 << 30))
-        return fail(MLA_ERR_INVALID_ARGUMENT, "batch must be at most 2^24 and num_pages at most 2^30");
+    if (batch > (1 << 16) || num_pages > (1 << 30))   // (a workgroup for each few rows plans all of them)
+        return fail(MLA_ERR_INVALID_ARGUMENT, "batch must be at most 2^16 and num_pages at most 2^30");
     if ((int64_t)max_pages * page_size > kMaxI32 || (int64_t)batch * max_pages > kMaxI32)
         return fail(MLA_ERR_INVALID_ARGUMENT, "max_pages * page_size and batch * max_pages must be "
                     "below 2^31");

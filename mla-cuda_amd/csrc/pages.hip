@@ -3,10 +3,8 @@
 // of cache8.hip's extend; a page is held by every table row that names it among its request's pages,
 // so that who holds what follows from the tables alone and nothing is counted between calls.
 //
-// What follows from all holders of a page is made by the workgroup that owns the page's range of the
-// pool: it reads the whole table and keeps a word a page in LDS, so that no memory has to be cleared
-// and no order of atomics shows in a result.  Past one range (a large pool) the next step is a launch
-// of its own; a small pool is done in one.
+// A small pool is done by one workgroup in one launch, with a word a page in LDS; a large one in launches
+// over parts of it, with the words in memory.  No order of atomics or of writers shows in a result.
 
 #include <algorithm>
 
@@ -22,6 +20,8 @@ typedef uint32_t v4u_t __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kRange = kPageRange;            // pages a workgroup owns
 constexpr int kPer = kRange / kThreads;       // consecutive ones a thread
+// a large pool's parts
+constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64, kPart = kPartThreads * kPer;
 
 // Sum over the threads in front of this one of a workgroup of W waves; *total that over all.
 template <int W = kWaves>
@@ -45,6 +45,16 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
     }
     *total = all;
     return before;
+}
+
+__global__ void __launch_bounds__(256) pages_clear_kernel(v4u_t* p, int64_t n) {
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = v4u_t{0, 0, 0, 0};
+}
+hipError_t clear_pages(void* p, int64_t bytes, hipStream_t stream) {   // 16-byte aligned, a multiple of 16
+    const int64_t n = bytes / 16;
+    hipLaunchKernelGGL(pages_clear_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 8 * kNumCUs)), dim3(256), 0,
+                       stream, static_cast<v4u_t*>(p), n);
+    return hipGetLastError();
 }
 
 __device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((int64_t)tokens + page - 1) / page); }
@@ -86,9 +96,9 @@ struct ForkArgs {
     int* table_out;
     int* state_out;
     int* copies;             // [B][2]
-    uint32_t* words;         // [num_pages] (past one range)
-    int* freed;              // [ranges]
-    int B, page, max_pages, num_pages, ranges;
+    uint32_t* words;         // [parts * kPart] (a large pool)
+    int* freed;              // [parts]
+    int B, page, max_pages, num_pages, parts;
 };
 
 struct ForkRow { int src, n; };
@@ -101,68 +111,53 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int b) {
     return {p, min(max(a.keep[b], 0), fork_len(a, p))};
 }
 
-// The words of pages [lo, lo + kRange), and how many of them nobody holds any more.  A wave reads kRows
-// rows at a time, 128 entries of each, all loads before the first mark; rows[kThreads] is scratch.
+// The marks of rows wave, wave + waves, .. of a.B, kRows of them at a time, 128 entries of each: all loads
+// before the first mark.
 struct ForkMark { int src, have, whole, held; };
-__device__ __forceinline__ int fork_words(const ForkArgs& a, int lo, uint32_t* words, ForkMark* rows, int* waves) {
-    constexpr int kRows = 4;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int pages = min(kRange, a.num_pages - lo);
-    for (int i = tid; i < kRange / 4; i += kThreads) reinterpret_cast<v4u_t*>(words)[i] = v4u_t{0, 0, 0, 0};
+__device__ __forceinline__ ForkMark fork_mark(const ForkArgs& a, int b) {
+    const ForkRow r = fork_row(a, b);
+    return {r.src, pages_of(fork_len(a, b), a.page), r.n / a.page, pages_of(r.n, a.page)};
+}
+template <int kRows, class Row>
+__device__ __forceinline__ void fork_marks(const ForkArgs& a, uint32_t* words, int b0, int nb, int wave, int waves, Row row) {
+    const int lane = threadIdx.x & 63;
     auto mark = [&](int page, uint32_t w) __attribute__((always_inline)) {
-        const uint32_t i = (uint32_t)page - (uint32_t)lo;
-        if (page >= lo && i < (uint32_t)pages) atomicMax(&words[i], w);
+        if (page >= 0 && page < a.num_pages) atomicMax(&words[page], w);
     };
-    for (int c0 = 0; c0 < a.B; c0 += kThreads) {
-        const int nb = min(kThreads, a.B - c0);
-        __syncthreads();
-        if (tid < nb) {
-            const ForkRow r = fork_row(a, c0 + tid);
-            rows[tid] = {r.src, pages_of(fork_len(a, c0 + tid), a.page), r.n / a.page, pages_of(r.n, a.page)};
+    for (int r0 = wave; r0 < nb; r0 += kRows * waves) {
+        ForkMark m[kRows];
+        int most = 0;
+        #pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            m[k] = r0 + k * waves < nb ? row(r0 + k * waves) : ForkMark{0, 0, 0, 0};
+            most = max(most, max(m[k].have, m[k].held));
         }
-        __syncthreads();
-        for (int r0 = wave; r0 < nb; r0 += kRows * kWaves) {
-            ForkMark m[kRows];
-            int most = 0;
+        for (int j0 = lane; j0 < most; j0 += 128) {
+            int own[kRows][2], from[kRows][2];
             #pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                m[k] = r0 + k * kWaves < nb ? rows[r0 + k * kWaves] : ForkMark{0, 0, 0, 0};
-                most = max(most, max(m[k].have, m[k].held));
-            }
-            for (int j0 = lane; j0 < most; j0 += 128) {
-                int own[kRows][2], from[kRows][2];
+            for (int k = 0; k < kRows; ++k)
                 #pragma unroll
-                for (int k = 0; k < kRows; ++k)
-                    #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int j = j0 + 64 * i;
-                        own[k][i] = j < m[k].have ? a.table[(int64_t)(c0 + r0 + k * kWaves) * a.max_pages + j] : -1;
-                        from[k][i] = j < m[k].held ? a.table[(int64_t)m[k].src * a.max_pages + j] : -1;
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    const int j = j0 + 64 * i;
+                    own[k][i] = j < m[k].have ? a.table[(int64_t)(b0 + r0 + k * waves) * a.max_pages + j] : -1;
+                    from[k][i] = j < m[k].held ? a.table[(int64_t)m[k].src * a.max_pages + j] : -1;
+                }
+            #pragma unroll
+            for (int k = 0; k < kRows; ++k)
                 #pragma unroll
-                for (int k = 0; k < kRows; ++k)
-                    #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        mark(own[k][i], kHeld);
-                        mark(from[k][i], j0 + 64 * i < m[k].whole ? kWhole : kOpen - (uint32_t)(c0 + r0 + k * kWaves));
-                    }
-            }
+                for (int i = 0; i < 2; ++i) {
+                    mark(own[k][i], kHeld);
+                    mark(from[k][i], j0 + 64 * i < m[k].whole ? kWhole : kOpen - (uint32_t)(b0 + r0 + k * waves));
+                }
         }
     }
-    __syncthreads();
-    const Words x = own_words(words);
-    int n = 0, total;
-    #pragma unroll
-    for (int i = 0; i < kPer; ++i) n += x.w[i] == kHeld;
-    block_scan(n, waves, &total);
-    return total;
 }
 
 // The plan of all requests: each one's copy, if it needs one and a free page is left for it.
 // put(b, row, old page, fresh page or kNoCopy, whether it is cut back to its whole pages)
-template <class Word, class Put>
+template <int W, class Word, class Put>
 __device__ __forceinline__ int fork_plan(const ForkArgs& a, int head, int count, int* waves, Word word, Put put) {
-    const int per = (a.B + kThreads - 1) / kThreads;
+    const int per = (a.B + 64 * W - 1) / (64 * W);
     const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
     auto needs = [&](int b, ForkRow r, int* old) __attribute__((always_inline)) {
         if (r.n % a.page == 0) return false;
@@ -171,7 +166,7 @@ __device__ __forceinline__ int fork_plan(const ForkArgs& a, int head, int count,
     };
     int n = 0, old = -1, total;
     for (int b = b0; b < b1; ++b) n += needs(b, fork_row(a, b), &old);
-    int order = block_scan(n, waves, &total);
+    int order = block_scan<W>(n, waves, &total);
     for (int b = b0; b < b1; ++b) {
         const ForkRow r = fork_row(a, b);
         const bool need = needs(b, r, &old), given = need && order < count;
@@ -190,21 +185,21 @@ __device__ __forceinline__ void fork_write(const ForkArgs& a, int b, int src, in
         to[j] = j >= held ? 0 : j < whole || fresh == kNoCopy ? from[j] : fresh;
 }
 
-// The pages of a range that nobody holds any more, behind the ring's tail: `before` of them come first.
-__device__ __forceinline__ void fork_free(const ForkArgs& a, int lo, const uint32_t* words, int before,
-                                          int head, int count, int* waves) {
-    const Words x = own_words(words);
+// The pages of `x`, from lo on, that nobody holds any more, behind the ring's tail: `before` of them come
+// first.  Their number.
+template <int W>
+__device__ __forceinline__ int fork_free(const ForkArgs& a, int lo, const Words& x, int before, int head, int count, int* waves) {
     int n = 0, total;
     #pragma unroll
     for (int i = 0; i < kPer; ++i) n += x.w[i] == kHeld;
-    int k = before + block_scan(n, waves, &total);
-    if (n == 0) return;
+    int k = before + block_scan<W>(n, waves, &total);
     #pragma unroll
     for (int i = 0; i < kPer; ++i)
         if (x.w[i] == kHeld) {
             if (k < a.num_pages - count) a.ring[ring_at(head, count + k, a.num_pages)] = lo + threadIdx.x * kPer + i;
             ++k;
         }
+    return total;
 }
 
 __device__ __forceinline__ void ring_state(const int* state, int n, int* head, int* count) {
@@ -215,71 +210,85 @@ __device__ __forceinline__ void ring_state(const int* state, int n, int* head, i
 
 struct ForkInfo { int src, n, fresh; };
 
-// ONE: one range and at most kThreads requests, all of it here.  Else the words and how many pages each
-// range frees.
-template <bool ONE>
-__global__ void __launch_bounds__(kThreads) fork_words_kernel(ForkArgs a) {
-    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
-    __shared__ int waves[kWaves];
-    __shared__ ForkMark rows[kThreads];
-    __shared__ ForkInfo info[ONE ? kThreads : 1];
-    const int tid = threadIdx.x, lo = blockIdx.x * kRange;
-    const int freed = fork_words(a, lo, words, rows, waves);
-    if (!ONE) {
-        if (tid == 0) a.freed[blockIdx.x] = freed;
-        for (int i = tid; i < min(kRange, a.num_pages - lo); i += kThreads) a.words[lo + i] = words[i];
-        return;
-    }
+// What a request's plan leaves behind, and its numbers for its row.
+__device__ __forceinline__ ForkInfo fork_put(const ForkArgs& a, int b, const ForkRow& r, int old, int fresh, bool cut) {
+    const int n = cut ? r.n / a.page * a.page : r.n;
+    a.lens_out[b] = n;
+    a.copies[2 * b] = fresh == kNoCopy ? -1 : old;
+    a.copies[2 * b + 1] = fresh == kNoCopy ? -1 : fresh;
+    return {r.src, n, fresh};
+}
+
+// A pool that a workgroup of W waves holds (kPer pages a thread) and at most a request a thread: few waves, where
+// that is enough, meet sooner (beams of 8 requests 6.0 us with 16 of them).
+template <int W>
+__global__ void __launch_bounds__(64 * W) fork_one_kernel(ForkArgs a) {
+    __shared__ __attribute__((aligned(16))) uint32_t words[64 * W * kPer];
+    __shared__ int waves[W];
+    __shared__ ForkMark rows[64 * W];
+    __shared__ ForkInfo info[64 * W];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    for (int i = tid; i < 64 * W * kPer / 4; i += 64 * W) reinterpret_cast<v4u_t*>(words)[i] = v4u_t{0, 0, 0, 0};
+    if (tid < a.B) rows[tid] = fork_mark(a, tid);
     int head, count;
     ring_state(a.state, a.num_pages, &head, &count);
-    const int taken = fork_plan(a, head, count, waves, [&](int page) { return words[page]; },
-                                [&](int b, ForkRow r, int old, int fresh, bool cut) __attribute__((always_inline)) {
-        const int n = cut ? r.n / a.page * a.page : r.n;
-        info[b] = {r.src, n, fresh};
-        a.lens_out[b] = n;
-        a.copies[2 * b] = fresh == kNoCopy ? -1 : old;
-        a.copies[2 * b + 1] = fresh == kNoCopy ? -1 : fresh;
+    __syncthreads();
+    fork_marks<4>(a, words, 0, a.B, wave, W, [&](int b) { return rows[b]; });
+    __syncthreads();
+    const int taken = fork_plan<W>(a, head, count, waves, [&](int page) { return words[page]; },
+                                        [&](int b, const ForkRow& r, int old, int fresh, bool cut) __attribute__((always_inline)) {
+        info[b] = fork_put(a, b, r, old, fresh, cut);
     });
+    const int freed = fork_free<W>(a, 0, own_words(words), 0, head, count, waves);
     if (tid == 0) {
         a.state_out[0] = ring_at(head, taken, a.num_pages);
         a.state_out[1] = min(count - taken + freed, a.num_pages);
     }
-    fork_free(a, lo, words, 0, head, count, waves);
     __syncthreads();
-    for (int b = tid >> 6; b < a.B; b += kWaves) fork_write(a, b, info[b].src, info[b].n, info[b].fresh);
+    for (int b = wave; b < a.B; b += W) fork_write(a, b, info[b].src, info[b].n, info[b].fresh);
 }
 
-// Workgroups [0, ranges) free pages, the others write kWaves rows each.
-__global__ void __launch_bounds__(kThreads) fork_emit_kernel(ForkArgs a) {
-    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
-    __shared__ int waves[kWaves];
-    __shared__ ForkInfo info[kWaves];
-    const int tid = threadIdx.x;
+// A large pool or batch: words in memory (cleared), the parts' freed pages, then those to the ring and the rows.
+__global__ void __launch_bounds__(256) fork_mark_kernel(ForkArgs a) {
+    const int wave = blockIdx.x * 4 + (threadIdx.x >> 6);
+    fork_marks<1>(a, a.words, 0, a.B, wave, gridDim.x * 4, [&](int b) { return fork_mark(a, b); });
+}
+__device__ __forceinline__ Words fork_part(const ForkArgs& a, int g) { return own_words(a.words + (int64_t)g * kPart); }
+
+__global__ void __launch_bounds__(kPartThreads) fork_freed_kernel(ForkArgs a) {
+    __shared__ int waves[kPartWaves];
+    const Words x = fork_part(a, blockIdx.x);
+    int n = 0, total;
+    #pragma unroll
+    for (int i = 0; i < kPer; ++i) n += x.w[i] == kHeld;
+    block_scan<kPartWaves>(n, waves, &total);
+    if (threadIdx.x == 0) a.freed[blockIdx.x] = total;
+}
+
+// Workgroups [0, parts) free pages, the others write kPartWaves rows each.
+__global__ void __launch_bounds__(kPartThreads) fork_emit_kernel(ForkArgs a) {
+    __shared__ int waves[kPartWaves];
+    __shared__ ForkInfo info[kPartWaves];
+    const int tid = threadIdx.x, g = blockIdx.x;
     int head, count;
     ring_state(a.state, a.num_pages, &head, &count);
-    if ((int)blockIdx.x < a.ranges) {
-        const int lo = blockIdx.x * kRange;
-        for (int i = tid; i < kRange; i += kThreads) words[i] = lo + i < a.num_pages ? a.words[lo + i] : 0;
+    if (g < a.parts) {
+        const Words x = fork_part(a, g);
         int n = 0, before;
-        for (int r = tid; r < (int)blockIdx.x; r += kThreads) n += a.freed[r];
-        block_scan(n, waves, &before);
-        fork_free(a, lo, words, before, head, count, waves);
+        for (int r = tid; r < g; r += kPartThreads) n += a.freed[r];
+        block_scan<kPartWaves>(n, waves, &before);
+        fork_free<kPartWaves>(a, g * kPart, x, before, head, count, waves);
         return;
     }
-    const int r0 = (blockIdx.x - a.ranges) * kWaves;
-    const int taken = fork_plan(a, head, count, waves, [&](int page) { return a.words[page]; },
-                                [&](int b, ForkRow r, int old, int fresh, bool cut) __attribute__((always_inline)) {
-        if (b < r0 || b >= r0 + kWaves) return;
-        const int n = cut ? r.n / a.page * a.page : r.n;
-        info[b - r0] = {r.src, n, fresh};
-        a.lens_out[b] = n;
-        a.copies[2 * b] = fresh == kNoCopy ? -1 : old;
-        a.copies[2 * b + 1] = fresh == kNoCopy ? -1 : fresh;
+    const int r0 = (g - a.parts) * kPartWaves;
+    const int taken = fork_plan<kPartWaves>(a, head, count, waves, [&](int page) { return a.words[page]; },
+                                            [&](int b, const ForkRow& r, int old, int fresh, bool cut) __attribute__((always_inline)) {
+        if (b >= r0 && b < r0 + kPartWaves) info[b - r0] = fork_put(a, b, r, old, fresh, cut);
     });
     if (r0 == 0) {
         int n = 0, freed;
-        for (int r = tid; r < a.ranges; r += kThreads) n += a.freed[r];
-        block_scan(n, waves, &freed);
+        for (int r = tid; r < a.parts; r += kPartThreads) n += a.freed[r];
+        block_scan<kPartWaves>(n, waves, &freed);
         if (tid == 0) {
             a.state_out[0] = ring_at(head, taken, a.num_pages);
             a.state_out[1] = (int)min((int64_t)count - taken + freed, (int64_t)a.num_pages);
@@ -313,25 +322,25 @@ struct CompactArgs {
     int B, page, max_pages, num_pages, ranges, room;
 };
 
-__device__ __forceinline__ int2 compact_words(const CompactArgs& a, int lo, uint32_t* words, int* waves) {
+// The words of a pool that a workgroup of W waves holds, and how many pages are held and free.
+template <int W>
+__device__ __forceinline__ int2 compact_words(const CompactArgs& a, uint32_t* words, int* waves) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int pages = min(kRange, a.num_pages - lo);
-    for (int i = tid; i < kRange; i += kThreads) words[i] = 0;
+    for (int i = tid; i < 64 * W * kPer / 4; i += 64 * W) reinterpret_cast<v4u_t*>(words)[i] = v4u_t{0, 0, 0, 0};
     int head, count;
     ring_state(a.state, a.num_pages, &head, &count);
     __syncthreads();
     auto mark = [&](int page, uint32_t w) __attribute__((always_inline)) {
-        const uint32_t i = (uint32_t)(page - lo);
-        if (page >= lo && i < (uint32_t)pages) atomicOr(&words[i], w);
+        if (page >= 0 && page < a.num_pages) atomicOr(&words[page], w);
     };
     constexpr int kRun = 8;
-    for (int b0 = wave; b0 < a.B; b0 += 4 * kWaves) {     // four rows at a time, 128 entries of each
+    for (int b0 = wave; b0 < a.B; b0 += 4 * W) {     // four rows at a time, 128 entries of each
         int have[4], most = 0;
         #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int b = min(b0 + k * kWaves, a.B - 1);
+            const int b = min(b0 + k * W, a.B - 1);
             const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
-            have[k] = b0 + k * kWaves < a.B ? pages_of(len, a.page) : 0;
+            have[k] = b0 + k * W < a.B ? pages_of(len, a.page) : 0;
             most = max(most, have[k]);
         }
         for (int j0 = lane; j0 < most; j0 += 128) {
@@ -339,17 +348,17 @@ __device__ __forceinline__ int2 compact_words(const CompactArgs& a, int lo, uint
             #pragma unroll
             for (int k = 0; k < kRun; ++k) {
                 const int j = j0 + 64 * (k & 1);
-                p[k] = j < have[k >> 1] ? a.table[(int64_t)(b0 + (k >> 1) * kWaves) * a.max_pages + j] : -1;
+                p[k] = j < have[k >> 1] ? a.table[(int64_t)(b0 + (k >> 1) * W) * a.max_pages + j] : -1;
             }
             #pragma unroll
             for (int k = 0; k < kRun; ++k) mark(p[k], kUsed);
         }
     }
-    for (int i = tid; i < count; i += kRun * kThreads) {
+    for (int i = tid; i < count; i += kRun * (64 * W)) {
         int p[kRun];
         #pragma unroll
         for (int k = 0; k < kRun; ++k)
-            p[k] = i + k * kThreads < count ? a.ring[ring_at(head, i + k * kThreads, a.num_pages)] : -1;
+            p[k] = i + k * (64 * W) < count ? a.ring[ring_at(head, i + k * (64 * W), a.num_pages)] : -1;
         #pragma unroll
         for (int k = 0; k < kRun; ++k) mark(p[k], kFree);
     }
@@ -361,8 +370,8 @@ __device__ __forceinline__ int2 compact_words(const CompactArgs& a, int lo, uint
         used += (x.w[i] & kUsed) != 0;
         free += x.w[i] == kFree;
     }
-    block_scan(used, waves, &all_used);
-    block_scan(free, waves, &all_free);
+    block_scan<W>(used, waves, &all_used);
+    block_scan<W>(free, waves, &all_free);
     return make_int2(all_used, all_free);
 }
 
@@ -437,14 +446,8 @@ __device__ __forceinline__ void compact_row(const CompactArgs& a, int b, int cut
     }
 }
 
-// A large pool, in parts of kPart pages: bytes a page, written plainly (all writers write 1), then sums,
-// then the moves.
-constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64, kPart = kPartThreads * kPer;
-
-__global__ void __launch_bounds__(256) compact_clear_kernel(v4u_t* p, int64_t n) {
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = v4u_t{0, 0, 0, 0};
-}
-
+// A large pool: bytes a page, cleared and written plainly (all writers write 1), then the parts' sums, then the
+// moves, then the table.
 // A wave marks a row of the table, and a workgroup its share of the ring.
 __global__ void __launch_bounds__(256) compact_mark_kernel(CompactArgs a) {
     const int lane = threadIdx.x & 63;
@@ -576,12 +579,13 @@ __global__ void __launch_bounds__(256) compact_table_kernel(CompactArgs a) {
         compact_row(a, b, cut, [&](int p) { return a.copies[2 * a.to[p] + 1]; });
 }
 
-// One range: all of it here, the moves in LDS.
-__global__ void __launch_bounds__(kThreads) compact_one_kernel(CompactArgs a) {
-    __shared__ __attribute__((aligned(16))) uint32_t words[kRange];
-    __shared__ int waves[kWaves], cut_at[2], holes[kRange / 2];
+// A pool that a workgroup holds: all of it here, the moves in LDS.
+template <int W>
+__global__ void __launch_bounds__(64 * W) compact_one_kernel(CompactArgs a) {
+    __shared__ __attribute__((aligned(16))) uint32_t words[64 * W * kPer];
+    __shared__ int waves[W], cut_at[2], holes[64 * W * kPer / 2];
     const int tid = threadIdx.x;
-    const int2 x = compact_words(a, 0, words, waves);
+    const int2 x = compact_words<W>(a, words, waves);
     const CompactSums s = {x.x, x.x + x.y, 0, 0};
     if (tid == 0) {
         cut_at[0] = a.num_pages;
@@ -590,24 +594,24 @@ __global__ void __launch_bounds__(kThreads) compact_one_kernel(CompactArgs a) {
     __syncthreads();
     int p, held;
     const Words own = own_words(words);
-    if (compact_cut<kWaves>(s, 0, own, waves, &p, &held)) {
+    if (compact_cut<W>(s, 0, own, waves, &p, &held)) {
         cut_at[0] = p;
         cut_at[1] = held;
     }
     __syncthreads();
     const int cut = cut_at[0], used_below = cut_at[1];
     // a page that moves keeps its move's number in its word, above the two bits
-    compact_emit<kWaves>(a, s, 0, own, used_below, waves,
+    compact_emit<W>(a, s, 0, own, used_below, waves,
                  [&](int p, int k) { words[p] |= (uint32_t)k << 2; a.copies[2 * k] = p; },
                  [&](int p, int k) { holes[k] = p; a.copies[2 * k + 1] = p; });
-    for (int k = s.U - used_below + tid; k < a.room; k += kThreads) a.copies[2 * k] = a.copies[2 * k + 1] = -1;
-    for (int k = s.all - s.U + tid; k < a.num_pages; k += kThreads) a.ring_out[k] = -1;
+    for (int k = s.U - used_below + tid; k < a.room; k += 64 * W) a.copies[2 * k] = a.copies[2 * k + 1] = -1;
+    for (int k = s.all - s.U + tid; k < a.num_pages; k += 64 * W) a.ring_out[k] = -1;
     if (tid == 0) {
         a.state_out[0] = 0;
         a.state_out[1] = s.all - s.U;
     }
     __syncthreads();
-    for (int b = tid >> 6; b < a.B; b += kWaves) compact_row(a, b, cut, [&](int q) { return holes[words[q] >> 2]; });
+    for (int b = tid >> 6; b < a.B; b += W) compact_row(a, b, cut, [&](int q) { return holes[words[q] >> 2]; });
 }
 
 // ---- copies ---------------------------------------------------------------------------------
@@ -664,14 +668,14 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(CopyArgs a) {
     }
 }
 
-int ranges_of(int num_pages) { return (int)(((int64_t)num_pages + kRange - 1) / kRange); }
+int parts_of(int num_pages) { return (int)(((int64_t)num_pages + kPart - 1) / kPart); }
 bool fork_in_one(int B, int num_pages) { return B <= kThreads && num_pages <= kRange; }
 
 }  // namespace
 
 size_t cache_fork_workspace(int B, int num_pages) {
     if (fork_in_one(B, num_pages)) return 0;
-    return ((size_t)num_pages + ranges_of(num_pages)) * 4;
+    return (size_t)parts_of(num_pages) * (kPart + 1) * 4;
 }
 
 hipError_t launch_cache_fork(const CacheFork& p, void* workspace, hipStream_t stream) {
@@ -680,25 +684,29 @@ hipError_t launch_cache_fork(const CacheFork& p, void* workspace, hipStream_t st
     a.state = p.free_state; a.ring = p.free_pages;
     a.lens_out = p.seq_lens_out; a.table_out = p.block_table_out; a.state_out = p.free_state_out;
     a.copies = p.copies;
+    a.parts = parts_of(p.num_pages);
     a.words = static_cast<uint32_t*>(workspace);
-    a.freed = static_cast<int*>(workspace) + p.num_pages;
+    a.freed = static_cast<int*>(workspace) + (size_t)a.parts * kPart;
     a.B = p.B; a.page = p.page_size; a.max_pages = p.max_pages; a.num_pages = p.num_pages;
-    a.ranges = ranges_of(p.num_pages);
     if (fork_in_one(p.B, p.num_pages)) {
-        hipLaunchKernelGGL(fork_words_kernel<true>, dim3(1), dim3(kThreads), 0, stream, a);
+        if (p.B <= kPartThreads && p.num_pages <= kPart)
+            hipLaunchKernelGGL(fork_one_kernel<kPartWaves>, dim3(1), dim3(kPartThreads), 0, stream, a);
+        else
+            hipLaunchKernelGGL(fork_one_kernel<kWaves>, dim3(1), dim3(kThreads), 0, stream, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(fork_words_kernel<false>, dim3((unsigned)a.ranges), dim3(kThreads), 0, stream, a);
-    hipError_t e = hipGetLastError();
+    const hipError_t e = clear_pages(workspace, (int64_t)a.parts * kPart * 4, stream);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(fork_emit_kernel, dim3((unsigned)(a.ranges + (p.B + kWaves - 1) / kWaves)), dim3(kThreads), 0,
-                       stream, a);
+    hipLaunchKernelGGL(fork_mark_kernel, dim3((unsigned)std::min((p.B + 3) / 4, 8 * kNumCUs)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(fork_freed_kernel, dim3((unsigned)a.parts), dim3(kPartThreads), 0, stream, a);
+    hipLaunchKernelGGL(fork_emit_kernel, dim3((unsigned)(a.parts + (p.B + kPartWaves - 1) / kPartWaves)), dim3(kPartThreads),
+                       0, stream, a);
     return hipGetLastError();
 }
 
 size_t cache_compact_workspace(int num_pages) {
     if (num_pages <= kRange) return 0;
-    const size_t parts = ((size_t)num_pages + kPart - 1) / kPart;
+    const size_t parts = parts_of(num_pages);
     return 2 * parts * kPart + parts * 8 + (size_t)num_pages * 4 + 4;
 }
 
@@ -709,7 +717,7 @@ hipError_t launch_cache_compact(const CacheCompact& p, void* workspace, hipStrea
     a.copies = p.copies;
     a.B = p.B; a.page = p.page_size; a.max_pages = p.max_pages; a.num_pages = p.num_pages;
     a.room = std::max(1, p.num_pages / 2);
-    a.ranges = (int)(((int64_t)p.num_pages + kPart - 1) / kPart);
+    a.ranges = parts_of(p.num_pages);
     const size_t bytes = (size_t)a.ranges * kPart;
     a.used = static_cast<uint8_t*>(workspace);
     a.free = a.used + bytes;
@@ -717,14 +725,14 @@ hipError_t launch_cache_compact(const CacheCompact& p, void* workspace, hipStrea
     a.to = reinterpret_cast<int*>(a.sums + a.ranges);
     a.cut = a.to + p.num_pages;
     if (p.num_pages <= kRange) {
-        hipLaunchKernelGGL(compact_one_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+        if (p.num_pages <= kPart) hipLaunchKernelGGL(compact_one_kernel<kPartWaves>, dim3(1), dim3(kPartThreads), 0, stream, a);
+        else hipLaunchKernelGGL(compact_one_kernel<kWaves>, dim3(1), dim3(kThreads), 0, stream, a);
         return hipGetLastError();
     }
-    const int64_t chunks = (int64_t)(2 * bytes / 16);
     const unsigned rows = (unsigned)std::min((p.B + 3) / 4, 8 * kNumCUs);
     const unsigned ring = (unsigned)std::min<int64_t>(((int64_t)p.num_pages + 1023) / 1024, 8 * kNumCUs);
-    hipLaunchKernelGGL(compact_clear_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 8 * kNumCUs)), dim3(256),
-                       0, stream, reinterpret_cast<v4u_t*>(workspace), chunks);
+    const hipError_t e = clear_pages(workspace, 2 * (int64_t)bytes, stream);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(compact_mark_kernel, dim3(std::max(rows, ring)), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(compact_sums_kernel, dim3((unsigned)a.ranges), dim3(kPartThreads), 0, stream, a);
     hipLaunchKernelGGL(compact_emit_kernel, dim3((unsigned)a.ranges), dim3(kPartThreads), 0, stream, a);

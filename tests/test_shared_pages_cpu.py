@@ -123,9 +123,9 @@ def compact_call(lib, batch=4, page=64, max_pages=8, pages=100, p=None, ws=None,
 
 @pytest.mark.parametrize("call,n_in,n", [(fork_call, 6, 10), (compact_call, 4, 8)])
 def test_table_refusals(lib, call, n_in, n):
-    for kw in ({"batch": 0}, {"batch": -1}, {"batch": (1 << 24) + 1}, {"page": 0}, {"page": 63}, {"page": -64},
+    for kw in ({"batch": 0}, {"batch": -1}, {"batch": (1 << 16) + 1}, {"page": 0}, {"page": 63}, {"page": -64},
                {"max_pages": 0}, {"pages": 0}, {"pages": (1 << 30) + 1}, {"max_pages": 1 << 25, "page": 64},
-               {"batch": 1 << 20, "max_pages": 1 << 12}):
+               {"batch": 1 << 16, "max_pages": 1 << 15}):
         assert call(lib, **kw) == INVALID, kw
         assert lib.mla_last_error()
     for i in range(n):
