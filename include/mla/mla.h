@@ -531,7 +531,8 @@ int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
  * first page (mla_cache_fork) are expanded once.  Table entries outside the pool read as zero rows.
  * Rounded on the way, in both types: keys, values and each key's weight (before the division by the
  * row's sum) to 11 bits as fp16 numbers, in bf16 under a power of two for each 64 keys that brings
- * their largest latent or rope value to [64, 128); weights down to 2^-22 of the row's largest; bf16
+ * their largest latent or rope value to [64, 128) (where a latent row's largest is more than 2^12 below that,
+ * one for each of their latent and rope rows); weights down to 2^-22 of the row's largest; bf16
  * queries to 11 bits down to 2^-14 of the row's largest; the output to its type.  Sums are float32.  A key
  * or value past fp16's range (65504, in bf16 times that power of two) stays there.  A latent row with a
  * NaN or an infinity makes the rows of the queries that see it NaN and reaches no other query.

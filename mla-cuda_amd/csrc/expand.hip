@@ -28,6 +28,8 @@ typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 constexpr int kUnit = kExpandUnit;            // rows a unit (and keys a step of the attention)
 constexpr int kR = 512, kD = 64, kN = 128;    // latent, rope, nope / value widths
 constexpr int kHead = 6;                      // log2 of a bf16 unit's largest value as it is stored
+constexpr int kSpread = 12;                   // log2 of how far a row's largest may lie below it
+constexpr int kMixed = 4096;                  // added to a mixed unit's exponent
 
 // ---- units ----------------------------------------------------------------------------------
 // Unit j of sequence b is its keys [64 j, 64 j + 64).  Sequences that continue one prompt hold the
@@ -120,9 +122,11 @@ __global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
 // A bf16 cache is fitted into fp16's range by a power of two for each unit, 2^e: its rows are stored
 // under it, the largest value in [2^kHead, 2^(kHead+1)), and the attention puts it back.  kHead leaves
 // 2^9 above for keys and values, sums of 512 products with weights (below 1 they cannot reach fp16's
-// end), and 2^20 below down to its subnormals, so that neither large rows nor weights cost the other rows
-// bits.  An fp16 cache is as it is (e = 0).  The latent rows keep the type of W_uk and W_uv, which they
-// are multiplied with; the rope rows are fp16.
+// end), and 2^20 below down to its subnormals.  Where a latent row is more than 2^kSpread below the largest value
+// the unit is `mixed`: each latent and each rope row has a power of two of its own, so that no row, hidden or
+// not, costs another its bits.
+// An fp16 cache is as it is (e = 0).  The latent rows keep the type of W_uk and W_uv, which they are
+// multiplied with; the rope rows are fp16.
 // A latent row with a value that is not finite makes every key and value of it NaN or infinite, and
 // with it every output of a query that sees it NaN (also under a weight of 0); the row is written as
 // zeros, so that queries in front of it are not touched by 0 * NaN, and the unit's first such row is
@@ -140,7 +144,8 @@ struct GatherArgs {
     const int* count;
     int* unit;               // [B][units] the unit's place in lat / rot
     int* bad;                // [places] first row that is not finite, or 64
-    int* exps;               // [places] e
+    int* exps;               // [places] e (its largest row's, plus kMixed)
+    int* row_exps;           // [places][2][64] the latent and the rope rows' own, of mixed units
     int* any_bad;
     int* rows;               // rows in all
     uint16_t* lat;
@@ -179,7 +184,7 @@ __device__ __forceinline__ float finite_max(float m, float x) {
 template <typename TL, bool F8>
 __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
     __shared__ int part[4], w_bad[4];
-    __shared__ float w_top[4];
+    __shared__ float row_top[2][kUnit];     // latent, rope
     const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.Sk) : a.Sk;
@@ -262,7 +267,20 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
         }
     }
     int worst = kUnit;
-    float top = 0.f;
+    float rope_top[2] = {0.f, 0.f};
+    if constexpr (!Half<TL>::kF16) {
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(y[i][k]);
+                rope_top[i] = finite_max(finite_max(rope_top[i], v[0]), v[1]);
+            }
+            #pragma unroll
+            for (int k = 1; k < 8; k *= 2) rope_top[i] = fmaxf(rope_top[i], __shfl_xor(rope_top[i], k));
+            if ((tid & 7) == 0) row_top[1][32 * i + (tid >> 3)] = rope_top[i];
+        }
+    }
     #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const bool odd = not_finite2<TL>(x[i][0]) || not_finite2<TL>(x[i][1]) || not_finite2<TL>(x[i][2]) ||
@@ -271,47 +289,61 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
             worst = min(worst, 16 * wave + i);
             x[i] = v4u{0, 0, 0, 0};
         }
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const v2f_t v = halves<TL>(x[i][k]);
-            top = fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1])));
+        if constexpr (!Half<TL>::kF16) {
+            float top = 0.f;
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(x[i][k]);
+                top = fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1])));
+            }
+            top = wave_reduce(top, OpMax());
+            if (lane == 0) row_top[0][16 * wave + i] = top;
         }
     }
-    #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const v2f_t v = halves<TL>(y[i][k]);
-            top = finite_max(finite_max(top, v[0]), v[1]);
-        }
-    top = wave_reduce(top, OpMax());
-    if (lane == 0) { w_bad[wave] = worst; w_top[wave] = top; }
+    if (lane == 0) w_bad[wave] = worst;
     __syncthreads();
     worst = min(min(w_bad[0], w_bad[1]), min(w_bad[2], w_bad[3]));
-    const int e = Half<TL>::kF16 ? 0 : exponent_of(fmaxf(fmaxf(w_top[0], w_top[1]), fmaxf(w_top[2], w_top[3]))) - kHead;
-    const float f = two_to(-e);
+    // the unit's exponent, and whether its latent rows (those that are not zero) keep near it; in a mixed unit
+    // those that are zero count as its largest latent row
+    int e = 0, lat_e = 0, rope_e = 0;
+    bool mixed = false;
+    if constexpr (!Half<TL>::kF16) {
+        const float top = row_top[0][lane], rope = row_top[1][lane];
+        e = exponent_of(wave_reduce(fmaxf(top, rope), OpMax())) - kHead;
+        lat_e = exponent_of(top > 0.f ? top : wave_reduce(top, OpMax())) - kHead;      // of row `lane`
+        mixed = __builtin_amdgcn_ballot_w64(top > 0.f && e - lat_e > kSpread) != 0;
+        rope_e = mixed && rope > 0.f ? exponent_of(rope) - kHead : e;
+        if (!mixed) lat_e = e;
+        else if (wave < 2) a.row_exps[((int64_t)place * 2 + wave) * kUnit + lane] = wave ? rope_e : lat_e;
+    }
     if (tid == 0) {
-        a.exps[place] = e;
+        a.exps[place] = mixed ? e + kMixed : e;
         a.bad[place] = worst;
         if (a.any_bad && worst < kUnit) *a.any_bad = 1;   // cleared by the plan; every writer writes the same
     }
     #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        v4u o;
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const v2f_t v = halves<TL>(x[i][k]);
-            o[k] = Half<TL>::pack2(v[0] * f, v[1] * f);
+        v4u o = x[i];
+        if constexpr (!Half<TL>::kF16) {
+            const float f = two_to(-__builtin_amdgcn_readlane(lat_e, 16 * wave + i));
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(x[i][k]);
+                o[k] = Half<TL>::pack2(v[0] * f, v[1] * f);
+            }
         }
         reinterpret_cast<v4u*>(lat + (16 * wave + i) * kR)[lane] = o;
     }
     #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        v4u o;
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const v2f_t v = halves<TL>(y[i][k]);
-            o[k] = pack_f16x2(v[0] * f, v[1] * f);
+        v4u o = y[i];
+        if constexpr (!Half<TL>::kF16) {
+            const float f = two_to(-__shfl(rope_e, 32 * i + (tid >> 3)));
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(y[i][k]);
+                o[k] = pack_f16x2(v[0] * f, v[1] * f);
+            }
         }
         reinterpret_cast<v4u*>(rot + (32 * i + (tid >> 3)) * kD)[tid & 7] = o;
     }
@@ -332,8 +364,10 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
 // fp16's subnormals, and rise to 2^(kBias + kRise) < 65504; their sum is of what is packed.
 // A unit's power of two is one number a step: its keys' goes into the factor of the scores, its values'
 // into the exponentials, as d = e - E <= 0 with the largest e so far in E (what is in the accumulators
-// is scaled when that grows); the sum takes it out again.  bf16 queries are made fp16 under a power of
-// two of their own.
+// is scaled when that grows); the sum takes it out again.  Where d is far below, or the unit is mixed, fp16
+// exponentials would lose it: there they stay without it, and the values' product, for rows of like
+// exponents at a time, is scaled in float32.  (As a path of its own: the ordinary one takes the time that
+// it takes without; with both in one run of registers 3% more.)  bf16 queries are made fp16 under a power of two of their own.
 // What bounds it: the matrix cores' power and the order of two waves on a SIMD.  4,096 causal rows of 128 heads
 // 725 us, 948 TFLOP/s (a large fp16 library product 1,318); the cores are busy 0.46 of the cycles, and
 // with operands of zeros a fifth faster.  A step without the exponentials takes 6% less, without its loads
@@ -349,6 +383,7 @@ struct HeadsArgs {
     const int* unit;
     const int* bad;
     const int* exps;
+    const int* row_exps;
     const int* any_bad;      // null: look for yourself
     const int* seq_lens;
     const int* new_lens;
@@ -422,6 +457,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     const int wave_first = w0 < a.Sq ? lim_of(w0) : -1, wave_last = w0 < a.Sq ? lim_of(min(w0 + 31, a.Sq - 1)) : -1;
     int n_tiles = (lim_of(min(r0 + kHRows, a.Sq) - 1) + kUnit) / kUnit;   // lim -1: 0
     int first = 0;               // SPLIT: a share of them
+    n_tiles = max(n_tiles, 0);
     if constexpr (SPLIT) {
         const int share = (n_tiles + a.splits - 1) / a.splits;
         first = sp * share;
@@ -502,17 +538,20 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     float m_ref = -INFINITY, l = 0.f;
     const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
 
-    int next = n_tiles > first ? load_uniform(units + first) : 0;
+    int next = n_tiles > first ? load_uniform(units + first) : 0, here = next;
     int e_next = n_tiles > first ? load_uniform(a.exps + next) : 0;
     if (n_tiles > first) issue(next, 0);
     next = n_tiles > first + 1 ? load_uniform(units + first + 1) : 0;
-    int E = e_next;
+    int E = -1000;               // below any unit's
     #pragma unroll 1
     for (int j = first; j < n_tiles; ++j) {
         const uint32_t st = ((j - first) & 1) * kStageBytes;
         wait_vm<0>();
         lds_barrier();      // step j has landed; every wave is done with step j - 1
-        const int e = e_next;
+        const int place = here, ee = e_next;
+        const bool mixed = !Half<TL>::kF16 && ee > kMixed / 2;
+        const int e = mixed ? ee - kMixed : ee;
+        here = next;
         if (j + 1 < n_tiles) {
             issue(next, kStageBytes - st);
             e_next = load_uniform(a.exps + next);
@@ -533,6 +572,35 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        // a mixed unit's scores again, nope and rope columns each under their row's power of two; the largest
+        // of its latent rows' is the unit's for the values
+        const int* const rows = a.row_exps + (int64_t)place * 2 * kUnit;
+        auto row_exps = [&](int rope, int kb, int i) __attribute__((always_inline)) {   // 4 keys from 8 i + 4 h on
+            return *reinterpret_cast<const v4i*>(rows + kUnit * rope + 32 * kb + 8 * i + 4 * hi);
+        };
+        int ev = e;
+        if (mixed) {
+            ev = rows[lane];
+            #pragma unroll
+            for (int i = 1; i < 64; i *= 2) ev = max(ev, __shfl_xor(ev, i));
+            ev = __builtin_amdgcn_readfirstlane(ev);
+            #pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                v16f r = {};
+                s[kb] = v16f{};
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) s[kb] = Mma<f16_t>::sub(k_frag(st, kb, i), qf[i], 0, s[kb]);
+                #pragma unroll
+                for (int i = 8; i < 12; ++i) r = Mma<f16_t>::sub(k_frag(st, kb, i), qf[i], 0, r);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v4i x = row_exps(0, kb, i), y = row_exps(1, kb, i);
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        s[kb][4 * i + k] = ldexpf(s[kb][4 * i + k], x[k] - e) + ldexpf(r[4 * i + k], y[k] - e);
+                }
+            }
+        }
         if (j * kUnit + kUnit - 1 > wave_first) {     // (opaque: 32 differences are not to stay in registers)
             int past = lim - j * kUnit - 4 * hi;
             asm volatile("" : "+v"(past));
@@ -542,10 +610,11 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                 for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + acc_row(i, 0) <= past ? s[kb][i] : -INFINITY;
         }
         // weights
-        const float ct = c * two_to(e);
-        if (e > E) {
-            const float f = e - E > 126 ? 0.f : two_to(E - e);
-            E = e;
+        // (not 0, which under zero queries and keys it could round to: a hidden score times it has to stay -infinity)
+        const float ct = fmaxf(c * two_to(e), 1.17549435e-38f);
+        if (ev > E) {
+            const float f = ev - E > 126 ? 0.f : two_to(E - ev);
+            E = ev;
             #pragma unroll
             for (int i = 0; i < 4; ++i)
                 #pragma unroll
@@ -570,32 +639,78 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[i][k] *= f;
         }
-        const int d = max(e - E, -100);
-        const float neg = (m_ref == -INFINITY ? 0.f : kBias - m_ref) + (float)d;
-        v4u vf[kWinV];
-        #pragma unroll
-        for (int i = 0; i < kWinV; ++i) vf[i] = v_frag(st, i);
+        const int d = ev - E;
         v4u p[4];
-        float sum = 0.f;
-        #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int kb = i >> 3, k = 2 * (i & 7);
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k], ct, neg));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k + 1], ct, neg));
-            s[kb][k] = x; s[kb][k + 1] = y;
-            const uint32_t w = pack_f16x2(x, y);
-            p[i >> 2][i & 3] = w;
-            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, w), ones, sum, false);
-        }
-        if (d < -8) {        // a unit of far smaller values: its weights' sum is not to go under fp16's end
-            sum = 0.f;
+        // Past 2^24 a reference is off its own score by more than a power of two, which a fused product would show.
+        const bool huge = __builtin_amdgcn_ballot_w64(fabsf(m_ref) > 16777216.f && fabsf(m_ref) < INFINITY) != 0;
+        if (__builtin_expect(!mixed && d >= -8 && !huge, 1)) {
+            const float neg = (m_ref == -INFINITY ? 0.f : kBias - m_ref) + (float)d;
+            float sum = 0.f;
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int kb = i >> 3, k = 2 * (i & 7);
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k], ct, neg));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k + 1], ct, neg));
+                const uint32_t w = pack_f16x2(x, y);
+                p[i >> 2][i & 3] = w;
+                sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, w), ones, sum, false);
+            }
+            l += sum * two_to(-d);
+        } else {
+            // score and reference rounded alike; exponentials without d, in float32; then levels of rows whose
+            // exponents are within kSpread of the largest one left
+            const float m = m_ref == -INFINITY ? 0.f : m_ref;
+            float sum = 0.f;
             #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum += s[kb][i];
+                for (int i = 0; i < 16; ++i) {
+                    s[kb][i] = __builtin_amdgcn_exp2f(fp32_pinned(s[kb][i] * ct) - m + kBias);
+                    sum += s[kb][i];
+                }
+            l += sum;
+            const int mine = mixed ? rows[lane] : e;       // row `lane`
+            int level = ev;
+            #pragma unroll 1
+            while (true) {
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    v4i x = {e, e, e, e};
+                    if (mixed) x = row_exps(0, i >> 2, i & 3);
+                    #pragma unroll
+                    for (int k = 0; k < 4; k += 2) {
+                        float v[2];
+                        #pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            const int ex = x[k + n];
+                            v[n] = ex <= level && ex >= level - kSpread ? s[i >> 2][4 * (i & 3) + k + n] * two_to(ex - level) : 0.f;
+                        }
+                        p[i >> 1][2 * (i & 1) + (k >> 1)] = pack_f16x2(v[0], v[1]);
+                    }
+                }
+                const float f = level - E < -126 ? 0.f : two_to(level - E);
+                #pragma unroll
+                for (int vb = 0; vb < 4; ++vb) {
+                    v16f t = {};
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) t = Mma<f16_t>::sub(v_frag(st, 4 * i + vb), p[i], 0, t);
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i) o[vb][i] = __builtin_fmaf(t[i], f, o[vb][i]);
+                }
+                int below = mine < level - kSpread ? mine : -0x7fffffff;
+                #pragma unroll
+                for (int i = 1; i < 64; i *= 2) below = max(below, __shfl_xor(below, i));
+                below = __builtin_amdgcn_readfirstlane(below);
+                if (below == -0x7fffffff) break;
+                level = below;
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = v4u{0, 0, 0, 0};     // and nothing more below
         }
-        l += sum * two_to(-d);
         // values
+        v4u vf[kWinV];
+        #pragma unroll
+        for (int i = 0; i < kWinV; ++i) vf[i] = v_frag(st, i);
         #pragma unroll
         for (int i = 0; i < 16; ++i) {
             o[i & 3] = Mma<f16_t>::sub(vf[i % kWinV], p[i >> 2], 0, o[i & 3]);
@@ -723,6 +838,7 @@ ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged) {
     p.off_unit = take(places * 4);
     p.off_bad = take(places * 4);
     p.off_exps = take(places * 4);
+    p.off_row_exps = take(places * 8 * kUnit);
     p.off_any = take(8);                      // any_bad, rows
     p.off_lat = take((size_t)p.rows_cap * kR * 2);
     p.off_rot = take((size_t)p.rows_cap * kD * 2);
@@ -758,7 +874,8 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     g.c_kv = p.c_kv; g.pe = p.pe; g.scales = static_cast<const uint8_t*>(p.scales);
     g.seq_lens = p.seq_lens; g.table = p.block_table;
     g.owner = u.owner; g.rank = u.rank; g.count = u.count;
-    g.unit = ints(plan.off_unit); g.bad = ints(plan.off_bad); g.exps = ints(plan.off_exps); g.rows = any_bad + 1;
+    g.unit = ints(plan.off_unit); g.bad = ints(plan.off_bad); g.exps = ints(plan.off_exps);
+    g.row_exps = ints(plan.off_row_exps); g.rows = any_bad + 1;
     g.any_bad = alone ? nullptr : any_bad; g.planned = p.block_table && p.B > 1;
     g.lat = half(plan.off_lat); g.rot = half(plan.off_rot);
     g.B = p.B; g.Sk = p.Sk; g.units = plan.units;
@@ -778,7 +895,7 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     HeadsArgs a;
     a.qn = static_cast<const uint16_t*>(p.q_nope); a.qr = static_cast<const uint16_t*>(p.q_rope);
     a.kv = half(plan.off_kv); a.rot = g.rot;
-    a.unit = g.unit; a.bad = g.bad; a.exps = g.exps; a.any_bad = g.any_bad;
+    a.unit = g.unit; a.bad = g.bad; a.exps = g.exps; a.row_exps = g.row_exps; a.any_bad = g.any_bad;
     a.seq_lens = p.seq_lens; a.new_lens = p.new_lens;
     a.order = p.block_table && p.B > 1 ? u.order : nullptr;
     a.part = reinterpret_cast<float*>(ws + plan.off_part);

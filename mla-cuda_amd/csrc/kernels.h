@@ -409,8 +409,8 @@ struct ExpandPlan {
     int64_t rows_cap = 0;            // rows of all of them
     int heads = 0;                   // expanded and attended to at a time
     int splits = 1;                  // of the keys
-    size_t off_owner, off_rank, off_count, off_order, off_unit, off_bad, off_exps, off_any, off_lat, off_rot, off_kv,
-        off_part, off_state, total;
+    size_t off_owner, off_rank, off_count, off_order, off_unit, off_bad, off_exps, off_row_exps, off_any,
+        off_lat, off_rot, off_kv, off_part, off_state, total;
 };
 ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged);
 hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* workspace, hipStream_t stream);

@@ -389,3 +389,116 @@ def test_random_batches(ext, seed):
     t = make(seed, B, Sq, lens, H, r.choice([BF, H16]), page=page)
     causal = r.random() < 0.7
     check_all(t, run_paged(ext, t, causal, new), lens, causal, new)
+
+
+@pytest.mark.parametrize("at", [0, 40, 129, 250, 299])
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 40, 1e30])
+def test_a_row_far_larger(ext, at, size):
+    """One key with a latent row or a rope row that is far larger than the others, seen or not: no
+    query loses bits by it, those that do not see it not one."""
+    Sq, lens = 140, [300]
+    t = make(23, 1, Sq, lens, 2, BF)
+    want = run_paged(ext, t, True)
+    check_all(t, want, lens, True)
+    page, row = t["table"][0, at // 64].item(), at % 64
+    first = max(0, at - (300 - Sq))             # the first query that sees it
+    old = t["c_kv"][page, row].clone(), t["pe"][page, row].clone()
+    t["c_kv"][page, row] *= size
+    got = run_paged(ext, t, True)
+    assert (got[0, :first].double() - want[0, :first].double()).norm() <= 2 ** -8 * want[0, :first].double().norm()
+    ref = E.attention(t["q_nope"][0], t["q_rope"][0], *rows_of(t, 0, 300), t["W_uk"], t["W_uv"], SCALE,
+                      E.limits(Sq, 300, Sq, True), BF)[0]
+    # with scores of such size a row's weights are nothing but 0 and 1, where the score is further from the others
+    # than the rounding of its key's components, 2^-11 of each, can bring it: 2^-11 sum |q k| / scale
+    big = t["c_kv"][page, row].double() @ t["W_uk"].double().transpose(1, 2)        # [H, 128]
+    s = (t["q_nope"][0, first:].double() * big[None]).sum(-1) / SCALE               # [rows, H]
+    off = 200 + 2.0 ** -11 * (t["q_nope"][0, first:].double() * big[None]).abs().sum(-1) / SCALE
+    gone, all_ = s < -off, s > off
+    d = (got[0, first:].double() - ref[first:]).norm(dim=-1)
+    n = ref[first:].norm(dim=-1)
+    assert (gone | all_).double().mean() > (0.9 if size > 1e5 else 0.5)
+    assert (d[gone | all_] <= 2 ** -7 * n[gone | all_]).all()
+    t["c_kv"][page, row], t["pe"][page, row] = old[0], old[1] * size
+    got = run_paged(ext, t, True)
+    assert (got[0, :first].double() - want[0, :first].double()).norm() <= 2 ** -8 * want[0, :first].double().norm()
+    ref = E.attention(t["q_nope"][0], t["q_rope"][0], *rows_of(t, 0, 300), t["W_uk"], t["W_uv"], SCALE,
+                      E.limits(Sq, 300, Sq, True), BF)[0]
+    s = (t["q_rope"][0, first:].double() * t["pe"][page, row].double()).sum(-1) / SCALE
+    # (rope components are exact; their float32 sums are off by less than 2^-18 of the sum of magnitudes)
+    sure = s.abs() > 200 + 2.0 ** -18 * (t["q_rope"][0, first:].double() * t["pe"][page, row].double()).abs().sum(-1) / SCALE
+    d, n = (got[0, first:].double() - ref[first:]).norm(dim=-1), ref[first:].norm(dim=-1)
+    assert (d[sure] <= 2 ** -7 * n[sure]).all()
+
+
+@pytest.mark.parametrize("B", [1, 2])
+def test_dense_rows_that_are_not_finite(ext, B):
+    t = make(24, B, 100, [130] * B, 3, BF)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    ckv, pe = normal(g, B, 130, R, dtype=BF), normal(g, B, 130, D, dtype=BF)
+    call = lambda: ext.mla_attention_expanded(t["q_nope"], t["q_rope"], ckv, pe, t["W_uk"], t["W_uv"], SCALE, True)
+    want = call()
+    ckv[0, 90, 3] = INF
+    got = call()
+    assert torch.equal(got[0, :60], want[0, :60]) and got[0, 60:].isnan().all() and torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens", [[0], [0, 0, 0]])
+def test_no_keys_at_all(ext, dtype, lens):
+    t = make(25, len(lens), 5, [1] * len(lens), 2, DT[dtype])
+    t["lens"].zero_()
+    assert not run_paged(ext, t, True).any()
+
+
+def test_small_units_behind_large_ones(ext):
+    """Units of very different size in one sequence, in either order, weights split over keys."""
+    t = make(26, 1, 64, [640], 2, BF, spread=0.01)
+    for j in range(10):
+        page = t["table"][0, j].item()
+        t["c_kv"][page] *= 2.0 ** [0, 3, 11, -2, -20, 0, -30, 12, -9, 1][j]
+        t["pe"][page] *= 2.0 ** [0, 3, 11, -2, -20, 0, -30, 12, -9, 1][j]
+    t["q_nope"] *= 2.0 ** -10
+    t["q_rope"] *= 2.0 ** -10
+    check_all(t, run_paged(ext, t, False), [640], False)
+
+
+def test_beyond_four_gib(ext):
+    """Pages behind the pool's first 2^32 bytes, and their copies."""
+    P, dt = 70000, BF
+    t = make(27, 1, 70, [200], 2, dt)
+    pools = [torch.empty(P, 64, w, dtype=dt, device=DEV) for w in (R, D)]
+    last = [P - 1, P - 3, 65600, 3]
+    for n, pool in zip(("c_kv", "pe"), pools):
+        pool[last] = t[n][t["table"][0, :4].long()]
+    want = run_paged(ext, t, True)
+    t.update(c_kv=pools[0], pe=pools[1], table=i32([last]))
+    assert torch.equal(run_paged(ext, t, True), want)
+    to = [P - 2, 1, 69000, 65537]
+    ext.cache_copy_pages(i32(list(zip(last, to))), pools)
+    for pool in pools:
+        for a, b in zip(last, to):
+            pool[a] = 0
+    t["table"] = i32([to])
+    assert torch.equal(run_paged(ext, t, True), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("what", ["queries", "keys", "both", "latent rows", "half the keys"])
+def test_zeros(ext, dtype, what):
+    """Queries, keys or both of zeros: averages of what a row sees, and never NaN."""
+    t = make(28, 2, 70, [150, 40], 2, DT[dtype])
+    if what in ("queries", "both"):
+        t["q_nope"][:, ::2], t["q_rope"][:, ::2] = 0, 0
+    if what in ("keys", "both", "latent rows"):
+        t["c_kv"].zero_()
+    if what in ("keys", "both"):
+        t["pe"].zero_()
+    if what == "half the keys":
+        t["c_kv"][t["table"][0, 0].item()], t["c_kv"][:, 32:] = 0, 0
+        t["pe"] *= 2.0 ** 9
+    got = run_paged(ext, t, True)
+    if what in ("keys", "both", "latent rows"):
+        assert not got.any()
+    else:
+        check_all(t, got, [150, 40], True)
