@@ -502,3 +502,73 @@ def test_zeros(ext, dtype, what):
         assert not got.any()
     else:
         check_all(t, got, [150, 40], True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_head_groups_by_eight(ext, dtype):
+    """Groups of 8, 8 and 3 heads."""
+    H, Sq, n = 19, 70, 300
+    t = make(29, 1, Sq, [n], H, DT[dtype])
+    table = torch.zeros(1, 6250, dtype=torch.int32, device=DEV)     # 2 GiB hold ten heads of 400,000 keys
+    table[:, :t["table"].size(1)] = t["table"]
+    t["table"] = table
+    check_all(t, run_paged(ext, t, True), [n], True)
+
+
+def test_two_streams_at_once(ext):
+    """Calls that overlap, with workspaces of their own."""
+    ts = [make(30 + i, 2, 130, [400 - 50 * i, 200], 4, BF) for i in range(2)]
+    ts[1]["c_kv"][ts[1]["table"][1, 0], 3] = NAN
+    want = [run_paged(ext, t, True) for t in ts]
+    streams = [torch.cuda.Stream() for _ in ts]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run_paged(ext, ts[i], True))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        for g in gs:
+            assert torch.equal(g.isnan(), w.isnan()) and torch.equal(g.nan_to_num(), w.nan_to_num())
+
+
+def test_two_graphs_share_a_workspace(ext):
+    """Graphs of one memory pool, of other shapes, types and paths (alone, planned, split), in any order."""
+    ts = [make(32, 1, 64, [300], 2, BF), make(33, 3, 100, [500, 100, 130], 3, H16), make(34, 1, 40, [6000], 2, BF)]
+    ts[1]["c_kv"][ts[1]["table"][0, 7], 0] = NAN
+    want = [run_paged(ext, t, True) for t in ts]
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], torch.cuda.graph_pool_handle()
+    for t in ts:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            out = run_paged(ext, t, True)
+            outs.append(out)
+    for i in (0, 1, 2, 1, 0, 2, 2, 0, 1, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        g = outs[i].clone()
+        assert torch.equal(g.isnan(), want[i].isnan()) and torch.equal(g.nan_to_num(), want[i].nan_to_num())
+        run_paged(ext, ts[(i + 1) % 3], True)
+        torch.cuda.synchronize()
+
+
+def test_many_sequences_of_one_prompt(ext):
+    """More sequences behind one first page than a plan compares with each other, and none of them wrong."""
+    B = 1100
+    t = make(35, 1, 2, [64], 1, BF)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(36)
+    P = 1 + 2 * B
+    c_kv, pe = normal(g, P, 64, R, dtype=BF), normal(g, P, 64, D, dtype=BF)
+    table = torch.arange(1, P, dtype=torch.int32, device=DEV).reshape(B, 2)
+    table[:, 0] = 0
+    table[1::2, 1] = 2                                  # and half of them behind a second page too
+    t.update(c_kv=c_kv, pe=pe, table=table, lens=i32([70 + b % 59 if b % 2 == 0 else 128 for b in range(B)]),
+             q_nope=normal(g, B, 2, 1, N, dtype=BF), q_rope=normal(g, B, 2, 1, D, dtype=BF))
+    got = run_paged(ext, t, True)
+    for b in (0, 1, 2, 3, 500, 501, 1023, 1024, 1025, 1026, 1098, 1099):
+        one = {**t, "table": table[b:b + 1].clone(), "lens": t["lens"][b:b + 1].clone(), "q_nope": t["q_nope"][b:b + 1],
+               "q_rope": t["q_rope"][b:b + 1]}
+        assert torch.equal(run_paged(ext, one, True)[0], got[b]), b

@@ -296,3 +296,41 @@ def test_shared_prompt_step(ext, blocked):
     head, count = state.tolist()
     free = [ring[(head + i) % P].item() for i in range(count)]
     assert sorted(free + list(held)) == list(range(P))
+
+
+# where one workgroup's waves become more, and one launch becomes several
+EDGES = [(256, 14, 4096), (257, 14, 4096), (256, 14, 4097), (1024, 14, 16384), (1024, 14, 16385), (1025, 14, 16384),
+         (4100, 3, 13000)]
+
+
+@pytest.mark.parametrize("B,max_pages,N", EDGES)
+def test_edges(ext, B, max_pages, N):
+    r = random.Random(B + N)
+    table, lens, ring, head, count = batch(r, B, max_pages, 64, N)
+    check_fork(ext, *plan(r, B, max_pages, 64), lens, table, ring, head, count, 64)
+    check_compact(ext, lens, table, ring, head, count, 64)
+
+
+def test_two_streams_at_once(ext):
+    """Large pools' calls that overlap, with workspaces of their own."""
+    r = random.Random(3)
+    made, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for N in (20000, 30000):
+        table, lens, ring, head, count = batch(r, 40, 100, 64, N)
+        parents, keep = plan(r, 40, 100, 64)
+        made.append((i32(parents), i32(keep), i32(lens), i32(table), i32(ring), i32([head, count])))
+
+    def calls(m):
+        ring = m[4].clone()
+        fork = ext.cache_fork(m[0], m[1], m[2], m[3], ring, m[5], 64)
+        return [ring] + fork + ext.cache_compact(fork[0], fork[1], ring, fork[2], 64)
+    want = [calls(m) for m in made]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(calls(made[i]))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        assert all(torch.equal(a, b) for g in gs for a, b in zip(g, w))
