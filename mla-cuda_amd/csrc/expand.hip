@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cstdlib>
+#include <type_traits>
 
 #include "kernels.h"
 #include "mma.h"
@@ -116,7 +117,9 @@ __global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
 }
 
 // ---- gather ---------------------------------------------------------------------------------
-// A workgroup copies a unit's rows, or only notes where its owner's are.
+// A workgroup copies a unit's rows, or only notes where its owner's are.  Few units are bound by the way to
+// memory and back, many by their bytes: 512 rows 7.1 us, 4,096 9.1, 32,768 16.8 (4.5 TB/s), 24,576 of the 8-bit
+// cache 14.4 (with four waves instead of eight and loads behind tests of their own 9.3, 11.5, 19.5 and 22.2).
 // Keys, values and weights are fp16 from here on, in bf16 too: 11 bits instead of 8 bring the outputs'
 // distance from the exact ones from 1.6 to 2.3 times that of their own rounding down to about it (bf16).
 // A bf16 cache is fitted into fp16's range by a power of two for each unit, 2^e: its rows are stored
@@ -181,13 +184,19 @@ __device__ __forceinline__ float finite_max(float m, float x) {
     return x < INFINITY ? fmaxf(m, x) : m;
 }
 
+constexpr int kGatherThreads = 512, kGatherWaves = kGatherThreads / 64;
+constexpr int kWaveRows = kUnit / kGatherWaves;
+
 template <typename TL, bool F8>
-__global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
-    __shared__ int part[4], w_bad[4];
+__global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArgs a) {
+    __shared__ int part[kGatherWaves], w_bad[kGatherWaves];
     __shared__ float row_top[2][kUnit];     // latent, rope
     const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.Sk) : a.Sk;
+    const int k0 = j * kUnit;
+    // (with the length, not behind it; the table spans all units)
+    const int page = a.table ? load_uniform(a.table + (int64_t)b * a.max_pages + k0 / a.page_size) : 0;
+    const int len = a.seq_lens ? min(max(load_uniform(a.seq_lens + b), 0), a.Sk) : a.Sk;
     const bool first = j == 0 && b == 0;
     const bool here = j * kUnit < len;
     if (!here && !first) return;     // the first workgroup leaves the number of rows, whatever it has
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
         own = here ? a.owner[at] : 0;
         // units of the sequences in front of the owner; the first workgroup also adds up all of them
         int sum = 0, all = 0;
-        for (int c = tid; c < (first ? a.B : own); c += 256) {
+        for (int c = tid; c < (first ? a.B : own); c += kGatherThreads) {
             const int n = a.count[c];
             all += n;
             sum += c < own ? n : 0;
@@ -205,13 +214,18 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
         sum = wave_sum(sum);
         if (lane == 0) part[wave] = sum;
         __syncthreads();
-        sum = part[0] + part[1] + part[2] + part[3];
+        auto total = [&]() __attribute__((always_inline)) {
+            int n = 0;
+            for (int w = 0; w < kGatherWaves; ++w) n += part[w];
+            return n;
+        };
+        sum = total();
         if (first) {
             __syncthreads();
             all = wave_sum(all);
             if (lane == 0) part[wave] = all;
             __syncthreads();
-            if (tid == 0) *a.rows = kUnit * (part[0] + part[1] + part[2] + part[3]);
+            if (tid == 0) *a.rows = kUnit * total();
         }
         if (!here) return;
         place = sum + a.rank[(int64_t)own * a.units + j];
@@ -225,68 +239,75 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
     if (!here) return;
 
     // where the unit's rows lie (a page is a whole number of units)
-    const int k0 = j * kUnit;
     int64_t r0 = (int64_t)b * a.Sk + k0;
     bool in = true;
     if (a.table) {
-        const int page = a.table[(int64_t)b * a.max_pages + k0 / a.page_size];
         in = page >= 0 && page < a.num_pages;
         r0 = (int64_t)page * a.page_size + k0 % a.page_size;
     }
     const int n = in ? min(kUnit, len - k0) : 0;
     uint16_t* lat = a.lat + (int64_t)place * kUnit * kR;
     uint16_t* rot = a.rot + (int64_t)place * kUnit * kD;
-    // latent rows: 16 a wave, 8 columns a lane; rope rows: 8 lanes a row, 2 of 8 columns a thread
-    v4u x[16], y[2];
+    // latent rows: 8 columns a lane; rope rows: 8 lanes a row.  All loads before their first use: rows behind the end
+    // read the last one, and are zeros.  A wave's rows, of both, are in one block of scales.
+    static_assert(kWaveRows == 8, "a wave's latent and rope rows are the same 8");
+    v4u x[kWaveRows], y;
+    const int w0 = kWaveRows * wave, yr = tid >> 3;
     #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int r = 16 * wave + i;
-        x[i] = v4u{0, 0, 0, 0};
-        if (r >= n) continue;
+    for (int i = 0; i < kWaveRows; ++i) x[i] = v4u{0, 0, 0, 0};
+    y = v4u{0, 0, 0, 0};
+    if (n > 0) {
+        typedef std::conditional_t<F8, v2u_t, v4u> Raw;
+        constexpr int kSize = F8 ? 1 : 2;
+        const uint8_t* lat_in = static_cast<const uint8_t*>(a.c_kv) + r0 * (kR * kSize);
+        const uint8_t* rot_in = static_cast<const uint8_t*>(a.pe) + r0 * (kD * kSize);
+        Raw u[kWaveRows], v;
+        float f = 1.f, g = 1.f;
         if constexpr (F8) {
-            const v2u_t c = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.c_kv) + (r0 + r) * kR)[lane];
-            const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift)] << 23);
-            const v2u_t lo = decode_half4<TL>(c[0], f), hi = decode_half4<TL>(c[1], f);
-            x[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
-        } else {
-            x[i] = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.c_kv) + (r0 + r) * kR)[lane];
+            const uint8_t* s = a.scales + 2 * ((r0 + w0) >> a.block_shift);
+            f = __uint_as_float((uint32_t)s[0] << 23);
+            g = __uint_as_float((uint32_t)s[1] << 23);
         }
-    }
-    #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = 32 * i + (tid >> 3), c = tid & 7;
-        y[i] = v4u{0, 0, 0, 0};
-        if (r >= n) continue;
-        if constexpr (F8) {
-            const v2u_t w = reinterpret_cast<const v2u_t*>(static_cast<const uint8_t*>(a.pe) + (r0 + r) * kD)[c];
-            const float f = __uint_as_float((uint32_t)a.scales[2 * ((r0 + r) >> a.block_shift) + 1] << 23);
-            const v2u_t lo = decode_half4<TL>(w[0], f), hi = decode_half4<TL>(w[1], f);
-            y[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
-        } else {
-            y[i] = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(a.pe) + (r0 + r) * kD)[c];
+        #pragma unroll
+        for (int i = 0; i < kWaveRows; ++i) u[i] = reinterpret_cast<const Raw*>(lat_in + min(w0 + i, n - 1) * (kR * kSize))[lane];
+        v = reinterpret_cast<const Raw*>(rot_in + min(yr, n - 1) * (kD * kSize))[tid & 7];
+        #pragma unroll
+        for (int i = 0; i < kWaveRows; ++i) {
+            if (w0 + i >= n) continue;
+            if constexpr (F8) {
+                const v2u_t lo = decode_half4<TL>(u[i][0], f), hi = decode_half4<TL>(u[i][1], f);
+                x[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
+            } else {
+                x[i] = u[i];
+            }
+        }
+        if (yr < n) {
+            if constexpr (F8) {
+                const v2u_t lo = decode_half4<TL>(v[0], g), hi = decode_half4<TL>(v[1], g);
+                y = v4u{lo[0], lo[1], hi[0], hi[1]};
+            } else {
+                y = v;
+            }
         }
     }
     int worst = kUnit;
-    float rope_top[2] = {0.f, 0.f};
     if constexpr (!Half<TL>::kF16) {
+        float top = 0.f;
         #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const v2f_t v = halves<TL>(y[i][k]);
-                rope_top[i] = finite_max(finite_max(rope_top[i], v[0]), v[1]);
-            }
-            #pragma unroll
-            for (int k = 1; k < 8; k *= 2) rope_top[i] = fmaxf(rope_top[i], __shfl_xor(rope_top[i], k));
-            if ((tid & 7) == 0) row_top[1][32 * i + (tid >> 3)] = rope_top[i];
+        for (int k = 0; k < 4; ++k) {
+            const v2f_t v = halves<TL>(y[k]);
+            top = finite_max(finite_max(top, v[0]), v[1]);
         }
+        #pragma unroll
+        for (int k = 1; k < 8; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+        if ((tid & 7) == 0) row_top[1][yr] = top;
     }
     #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < kWaveRows; ++i) {
         const bool odd = not_finite2<TL>(x[i][0]) || not_finite2<TL>(x[i][1]) || not_finite2<TL>(x[i][2]) ||
                          not_finite2<TL>(x[i][3]);
         if (__builtin_amdgcn_ballot_w64(odd) != 0) {
-            worst = min(worst, 16 * wave + i);
+            worst = min(worst, w0 + i);
             x[i] = v4u{0, 0, 0, 0};
         }
         if constexpr (!Half<TL>::kF16) {
@@ -297,12 +318,12 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
                 top = fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1])));
             }
             top = wave_reduce(top, OpMax());
-            if (lane == 0) row_top[0][16 * wave + i] = top;
+            if (lane == 0) row_top[0][w0 + i] = top;
         }
     }
     if (lane == 0) w_bad[wave] = worst;
     __syncthreads();
-    worst = min(min(w_bad[0], w_bad[1]), min(w_bad[2], w_bad[3]));
+    for (int w = 0; w < kGatherWaves; ++w) worst = min(worst, w_bad[w]);
     // the unit's exponent, and whether its latent rows (those that are not zero) keep near it; in a mixed unit
     // those that are zero count as its largest latent row
     int e = 0, lat_e = 0, rope_e = 0;
@@ -322,31 +343,28 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
         if (a.any_bad && worst < kUnit) *a.any_bad = 1;   // cleared by the plan; every writer writes the same
     }
     #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < kWaveRows; ++i) {
         v4u o = x[i];
         if constexpr (!Half<TL>::kF16) {
-            const float f = two_to(-__builtin_amdgcn_readlane(lat_e, 16 * wave + i));
+            const float f = two_to(-__builtin_amdgcn_readlane(lat_e, w0 + i));
             #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const v2f_t v = halves<TL>(x[i][k]);
                 o[k] = Half<TL>::pack2(v[0] * f, v[1] * f);
             }
         }
-        reinterpret_cast<v4u*>(lat + (16 * wave + i) * kR)[lane] = o;
+        reinterpret_cast<v4u*>(lat + (w0 + i) * kR)[lane] = o;
     }
-    #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        v4u o = y[i];
-        if constexpr (!Half<TL>::kF16) {
-            const float f = two_to(-__shfl(rope_e, 32 * i + (tid >> 3)));
-            #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const v2f_t v = halves<TL>(y[i][k]);
-                o[k] = pack_f16x2(v[0] * f, v[1] * f);
-            }
+    v4u o = y;
+    if constexpr (!Half<TL>::kF16) {
+        const float f = two_to(-__shfl(rope_e, yr));
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const v2f_t v = halves<TL>(y[k]);
+            o[k] = pack_f16x2(v[0] * f, v[1] * f);
         }
-        reinterpret_cast<v4u*>(rot + (32 * i + (tid >> 3)) * kD)[tid & 7] = o;
     }
+    reinterpret_cast<v4u*>(rot + yr * kD)[tid & 7] = o;
 }
 
 // ---- attention ------------------------------------------------------------------------------
@@ -368,12 +386,15 @@ __global__ void __launch_bounds__(256) expand_gather_kernel(GatherArgs a) {
 // exponentials would lose it: there they stay without it, and the values' product, for rows of like
 // exponents at a time, is scaled in float32.  Such steps are done outside the loop of the ordinary ones, which
 // so keeps its registers (inside it they cost up to 28%).  bf16 queries are made fp16 under a power of two of their own.
-// What bounds it: the matrix cores' power and the order of two waves on a SIMD.  4,096 causal rows of 128 heads
-// 725 us, 948 TFLOP/s (a large fp16 library product 1,318); the cores are busy 0.46 of the cycles, and
-// with operands of zeros a fifth faster.  A step without the exponentials takes 6% less, without its loads
-// 10%.  Other structures, each on one card against this one: the next step's scores and the last one's
-// values between the exponentials of a step (+6%), the same with 64 rows a wave in 512 registers (+60%) or
-// eight waves a workgroup (+10%), loads between the score MFMAs (+12%), the MFMAs at a higher wave priority
+// What bounds it: the matrix cores' power.  4,096 causal rows of 128 heads 725 to 790 us by the card, 870 to 948
+// TFLOP/s; 2,048 rows over 32,768 keys of 16 heads 650, 1,000 TFLOP/s (a large fp16 library product 1,318).  The
+// second, without exponentials, reads of fragments and all else but its matrix instructions, barriers and loads of
+// stages, takes 86% of its time, and the cores are busy 0.46 of the cycles, at the clock that they leave; with
+// operands of zeros it is a fifth faster.  Other structures, each on one card against this one: the next step's
+// scores and the last one's values between the exponentials of a step (+6%), the same with 64 rows a wave in 512
+// registers (+60%) or eight waves a workgroup (+10%); eight waves of which four have matrix instructions between
+// two barriers while four have exponentials (-3% where most keys are visible, +4 to +10% where tiles of 256 rows
+// meet the diagonal or a chunk's end); loads between the score MFMAs (+12%), the MFMAs at a higher wave priority
 // (+1%), windows of 3 and 4 fragments (+0.3%, +1.5%), left to the compiler's order (+5%).
 struct HeadsArgs {
     const uint16_t* qn;      // [B, Sq, H, 128]
@@ -914,11 +935,11 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     g.block_shift = p.scale_block == 16 ? 4 : p.scale_block == 32 ? 5 : 6;
     const dim3 gather((unsigned)plan.units, (unsigned)p.B);
     if (p.scales) {
-        if (p.f16) hipLaunchKernelGGL((expand_gather_kernel<f16_t, true>), gather, dim3(256), 0, stream, g);
-        else hipLaunchKernelGGL((expand_gather_kernel<bf16_t, true>), gather, dim3(256), 0, stream, g);
+        if (p.f16) hipLaunchKernelGGL((expand_gather_kernel<f16_t, true>), gather, dim3(kGatherThreads), 0, stream, g);
+        else hipLaunchKernelGGL((expand_gather_kernel<bf16_t, true>), gather, dim3(kGatherThreads), 0, stream, g);
     } else {
-        if (p.f16) hipLaunchKernelGGL((expand_gather_kernel<f16_t, false>), gather, dim3(256), 0, stream, g);
-        else hipLaunchKernelGGL((expand_gather_kernel<bf16_t, false>), gather, dim3(256), 0, stream, g);
+        if (p.f16) hipLaunchKernelGGL((expand_gather_kernel<f16_t, false>), gather, dim3(kGatherThreads), 0, stream, g);
+        else hipLaunchKernelGGL((expand_gather_kernel<bf16_t, false>), gather, dim3(kGatherThreads), 0, stream, g);
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
