@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
 
 // ---- gather ---------------------------------------------------------------------------------
 // A workgroup copies a unit's rows, or only notes where its owner's are.  Few units are bound by the way to
-// memory and back, many by their bytes: 512 rows 7.1 us, 4,096 9.1, 32,768 16.8 (4.5 TB/s), 24,576 of the 8-bit
+// memory and back, many by their bytes: 512 rows 7.1 us, 4,096 9.1, 32,768 16.8 (4.5 TB/s), 13,216 of the 8-bit
 // cache 14.4 (with four waves instead of eight and loads behind tests of their own 9.3, 11.5, 19.5 and 22.2).
 // Keys, values and weights are fp16 from here on, in bf16 too: 11 bits instead of 8 bring the outputs'
 // distance from the exact ones from 1.6 to 2.3 times that of their own rounding down to about it (bf16).
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArg
 // What bounds it: the matrix cores' power.  4,096 causal rows of 128 heads 725 to 790 us by the card, 870 to 948
 // TFLOP/s; 2,048 rows over 32,768 keys of 16 heads 650, 1,000 TFLOP/s (a large fp16 library product 1,318).  The
 // second, without exponentials, reads of fragments and all else but its matrix instructions, barriers and loads of
-// stages, takes 86% of its time, and the cores are busy 0.46 of the cycles, at the clock that they leave; with
+// stages, takes 86% of its time; the cores are busy 0.55 and 0.66 of the cycles, at the clock that they leave; with
 // operands of zeros it is a fifth faster.  Other structures, each on one card against this one: the next step's
 // scores and the last one's values between the exponentials of a step (+6%), the same with 64 rows a wave in 512
 // registers (+60%) or eight waves a workgroup (+10%); eight waves of which four have matrix instructions between
