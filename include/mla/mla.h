@@ -540,7 +540,8 @@ int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
  * On inputs of unit spread the outputs' relative distance (RMS) from the exact ones is 1.7e-3 in bf16 (the output's
  * own rounding 1.66e-3; the absorbed form 2.5 to 3.8e-3) and 2.6 to 3.7e-4 in fp16, up to 5e-4 over the 8-bit cache
  * (rounding 2.1e-4; the absorbed form as here).
- * The workspace holds keys and values of as many heads at a time as 2 GiB take (one at least). */
+ * The workspace holds keys and values of as many heads at a time as 2 GiB take (one at least), and 1.2 KB for each
+ * key of batch * dims->sk: of a wide table give the columns up to the longest sequence's (grids go by them too). */
 size_t mla_attention_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims, int causal);
 int mla_attention_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
                            const void* q_rope, const void* c_kv, const void* pe_cache,
