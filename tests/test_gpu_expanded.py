@@ -572,3 +572,39 @@ def test_many_sequences_of_one_prompt(ext):
         one = {**t, "table": table[b:b + 1].clone(), "lens": t["lens"][b:b + 1].clone(), "q_nope": t["q_nope"][b:b + 1],
                "q_rope": t["q_rope"][b:b + 1]}
         assert torch.equal(run_paged(ext, one, True)[0], got[b]), b
+
+
+def test_most_sequences(ext):
+    """As many sequences as a call takes, all behind one page or none, one key each or a page and one."""
+    B = 65535
+    g = torch.Generator(device=DEV)
+    g.manual_seed(37)
+    t = make(38, 1, 1, [64], 1, BF)
+    P = 3000
+    table = torch.stack((torch.zeros(B, dtype=torch.int32, device=DEV),
+                         torch.arange(B, dtype=torch.int32, device=DEV) % (P - 1) + 1), 1).contiguous()
+    lens = i32([65, 1, 0] * (B // 3))
+    t.update(c_kv=normal(g, P, 64, R, dtype=BF), pe=normal(g, P, 64, D, dtype=BF), table=table, lens=lens,
+             q_nope=normal(g, B, 1, 1, N, dtype=BF), q_rope=normal(g, B, 1, 1, D, dtype=BF))
+    got = run_paged(ext, t, True)
+    assert not got[2::3].any()
+    for b in (0, 1, 3, 4, 1500, 1501, 4095, 32768, 65532, 65533):
+        one = {**t, "table": table[b:b + 1].clone(), "lens": lens[b:b + 1].clone(),
+               "q_nope": t["q_nope"][b:b + 1], "q_rope": t["q_rope"][b:b + 1]}
+        assert torch.equal(run_paged(ext, one, True)[0], got[b]), b
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [5, 128, 700])
+def test_q_heads_apart(ext, dtype, rows, monkeypatch):
+    """With RoPE in a launch of its own the same queries, bit for bit."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(39)
+    H, hidden, ql, dt = 16, 512, 256, DT[dtype]
+    args = (normal(g, 1, rows, hidden, dtype=dt), normal(g, hidden, ql, dtype=dt, std=hidden ** -0.5),
+            torch.ones(ql, dtype=dt, device=DEV), normal(g, ql, H * (N + D), dtype=dt, std=ql ** -0.5),
+            torch.arange(rows, device=DEV) + 40, N, D, 1e-6)
+    want = ext.q_heads(*args)
+    monkeypatch.setenv("MLA_QUP_FUSE", "0")
+    got = ext.q_heads(*args)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
