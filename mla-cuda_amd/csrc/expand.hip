@@ -435,10 +435,14 @@ __device__ __forceinline__ uint32_t to_half2(float x, float y) {
     return Half<TL>::pack2(x, y);
 }
 
-template <typename TL, bool SPLIT>
+// PAIR: chunks of up to 64 rows, which two waves have; the other two take the second half of each step's keys, and
+// the halves are joined at the end (a call of 64 rows over 512 keys 49.2 -> 46.2 us, eight of 64 over 512 240 -> 233,
+// 64 over 8,256 485 -> 478).
+template <typename TL, bool SPLIT, bool PAIR>
 __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStageBytes];
     constexpr float kRise = 6.f, kBias = 8.f;
+    constexpr int KB = PAIR ? 1 : 2;              // 32 keys, of a step's 64, a wave
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, q = lane & 31;
     const uint32_t lds0 = lds_addr(smem);
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     auto lim_of = [&](int row) __attribute__((always_inline)) {
         return a.causal ? min(len - a.Sq + row, len - 1) : len - 1;
     };
-    const int w0 = r0 + 32 * wave;
+    const int w0 = r0 + 32 * (PAIR ? wave & 1 : wave), kh = PAIR ? 32 * (wave >> 1) : 0;   // first row, and key of a step
     const int row = min(w0 + q, a.Sq - 1);
     const int lim = lim_of(row);
     const int wave_first = w0 < a.Sq ? lim_of(w0) : -1, wave_last = w0 < a.Sq ? lim_of(min(w0 + 31, a.Sq - 1)) : -1;
@@ -544,9 +548,9 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     };
 
     // ---- fragments
-    const uint32_t k_rd = (uint32_t)q * 64 + 16 * (hi ^ ((q >> 2) & 3));
+    const uint32_t k_rd = (uint32_t)(kh + q) * 64 + 16 * (hi ^ ((q >> 2) & 3));
     const int G4 = lane >> 4, q4 = (lane >> 2) & 3, i4 = lane & 3;
-    const uint32_t v_rd = (uint32_t)(4 * (G4 >> 1) + q4) * 64 + 32 * (G4 & 1) + 8 * i4;
+    const uint32_t v_rd = (uint32_t)(kh + 4 * (G4 >> 1) + q4) * 64 + 32 * (G4 & 1) + 8 * i4;
     typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
     auto k_frag = [&](uint32_t st, int kb, int i) __attribute__((always_inline)) {   // i: 16 of 192 columns
@@ -586,12 +590,12 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             next = j + 2 < n_tiles ? load_uniform(units + j + 2) : 0;
         }
     };
-    auto hide = [&](v16f (&s)[2]) __attribute__((always_inline)) {
+    auto hide = [&](v16f (&s)[KB]) __attribute__((always_inline)) {
         if (j * kUnit + kUnit - 1 <= wave_first) return;
-        int past = lim - j * kUnit - 4 * hi;                // (opaque: 32 differences are not to stay in registers)
+        int past = lim - j * kUnit - kh - 4 * hi;                // (opaque: 32 differences are not to stay in registers)
         asm volatile("" : "+v"(past));
         #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
             #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + acc_row(i, 0) <= past ? s[kb][i] : -INFINITY;
     };
@@ -613,12 +617,12 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     // Moves the references of rows whose scores passed them (those only: a row's bits do not depend on the others
     // of its wave).  Past 2^24 a reference is off its own score by more than a power of two, which a fused
     // product would show: `huge`.
-    auto refer = [&](const v16f (&s)[2], float ct) __attribute__((always_inline)) {
+    auto refer = [&](const v16f (&s)[KB], float ct) __attribute__((always_inline)) {
         float top = fmaxf(s[0][0], s[0][1]);
         #pragma unroll
         for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(s[0][i], s[0][i + 1]), top);
         #pragma unroll
-        for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(s[1][i], s[1][i + 1]), top);
+        for (int i = 16; i < 16 * KB; i += 2) top = fmaxf(fmaxf(s[i >> 4][i & 15], s[i >> 4][(i & 15) + 1]), top);
         if (__builtin_amdgcn_ballot_w64(top * ct > m_ref + kRise)) {
             const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * ct;
@@ -636,17 +640,19 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         #pragma unroll 1
         for (; j < n_tiles; ++j) {
             begin();
-            if (j * kUnit > wave_last) continue;
+            if (j * kUnit + kh > wave_last) continue;
             if (__builtin_expect(huge || ee > kMixed / 2 || E - ee > 8, 0)) break;
             // scores; a fragment's place is read again as soon as it is used
-            v16f s[2] = {v16f{}, v16f{}};
-            v4u kf[kWinK][2];
+            v16f s[KB] = {};
+            v4u kf[kWinK][KB];
             #pragma unroll
-            for (int i = 0; i < kWinK; ++i) { kf[i][0] = k_frag(st, 0, i); kf[i][1] = k_frag(st, 1, i); }
+            for (int i = 0; i < kWinK; ++i)
+                #pragma unroll
+                for (int kb = 0; kb < KB; ++kb) kf[i][kb] = k_frag(st, kb, i);
             #pragma unroll
             for (int i = 0; i < 12; ++i) {
                 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
+                for (int kb = 0; kb < KB; ++kb) {
                     s[kb] = Mma<f16_t>::sub(kf[i % kWinK][kb], qf[i], 0, s[kb]);
                     if (i + kWinK < 12) kf[i % kWinK][kb] = k_frag(st, kb, i + kWinK);
                 }
@@ -661,9 +667,9 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             const int d = ee - E;
             const float neg = (m_ref == -INFINITY ? 0.f : kBias - m_ref) + (float)d;
             float sum = 0.f;
-            v4u p[4];
+            v4u p[2 * KB];
             #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 8 * KB; ++i) {
                 const int kb = i >> 3, k = 2 * (i & 7);
                 const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k], ct, neg));
                 const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][k + 1], ct, neg));
@@ -677,9 +683,9 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             #pragma unroll
             for (int i = 0; i < kWinV; ++i) vf[i] = v_frag(st, i);
             #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 8 * KB; ++i) {
                 o[i & 3] = Mma<f16_t>::sub(vf[i % kWinV], p[i >> 2], 0, o[i & 3]);
-                if (i + kWinV < 16) vf[i % kWinV] = v_frag(st, i + kWinV);
+                if (i + kWinV < 8 * KB) vf[i % kWinV] = v_frag(st, i + kWinV);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -690,16 +696,16 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         const int e = mixed ? ee - kMixed : ee;
         const int* const rows = a.row_exps + (int64_t)place * 2 * kUnit;
         auto row_exps = [&](int rope, int kb, int i) __attribute__((always_inline)) {   // 4 keys from 8 i + 4 h on
-            return mixed ? *reinterpret_cast<const v4i*>(rows + kUnit * rope + 32 * kb + 8 * i + 4 * hi) : v4i{e, e, e, e};
+            return mixed ? *reinterpret_cast<const v4i*>(rows + kUnit * rope + kh + 32 * kb + 8 * i + 4 * hi) : v4i{e, e, e, e};
         };
         const int mine = mixed ? rows[lane] : e;           // row `lane`
         int ev = mine;
         #pragma unroll
         for (int i = 1; i < 64; i *= 2) ev = max(ev, __shfl_xor(ev, i));
         ev = __builtin_amdgcn_readfirstlane(ev);
-        v16f s[2];
+        v16f s[KB];
         #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < KB; ++kb) {
             v16f r = {};
             s[kb] = v16f{};
             #pragma unroll
@@ -723,7 +729,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         const float m = m_ref == -INFINITY ? 0.f : m_ref;
         float sum = 0.f;
         #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
             #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[kb][i] = __builtin_amdgcn_exp2f(fp32_pinned(s[kb][i] * ct) - m + kBias);
@@ -733,9 +739,9 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         int level = ev;
         #pragma unroll 1
         while (true) {
-            v4u p[4];
+            v4u p[2 * KB];
             #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4 * KB; ++i) {
                 const v4i x = row_exps(0, i >> 2, i & 3);
                 #pragma unroll
                 for (int k = 0; k < 4; k += 2) {
@@ -753,7 +759,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             for (int vb = 0; vb < 4; ++vb) {
                 v16f t = {};
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) t = Mma<f16_t>::sub(v_frag(st, 4 * i + vb), p[i], 0, t);
+                for (int i = 0; i < 2 * KB; ++i) t = Mma<f16_t>::sub(v_frag(st, 4 * i + vb), p[i], 0, t);
                 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[vb][i] = __builtin_fmaf(t[i], f, o[vb][i]);
             }
@@ -770,6 +776,31 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     {
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
         l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    if constexpr (PAIR) {
+        // 16 KB of outputs, references, sums and powers of two from each wave of the second halves
+        float* const theirs = reinterpret_cast<float*>(smem) + (wave & 1) * (67 * 64) + lane;
+        __syncthreads();
+        if (kh) {
+            #pragma unroll
+            for (int i = 0; i < 64; ++i) theirs[64 * i] = o[i >> 4][i & 15];
+            theirs[64 * 64] = m_ref;
+            theirs[64 * 65] = l;
+            theirs[64 * 66] = __int_as_float(E);
+        }
+        __syncthreads();
+        if (kh) return;
+        const float m1 = theirs[64 * 64], l1 = theirs[64 * 65];
+        const int E1 = __float_as_int(theirs[64 * 66]), top = max(E, E1);
+        const float m = fmaxf(m_ref, m1);
+        float f0 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m_ref - m), f1 = l1 == 0.f ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
+        l = l * f0 + l1 * f1;
+        f0 = top - E > 126 ? 0.f : f0 * two_to(E - top);
+        f1 = top - E1 > 126 ? 0.f : f1 * two_to(E1 - top);
+        m_ref = m;
+        E = top;
+        #pragma unroll
+        for (int i = 0; i < 64; ++i) o[i >> 4][i & 15] = o[i >> 4][i & 15] * f0 + theirs[64 * i] * f1;
     }
     float f = l == 0.f ? 0.f : two_to(E) / l;
     if (!a.any_bad || load_uniform(a.any_bad)) {
@@ -833,6 +864,12 @@ __global__ void __launch_bounds__(256) heads_merge_kernel(HeadsArgs a) {
     const float f = total == 0.f ? 0.f : 1.f / total;
     uint16_t* const dst = a.out + (bi * a.H + a.h0 + hl) * kN;
     reinterpret_cast<v2u_t*>(dst)[lane] = v2u_t{to_half2<TL>(o[0] * f, o[1] * f), to_half2<TL>(o[2] * f, o[3] * f)};
+}
+
+template <typename TL, bool SPLIT>
+void launch_heads(const HeadsArgs& a, dim3 grid, hipStream_t stream) {
+    if (a.Sq <= 64) hipLaunchKernelGGL((heads_kernel<TL, SPLIT, true>), grid, dim3(kHThreads), 0, stream, a);
+    else hipLaunchKernelGGL((heads_kernel<TL, SPLIT, false>), grid, dim3(kHThreads), 0, stream, a);
 }
 
 // ---- queries per head -----------------------------------------------------------------------
@@ -975,18 +1012,18 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
         e = launch_kv_expand(k, stream);
         if (e != hipSuccess) return e;
         a.h0 = h0; a.heads = heads;
-        const dim3 grid((unsigned)(tiles * p.B * heads * plan.splits)), block(kHThreads);
+        const dim3 grid((unsigned)(tiles * p.B * heads * plan.splits));
         if (plan.splits > 1) {
-            if (p.f16) hipLaunchKernelGGL((heads_kernel<f16_t, true>), grid, block, 0, stream, a);
-            else hipLaunchKernelGGL((heads_kernel<bf16_t, true>), grid, block, 0, stream, a);
+            if (p.f16) launch_heads<f16_t, true>(a, grid, stream);
+            else launch_heads<bf16_t, true>(a, grid, stream);
             e = hipGetLastError();
             if (e != hipSuccess) return e;
             const dim3 merge((unsigned)(((int64_t)p.B * p.Sq * heads + 7) / 8));
             if (p.f16) hipLaunchKernelGGL(heads_merge_kernel<f16_t>, merge, dim3(256), 0, stream, a);
             else hipLaunchKernelGGL(heads_merge_kernel<bf16_t>, merge, dim3(256), 0, stream, a);
         } else {
-            if (p.f16) hipLaunchKernelGGL((heads_kernel<f16_t, false>), grid, block, 0, stream, a);
-            else hipLaunchKernelGGL((heads_kernel<bf16_t, false>), grid, block, 0, stream, a);
+            if (p.f16) launch_heads<f16_t, false>(a, grid, stream);
+            else launch_heads<bf16_t, false>(a, grid, stream);
         }
         e = hipGetLastError();
         if (e != hipSuccess) return e;

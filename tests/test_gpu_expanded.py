@@ -608,3 +608,37 @@ def test_q_heads_apart(ext, dtype, rows, monkeypatch):
     monkeypatch.setenv("MLA_QUP_FUSE", "0")
     got = ext.q_heads(*args)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("Sq", [1, 33, 64, 65])
+@pytest.mark.parametrize("at", [0, 31, 32, 200, 270, 299])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_a_large_row_and_few_queries(ext, Sq, at, splits, monkeypatch):
+    """A key whose latent row is 2^13 times the others', under queries that are as much smaller, so that
+    scores are ordinary and the row shows in its values.  A row's distance is at most its output's rounding
+    (2^-9), twice what the scores are off (2^-11 sum |q k| / scale, some 2^-11 * 6, in weights and in their sum), and
+    a half step of 11 bits for weights and values each: 0.0088."""
+    monkeypatch.setenv("MLA_EXPAND_SPLITS", str(splits))
+    t = make(40 + Sq, 1, Sq, [300], 2, BF)
+    t["q_nope"] *= 2.0 ** -13
+    page, row = t["table"][0, at // 64].item(), at % 64
+    t["c_kv"][page, row] *= 2.0 ** 13
+    got = run_paged(ext, t, True)[0]
+    ref = E.attention(t["q_nope"][0], t["q_rope"][0], *rows_of(t, 0, 300), t["W_uk"], t["W_uv"], SCALE,
+                      E.limits(Sq, 300, Sq, True), BF)[0]
+    d, n = (got.double() - ref).norm(dim=-1), ref.norm(dim=-1)
+    assert (d <= 2 ** -6 * n).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Sq,lens,H,splits", [(1, 64, [64], 3, 1), (2, 64, [65, 1000], 8, 4), (3, 17, [32, 33, 700], 2, 64),
+                                                (1, 3, [31], 16, 2), (4, 50, [500, 0, 51, 640], 5, 3)])
+def test_few_queries(ext, dtype, B, Sq, lens, H, splits, monkeypatch):
+    monkeypatch.setenv("MLA_EXPAND_SPLITS", str(splits))
+    t = make(60 + Sq, B, Sq, lens, H, DT[dtype])
+    for causal in (True, False):
+        got = run_paged(ext, t, causal)
+        check_all(t, got, lens, causal)
+    t["c_kv"][t["table"][0, 0], 5] = INF
+    hurt = run_paged(ext, t, False)
+    assert hurt[0].isnan().all() and torch.equal(hurt[1:], got[1:])
