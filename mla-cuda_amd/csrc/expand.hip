@@ -386,8 +386,8 @@ __global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArg
 // exponentials would lose it: there they stay without it, and the values' product, for rows of like
 // exponents at a time, is scaled in float32.  Such steps are done outside the loop of the ordinary ones, which
 // so keeps its registers (inside it they cost up to 28%).  bf16 queries are made fp16 under a power of two of their own.
-// What bounds it: the matrix cores' power.  4,096 causal rows of 128 heads 747 us, 920 TFLOP/s; 2,048 rows over
-// 32,768 keys of 16 heads 650 to 690 by the card, 965 to 1,024 TFLOP/s (a large fp16 library product 1,318).  The
+// What bounds it: the matrix cores' power.  4,096 causal rows of 128 heads 718 us, 957 TFLOP/s; 2,048 rows over
+// 32,768 keys of 16 heads 640, 1,040 TFLOP/s (a large fp16 library product 1,318).  The
 // second, without exponentials, reads of fragments and all else but its matrix instructions, barriers and loads of
 // stages, takes 86% of its time; the cores are busy 0.57 and 0.66 of the cycles, at the clock that they leave; with
 // operands of zeros it is a fifth faster.  Other structures, each on one card against this one: the next step's
