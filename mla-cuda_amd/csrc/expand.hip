@@ -614,10 +614,11 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         scale_out(f);
     };
     bool huge = false;
-    // Moves the references of rows whose scores passed them (those only: a row's bits do not depend on the others
-    // of its wave).  Past 2^24 a reference is off its own score by more than a power of two, which a fused
-    // product would show: `huge`.
-    auto refer = [&](const v16f (&s)[KB], float ct) __attribute__((always_inline)) {
+    // Moves the references of rows whose scores passed them (those only).  Past 2^24 a reference is off its own score by
+    // more than a power of two, which a fused product would show, and so would another order of sums: `huge`.  An
+    // ordinary step that finds it leaves everything as it is to the step that is done apart, which refers to scores
+    // of its own making.
+    auto refer = [&](const v16f (&s)[KB], float ct, bool ordinary) __attribute__((always_inline)) {
         float top = fmaxf(s[0][0], s[0][1]);
         #pragma unroll
         for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(s[0][i], s[0][i + 1]), top);
@@ -628,11 +629,12 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * ct;
             const bool over = top > m_ref + kRise;
             const float m = over ? top : m_ref;
+            huge = __builtin_amdgcn_ballot_w64(fabsf(m) > 16777216.f && fabsf(m) < INFINITY) != 0;
+            if (ordinary && huge) return;
             const float f = over ? __builtin_amdgcn_exp2f(m_ref - m) : 1.f;
             m_ref = m;
             l *= f;
             scale_out(f);
-            huge = __builtin_amdgcn_ballot_w64(fabsf(m) > 16777216.f && fabsf(m) < INFINITY) != 0;
         }
     };
     #pragma unroll 1
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             // weights
             const float ct = factor(ee);
             grow(ee);
-            refer(s, ct);
+            refer(s, ct, true);
             if (__builtin_expect(huge, 0)) break;
             const int d = ee - E;
             const float neg = (m_ref == -INFINITY ? 0.f : kBias - m_ref) + (float)d;
@@ -723,7 +725,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         hide(s);
         const float ct = factor(e);
         grow(ev);
-        refer(s, ct);
+        refer(s, ct, false);
         // score and reference rounded alike; exponentials without a unit's power of two, in float32; then the values'
         // product in levels of rows whose exponents are within kSpread of the largest one left
         const float m = m_ref == -INFINITY ? 0.f : m_ref;
