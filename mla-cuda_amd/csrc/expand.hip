@@ -125,9 +125,9 @@ __global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
 // A bf16 cache is fitted into fp16's range by a power of two for each unit, 2^e: its rows are stored
 // under it, the largest value in [2^kHead, 2^(kHead+1)), and the attention puts it back.  kHead leaves
 // 2^9 above for keys and values, sums of 512 products with weights (below 1 they cannot reach fp16's
-// end), and 2^20 below down to its subnormals.  Where a latent row is more than 2^kSpread below the largest value
-// the unit is `mixed`: each latent and each rope row has a power of two of its own, so that no row, hidden or
-// not, costs another its bits.
+// end), and 2^20 below down to its subnormals.  Where a latent row (where that is zeros: a rope row) is more than
+// 2^kSpread below the largest value the unit is `mixed`: each latent and each rope row has a power of two of its own, so
+// that no row, hidden or not, costs another its bits.
 // An fp16 cache is as it is (e = 0).  The latent rows keep the type of W_uk and W_uv, which they are
 // multiplied with; the rope rows are fp16.
 // A latent row with a value that is not finite makes every key and value of it NaN or infinite, and
@@ -332,8 +332,9 @@ __global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArg
         const float top = row_top[0][lane], rope = row_top[1][lane];
         e = exponent_of(wave_reduce(fmaxf(top, rope), OpMax())) - kHead;
         lat_e = exponent_of(top > 0.f ? top : wave_reduce(top, OpMax())) - kHead;      // of row `lane`
-        mixed = __builtin_amdgcn_ballot_w64(top > 0.f && e - lat_e > kSpread) != 0;
-        rope_e = mixed && rope > 0.f ? exponent_of(rope) - kHead : e;
+        rope_e = rope > 0.f ? exponent_of(rope) - kHead : e;
+        mixed = __builtin_amdgcn_ballot_w64(e - (top > 0.f ? lat_e : rope_e) > kSpread) != 0;
+        if (!mixed) rope_e = e;
         if (!mixed) lat_e = e;
         else if (wave < 2) a.row_exps[((int64_t)place * 2 + wave) * kUnit + lane] = wave ? rope_e : lat_e;
     }
@@ -384,7 +385,9 @@ __global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArg
 // into the exponentials, as d = e - E <= 0 with the largest e so far in E (what is in the accumulators
 // is scaled when that grows); the sum takes it out again.  Where d is far below, or the unit is mixed, fp16
 // exponentials would lose it: there they stay without it, and the values' product, for rows of like
-// exponents at a time, is scaled in float32.  Such steps are done outside the loop of the ordinary ones, which
+// exponents at a time, is scaled in float32.  Where d is far above (2^kGrow, past which what is in the accumulators could
+// leave float32), too: the power of two of a row then rises where the unit has something under a weight for it, and stays
+// where the row does not see the keys that are so large.  Such steps are done outside the loop of the ordinary ones, which
 // so keeps its registers (inside it they cost up to 28%).  bf16 queries are made fp16 under a power of two of their own.
 // What bounds it: the matrix cores' power.  4,096 causal rows of 128 heads 718 us, 957 TFLOP/s; 2,048 rows over
 // 32,768 keys of 16 heads 640, 1,040 TFLOP/s (a large fp16 library product 1,318).  The
@@ -418,6 +421,8 @@ struct HeadsArgs {
 };
 
 constexpr int kHRows = 128, kHThreads = 256;
+constexpr int kLeast = 100 + kHead;          // the least unit's power of two is 2^-kLeast
+constexpr int kGrow = 32;                    // powers of two that an ordinary step raises a wave's by
 constexpr int kWinK = 2, kWinV = 3;          // fragments read ahead (keys by pairs)
 constexpr int kKBytes = kUnit * 2 * kN, kRBytes = kUnit * 2 * kD;       // a stage's parts
 constexpr int kKeyBytes = kKBytes + kRBytes;                            // keys: nope and rope columns
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         #pragma unroll
         for (int i = 0; i < 4; ++i) qf[8 + i] = *reinterpret_cast<const v4u*>(r + 16 * i);
     }
-    float c = a.c;
+    int qe = 0;                  // bf16: the row's power of two
     if constexpr (!Half<TL>::kF16) {
         float top = 0.f;
         #pragma unroll
@@ -515,9 +520,8 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                 top = finite_max(finite_max(top, v[0]), v[1]);
             }
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        const int e = min(exponent_of(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]))), 126);
-        const float f = two_to(-e);
-        c *= two_to(e);
+        qe = min(exponent_of(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]))), 126);
+        const float f = two_to(-qe);
         #pragma unroll
         for (int i = 0; i < 12; ++i)
             #pragma unroll
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
     int e_next = n_tiles > first ? load_uniform(a.exps + next) : 0;
     if (n_tiles > first) issue(next, 0);
     next = n_tiles > first + 1 ? load_uniform(units + first + 1) : 0;
-    int E = -1000;               // below any unit's
+    int E = -1000;               // below any unit's (-kLeast)
 
     // ---- steps
     int j = first, place = 0, ee = 0;
@@ -600,7 +604,9 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + acc_row(i, 0) <= past ? s[kb][i] : -INFINITY;
     };
     // (not 0, which under zero queries and keys it could round to: a hidden score times it has to stay -infinity)
-    auto factor = [&](int e) __attribute__((always_inline)) { return fmaxf(c * two_to(e), 1.17549435e-38f); };
+    auto factor = [&](int e) __attribute__((always_inline)) {
+        return fmaxf(Half<TL>::kF16 ? a.c : ldexpf(a.c, qe + e), 1.17549435e-38f);
+    };
     auto scale_out = [&](float f) __attribute__((always_inline)) {
         #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -613,7 +619,8 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         E = ev;
         scale_out(f);
     };
-    bool huge = false;
+    bool huge = false, apart = false;   // apart: the rows of the wave have powers of two of their own,
+    int Er = 0;                         // 2^Er, in place of 2^E
     // Moves the references of rows whose scores passed them (those only).  Past 2^24 a reference is off its own score by
     // more than a power of two, which a fused product would show, and so would another order of sums: `huge`.  An
     // ordinary step that finds it leaves everything as it is to the step that is done apart, which refers to scores
@@ -643,7 +650,7 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         for (; j < n_tiles; ++j) {
             begin();
             if (j * kUnit + kh > wave_last) continue;
-            if (__builtin_expect(huge || ee > kMixed / 2 || E - ee > 8, 0)) break;
+            if (__builtin_expect(huge || apart || ee > kMixed / 2 || E - ee > 8 || (ee - E > kGrow && E >= -kLeast), 0)) break;
             // scores; a fragment's place is read again as soon as it is used
             v16f s[KB] = {};
             v4u kf[kWinK][KB];
@@ -692,8 +699,8 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             }
         }
         if (j >= n_tiles) break;
-        // A step that is not ordinary.  A mixed unit's scores have its nope and rope columns each under their
-        // row's power of two, and the largest of its latent rows' is the unit's for the values.
+        // A step that is not ordinary.  A mixed unit's scores have its nope and rope columns each under their row's power
+        // of two.  They are made in their own units, 2^qe and a.c in them: nothing of a row's passes through another's.
         const bool mixed = ee > kMixed / 2;
         const int e = mixed ? ee - kMixed : ee;
         const int* const rows = a.row_exps + (int64_t)place * 2 * kUnit;
@@ -701,10 +708,6 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             return mixed ? *reinterpret_cast<const v4i*>(rows + kUnit * rope + kh + 32 * kb + 8 * i + 4 * hi) : v4i{e, e, e, e};
         };
         const int mine = mixed ? rows[lane] : e;           // row `lane`
-        int ev = mine;
-        #pragma unroll
-        for (int i = 1; i < 64; i *= 2) ev = max(ev, __shfl_xor(ev, i));
-        ev = __builtin_amdgcn_readfirstlane(ev);
         v16f s[KB];
         #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -719,13 +722,11 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                 const v4i x = row_exps(0, kb, i), y = row_exps(1, kb, i);
                 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    s[kb][4 * i + k] = ldexpf(s[kb][4 * i + k], x[k] - e) + ldexpf(r[4 * i + k], y[k] - e);
+                    s[kb][4 * i + k] = ldexpf(s[kb][4 * i + k] * a.c, x[k] + qe) + ldexpf(r[4 * i + k] * a.c, y[k] + qe);
             }
         }
         hide(s);
-        const float ct = factor(e);
-        grow(ev);
-        refer(s, ct, false);
+        refer(s, 1.f, false);
         // score and reference rounded alike; exponentials without a unit's power of two, in float32; then the values'
         // product in levels of rows whose exponents are within kSpread of the largest one left
         const float m = m_ref == -INFINITY ? 0.f : m_ref;
@@ -734,11 +735,15 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         for (int kb = 0; kb < KB; ++kb)
             #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(fp32_pinned(s[kb][i] * ct) - m + kBias);
+                s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] - m + kBias);
                 sum += s[kb][i];
             }
         l += sum;
-        int level = ev;
+        if (!apart) Er = E;
+        int level = mine;
+        #pragma unroll
+        for (int i = 1; i < 64; i *= 2) level = max(level, __shfl_xor(level, i));
+        level = __builtin_amdgcn_readfirstlane(level);
         #pragma unroll 1
         while (true) {
             v4u p[2 * KB];
@@ -756,12 +761,27 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
                     p[i >> 1][2 * (i & 1) + (k >> 1)] = pack_f16x2(v[0], v[1]);
                 }
             }
-            const float f = level - E < -126 ? 0.f : two_to(level - E);
-            #pragma unroll
-            for (int vb = 0; vb < 4; ++vb) {
+            auto product = [&](int vb) __attribute__((always_inline)) {
                 v16f t = {};
                 #pragma unroll
                 for (int i = 0; i < 2 * KB; ++i) t = Mma<f16_t>::sub(v_frag(st, 4 * i + vb), p[i], 0, t);
+                return t;
+            };
+            // a row's power of two rises where the level gives it something, not for keys that it does not see
+            float most = 0.f;
+            #pragma unroll 1
+            for (int vb = 0; vb < 4; ++vb) {
+                const v16f t = product(vb);
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(t[i]));
+            }
+            const int up = most > 0.f ? max(Er, level) : Er;
+            if (__builtin_amdgcn_ballot_w64(up > Er)) scale_out(up - Er > 126 ? 0.f : two_to(Er - up));
+            Er = up;
+            const float f = level > Er || level - Er < -126 ? 0.f : two_to(level - Er);
+            #pragma unroll
+            for (int vb = 0; vb < 4; ++vb) {
+                const v16f t = product(vb);
                 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[vb][i] = __builtin_fmaf(t[i], f, o[vb][i]);
             }
@@ -772,8 +792,11 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             if (below == -0x7fffffff) break;
             level = below;
         }
+        E = __builtin_amdgcn_readfirstlane(Er);
+        apart = __builtin_amdgcn_ballot_w64(Er != E) != 0;
         ++j;
     }
+    if (!apart) Er = E;
 
     {
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -788,23 +811,23 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
             for (int i = 0; i < 64; ++i) theirs[64 * i] = o[i >> 4][i & 15];
             theirs[64 * 64] = m_ref;
             theirs[64 * 65] = l;
-            theirs[64 * 66] = __int_as_float(E);
+            theirs[64 * 66] = __int_as_float(Er);
         }
         __syncthreads();
         if (kh) return;
         const float m1 = theirs[64 * 64], l1 = theirs[64 * 65];
-        const int E1 = __float_as_int(theirs[64 * 66]), top = max(E, E1);
+        const int E1 = __float_as_int(theirs[64 * 66]), top = max(Er, E1);
         const float m = fmaxf(m_ref, m1);
         float f0 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m_ref - m), f1 = l1 == 0.f ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
         l = l * f0 + l1 * f1;
-        f0 = top - E > 126 ? 0.f : f0 * two_to(E - top);
+        f0 = top - Er > 126 ? 0.f : f0 * two_to(Er - top);
         f1 = top - E1 > 126 ? 0.f : f1 * two_to(E1 - top);
         m_ref = m;
-        E = top;
+        Er = top;
         #pragma unroll
         for (int i = 0; i < 64; ++i) o[i >> 4][i & 15] = o[i >> 4][i & 15] * f0 + theirs[64 * i] * f1;
     }
-    float f = l == 0.f ? 0.f : two_to(E) / l;
+    float f = l == 0.f || Er < -kLeast ? 0.f : two_to(Er) / l;      // (without any value that counts: zeros)
     if (!a.any_bad || load_uniform(a.any_bad)) {
         int worst = 0x7fffffff;
         for (int j = first + lane; j < n_tiles; j += 64) {

@@ -1,4 +1,5 @@
-"""GPU checks of the expanded attention where values and scores lie far apart (bounds of tests/expanded_ref.py)."""
+"""GPU checks of the expanded attention where values and scores lie far apart: what a query does not see costs
+it nothing (bounds of tests/expanded_ref.py)."""
 
 from __future__ import annotations
 
@@ -11,6 +12,61 @@ import expanded_ref as E
 from test_gpu_expanded import BF, DEV, DT, SCALE, ext, make, rows_of, run_paged  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+MOST = 3.3e38                                    # near bf16's end
+
+
+def visible(t, got, at, dtype=BF):
+    """The queries in front of key `at` of the one sequence, against the keys in front of it."""
+    Sq, n = got.size(1), int(t["lens"][0])
+    first = max(0, at - (n - Sq))
+    lat, rot = (x[:at] for x in rows_of(t, 0, n))
+    lims = E.limits(Sq, n, Sq, True)[:first]
+    ref = E.attention(t["q_nope"][0, :first], t["q_rope"][0, :first], lat, rot, t["W_uk"], t["W_uv"], SCALE, lims, dtype)
+    return (got[0, :first],) + ref
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("Sq", [60, 140])
+@pytest.mark.parametrize("at", [255, 257, 290, 299])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -9, 2.0 ** -30])
+@pytest.mark.parametrize("what", ["latent", "rope"])
+def test_a_hidden_row_near_the_end_of_the_type(ext, what, size, at, Sq, splits, monkeypatch):
+    """A key whose values are near bf16's largest, behind ordinary and behind small ones: queries that do not see
+    it keep the bounds that they have over the keys they see."""
+    monkeypatch.setenv("MLA_EXPAND_SPLITS", str(splits))
+    t = make(50 + Sq, 1, Sq, [300], 2, BF)
+    t["c_kv"] *= size
+    t["pe"] *= size
+    t["q_nope"] /= size
+    t["q_rope"] /= size
+    page, row = t["table"][0, at // 64].item(), at % 64
+    n = "c_kv" if what == "latent" else "pe"
+    t[n][page, row] = MOST * torch.sign(t[n][page, row].float()).to(BF)
+    E.check(*visible(t, run_paged(ext, t, True), at), name=f"{what} {at}")
+
+
+@pytest.mark.parametrize("Sq", [60, 140])
+@pytest.mark.parametrize("at", [257, 290, 299])
+def test_a_hidden_row_behind_rows_of_zeros(ext, at, Sq):
+    """The same where the keys of its 64 in front of it have latent rows of zeros."""
+    t = make(51, 1, Sq, [300], 2, BF)
+    page, row = t["table"][0, at // 64].item(), at % 64
+    t["c_kv"][page, :row] = 0
+    t["c_kv"][page, row] = MOST
+    E.check(*visible(t, run_paged(ext, t, True), at), name=str(at))
+
+
+@pytest.mark.parametrize("at", [129, 161, 250, 299])
+@pytest.mark.parametrize("size", [2.0 ** 13, 2.0 ** 14, 2.0 ** 40, 1e30])
+@pytest.mark.parametrize("what", ["latent", "rope"])
+def test_a_far_larger_row_costs_no_bits(ext, what, size, at):
+    """A key that is far larger than the others leaves the queries in front of it within the bounds over their own
+    keys, which do not know of it."""
+    t = make(52, 1, 140, [300], 2, BF)
+    page, row = t["table"][0, at // 64].item(), at % 64
+    t["c_kv" if what == "latent" else "pe"][page, row] *= size
+    E.check(*visible(t, run_paged(ext, t, True), at), name=f"{what} {at}")
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
