@@ -901,7 +901,7 @@ int run_expanded(ExpandProblem p, mla_dtype_t dtype, const mla_dims_t* dims, con
     MLA_CHECK(check_ptr(W_uk, "W_uk"));
     MLA_CHECK(check_ptr(W_uv, "W_uv"));
     MLA_CHECK(check_ptr(out, "out"));
-    const ExpandPlan plan = plan_expand(dims->batch, dims->sq, dims->sk, dims->heads, p.block_table != nullptr);
+    const ExpandPlan plan = plan_expand(dims->batch, dims->sq, dims->sk, dims->heads, p.block_table != nullptr, is_f16(dtype));
     MLA_CHECK(check_ws(workspace, workspace_bytes, plan.total));
     p.f16 = is_f16(dtype);
     p.q_nope = q_nope; p.q_rope = q_rope; p.W_uk = W_uk; p.W_uv = W_uv; p.out = out;
@@ -1884,7 +1884,7 @@ int mla_attention_paged_fp8blk(mla_dtype_t dtype, const mla_dims_t* dims, const 
 
 size_t mla_attention_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims, int causal) {
     if (check_expanded(dtype, dims, causal) != MLA_OK) return 0;
-    return plan_expand(dims->batch, dims->sq, dims->sk, dims->heads, false).total;
+    return plan_expand(dims->batch, dims->sq, dims->sk, dims->heads, false, is_f16(dtype)).total;
 }
 
 int mla_attention_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
@@ -1903,7 +1903,7 @@ int mla_attention_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void
 size_t mla_attention_paged_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims,
                                                     int causal, int32_t page_size) {
     if (check_expanded(dtype, dims, causal) != MLA_OK || check_pages(dims, page_size) != MLA_OK) return 0;
-    return plan_expand(dims->batch, dims->sq, dims->sk, dims->heads, true).total;
+    return plan_expand(dims->batch, dims->sq, dims->sk, dims->heads, true, is_f16(dtype)).total;
 }
 
 int mla_attention_paged_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,

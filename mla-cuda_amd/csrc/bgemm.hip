@@ -60,6 +60,7 @@ struct BArgs {
     QUpEpilogue q;                               // QUP kernels: 2a2 with 2b
     const int* rows;                             // EXPAND kernels: M, on the device
     int64_t b_hi;                                // and what B's rows past 128 of a group lie further on
+    const int* w_flag; const uint16_t* w_copy;   // and groups whose rows are read from a copy (KvExpand)
 };
 
 // EXPAND: the keys and values of the expanded attention (expand.hip).  The groups are heads, all of
@@ -78,6 +79,14 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
         __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, 1);   // hwreg(MODE, bit 23, 1 bit)
         a.M = load_uniform(a.rows);
         a.tiles_m = (a.M + BM - 1) / BM;
+    }
+    bool copies = false;                         // EXPAND: some group is read from the copy
+    if constexpr (EXPAND) {
+        if (a.w_copy) {
+            int any = 0;
+            for (int i = threadIdx.x & 63; i < 2 * a.G; i += 64) any |= a.w_flag[i];
+            copies = __builtin_amdgcn_ballot_w64((any & 1) != 0) != 0;
+        }
     }
     constexpr int RB = BM / 64, CB = BN / 128;         // 32x32 blocks per wave
     constexpr int kAStage = BM * 2 * kBKS, kBStage = BN * 2 * kBKS;
@@ -147,8 +156,12 @@ __global__ void __launch_bounds__(kBThreads, MINB) bgemm_kernel(BArgs a) {
         j.a_base = reinterpret_cast<uint64_t>(a.A + j.g * a.sAg + (int64_t)j.m0 * a.lda + k0);
         j.b_base = reinterpret_cast<uint64_t>(
             a.B + j.g * a.sBg + (NT ? (int64_t)j.n0 * a.ldb + k0 : (int64_t)k0 * a.ldb + j.n0));
-        if constexpr (EXPAND)
-            if (j.n0 + (BN / 8) * wave >= 128) j.b_base += 2 * (uint64_t)a.b_hi;   // this wave's rows
+        if constexpr (EXPAND) {
+            const int hi = j.n0 + (BN / 8) * wave >= 128;                          // this wave's rows
+            if (hi) j.b_base += 2 * (uint64_t)a.b_hi;
+            if (copies && (load_uniform(a.w_flag + 2 * j.g + hi) & 1))
+                j.b_base = reinterpret_cast<uint64_t>(a.w_copy + ((int64_t)j.g * 256 + j.n0) * a.ldb);
+        }
         const int rows = min(BM, a.M - j.m0), cols = min(BN, a.N - j.n0);
         j.a_bytes = (uint32_t)(rows - 1) * (uint32_t)a.lda * 2u + 2u * kBKS;
         j.b_bytes = NT ? (uint32_t)(cols - 1) * (uint32_t)a.ldb * 2u + 2u * kBKS
@@ -558,6 +571,7 @@ hipError_t launch_kv_expand(const KvExpand& p, hipStream_t stream) {
     a.C16 = p.kv; a.ldc = 2 * kN; a.sCg = p.rows_cap * 2 * kN;
     a.N = 2 * kN; a.K = kR; a.G = p.heads; a.split = 1; a.k_chunk = kR;
     a.rows = p.rows;
+    a.w_flag = p.w_flag; a.w_copy = p.w_copy;
     // tiles of 128 x 128 (two workgroups a CU) while those of 256 x 256 are fewer than the CUs
     const bool small = (p.rows_cap + 255) / 256 * p.heads < kNumCUs;
     const int bm = small ? 128 : 256;

@@ -153,7 +153,12 @@ struct GatherArgs {
     int* rows;               // rows in all
     uint16_t* lat;
     uint16_t* rot;
-    int B, Sk, units, max_pages, page_size, num_pages, block_shift;
+    const uint16_t* W_uk;    // [H][128][512]
+    const uint16_t* W_uv;
+    int* w_flag;             // [H][2] of W_uk and W_uv: kScaled, kOdd
+    int* w_exps;             // [H][2][128] their rows' powers of two, or kOddRow (where flagged)
+    uint16_t* w_copy;        // [H][2][128][512] rows under them (where scaled)
+    int B, Sk, units, max_pages, page_size, num_pages, block_shift, H, w_groups;
 };
 
 template <typename TL>
@@ -187,12 +192,89 @@ __device__ __forceinline__ float finite_max(float m, float x) {
 constexpr int kGatherThreads = 512, kGatherWaves = kGatherThreads / 64;
 constexpr int kWaveRows = kUnit / kGatherWaves;
 
+// ---- weights --------------------------------------------------------------------------------
+// fp16 keys and values have bf16's range only as far as the weights are of ordinary size.  Where the largest weight of
+// every row (of a head's W_uk or W_uv, zeros aside) is in [2^-9, 1) they are: 512 products with latents below 2^(kHead+1)
+// stay below 65504, and a latent row as far below its unit's largest as kSpread lets it be still leaves 11 bits.  A head's
+// W_uk or W_uv with a row outside is `scaled`: the product reads a copy whose rows are each brought to [1/2, 1) by
+// a power of two, which the attention puts into the query's columns (W_uk) or into the output's (W_uv); so the function
+// stays what it is, and the head's numbers do not depend on the weights' unit.  A row with a weight that is not
+// finite is `odd` (in fp16 too, whose weights are otherwise as they are): its output column, or for W_uk all of the head,
+// is NaN where a query sees a key.  A workgroup has 128 rows, beside the gather's: 128 heads' 33.5 MB make that launch 7.5 ->
+// 11.1 us at 512 rows and 10.7 -> 15.1 at 3,400, and the product behind it 23.4 -> 24.3 and (weights on the
+// chip by then) 145 -> 134; 16 rows of a wave in flight instead of 8 are not faster (12.0).
+constexpr int kScaled = 1, kOdd = 2;          // flags
+constexpr int kOddRow = 1 << 16;
+constexpr float kSmallRow = 1.f / 512;        // rows from here to 1 are as they are
+
+typedef uint16_t v2h_t __attribute__((ext_vector_type(2)));
+template <typename TL>
+__device__ __forceinline__ void expand_weights(const GatherArgs& a, int h, int half) {
+    __shared__ int row_e[kN], w_flags[kGatherWaves];
+    constexpr uint32_t kInf = Half<TL>::kF16 ? 0x7c00u : 0x7f80u;
+    constexpr int kRows = kN / kGatherWaves, kRun = 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const v4u* const src = reinterpret_cast<const v4u*>((half ? a.W_uv : a.W_uk) + (int64_t)h * kN * kR) + kRows * wave * 64 + lane;
+    int flag = 0;
+    #pragma unroll 1
+    for (int r0 = 0; r0 < kRows; r0 += kRun) {
+        v4u x[kRun];
+        #pragma unroll
+        for (int i = 0; i < kRun; ++i) x[i] = src[(r0 + i) * 64];
+        #pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+            v2h_t m = {0, 0};
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2h_t, x[i][k] & 0x7fff7fffu));
+            const uint32_t u = min((uint32_t)max(m[0], m[1]), kInf);      // magnitudes, NaN as infinity
+            const float top = wave_reduce(Half<TL>::to_f32(u), OpMax());
+            int e = 0;
+            if (!(top < INFINITY)) {
+                e = kOddRow;
+                flag |= kOdd | (Half<TL>::kF16 ? 0 : kScaled);
+            } else if (!Half<TL>::kF16 && top > 0.f) {
+                e = exponent_of(top) + 1;
+                if (!(top >= kSmallRow && top < 1.f)) flag |= kScaled;
+            }
+            if (lane == 0) row_e[kRows * wave + r0 + i] = e;
+        }
+    }
+    if (lane == 0) w_flags[wave] = flag;
+    __syncthreads();
+    flag = 0;
+    for (int w = 0; w < kGatherWaves; ++w) flag |= w_flags[w];
+    flag = __builtin_amdgcn_readfirstlane(flag);
+    const int at = 2 * h + half;
+    if (tid == 0) a.w_flag[at] = flag;
+    if (flag == 0) return;
+    if (tid < kN) a.w_exps[at * kN + tid] = row_e[tid];
+    if constexpr (!Half<TL>::kF16) {
+        v4u* const dst = reinterpret_cast<v4u*>(a.w_copy + (int64_t)at * kN * kR) + kRows * wave * 64 + lane;
+        #pragma unroll 1
+        for (int i = 0; i < kRows; ++i) {
+            const int e = row_e[kRows * wave + i];
+            v4u x = src[i * 64];
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(x[k]);
+                x[k] = e == kOddRow ? 0u : Half<TL>::pack2(ldexpf(v[0], -e), ldexpf(v[1], -e));
+            }
+            dst[i * 64] = x;
+        }
+    }
+}
+
 template <typename TL, bool F8>
 __global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArgs a) {
     __shared__ int part[kGatherWaves], w_bad[kGatherWaves];
     __shared__ float row_top[2][kUnit];     // latent, rope
     const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (j >= a.units) {
+        const int i = b * a.w_groups + j - a.units;
+        if (i < 2 * a.H) expand_weights<TL>(a, i >> 1, i & 1);
+        return;
+    }
     const int k0 = j * kUnit;
     // (with the length, not behind it; the table spans all units)
     const int page = a.table ? load_uniform(a.table + (int64_t)b * a.max_pages + k0 / a.page_size) : 0;
@@ -409,6 +491,8 @@ struct HeadsArgs {
     const int* exps;
     const int* row_exps;
     const int* any_bad;      // null: look for yourself
+    const int* w_flag;       // as the gather's
+    const int* w_exps;
     const int* seq_lens;
     const int* new_lens;
     const int* order;        // null: as they come
@@ -510,7 +594,36 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         for (int i = 0; i < 4; ++i) qf[8 + i] = *reinterpret_cast<const v4u*>(r + 16 * i);
     }
     int qe = 0;                  // bf16: the row's power of two
-    if constexpr (!Half<TL>::kF16) {
+    if (!Half<TL>::kF16 && (load_uniform(a.w_flag + 2 * h) & kScaled)) {
+        // columns that W_uk's rows have left their powers of two to
+        auto column = [&](int i, int k) __attribute__((always_inline)) {
+            if (i >= 8) return 0;
+            const int e = a.w_exps[2 * kN * h + 16 * i + 8 * hi + k];
+            return e == kOddRow ? 0 : e;
+        };
+        int top = -1000;
+        #pragma unroll
+        for (int i = 0; i < 12; ++i)
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(qf[i][k]);
+                #pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float x = fabsf(v[n]);
+                    if (x > 0.f && x < INFINITY) top = max(top, exponent_of(x) + column(i, 2 * k + n));
+                }
+            }
+        const auto x = __builtin_amdgcn_permlane32_swap((uint32_t)top, (uint32_t)top, false, false);
+        qe = max((int)x[0], (int)x[1]);
+        if (qe == -1000) qe = 0;
+        #pragma unroll
+        for (int i = 0; i < 12; ++i)
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const v2f_t v = halves<TL>(qf[i][k]);
+                qf[i][k] = pack_f16x2(ldexpf(v[0], column(i, 2 * k) - qe), ldexpf(v[1], column(i, 2 * k + 1) - qe));
+            }
+    } else if constexpr (!Half<TL>::kF16) {
         float top = 0.f;
         #pragma unroll
         for (int i = 0; i < 12; ++i)
@@ -838,28 +951,37 @@ __global__ void __launch_bounds__(kHThreads, 2) heads_kernel(HeadsArgs a) {
         for (int i = 1; i < 64; i *= 2) worst = min(worst, __shfl_xor(worst, i));
         if (worst <= lim) l = f = __uint_as_float(0x7fc00000u);
     }
+    const int w_uk = load_uniform(a.w_flag + 2 * h), w_uv = load_uniform(a.w_flag + 2 * h + 1);
+    if ((w_uk & kOdd) && l != 0.f) l = f = __uint_as_float(0x7fc00000u);
+    if (w0 + q >= a.Sq) return;
+    auto outputs = [&](int vb, int i) __attribute__((always_inline)) {     // four columns from 32 vb + 2 i + 4 hi on
+        v4f x = {o[vb][i], o[vb][i + 1], o[vb][i + 2], o[vb][i + 3]};
+        if (w_uv == 0) return x * f;
+        // W_uv's rows' powers of two
+        const v4i e = *reinterpret_cast<const v4i*>(a.w_exps + (2 * h + 1) * kN + 32 * vb + 2 * i + 4 * hi);
+        const float g = f == 0.f ? 0.f : f != f ? f : 1.f / l;
+        #pragma unroll
+        for (int k = 0; k < 4; ++k)
+            x[k] = e[k] != kOddRow ? ldexpf(x[k] * g, Er + e[k]) : l == 0.f ? 0.f : __uint_as_float(0x7fc00000u);
+        return x;
+    };
     if constexpr (SPLIT) {
-        if (w0 + q >= a.Sq) return;
         const int64_t at = ((int64_t)(sp * a.B + b) * a.Sq + row) * a.heads + hl;
         if (hi == 0) a.state[at] = make_float2(m_ref, l);
         float* const dst = a.part + at * kN + 4 * hi;
         #pragma unroll
         for (int vb = 0; vb < 4; ++vb)
             #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<v4f*>(dst + 32 * vb + 2 * i) =
-                    v4f{o[vb][i] * f, o[vb][i + 1] * f, o[vb][i + 2] * f, o[vb][i + 3] * f};
-        return;
-    }
-    if (w0 + q < a.Sq) {
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<v4f*>(dst + 32 * vb + 2 * i) = outputs(vb, i);
+    } else {
         uint16_t* const dst = out + row * row_stride + 4 * hi;
         #pragma unroll
         for (int vb = 0; vb < 4; ++vb)
             #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<v2u_t*>(dst + 32 * vb + 2 * i) =
-                    v2u_t{to_half2<TL>(o[vb][i] * f, o[vb][i + 1] * f),
-                          to_half2<TL>(o[vb][i + 2] * f, o[vb][i + 3] * f)};
+            for (int i = 0; i < 16; i += 4) {
+                const v4f x = outputs(vb, i);
+                *reinterpret_cast<v2u_t*>(dst + 32 * vb + 2 * i) = v2u_t{to_half2<TL>(x[0], x[1]), to_half2<TL>(x[2], x[3])};
+            }
     }
 }
 
@@ -939,7 +1061,7 @@ int expand_splits(int64_t items, int units) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * kNumCUs / items, 16), units / 8));
 }
 
-ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged) {
+ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged, bool f16) {
     ExpandPlan p;
     p.units = (Sk + kUnit - 1) / kUnit;
     const int64_t places = (int64_t)B * p.units;
@@ -960,6 +1082,9 @@ ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged) {
     p.off_exps = take(places * 4);
     p.off_row_exps = take(places * 8 * kUnit);
     p.off_any = take(8);                      // any_bad, rows
+    p.off_w_flag = take((size_t)H * 8);
+    p.off_w_exps = take((size_t)H * 8 * kN);
+    p.off_w_copy = take(f16 ? 0 : (size_t)H * 4 * kN * kR);
     p.off_lat = take((size_t)p.rows_cap * kR * 2);
     p.off_rot = take((size_t)p.rows_cap * kD * 2);
     p.off_kv = take((size_t)p.heads * p.rows_cap * 512);
@@ -1001,7 +1126,10 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     g.B = p.B; g.Sk = p.Sk; g.units = plan.units;
     g.page_size = p.page_size; g.max_pages = u.max_pages; g.num_pages = p.num_pages;
     g.block_shift = p.scale_block == 16 ? 4 : p.scale_block == 32 ? 5 : 6;
-    const dim3 gather((unsigned)plan.units, (unsigned)p.B);
+    g.W_uk = static_cast<const uint16_t*>(p.W_uk); g.W_uv = static_cast<const uint16_t*>(p.W_uv);
+    g.w_flag = ints(plan.off_w_flag); g.w_exps = ints(plan.off_w_exps); g.w_copy = half(plan.off_w_copy);
+    g.H = p.H; g.w_groups = (2 * p.H + p.B - 1) / p.B;
+    const dim3 gather((unsigned)(plan.units + g.w_groups), (unsigned)p.B);
     if (p.scales) {
         if (p.f16) hipLaunchKernelGGL((expand_gather_kernel<f16_t, true>), gather, dim3(kGatherThreads), 0, stream, g);
         else hipLaunchKernelGGL((expand_gather_kernel<bf16_t, true>), gather, dim3(kGatherThreads), 0, stream, g);
@@ -1016,6 +1144,7 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     a.qn = static_cast<const uint16_t*>(p.q_nope); a.qr = static_cast<const uint16_t*>(p.q_rope);
     a.kv = half(plan.off_kv); a.rot = g.rot;
     a.unit = g.unit; a.bad = g.bad; a.exps = g.exps; a.row_exps = g.row_exps; a.any_bad = g.any_bad;
+    a.w_flag = g.w_flag; a.w_exps = g.w_exps;
     a.seq_lens = p.seq_lens; a.new_lens = p.new_lens;
     a.order = p.block_table && p.B > 1 ? u.order : nullptr;
     a.part = reinterpret_cast<float*>(ws + plan.off_part);
@@ -1033,6 +1162,8 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
         k.lat = g.lat; k.kv = half(plan.off_kv);
         k.W_uk = static_cast<const uint16_t*>(p.W_uk) + (int64_t)h0 * kN * kR;
         k.W_uv = static_cast<const uint16_t*>(p.W_uv) + (int64_t)h0 * kN * kR;
+        k.w_flag = g.w_flag + 2 * h0;
+        k.w_copy = p.f16 ? nullptr : g.w_copy + (int64_t)h0 * 2 * kN * kR;
         k.rows = g.rows; k.rows_cap = plan.rows_cap; k.heads = heads;
         e = launch_kv_expand(k, stream);
         if (e != hipSuccess) return e;

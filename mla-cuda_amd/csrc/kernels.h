@@ -410,9 +410,9 @@ struct ExpandPlan {
     int heads = 0;                   // expanded and attended to at a time
     int splits = 1;                  // of the keys
     size_t off_owner, off_rank, off_count, off_order, off_unit, off_bad, off_exps, off_row_exps, off_any,
-        off_lat, off_rot, off_kv, off_part, off_state, total;
+        off_w_flag, off_w_exps, off_w_copy, off_lat, off_rot, off_kv, off_part, off_state, total;
 };
-ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged);
+ExpandPlan plan_expand(int B, int Sq, int Sk, int H, bool paged, bool f16);
 hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* workspace, hipStream_t stream);
 // its product (bgemm.hip): kv [heads][rows_cap][256] from lat [rows][512]; *rows on the device
 struct KvExpand {
@@ -420,6 +420,8 @@ struct KvExpand {
     const uint16_t* lat = nullptr;
     const uint16_t* W_uk = nullptr;
     const uint16_t* W_uv = nullptr;
+    const int* w_flag = nullptr;       // [heads][2] bit 0: rows from w_copy [heads][2][128][512], where it is given
+    const uint16_t* w_copy = nullptr;
     uint16_t* kv = nullptr;
     const int* rows = nullptr;
     int64_t rows_cap = 0;

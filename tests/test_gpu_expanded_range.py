@@ -1,5 +1,5 @@
-"""GPU checks of the expanded attention where values and scores lie far apart: what a query does not see costs
-it nothing (bounds of tests/expanded_ref.py)."""
+"""GPU checks of the expanded attention where values, weights and scores lie far apart: what a query does not see
+costs it nothing, and powers of two in the weights cost no bits (bounds of tests/expanded_ref.py)."""
 
 from __future__ import annotations
 
@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import expanded_ref as E
-from test_gpu_expanded import BF, DEV, DT, SCALE, ext, make, rows_of, run_paged  # noqa: F401
+from test_gpu_expanded import BF, DEV, DT, N, SCALE, ext, make, rows_of, run_paged  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,153 @@ def test_scores_past_float32s_steps(ext, dtype, Sq, n, power):
         d, size = (got[sure, h] - v[best[sure]]).norm(dim=-1), v[best[sure]].norm(dim=-1)
         assert (d <= 2 ** -7 * size).all()
     assert tested > Sq
+
+
+def columns(got, ref, name):
+    """E.check's 2-norms, of every output column of its own."""
+    out, _, usual = ref
+    d = (got.double() - out).norm(dim=0)
+    assert torch.isfinite(got).all(), name
+    assert (d <= usual.norm(dim=0)).all(), f"{name}: {(d / usual.norm(dim=0)).max().item():.3f} of the bound"
+
+
+@pytest.mark.parametrize("uk,uv", [(0, -30), (0, -12), (0, 12), (0, 60), (-30, 0), (-12, 0), (12, 0), (60, 0), (-40, 40), (5, 5)])
+@pytest.mark.parametrize("Sq,lens,splits", [(60, [300], 1), (140, [300], 3), (140, [140, 400], 1)])
+def test_powers_of_two_in_the_weights(ext, uk, uv, Sq, lens, splits, monkeypatch):
+    """W_uk under 2^uk, with queries under 2^-uk, and W_uv under 2^uv: the same function, and the same bits of it."""
+    monkeypatch.setenv("MLA_EXPAND_SPLITS", str(splits))
+    t = make(54, len(lens), Sq, lens, 3, BF)
+    t["W_uk"] *= 2.0 ** uk
+    t["q_nope"] *= 2.0 ** -uk
+    t["W_uv"] *= 2.0 ** uv
+    got = run_paged(ext, t, True)
+    for b, n in enumerate(lens):
+        ref = E.attention(t["q_nope"][b], t["q_rope"][b], *rows_of(t, b, n), t["W_uk"], t["W_uv"], SCALE,
+                          E.limits(Sq, n, Sq, True), BF)
+        columns(got[b], ref, f"{uk} {uv} {b}")
+
+
+@pytest.mark.parametrize("Sq,n", [(64, 64), (200, 333)])
+@pytest.mark.parametrize("most", [8, 40])
+def test_weights_of_rows_far_apart(ext, Sq, n, most):
+    """Every row of W_uk and W_uv under a power of two of its own, some rows zeros, in some of the heads."""
+    t = make(55, 1, Sq, [n], 4, BF)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(most)
+    for name in ("W_uk", "W_uv"):
+        e = torch.randint(-most, most + 1, (4, N), generator=g, device=DEV).float()
+        e[1] = 0
+        t[name] *= torch.exp2(e)[..., None].to(BF)
+        if name == "W_uk":
+            t["q_nope"] *= torch.exp2(-e).to(BF)[None, None]
+        t[name][2, 5] = 0
+    got = run_paged(ext, t, True)
+    ref = E.attention(t["q_nope"][0], t["q_rope"][0], *rows_of(t, 0, n), t["W_uk"], t["W_uv"], SCALE,
+                      E.limits(Sq, n, Sq, True), BF)
+    columns(got[0], ref, f"{Sq} {n}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("Sq,n,splits", [(64, 200, 1), (70, 200, 1), (130, 700, 2), (30, 20, 1)])
+def test_weights_that_are_not_finite(ext, dtype, Sq, n, splits, monkeypatch):
+    """A weight that is not finite makes its output column (W_uv) or its head (W_uk) NaN where a query sees a key, and
+    changes nothing else."""
+    monkeypatch.setenv("MLA_EXPAND_SPLITS", str(splits))
+    t = make(56, 1, max(Sq, n), [n], 3, DT[dtype])
+    for k in ("q_nope", "q_rope"):
+        t[k] = t[k][:, -Sq:].contiguous()
+    want = run_paged(ext, t, True)
+    empty = max(0, Sq - n)
+    t["W_uv"][1, 7, 100] = math.inf
+    t["W_uk"][2, 9, 3] = math.nan
+    got = run_paged(ext, t, True)
+    assert not got[:, :empty].any()
+    assert torch.equal(got[:, :, 0], want[:, :, 0])
+    assert got[:, empty:, 1, 7].isnan().all()
+    keep = [i for i in range(N) if i != 7]
+    assert torch.equal(got[:, :, 1, keep], want[:, :, 1, keep])
+    assert got[:, empty:, 2].isnan().all()
+
+
+def own(t):
+    """Weights and queries of their own memory."""
+    return {**t, "W_uk": t["W_uk"].clone(), "W_uv": t["W_uv"].clone(), "q_nope": t["q_nope"].clone()}
+
+
+def scaled(t, uk, uv):
+    """Heads of W_uk and W_uv under powers of two of their own, the queries' columns under W_uk's inverse."""
+    u = own(t)
+    k, v = (torch.exp2(torch.tensor(e, dtype=torch.float32, device=DEV)).to(BF) for e in (uk, uv))
+    u["W_uk"] *= k[:, None, None]
+    u["q_nope"] /= k[:, None]
+    u["W_uv"] *= v[:, None, None]
+    return u, v[:, None]
+
+
+@pytest.mark.parametrize("B,Sq,lens,span", [(1, 130, [300], 1400000), (40, 3, [3 + 5 * b for b in range(40)], 0), (2, 64, [64, 1000], 0)])
+def test_heads_under_powers_of_their_own(ext, B, Sq, lens, span):
+    """Groups of heads, more sequences than heads, few queries: the outputs are those of ordinary weights under W_uv's
+    powers of two, bit for bit (every rounding on the way is under powers of two that are taken out again)."""
+    t = make(57, B, Sq, lens, 5, BF)
+    t["q_rope"].zero_()             # (whose scores lie beside those of scaled columns)
+    if span:                        # 2 GiB hold three heads of that many keys
+        table = torch.zeros(1, span // 64, dtype=torch.int32, device=DEV)
+        table[:, :t["table"].size(1)] = t["table"]
+        t["table"] = table
+    want = run_paged(ext, t, True)
+    u, v = scaled(t, [0, 20, -20, 0, -14], [0, 0, 30, -30, 14])
+    assert torch.equal(run_paged(ext, u, True), want * v)
+
+
+def test_weights_change_between_replays(ext):
+    """A captured call looks at its weights in every replay; eager calls in between."""
+    t = make(58, 2, 70, [200, 130], 5, BF)
+    t["q_rope"].zero_()
+    u = own(t)
+    steps = [([0] * 5, [0] * 5), ([0, 20, -20, 0, -14], [0, 0, 30, -30, 14]), ([0] * 5, [0] * 5), ([-20] * 5, [14, 0, 0, 0, 0])]
+    want = run_paged(ext, t, True)
+    run_paged(ext, u, True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run_paged(ext, u, True)
+    for uk, uv in steps:
+        s, v = scaled(t, uk, uv)
+        for k in ("W_uk", "W_uv", "q_nope"):
+            u[k].copy_(s[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want * v)
+        assert torch.equal(run_paged(ext, s, True), want * v)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("block", [0, 32])
+def test_scaled_weights_over_other_caches(ext, block):
+    """The dense cache and the one in 8 bits."""
+    t = make(59, 2, 40, [128, 128], 4, BF)
+    t["q_rope"].zero_()
+    u, v = scaled(t, [20, 0, -20, 1], [30, -30, 0, 1])
+    if block:
+        codes = [torch.nan_to_num(t[n].float()).mul(40).to(torch.float8_e4m3fn) for n in ("c_kv", "pe")]
+        scales = torch.full((t["c_kv"].size(0), 64 // block, 2), 122, dtype=torch.uint8, device=DEV)
+        call = lambda x: ext.mla_attention_paged_fp8blk_expanded(x["q_nope"], x["q_rope"], *codes, scales, t["table"], t["lens"],
+                                                                 x["W_uk"], x["W_uv"], SCALE, True)
+    else:
+        rows = [torch.stack([rows_of(t, b, 128)[i] for b in range(2)]).contiguous() for i in range(2)]
+        call = lambda x: ext.mla_attention_expanded(x["q_nope"], x["q_rope"], *rows, x["W_uk"], x["W_uv"], SCALE, True)
+    assert torch.equal(call(u), call(t) * v)
+
+
+@pytest.mark.parametrize("weight", [2.0 ** -9, 255 / 256, 1.0, 255 / 128, 255.0])
+@pytest.mark.parametrize("Sq,n", [(64, 64), (130, 200)])
+def test_the_largest_values(ext, Sq, n, weight):
+    """Latent rows along the weights' rows, each at its largest: 512 products of one sign, 65,025 in the scale that fp16
+    holds them in."""
+    t = make(60, 1, Sq, [n], 2, BF)
+    sign = torch.sign(t["W_uv"][0, 0].float()).to(BF)
+    t["W_uv"][0] = weight * sign
+    for j in range(-(-n // 64)):
+        t["c_kv"][t["table"][0, j]] = 127.5 * sign
+    got = run_paged(ext, t, True)
+    assert (got[0, :, 0] == torch.tensor(512 * 127.5 * weight, device=DEV).to(BF)).all()
