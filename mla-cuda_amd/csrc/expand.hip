@@ -1102,7 +1102,7 @@ hipError_t launch_expand(const ExpandProblem& p, const ExpandPlan& plan, void* w
     auto ints = [&](size_t off) { return reinterpret_cast<int*>(ws + off); };
     auto half = [&](size_t off) { return reinterpret_cast<uint16_t*>(ws + off); };
     const int64_t tiles = (p.Sq + kHRows - 1) / kHRows;
-    if (p.B > 65535 || plan.rows_cap > 0x7fffffff || tiles * p.B * plan.heads * plan.splits > 0x7fffffff)
+    if (p.B > 65535 || plan.rows_cap > 0x7fffffff || tiles * p.B * plan.heads * plan.splits > 0xffffffffll / kHThreads)
         return hipErrorInvalidValue;
     int* any_bad = ints(plan.off_any);
     PlanArgs u;
