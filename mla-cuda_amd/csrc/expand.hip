@@ -204,7 +204,7 @@ constexpr int kWaveRows = kUnit / kGatherWaves;
 // 11.1 us at 512 rows and 10.7 -> 15.1 at 3,400, and the product behind it 23.4 -> 24.3 and (weights on the
 // chip by then) 145 -> 134; 16 rows of a wave in flight instead of 8 are not faster (12.0).
 constexpr int kScaled = 1, kOdd = 2;          // flags
-constexpr int kOddRow = 1 << 16;
+constexpr int kOddRow = 1 << 16, kZeroRow = -400;   // (zeros count as so small that their query columns weigh nothing)
 constexpr float kSmallRow = 1.f / 512;        // rows from here to 1 are as they are
 
 typedef uint16_t v2h_t __attribute__((ext_vector_type(2)));
@@ -228,7 +228,7 @@ __device__ __forceinline__ void expand_weights(const GatherArgs& a, int h, int h
             for (int k = 0; k < 4; ++k) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2h_t, x[i][k] & 0x7fff7fffu));
             const uint32_t u = min((uint32_t)max(m[0], m[1]), kInf);      // magnitudes, NaN as infinity
             const float top = wave_reduce(Half<TL>::to_f32(u), OpMax());
-            int e = 0;
+            int e = Half<TL>::kF16 ? 0 : kZeroRow;
             if (!(top < INFINITY)) {
                 e = kOddRow;
                 flag |= kOdd | (Half<TL>::kF16 ? 0 : kScaled);

@@ -103,7 +103,7 @@ def test_scores_past_float32s_steps(ext, dtype, Sq, n, power):
 
 
 def columns(got, ref, name):
-    """E.check's 2-norms, of every output column of its own."""
+    """E.check's 2-norms, of every head and output column of its own."""
     out, _, usual = ref
     d = (got.double() - out).norm(dim=0)
     assert torch.isfinite(got).all(), name
@@ -144,6 +144,19 @@ def test_weights_of_rows_far_apart(ext, Sq, n, most):
     ref = E.attention(t["q_nope"][0], t["q_rope"][0], *rows_of(t, 0, n), t["W_uk"], t["W_uv"], SCALE,
                       E.limits(Sq, n, Sq, True), BF)
     columns(got[0], ref, f"{Sq} {n}")
+
+
+@pytest.mark.parametrize("uk", [-30, -12, 20])
+def test_rows_of_zeros_among_scaled_weights(ext, uk):
+    """Query columns that meet rows of zeros, with the size of the others' scaled ones, cost those no bits."""
+    t = make(61, 1, 70, [200], 3, BF)
+    t["W_uk"] *= 2.0 ** uk
+    t["q_nope"] *= 2.0 ** -uk
+    t["W_uk"][1, 5], t["W_uk"][2, 64:], t["W_uv"][0, 3:90] = 0, 0, 0
+    got = run_paged(ext, t, True)
+    ref = E.attention(t["q_nope"][0], t["q_rope"][0], *rows_of(t, 0, 200), t["W_uk"], t["W_uv"], SCALE,
+                      E.limits(70, 200, 70, True), BF)
+    columns(got[0], ref, str(uk))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
