@@ -471,11 +471,12 @@ __global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArg
 // leave float32), too: the power of two of a row then rises where the unit has something under a weight for it, and stays
 // where the row does not see the keys that are so large.  Such steps are done outside the loop of the ordinary ones, which
 // so keeps its registers (inside it they cost up to 28%).  bf16 queries are made fp16 under a power of two of their own.
-// What bounds it: the matrix cores' power.  4,096 causal rows of 128 heads 718 us, 957 TFLOP/s; 2,048 rows over
-// 32,768 keys of 16 heads 640, 1,040 TFLOP/s (a large fp16 library product 1,318).  The
-// second, without exponentials, reads of fragments and all else but its matrix instructions, barriers and loads of
-// stages, takes 86% of its time; the cores are busy 0.57 and 0.66 of the cycles, at the clock that they leave; with
-// operands of zeros it is a fifth faster.  Other structures, each on one card against this one: the next step's
+// What bounds it: the matrix cores' power, and what does not fit beside them.  4,096 causal rows of 128 heads 718 us, 957
+// TFLOP/s; 2,048 rows over 32,768 keys of 16 heads 640, 1,040 TFLOP/s (a large fp16 library product 1,318).  The second
+// (666 in the run of these) takes 629 us without exponentials, 609 without reads of fragments, 559 without softmax and
+// reads, that is with its matrix instructions, barriers and loads of stages alone, and 471 without any matrix
+// instruction; the cores are busy 0.57 and 0.66 of the cycles and the VALU issues in 0.43, at the clock that they leave
+// (no counter here shows it; with operands of zeros the second is a fifth faster).  Other structures, each on one card against this one: the next step's
 // scores and the last one's values between the exponentials of a step (+6%), the same with 64 rows a wave in 512
 // registers (+60%) or eight waves a workgroup (+10%); eight waves of which four have matrix instructions between
 // two barriers while four have exponentials (-3% where most keys are visible, +4 to +10% where tiles of 256 rows
@@ -1051,7 +1052,8 @@ int expand_heads(int H, int64_t rows) {
 
 // Key splits of the attention, where its workgroups are fewer than two a CU (which share the matrix cores' and
 // the VALU's time): 256 of them over 512 units 1,023 us unsplit, 836 in 2, 871 in 3, 836 in 4.  A
-// share is at least 8 units: 128 workgroups over 8 units 51.1 us unsplit, 52.0 in 2, 54.8 in 4.
+// share is at least 8 units of the span (128 workgroups over 8 units 51.1 us unsplit, 52.0 in 2, 54.8 in 4); how much
+// of it the sequences hold is not known here, and a tile that sees less has as many, smaller shares.
 // MLA_EXPAND_SPLITS overrides the rule.
 int expand_splits(int64_t items, int units) {
     if (const char* e = std::getenv("MLA_EXPAND_SPLITS")) {
