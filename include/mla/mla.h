@@ -520,9 +520,10 @@ int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
  *   k[j, h] = W_uk[h] c_kv[j],  v[j, h] = W_uv[h] c_kv[j],
  *   out[b, i, h] = softmax_j((q_nope[b, i, h] . k[j, h] + q_rope[b, i, h] . pe[j]) / scale) . v[j, h],
  * mla_attention's function of unabsorbed queries: 640 operations a pair and head instead of 2,176, and
- * 262,144 a key and head once.  It pays from about 60 new tokens a sequence where they are most of its keys, 180
- * behind 1,024 others and 260 behind 8,192 or more (128 heads); below that mla_q_absorbed and the attention over the
- * latents are faster.  bf16 or fp16 (queries, weights, output, and the cache where
+ * 262,144 a key and head once.  It pays from about 130 new tokens of one sequence (of eight: 30 each) where they are all
+ * of its keys, 190 behind 1,024 others, 270 behind 8,192 and 300 behind 32,768 (128 heads, bf16, with the Q path); below
+ * that mla_q_absorbed and the attention over the latents are faster, far from there by up to ten times (16 tokens behind
+ * 8,192), and a caller chooses.  bf16 or fp16 (queries, weights, output, and the cache where
  * it is not in 8 bits), kv_rank 512, rope 64, nope and v 128 (MLA_ERR_UNSUPPORTED otherwise).
  *   q_nope [B, Sq, H, 128], q_rope [B, Sq, H, 64]     mla_q_heads
  *   W_uk [H, 128, 512], W_uv [H, 128, 512], out [B, Sq, H, 128]
@@ -544,7 +545,8 @@ int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
  * own rounding 1.66e-3; the absorbed form 2.5 to 3.8e-3) and 2.6 to 3.7e-4 in fp16, up to 5e-4 over the 8-bit cache
  * (rounding 2.1e-4; the absorbed form as here).
  * The workspace holds keys and values of as many heads at a time as 2 GiB take (one at least), 256 KB a head in bf16
- * (its weights, should they need powers of two) and 1.2 KB for each key of batch * dims->sk: of a wide table give the columns up to the longest sequence's (grids go by them too). */
+ * (its weights, should they need powers of two) and 1.2 KB for each key of batch * dims->sk: of a wide table give the
+ * columns up to the longest sequence's (grids go by them too). */
 size_t mla_attention_expanded_workspace_bytes(mla_dtype_t dtype, const mla_dims_t* dims, int causal);
 int mla_attention_expanded(mla_dtype_t dtype, const mla_dims_t* dims, const void* q_nope,
                            const void* q_rope, const void* c_kv, const void* pe_cache,

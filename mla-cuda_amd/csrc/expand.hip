@@ -119,7 +119,8 @@ __global__ void __launch_bounds__(kPlanThreads) expand_plan_kernel(PlanArgs a) {
 // ---- gather ---------------------------------------------------------------------------------
 // A workgroup copies a unit's rows, or only notes where its owner's are.  Few units are bound by the way to
 // memory and back, many by their bytes: 512 rows 7.1 us, 4,096 9.1, 32,768 16.8 (4.5 TB/s), 13,216 of the 8-bit
-// cache 14.4 (with four waves instead of eight and loads behind tests of their own 9.3, 11.5, 19.5 and 22.2).
+// cache 14.4 (with four waves instead of eight and loads behind tests of their own 9.3, 11.5, 19.5 and 22.2); with the
+// weights of 128 heads (16 in the third) beside them 10.8, 14.3, 20.0 and 17.6.
 // Keys, values and weights are fp16 from here on, in bf16 too: 11 bits instead of 8 bring the outputs'
 // distance from the exact ones from 1.6 to 2.3 times that of their own rounding down to about it (bf16).
 // A bf16 cache is fitted into fp16's range by a power of two for each unit, 2^e: its rows are stored
@@ -200,9 +201,9 @@ constexpr int kWaveRows = kUnit / kGatherWaves;
 // a power of two, which the attention puts into the query's columns (W_uk) or into the output's (W_uv); so the function
 // stays what it is, and the head's numbers do not depend on the weights' unit.  A row with a weight that is not
 // finite is `odd` (in fp16 too, whose weights are otherwise as they are): its output column, or for W_uk all of the head,
-// is NaN where a query sees a key.  A workgroup has 128 rows, beside the gather's: 128 heads' 33.5 MB make that launch 7.5 ->
-// 11.1 us at 512 rows and 10.7 -> 15.1 at 3,400, and the product behind it 23.4 -> 24.3 and (weights on the
-// chip by then) 145 -> 134; 16 rows of a wave in flight instead of 8 are not faster (12.0).
+// is NaN where a query sees a key.  A workgroup has 128 rows, beside the gather's: 128 heads' 33.5 MB make that
+// launch 7.4 -> 10.8 us at 512 rows and 9.5 -> 14.0 at 3,400, and the product behind it 23.9 -> 24.9 and (weights on the
+// chip by then) 138 -> 121; 16 rows of a wave in flight instead of 8 are not faster (+0.9 us).
 constexpr int kScaled = 1, kOdd = 2;          // flags
 constexpr int kOddRow = 1 << 16, kZeroRow = -400;   // (zeros count as so small that their query columns weigh nothing)
 constexpr float kSmallRow = 1.f / 512;        // rows from here to 1 are as they are
@@ -471,17 +472,17 @@ __global__ void __launch_bounds__(kGatherThreads) expand_gather_kernel(GatherArg
 // leave float32), too: the power of two of a row then rises where the unit has something under a weight for it, and stays
 // where the row does not see the keys that are so large.  Such steps are done outside the loop of the ordinary ones, which
 // so keeps its registers (inside it they cost up to 28%).  bf16 queries are made fp16 under a power of two of their own.
-// What bounds it: the matrix cores' power, and what does not fit beside them.  4,096 causal rows of 128 heads 718 us, 957
+// What bounds it: the matrix cores' power, and what does not fit beside them.  4,096 causal rows of 128 heads 711 us, 967
 // TFLOP/s; 2,048 rows over 32,768 keys of 16 heads 640, 1,040 TFLOP/s (a large fp16 library product 1,318).  The second
 // (666 in the run of these) takes 629 us without exponentials, 609 without reads of fragments, 559 without softmax and
 // reads, that is with its matrix instructions, barriers and loads of stages alone, and 471 without any matrix
-// instruction; the cores are busy 0.57 and 0.66 of the cycles and the VALU issues in 0.43, at the clock that they leave
-// (no counter here shows it; with operands of zeros the second is a fifth faster).  Other structures, each on one card against this one: the next step's
-// scores and the last one's values between the exponentials of a step (+6%), the same with 64 rows a wave in 512
-// registers (+60%) or eight waves a workgroup (+10%); eight waves of which four have matrix instructions between
-// two barriers while four have exponentials (-3% where most keys are visible, +4 to +10% where tiles of 256 rows
-// meet the diagonal or a chunk's end); loads between the score MFMAs (+12%), the MFMAs at a higher wave priority
-// (+1%), windows of 3 and 4 fragments (+0.3%, +1.5%), left to the compiler's order (+5%).
+// instruction; the cores are busy 0.58 and 0.67 of the cycles and the VALU issues in 0.44, at the clock that they leave
+// (no counter here shows it; with operands of zeros the second is a fifth faster).  Other structures, each on one card
+// against this one: the next step's scores and the last one's values between the exponentials of a step (+6%), the same
+// with 64 rows a wave in 512 registers (+60%) or eight waves a workgroup (+10%); eight waves of which four have matrix
+// instructions between two barriers while four have exponentials (-3% where most keys are visible, +4 to +10% where tiles
+// of 256 rows meet the diagonal or a chunk's end); loads between the score MFMAs (+12%), the MFMAs at a higher wave
+// priority (+1%), windows of 3 and 4 fragments (+0.3%, +1.5%), left to the compiler's order (+5%).
 struct HeadsArgs {
     const uint16_t* qn;      // [B, Sq, H, 128]
     const uint16_t* qr;      // [B, Sq, H, 64]
