@@ -533,8 +533,8 @@ int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
  * first page (mla_cache_fork) are expanded once.  Table entries outside the pool read as zero rows.
  * Rounded on the way, in both types: keys, values and each key's weight (before the division by the
  * row's sum) to 11 bits as fp16 numbers, in bf16 under a power of two for each 64 keys that brings
- * their largest latent or rope value to [64, 128) (where a latent row's largest is more than 2^12 below that,
- * one for each of their latent and rope rows); weights down to 2^-22 of the row's largest, for keys whose
+ * their largest latent or rope value to [64, 128) (sizes below 2^-100 count as that; where a latent row's largest
+ * is more than 2^12 below theirs, one for each of their latent and rope rows); weights down to 2^-22 of the row's largest, for keys whose
  * power of two is 2^k below the largest so far 2^(k-22) (k up to 12); bf16 queries to 11 bits down to 2^-14 of the
  * row's largest; the output to its type.  Sums are float32.  In bf16 rows of W_uk and W_uv whose largest
  * value is below 2^-9 or at least 1 count as if brought to [1/2, 1) by a power of two (with all of that weight and
@@ -542,7 +542,7 @@ int mla_cache_copy_pages(const int32_t* copies, int64_t n, int32_t num_pages,
  * 65504 stays there.  A latent row with a NaN or an infinity makes the rows of the queries that see it NaN and reaches no
  * other query; a row of W_uv with one makes its output column NaN, one of W_uk all of its head (where a query sees a key).
  * On inputs of unit spread the outputs' relative distance (RMS) from the exact ones is 1.7e-3 in bf16 (the output's
- * own rounding 1.66e-3; the absorbed form 2.5 to 3.8e-3) and 2.6 to 3.7e-4 in fp16, up to 5e-4 over the 8-bit cache
+ * own rounding 1.66e-3; the absorbed form 2.5 to 3.8e-3) and 2.6 to 3.7e-4 in fp16, about 5e-4 over the 8-bit cache
  * (rounding 2.1e-4; the absorbed form as here).
  * The workspace holds keys and values of as many heads at a time as 2 GiB take (one at least), 256 KB a head in bf16
  * (its weights, should they need powers of two) and 1.2 KB for each key of batch * dims->sk: of a wide table give the

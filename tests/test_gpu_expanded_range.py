@@ -4,6 +4,7 @@ costs it nothing, and powers of two in the weights cost no bits (bounds of tests
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -263,3 +264,39 @@ def test_the_largest_values(ext, Sq, n, weight):
         t["c_kv"][t["table"][0, j]] = 127.5 * sign
     got = run_paged(ext, t, True)
     assert (got[0, :, 0] == torch.tensor(512 * 127.5 * weight, device=DEV).to(BF)).all()
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_rows_weights_and_units_of_any_size(ext, seed, monkeypatch):
+    """Rows, units or a few rows under powers of two of their own, in half of the batches the weights' rows too: every
+    query of every head keeps the bounds' 2-norm, its columns each in its W_uv row's unit."""
+    r = random.Random(seed)
+    Sq = r.choice([5, 33, 60, 64, 65, 140, 300])
+    n = Sq + r.choice([0, 1, 30, 64, 200, 500])
+    monkeypatch.setenv("MLA_EXPAND_SPLITS", str(r.choice([1, 1, 2, 5])))
+    span, mode = r.choice([3, 10, 14, 40, 60]), r.choice(["rows", "units", "a few"])
+    t = make(70 + seed, 1, Sq, [n], 3, BF)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    P = t["c_kv"].size(0)
+    powers = {}
+    for k in ("c_kv", "pe"):
+        e = torch.randint(-span, span + 1, (P, 1 if mode == "units" else 64), generator=g, device=DEV).float().expand(P, 64)
+        if mode == "a few":
+            e = torch.where(torch.rand(P, 64, generator=g, device=DEV) < 0.03, float(span), 0.0)
+        powers[k] = powers["c_kv"] if mode == "units" and k == "pe" else e
+        t[k] *= torch.exp2(powers[k])[..., None].to(BF)
+    t["q_nope"] *= 2.0 ** -span
+    t["q_rope"] *= 2.0 ** -span
+    if r.random() < 0.5:
+        for k in ("W_uk", "W_uv"):
+            e = torch.randint(-30, 31, (3, N), generator=g, device=DEV).float()
+            t[k] *= torch.exp2(e)[..., None].to(BF)
+            if k == "W_uk":
+                t["q_nope"] *= torch.exp2(-e)[None, None].to(BF)
+    got = run_paged(ext, t, True)[0]
+    out, _, usual = E.attention(t["q_nope"][0], t["q_rope"][0], *rows_of(t, 0, n), t["W_uk"], t["W_uv"], SCALE,
+                                E.limits(Sq, n, Sq, True), BF)
+    assert torch.isfinite(got).all()
+    unit = t["W_uv"].double().norm(dim=-1)
+    assert (((got.double() - out) / unit).norm(dim=-1) <= (usual / unit).norm(dim=-1)).all()
